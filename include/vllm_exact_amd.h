@@ -268,6 +268,70 @@ int vxa_exact_linear_op_noalloc(const void* x, int x_dtype, int64_t ldx, const i
                                 int64_t ldo, int64_t m, int64_t n, int64_t k, int f, int trunc,
                                 const int32_t* cfg, int cfg_len, vxa_stream_t stream);
 
+/*
+ * Causal attention over whole prompts (prompt_attn.prompt_attention): sequences of different lengths, their rows
+ * packed one after the other. q [tokens, num_heads, head_dim], k and v [tokens, num_kv_heads, head_dim] of `dtype`
+ * (bf16 or fp16) with element strides of rows and heads; starts [n + 1] int32 on the GPU, the packed rows where the
+ * sequences begin and the last one ends. Row i of a sequence attends to its rows 0 .. i. out may be fp32, bf16 or
+ * fp16. Rows outside the sequences are not written; starts outside [0, tokens] are clamped to it. head_dim 64, 128 or
+ * 256, rows aligned to 16 bytes, else VXA_ERR_UNSUPPORTED. A row's bits depend on its own sequence only.
+ */
+int vxa_prompt_attention(const void* q, int64_t stride_qt, int64_t stride_qh, const void* k, int64_t stride_kt,
+                         int64_t stride_kh, const void* v, int64_t stride_vt, int64_t stride_vh, int dtype,
+                         const int32_t* starts, int64_t n, int64_t tokens, float scale, void* out, int out_dtype,
+                         int64_t stride_ot, int64_t stride_oh, int64_t num_heads, int64_t num_kv_heads,
+                         int64_t head_dim, vxa_stream_t stream);
+
+/*
+ * A paged KV cache in 8 bits (int8_cache): k_cache, v_cache [num_blocks, block_size, num_kv_heads, head_dim] int8 by
+ * strides (block, token in block, head; elements, multiples of 16), k_scale, v_scale [num_blocks, block_size,
+ * num_kv_heads] fp32 by strides. A (token, head) row x is held as q = round(127 x / max|x|) and the scale
+ * max|x| / 127; a row with an infinity or NaN as zeros and the scale NaN.
+ *
+ * write: key, value [tokens, num_kv_heads, head_dim] of `dtype` into the slots block * block_size + place of
+ * slots [tokens] (int64 on the GPU). Slots outside the cache, -1 for one, are skipped.
+ * read: packed rows starts[i] .. starts[i + 1] of key and value (fp32, bf16 or fp16) are tokens first[i], first[i] + 1, ...
+ * of sequence i (first null: from 0), found through block_table [n, bt_cols]. A row past its block table or on a block
+ * that the cache does not have is NaN; rows of no sequence are not written.
+ */
+int vxa_int8_cache_write(const void* key, int64_t stride_kt, int64_t stride_kh, const void* value, int64_t stride_vt,
+                         int64_t stride_vh, int dtype, int64_t tokens, int64_t num_kv_heads, int64_t head_dim,
+                         int8_t* k_cache, int64_t stride_kcb, int64_t stride_kcp, int64_t stride_kch, int8_t* v_cache,
+                         int64_t stride_vcb, int64_t stride_vcp, int64_t stride_vch, float* k_scale,
+                         int64_t stride_ksb, int64_t stride_ksp, int64_t stride_ksh, float* v_scale,
+                         int64_t stride_vsb, int64_t stride_vsp, int64_t stride_vsh, int64_t num_blocks,
+                         int64_t block_size, const int64_t* slots, vxa_stream_t stream);
+int vxa_int8_cache_read(const int8_t* k_cache, int64_t stride_kcb, int64_t stride_kcp, int64_t stride_kch,
+                        const int8_t* v_cache, int64_t stride_vcb, int64_t stride_vcp, int64_t stride_vch,
+                        const float* k_scale, int64_t stride_ksb, int64_t stride_ksp, int64_t stride_ksh,
+                        const float* v_scale, int64_t stride_vsb, int64_t stride_vsp, int64_t stride_vsh,
+                        int64_t num_blocks, int64_t block_size, const int32_t* block_table, int64_t stride_bt,
+                        int64_t bt_cols, const int32_t* starts, const int32_t* first, int64_t n, int64_t tokens,
+                        int64_t num_kv_heads, int64_t head_dim, void* key, int64_t stride_kt, int64_t stride_kh,
+                        void* value, int64_t stride_vt, int64_t stride_vh, int dtype, vxa_stream_t stream);
+
+/*
+ * Attention of drafted tokens over a paged cache (tree_attn.tree_decode). Request i has
+ * T = query_starts[i + 1] - query_starts[i] nodes, the packed query rows from query_starts[i] on, whose keys and values
+ * are the last T of its seq_lens[i] cached ones. A node attends to the context before them and to the drafted key j
+ * where bit j of its tree_mask [tokens] is set (null: to the drafted keys up to its own). A node that attends to
+ * nothing gives zeros. The cache: the query's type, or int8 with k_scale and v_scale as above (both null: not int8).
+ * max_nodes <= 64 and max_seq_len bound T and seq_lens; a request beyond them, shorter than its nodes, or with a block
+ * that the cache does not have gets NaN rows. The workspace holds the partial sums of 512-key segments.
+ */
+int vxa_tree_decode_workspace(int64_t tokens, int64_t num_heads, int64_t head_dim, int64_t max_seq_len,
+                              size_t* ws_bytes);
+int vxa_tree_decode(const void* q, int64_t stride_qt, int64_t stride_qh, int q_dtype, const void* k_cache,
+                    int64_t stride_kcb, int64_t stride_kcp, int64_t stride_kch, const void* v_cache,
+                    int64_t stride_vcb, int64_t stride_vcp, int64_t stride_vch, const float* k_scale,
+                    int64_t stride_ksb, int64_t stride_ksp, int64_t stride_ksh, const float* v_scale,
+                    int64_t stride_vsb, int64_t stride_vsp, int64_t stride_vsh, int64_t num_blocks, int64_t block_size,
+                    const int32_t* block_table, int64_t stride_bt, int64_t bt_cols, const int32_t* seq_lens,
+                    const int32_t* query_starts, const int64_t* tree_mask, float scale, void* out, int out_dtype,
+                    int64_t stride_ot, int64_t stride_oh, int64_t n, int64_t tokens, int64_t num_heads,
+                    int64_t num_kv_heads, int64_t head_dim, int64_t max_nodes, int64_t max_seq_len, void* ws,
+                    size_t ws_bytes, vxa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,114 @@
+// Device helpers that the attention kernels share (gfx950): the softmax's constants, exchanges
+// between the lane rows of a wave, and the 16-bit element types with their matrix instructions.
+#pragma once
+
+#include <type_traits>
+
+#include "common.h"
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+constexpr float kNegInf = -__builtin_huge_valf();
+// Where a unit's running maximum starts: below every finite score, so that the first tile replaces it,
+// and finite, so that keys scoring -inf weigh exp2(-inf - m) = 0 also where nothing else has been seen
+// (-inf - -inf would be NaN). Such a unit's state is (kLowest, 0, 0), which adds 0 to any merge.
+constexpr float kLowest = -3.402823466e38f;  // -FLT_MAX
+
+__device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Exchanges between the four 16-lane rows of a wave on the vector ALU (gfx950 lane swaps), in
+// place of ds_bpermute round trips through the LDS pipe. The fp32 pairs come back as
+// {x of the lower row or half, x of the upper}, for both sides.
+__device__ inline void swap32(float& a, float& b) {  // a's upper half <-> b's lower half
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  a = __uint_as_float(r[0]);
+  b = __uint_as_float(r[1]);
+}
+__device__ inline void swap16(float& a, float& b) {  // a's odd rows <-> b's even rows
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  a = __uint_as_float(r[0]);
+  b = __uint_as_float(r[1]);
+}
+__device__ inline float rows_max(float v) {
+  float a = v, b = v;
+  swap16(a, b);
+  v = fmaxf(a, b);
+  a = v, b = v;
+  swap32(a, b);
+  return fmaxf(a, b);
+}
+__device__ inline float rows_sum(float v) {
+  float a = v, b = v;
+  swap16(a, b);
+  v = a + b;
+  a = v, b = v;
+  swap32(a, b);
+  return a + b;
+}
+template <int N, typename F, int I = 0>
+__device__ inline void static_for(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for<N, F, I + 1>(static_cast<F&&>(f));
+  }
+}
+
+
+// The two 16-bit element types. Operands of the matrix instructions are held as four dwords of
+// two elements each; products of two such elements are exact in fp32.
+struct BF16 {
+  static constexpr uint32_t kExpMask = 0x7F80u, kOne = 0x3F80u;
+  static constexpr int kDtype = VXA_BF16;
+  static __device__ inline float to_f32(uint16_t b) { return bf16_to_f32(b); }
+  static __device__ inline uint32_t pack(float a, float b) {  // round to nearest even
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
+  }
+  static __device__ inline v2f unpack(uint32_t w) {
+    return v2f{__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)};
+  }
+  static __device__ inline v4f mfma16(v4u32 a, v4u32 b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  }
+  static __device__ inline v16f mfma32(v4u32 a, v4u32 b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  }
+};
+struct FP16 {
+  static constexpr uint32_t kExpMask = 0x7C00u, kOne = 0x3C00u;
+  static constexpr int kDtype = VXA_F16;
+  static __device__ inline float to_f32(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
+  static __device__ inline uint32_t pack(float a, float b) {  // round to nearest even
+    return __builtin_bit_cast(uint32_t, v2h{(_Float16)a, (_Float16)b});
+  }
+  static __device__ inline v2f unpack(uint32_t w) { return __builtin_convertvector(__builtin_bit_cast(v2h, w), v2f); }
+  static __device__ inline v4f mfma16(v4u32 a, v4u32 b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  }
+  static __device__ inline v16f mfma32(v4u32 a, v4u32 b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  }
+};
+
+// Whether one of a dword's two elements is an infinity or NaN.
+template <typename T>
+__device__ inline bool any_special(uint32_t w) {
+  constexpr uint32_t m = T::kExpMask;
+  return (w & m) == m || ((w >> 16) & m) == m;
+}
+// The dword with its infinities and NaN replaced by 0, and which of its elements add +inf (SIGN = 0: +inf
+// and NaN) or -inf (SIGN = 1: -inf and NaN), as elements 1 and 0.
+template <typename T>
+__device__ inline uint32_t only_finite(uint32_t w) {
+  constexpr uint32_t m = T::kExpMask;
+  return ((w & m) == m ? 0u : w & 0xFFFFu) | (((w >> 16) & m) == m ? 0u : w & 0xFFFF0000u);
+}
+template <typename T, int SIGN>
+__device__ inline uint32_t special_flags(uint32_t w) {
+  constexpr uint32_t m = T::kExpMask, other = m | (SIGN ? 0u : 0x8000u);  // the infinity that does not count
+  const uint32_t lo = w & 0xFFFFu, hi = w >> 16;
+  return ((lo & m) == m && lo != other ? T::kOne : 0u) | ((hi & m) == m && hi != other ? T::kOne << 16 : 0u);
+}

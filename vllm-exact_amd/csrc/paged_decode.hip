@@ -42,7 +42,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "common.h"
+#include "attention_common.h"
 
 namespace {
 
@@ -75,14 +75,6 @@ struct PagedParams {
   int64_t sot, soh;
   int32_t out_dtype;
 };
-
-constexpr float kNegInf = -__builtin_huge_valf();
-// Where a unit's running maximum starts: below every finite score, so that the first tile replaces it,
-// and finite, so that keys scoring -inf weigh exp2(-inf - m) = 0 also where nothing else has been seen
-// (-inf - -inf would be NaN). Such a unit's state is (kLowest, 0, 0), which adds 0 to any merge.
-constexpr float kLowest = -3.402823466e38f;  // -FLT_MAX
-
-__device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Fixed-order merge of a softmax state (m, l, a) with another (ms, ls, as_)
 // (paged_attn.py:84-93, base-2 logits). A state with m == -inf contributes exactly 0.
@@ -119,47 +111,10 @@ struct DimTraits {
 // the wave's running state, so that units can also be computed apart and merged later.
 constexpr int kUnit = 64;
 
-// Exchanges between the four 16-lane rows of a wave on the vector ALU (gfx950 lane swaps), in
-// place of ds_bpermute round trips through the LDS pipe. The fp32 pairs come back as
-// {x of the lower row or half, x of the upper}, for both sides.
-__device__ inline void swap32(float& a, float& b) {  // a's upper half <-> b's lower half
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-  a = __uint_as_float(r[0]);
-  b = __uint_as_float(r[1]);
-}
-__device__ inline void swap16(float& a, float& b) {  // a's odd rows <-> b's even rows
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-  a = __uint_as_float(r[0]);
-  b = __uint_as_float(r[1]);
-}
-__device__ inline float rows_max(float v) {
-  float a = v, b = v;
-  swap16(a, b);
-  v = fmaxf(a, b);
-  a = v, b = v;
-  swap32(a, b);
-  return fmaxf(a, b);
-}
-__device__ inline float rows_sum(float v) {
-  float a = v, b = v;
-  swap16(a, b);
-  v = a + b;
-  a = v, b = v;
-  swap32(a, b);
-  return a + b;
-}
 // Lane H of the caller's 16-lane row, for every lane of the row (a DPP operand, no LDS).
 template <int H>
 __device__ inline float row_lane(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + H, 0xf, 0xf, false));
-}
-
-template <int N, typename F, int I = 0>
-__device__ inline void static_for(F&& f) {
-  if constexpr (I < N) {
-    f(std::integral_constant<int, I>{});
-    static_for<N, F, I + 1>(static_cast<F&&>(f));
-  }
 }
 
 // 16-byte (8-byte for D = 64) pieces of V a lane reads per key, raw.

@@ -47,6 +47,11 @@ EXPORTED = (
     "vxa_exact_linear_op_noalloc",
     "vxa_exact_linear_op_scratch",
     "vxa_exact_linear_op",
+    "vxa_prompt_attention",
+    "vxa_int8_cache_write",
+    "vxa_int8_cache_read",
+    "vxa_tree_decode_workspace",
+    "vxa_tree_decode",
 )
 
 _i64, _i32, _int, _vp, _sz = ctypes.c_int64, ctypes.c_int32, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
@@ -103,6 +108,25 @@ _SIGNATURES = {
         _int,
         [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, _vp,
          _int, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp],
+    ),
+    "vxa_prompt_attention": (
+        _int,
+        [_vp, _i64, _i64] * 3 + [_int, _vp, _i64, _i64, ctypes.c_float, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp],
+    ),
+    "vxa_int8_cache_write": (
+        _int,
+        [_vp, _i64, _i64] * 2 + [_int, _i64, _i64, _i64] + [_vp, _i64, _i64, _i64] * 4 + [_i64, _i64, _vp, _vp],
+    ),
+    "vxa_int8_cache_read": (
+        _int,
+        [_vp, _i64, _i64, _i64] * 4 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64]
+        + [_vp, _i64, _i64] * 2 + [_int, _vp],
+    ),
+    "vxa_tree_decode_workspace": (_int, [_i64, _i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "vxa_tree_decode": (
+        _int,
+        [_vp, _i64, _i64, _int] + [_vp, _i64, _i64, _i64] * 4 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+         ctypes.c_float, _vp, _int] + [_i64] * 9 + [_vp, _sz, _vp],
     ),
 }
 
@@ -231,4 +255,16 @@ def paged_units_workspace(n, H, KV, D, max_len, split, blk, waves):
     ws = _sz()
     check(lib().vxa_paged_decode_units_workspace(n, H, KV, D, max_len, split, blk, waves, ctypes.byref(ws)),
           "paged_decode_units_workspace")
+    return ws.value
+
+
+def strided(t, *axes):
+    """(pointer, strides of `axes`) as the entry points take a tensor; nulls and zeros for None."""
+    return (None,) + (0,) * len(axes) if t is None else (t.data_ptr(),) + tuple(t.stride(a) for a in axes)
+
+
+@functools.lru_cache(maxsize=1024)
+def tree_workspace(tokens, H, D, max_seq_len):
+    ws = _sz()
+    check(lib().vxa_tree_decode_workspace(tokens, H, D, max_seq_len, ctypes.byref(ws)), "tree_decode_workspace")
     return ws.value
