@@ -3,16 +3,21 @@
 //   o_i = sum_{j <= i} p_ij v_j / sum_{j <= i} p_ij,   p_ij = exp(scale q_i.k_j - max_j scale q_i.k_j)
 // for every row i of every sequence, with groups of G = H / KV query heads on one key/value head.
 //
-// Work split. A workgroup of 4 waves computes 128 rows of one (sequence, head), 32 rows a wave, and walks the
-// keys up to its last row in tiles of 64 (32 at 256 dims) with one running maximum and sum: every score is computed once and kept
-// in registers. A wave's rows are the columns of S^T = K Q^T (32 x 32 x 16 MFMAs) and of O^T = V^T P^T, so a lane
-// holds scores of one row only, and with the keys of the second product taken in the order in which the first one
-// leaves them in the lane, P goes from one product to the other without leaving the lane. The tiles of K and V go
-// through registers into LDS, V transposed on the way (a byte permute for two elements), two tiles in turn.
+// Work split. A workgroup of 4 waves computes 32 rows of four heads of one KV head (64 rows of two, 128 of one where
+// the group has no more), 32 rows of one head a wave, and walks the keys up to its last row in tiles of 64 (32 at 256
+// dims) with one running maximum and sum: every score is computed once and kept in registers. A wave's rows are the
+// columns of S^T = K Q^T (32 x 32 x 16 MFMAs) and of O^T = V^T P^T, so a lane holds scores of one row only, and with the
+// keys of the second product taken in the order in which the first one leaves them in the lane, P goes from one product
+// to the other without leaving the lane. The tiles of K and V are copied straight into LDS, two in turn; V is transposed
+// as it is read from there. Two workgroups share a CU, so that one's softmax runs beside the other's products.
 // A row's order of operations depends on its place in its sequence alone, not on the batch.
 //
 // Rounding. Scores, maxima, sums and accumulators are fp32; P is rounded to the 16-bit element type for the second
 // product, an error of the size of the output's own rounding, while its sum takes the fp32 values.
+//
+// Measured (one prompt of 8192 tokens, 32 heads on 8, 128 dims, bf16): 525 us, 1048 TFLOP/s of the scores that count; a
+// large library matrix product reaches 1185 on the same card. The matrix pipes are busy 52 % of the cycles, the vector
+// ALU's softmax takes most of the others, and the clock falls below 2 GHz.
 
 #include <algorithm>
 #include <cmath>
@@ -21,8 +26,11 @@
 
 namespace {
 
-constexpr int kRows = 128;  // query rows of a workgroup
-constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+// A running maximum stays until a score passes it by this much (in powers of two): weights up to 2^8 are as precise as
+// weights up to 1 in every type here, and a tile seldom passes it, so the accumulators are seldom rescaled.
+constexpr float kSlack = 8.0f;
 
 struct PromptParams {
   const uint16_t* q;
@@ -35,12 +43,14 @@ struct PromptParams {
   float scale_log2;  // > 0: the sign and a zero of the scale are in q's elements,
   uint32_t q_and, q_xor;  // (q & q_and) ^ q_xor, so that scaled scores keep the order of the products
   int32_t n, total, H, G, tiles;
+  int32_t heads, rows;  // of a workgroup: heads of one KV head, and rows of each; 4 waves of 32 rows in all
   void* out;
   int64_t sot, soh;
   int32_t out_dtype;
+  bool out_wide;  // the output has the input's type and its rows start on 8 bytes
 };
 
-// The sequence and rows of tile `tile`, counted over the sequences' tiles of kRows rows in order.
+// The sequence and rows of tile `tile`, counted over the sequences' tiles of p.rows rows in order.
 struct Tile {
   int base, len, row0;  // first packed row of the sequence, its length (0: no such tile), the tile's first row in it
 };
@@ -54,7 +64,7 @@ __device__ inline Tile find_tile(const PromptParams& p, int tile) {
       lo = max(p.cu[j], 0);
       len = max(min(p.cu[j + 1], p.total) - lo, 0);
     }
-    const int mine = (len + kRows - 1) / kRows;
+    const int mine = (len + p.rows - 1) / p.rows;
     int sum = mine;  // inclusive over the lanes
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) {
@@ -65,68 +75,59 @@ __device__ inline Tile find_tile(const PromptParams& p, int tile) {
     if (hit != 0) {
       const int at = __builtin_ctzll(hit);
       const int first = before + __shfl(sum - mine, at);
-      return Tile{__shfl(lo, at), __shfl(len, at), (tile - first) * kRows};
+      return Tile{__shfl(lo, at), __shfl(len, at), (tile - first) * p.rows};
     }
     before += __shfl(sum, 63);
   }
   return Tile{0, 0, 0};
 }
 
-// Values of keys that some rows do not attend to may be infinities or NaN, and 0 times those is NaN. In a tile with
-// masked keys they enter the product as 0, and what they add is added to the rows that attend to them. a: 8 keys
-// (key0 + j % 4 + 8 (j / 4)) of one dim.
-template <typename T>
-__device__ inline void add_special(v4u32& a, int key0, int row, v16f& acc) {
-  if (!__any(any_special<T>(a[0]) || any_special<T>(a[1]) || any_special<T>(a[2]) || any_special<T>(a[3]))) return;
-  v4u32 plus, minus, seen;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    plus[i] = special_flags<T, 0>(a[i]);
-    minus[i] = special_flags<T, 1>(a[i]);
-    a[i] = only_finite<T>(a[i]);
-    const int key = key0 + 2 * (i % 2) + 8 * (i / 2);
-    seen[i] = (key <= row ? (uint32_t)T::kOne : 0u) | (key + 1 <= row ? (uint32_t)T::kOne << 16 : 0u);
-  }
-  const v16f zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  const v16f up = T::mfma32(plus, seen, zero);
-#pragma unroll
-  for (int r = 0; r < 16; ++r)
-    if (up[r] > 0.0f) acc[r] += __builtin_huge_valf();
-  const v16f down = T::mfma32(minus, seen, zero);
-#pragma unroll
-  for (int r = 0; r < 16; ++r)
-    if (down[r] > 0.0f) acc[r] += kNegInf;
+// Four 16-bit elements of one column, from four rows that the 16 lanes of a group address together (8 bytes a lane,
+// four lanes a row): gfx950's transposing LDS read.
+__device__ inline v2u32 read_transposed(const char* lds) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4s lds_v4s;
+  return __builtin_bit_cast(v2u32, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)lds));
 }
 
+typedef __attribute__((address_space(3))) void lds_void_t;
+
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void prompt_kernel(PromptParams p) {
-  constexpr int kKeys = D == 256 ? 32 : 64;  // keys of a tile: at 256 dims 64 keys leave no registers for the loads ahead
-  constexpr int KU = kKeys / 32, KCH = kKeys / 8;
-  constexpr int QS = D / 16;   // MFMA steps over the head's dims
-  constexpr int DB = D / 32;   // 32-dim blocks of O^T
-  constexpr int KC = D / 8;    // 16-byte chunks of a key
-  constexpr int KL = kKeys * KC / kThreads;             // chunks of K a thread stages
-  constexpr int VD = D == 64 ? 2 : 4;                   // dims of a unit of V, 8 keys
-  constexpr int VU = kKeys / 8 * (D / VD) / kThreads;   // units of V a thread stages
-  __shared__ v4u32 s_k[2][kKeys * KC];   // [key][chunk ^ key]
-  __shared__ v4u32 s_v[2][D * KCH];        // [dim][chunk of 8 keys, swizzled]
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_kernel(PromptParams p) {
+  constexpr int kKeys = D == 256 ? 32 : 64;  // keys of a tile: at 256 dims 64 keys' scores leave too few registers
+  constexpr int KU = kKeys / 32;
+  constexpr int QS = D / 16;       // MFMA steps over the head's dims
+  constexpr int DB = D / 32;       // 32-dim blocks of O^T
+  constexpr int kRow = 2 * D;      // bytes of a key in LDS
+  constexpr int kTileBytes = kKeys * kRow;
+  constexpr int kPer = 1024 / kRow;                   // keys that one wave's copy moves
+  constexpr int kRound = kPer * kWaves;               // ... that all waves' copies move
+  constexpr int kCopies = kKeys / kRound;             // copies of a wave for a tile of K, and of V
+  constexpr int kBases = kRound < 16 && D > 64 ? 16 / kRound : 1;  // copies after which K's swizzle repeats
+  __shared__ __attribute__((aligned(1024))) char s_kv[2][2][kTileBytes];  // [buffer][K, V][key][16-byte chunk, swizzled]
+  // A key's chunk c lies at c ^ swizzle(key): 16 lanes that read one chunk of 16 keys (K), or four chunks of four keys
+  // (V, transposed), meet 16 different 16-byte columns of the 256 bytes that the banks deliver.
+  auto swk = [](int key) { return D == 64 ? (key >> 1) & 7 : key & 15; };
+  auto swv = [](int key) { return D == 64 ? 4 * ((key >> 1) & 1) : 4 * (key & 3); };
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
 
   // Workgroups of one KV head run on one XCD, longest rows first.
-  const int x = (int)(blockIdx.x % p.H);
-  const int head = p.H % 8 == 0 ? (x % 8) * (p.H / 8) + x / 8 : x;
-  const Tile tile = find_tile(p, p.tiles - 1 - (int)(blockIdx.x / p.H));
+  const int groups = p.H / p.heads;
+  const int x = (int)(blockIdx.x % groups);
+  const int head = (groups % 8 == 0 ? (x % 8) * (groups / 8) + x / 8 : x) * p.heads + wave % p.heads;
+  const Tile tile = find_tile(p, p.tiles - 1 - (int)(blockIdx.x / groups));
   if (tile.len == 0) return;
   const int base = __builtin_amdgcn_readfirstlane(tile.base);
   const int len = __builtin_amdgcn_readfirstlane(tile.len);
   const int row0 = __builtin_amdgcn_readfirstlane(tile.row0);
-  const uint16_t* kh = p.k + (int64_t)base * p.skt + (int64_t)(head / p.G) * p.skh;
-  const uint16_t* vh = p.v + (int64_t)base * p.svt + (int64_t)(head / p.G) * p.svh;
+  const char* kh = reinterpret_cast<const char*>(p.k + (int64_t)base * p.skt + (int64_t)(head / p.G) * p.skh);
+  const char* vh = reinterpret_cast<const char*>(p.v + (int64_t)base * p.svt + (int64_t)(head / p.G) * p.svh);
+  const int64_t skt = 2 * p.skt, svt = 2 * p.svt;
 
-  const int wrow = row0 + 32 * wave;  // the wave's first row
+  const int wrow = row0 + wave / p.heads * 32;  // the wave's first row
   const int row = wrow + col;
   v4u32 qf[QS];
   {
@@ -135,148 +136,188 @@ __global__ __launch_bounds__(kThreads) void prompt_kernel(PromptParams p) {
     for (int i = 0; i < QS; ++i) qf[i] = (*reinterpret_cast<const v4u32*>(q + 16 * i) & p.q_and) ^ p.q_xor;
   }
 
-  const int last = min(row0 + kRows, len);              // keys of the workgroup
+  const int last = min(row0 + p.rows, len);  // keys of the workgroup
   const int tiles = (last + kKeys - 1) / kKeys;
-  v4u32 kr[KL];
-  uint32_t vr[VU][8][VD / 2];
-  // V's slots: chunk c of a tile holds, for j = 0..7, the key 32 (c / 4) + 16 (c / 2 % 2) + 4 (c % 2) + (j % 4) + 8 (j / 4),
-  // which is the order in which an S^T tile's registers hold a lane's keys.
-  auto load = [&](int t) {
+
+  // Tiles go straight from memory into LDS (global_load_lds_dwordx4: lane i's 16 bytes land at M0 + 16 i), from inline
+  // asm: with the builtin the compiler, which cannot tell the buffers apart, waits for the next tile's copies before it
+  // reads this one. Only the waits below order them. Copy i of a wave moves keys i * kRound + wave * kPer + [0, kPer).
+  const int key_l = wave * kPer + lane / (kRow / 16), chunk = lane % (kRow / 16);
+  const char* ksrc[kBases];
 #pragma unroll
-    for (int i = 0; i < KL; ++i) {
-      const int u = threadIdx.x + i * kThreads;
-      kr[i] = *reinterpret_cast<const v4u32*>(kh + (int64_t)min(t * kKeys + u / KC, len - 1) * p.skt + 8 * (u % KC));
-    }
-#pragma unroll
-    for (int i = 0; i < VU; ++i) {
-      const int u = threadIdx.x + i * kThreads;
-      const int c = u / (D / VD), d = VD * (u % (D / VD));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int key = t * kKeys + 32 * (c / 4) + 16 * (c / 2 % 2) + 4 * (c % 2) + j % 4 + 8 * (j / 4);
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(vh + (int64_t)min(key, len - 1) * p.svt + d);
-        if constexpr (VD == 2) {
-          vr[i][j][0] = *src;
-        } else {
-          const v2u32 w = *reinterpret_cast<const v2u32*>(src);
-          vr[i][j][0] = w.x, vr[i][j][1] = w.y;
-        }
-      }
-    }
+  for (int i = 0; i < kBases; ++i) ksrc[i] = kh + (key_l + i * kRound) * skt + 16 * (chunk ^ swk(key_l + i * kRound));
+  const char* vsrc = vh + key_l * svt + 16 * (chunk ^ swv(key_l));
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t*)&s_kv[0][0][0]) + wave * 1024;
+  auto copy = [&](const char* src, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
   };
-  auto vslot = [](int d, int c) { return d * KCH + (c ^ ((d ^ (d >> 3)) & (KCH - 1))); };
-  auto store = [&](int buf) {
+  auto load = [&](int t, int buf) {
+    const uint32_t dst = lds0 + buf * 2 * kTileBytes;
+    if ((t + 1) * kKeys <= len) {
 #pragma unroll
-    for (int i = 0; i < KL; ++i) {
-      const int u = threadIdx.x + i * kThreads;
-      const int key = u / KC, c = u % KC;
-      s_k[buf][key * KC + (c ^ (key & (KC < 16 ? 7 : 15)))] = kr[i];
-    }
+      for (int i = 0; i < kCopies; ++i) {
+        copy(ksrc[i % kBases] + (int64_t)(t * kKeys + i / kBases * kBases * kRound) * skt, dst + i * kWaves * 1024);
+        copy(vsrc + (int64_t)(t * kKeys + i * kRound) * svt, dst + kTileBytes + i * kWaves * 1024);
+      }
+    } else {  // keys past the sequence's end repeat its last one
 #pragma unroll
-    for (int i = 0; i < VU; ++i) {
-      const int u = threadIdx.x + i * kThreads;
-      const int c = u / (D / VD), d = VD * (u % (D / VD));
-#pragma unroll
-      for (int e = 0; e < VD; ++e) {
-        v4u32 w;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = __builtin_amdgcn_perm(vr[i][2 * j + 1][e / 2], vr[i][2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
-        s_v[buf][vslot(d + e, c)] = w;
+      for (int i = 0; i < kCopies; ++i) {
+        const int in_tile = i * kRound + key_l, key = min(t * kKeys + in_tile, len - 1);
+        copy(kh + key * skt + 16 * (chunk ^ swk(in_tile)), dst + i * kWaves * 1024);
+        copy(vh + key * svt + 16 * (chunk ^ swv(in_tile)), dst + kTileBytes + i * kWaves * 1024);
       }
     }
   };
 
-  float m = kLowest, l = 0.0f;
+  // Where this lane reads: K's row `col` of a 32-key block, V's rows 4 half + (lane % 16) / 4 and 8 further.
+  const int vkey = 4 * half + (lane & 15) / 4;
+  const int vdim = 2 * ((lane >> 4) & 1) + (lane & 3) / 2;  // chunk in a 32-dim block
+  const int vbyte = vkey * kRow + 8 * (lane & 1);
+
+  float m, l[4];
   v16f acc[DB];
-#pragma unroll
-  for (int i = 0; i < DB; ++i) acc[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
-  load(0);
-  store(0);
-  for (int t = 0; t < tiles; ++t) {
+  // One tile. MASKED: some of its keys may come after some of the wave's rows.
+  // CAREFUL: values of keys that some rows do not attend to may be infinities or NaN, and 0 times those is NaN; here they
+  // enter the product as 0, and the rows that attend to them add them at the end. The pass that does not look ends with
+  // NaN wherever that mattered.
+  auto step = [&](int t, auto masked_c, auto careful_c) {
+    constexpr bool MASKED = decltype(masked_c)::value, CAREFUL = decltype(careful_c)::value;
+    // Tile t has landed, for every wave, and every wave has read tile t - 1: its buffer takes tile t + 1.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int buf = t & 1;
-    __syncthreads();
-    if (t + 1 < tiles) load(t + 1);
+    if (t + 1 < tiles) load(t + 1, buf ^ 1);
     const int key0 = t * kKeys;
-    if (key0 <= wrow + 31) {  // some row of the wave attends to the tile
-      v16f s[KU];
+    if (MASKED && key0 > wrow + 31) return;  // no row of the wave attends to the tile
+    const char* kt = s_kv[buf][0] + col * kRow;
+    const char* vt = s_kv[buf][1] + vbyte;
+    v16f s[KU];
 #pragma unroll
-      for (int u = 0; u < KU; ++u) {
-        s[u] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-        const int key = 32 * u + col;
+    for (int u = 0; u < KU; ++u) s[u] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < QS; ++i)
-          s[u] = T::mfma32(s_k[buf][key * KC + ((2 * i + half) ^ (key & (KC < 16 ? 7 : 15)))], qf[i], s[u]);
-      }
-      const bool masked = key0 + kKeys - 1 > wrow;
-      if (masked) {
+    for (int i = 0; i < QS; ++i)
 #pragma unroll
-        for (int u = 0; u < KU; ++u)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (key0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * half > row) s[u][r] = kNegInf;
-      }
-      float top = s[0][0];
+      for (int u = 0; u < KU; ++u)
+        s[u] = T::mfma32(*reinterpret_cast<const v4u32*>(kt + 32 * u * kRow + 16 * ((2 * i + half) ^ swk(col))), qf[i], s[u]);
+    if constexpr (MASKED) {
 #pragma unroll
       for (int u = 0; u < KU; ++u)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-      float ta = top, tb = top;
-      swap32(ta, tb);
-      top = fmaxf(ta, tb) * p.scale_log2;
-      if (__any(top > m)) {
-        const float mn = fmaxf(m, top);
-        const float c = exp2_hw(m - mn);
-        l *= c;
-#pragma unroll
-        for (int i = 0; i < DB; ++i) acc[i] = acc[i] * c;
-        m = mn;
-      }
-      v4u32 pf[2 * KU];
-#pragma unroll
-      for (int u = 0; u < KU; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float a = exp2_hw(fmaf(s[u][r], p.scale_log2, -m)), b = exp2_hw(fmaf(s[u][r + 1], p.scale_log2, -m));
-          l += a;
-          l += b;
-          pf[2 * u + r / 8][r % 8 / 2] = T::pack(a, b);
-        }
-#pragma unroll
-      for (int c = 0; c < 2 * KU; ++c)
-#pragma unroll
-        for (int i = 0; i < DB; ++i) {
-          v4u32 a = s_v[buf][vslot(32 * i + col, 2 * c + half)];
-          if (masked) add_special<T>(a, key0 + 32 * (c / 2) + 16 * (c % 2) + 4 * half, row, acc[i]);
-          acc[i] = T::mfma32(a, pf[c], acc[i]);
-        }
+        for (int r = 0; r < 16; ++r)
+          if (key0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * half > row) s[u][r] = kNegInf;
     }
-    if (t + 1 < tiles) store(buf ^ 1);
-  }
-  float la = l, lb = l;
-  swap32(la, lb);
-  l = la + lb;
-  if (row >= len) return;
-  const int64_t at = (int64_t)(base + row) * p.sot + (int64_t)head * p.soh;
+    float top = s[0][0];
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+    float ta = top, tb = top;
+    swap32(ta, tb);
+    top = fmaxf(ta, tb) * p.scale_log2;
+    if (__any(top > m + kSlack)) {
+      const float mn = fmaxf(m, top);
+      const float c = exp2_hw(m - mn);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l[i] *= c;
+#pragma unroll
+      for (int i = 0; i < DB; ++i) acc[i] = acc[i] * c;
+      m = mn;
+    }
+    v4u32 pf[2 * KU];
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float a = exp2_hw(fmaf(s[u][r], p.scale_log2, -m)), b = exp2_hw(fmaf(s[u][r + 1], p.scale_log2, -m));
+        l[r % 4] += a;
+        l[r % 4 + 1] += b;
+        pf[2 * u + r / 8][r % 8 / 2] = T::pack(a, b);
+      }
+    // Chunk c of P holds, for j = 0..7, the keys 16 c + 4 half + j % 4 + 8 (j / 4): the order of the lane's scores.
+    auto values = [&](int c, int i) {
+      const char* at = vt + 16 * c * kRow + 16 * ((4 * i + vdim) ^ swv(vkey));
+      const v2u32 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
+      return v4u32{lo.x, lo.y, hi.x, hi.y};
+    };
+#pragma unroll
+    for (int c = 0; c < 2 * KU; ++c)
+#pragma unroll
+      for (int i = 0; i < DB; ++i) {
+        v4u32 a = values(c, i);
+        if constexpr (CAREFUL) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) a[j] = only_finite<T>(a[j]);
+        }
+        acc[i] = T::mfma32(a, pf[c], acc[i]);
+      }
+  };
+  const int full = min((wrow + 1) / kKeys, tiles);  // tiles without masked keys
+  auto start = [&] {
+    m = kLowest;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l[i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DB; ++i) acc[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    load(0, 0);
+  };
+  start();
+  int t = 0;
+  for (; t < full; ++t) step(t, std::false_type{}, std::false_type{});
+  for (; t < tiles; ++t) step(t, std::true_type{}, std::false_type{});
+  float odd = 0.0f;  // 0 where all sums are finite, else NaN
 #pragma unroll
   for (int i = 0; i < DB; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      store_f32_as(p.out, p.out_dtype, at + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half, acc[i][r] / l);
+    for (int r = 0; r < 16; ++r) odd = fmaf(acc[i][r], 0.0f, odd);
+  const bool careful = __syncthreads_or(odd != 0.0f);
+  if (careful) {
+    start();
+    for (t = 0; t < tiles; ++t) step(t, std::true_type{}, std::true_type{});
+  }
+  float la = (l[0] + l[1]) + (l[2] + l[3]), lb = la;
+  swap32(la, lb);
+  const float inv = 1.0f / (la + lb);
+  if (row >= len) return;
+  const int64_t at = (int64_t)(base + row) * p.sot + (int64_t)head * p.soh + 4 * half;
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      float o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = acc[i][r + j] * inv;
+      if (careful) {
+#pragma unroll 1
+        for (int key = 0; key <= row; ++key) {
+          const v2u32 w = *reinterpret_cast<const v2u32*>(vh + key * svt + 64 * i + 4 * r + 8 * half);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float f = T::to_f32((uint16_t)(w[j / 2] >> (16 * (j % 2))));
+            if (!__builtin_isfinite(f)) o[j] += f;
+          }
+        }
+      }
+      const int64_t to = at + 32 * i + 2 * r;
+      if (p.out_wide) {
+        reinterpret_cast<v2u32*>(reinterpret_cast<uint16_t*>(p.out) + to)[0] = v2u32{T::pack(o[0], o[1]), T::pack(o[2], o[3])};
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) store_f32_as(p.out, p.out_dtype, to + j, o[j]);
+      }
+    }
 }
 
 template <typename T>
 hipError_t launch_prompt(int64_t D, const PromptParams& p, hipStream_t st) {
-  const int64_t blocks = (int64_t)p.tiles * p.H;
+  const int64_t blocks = (int64_t)p.tiles * (p.H / p.heads);
   if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)blocks), threads(kThreads);
   if (D == 64)
-    hipLaunchKernelGGL((prompt_kernel<T, 64>), grid, threads, 0, st, p);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, 64>), grid, threads, 0, st, p);
   else if (D == 128)
-    hipLaunchKernelGGL((prompt_kernel<T, 128>), grid, threads, 0, st, p);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, 128>), grid, threads, 0, st, p);
   else
-    hipLaunchKernelGGL((prompt_kernel<T, 256>), grid, threads, 0, st, p);
+    hipLaunchKernelGGL((prompt_attention_kernel<T, 256>), grid, threads, 0, st, p);
   return hipGetLastError();
 }
 
@@ -307,9 +348,12 @@ extern "C" int vxa_prompt_attention(const void* q, int64_t sqt, int64_t sqh, con
   p.q_and = scale == 0.0f ? 0u : 0xFFFFFFFFu;
   p.q_xor = scale < 0.0f ? 0x80008000u : 0u;
   p.n = (int32_t)n, p.total = (int32_t)tokens, p.H = (int32_t)num_heads, p.G = (int32_t)(num_heads / num_kv_heads);
+  p.heads = p.G % 4 == 0 ? 4 : p.G % 2 == 0 ? 2 : 1;
+  p.rows = 32 * kWaves / p.heads;
   // At most this many tiles: each sequence's last one may be part filled.
-  p.tiles = (int32_t)std::min<int64_t>(cdiv<int64_t>(tokens, kRows) + n, tokens);
+  p.tiles = (int32_t)std::min<int64_t>(cdiv<int64_t>(tokens, p.rows) + n, tokens);
   p.out = out, p.sot = sot, p.soh = soh, p.out_dtype = out_dtype;
+  p.out_wide = out_dtype == dtype && (uintptr_t)out % 8 == 0 && sot % 4 == 0 && soh % 4 == 0;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const hipError_t err = dtype == VXA_BF16 ? launch_prompt<BF16>(head_dim, p, st) : launch_prompt<FP16>(head_dim, p, st);
   if (err == hipErrorInvalidConfiguration) return VXA_ERR_UNSUPPORTED;
