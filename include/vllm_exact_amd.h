@@ -317,7 +317,8 @@ int vxa_int8_cache_read(const int8_t* k_cache, int64_t stride_kcb, int64_t strid
  * where bit j of its tree_mask [tokens] is set (null: to the drafted keys up to its own). A node that attends to
  * nothing gives zeros. The cache: the query's type, or int8 with k_scale and v_scale as above (both null: not int8).
  * max_nodes <= 64 and max_seq_len bound T and seq_lens; a request beyond them, shorter than its nodes, or with a block
- * that the cache does not have gets NaN rows. The workspace holds the partial sums of 512-key segments.
+ * that the cache does not have gets NaN rows. The workspace (on 16 bytes) holds the partial sums of groups of
+ * four 512-key segments, four for each group.
  */
 int vxa_tree_decode_workspace(int64_t tokens, int64_t num_heads, int64_t head_dim, int64_t max_seq_len,
                               size_t* ws_bytes);

@@ -17,6 +17,9 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // and finite, so that keys scoring -inf weigh exp2(-inf - m) = 0 also where nothing else has been seen
 // (-inf - -inf would be NaN). Such a unit's state is (kLowest, 0, 0), which adds 0 to any merge.
 constexpr float kLowest = -3.402823466e38f;  // -FLT_MAX
+// A running maximum stays until a score passes it by this much (in powers of two): weights up to 2^8 are as precise as
+// weights up to 1 in every type here, and a tile seldom passes it, so the accumulators are seldom rescaled.
+constexpr float kSlack = 8.0f;
 
 __device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -28,9 +28,6 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-// A running maximum stays until a score passes it by this much (in powers of two): weights up to 2^8 are as precise as
-// weights up to 1 in every type here, and a tile seldom passes it, so the accumulators are seldom rescaled.
-constexpr float kSlack = 8.0f;
 
 struct PromptParams {
   const uint16_t* q;

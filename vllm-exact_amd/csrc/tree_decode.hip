@@ -15,9 +15,11 @@
 // V is loaded by rows, each lane 8 keys of the same D / 16 dims, and transposed in registers, one byte permute
 // for every two elements. K and V go from HBM to registers; LDS holds only the segment's row offsets and scales.
 //
-// Order. Keys are cut into segments of kSeg. A wave of a workgroup takes the segment's 32-key tiles w, w + 4,
-// ... with one running maximum, the 4 waves are merged as ((0 + 2) + (1 + 3)), segments in order. It depends on
-// a request's own length only, so its bits do not change with the batch.
+// Order. Keys are cut into segments of kSeg and groups of kGroup segments. Strand w of a segment, its 32-key tiles w,
+// w + 4, ..., is summed with one running maximum; the segments of a strand are folded in order, the four strands of a
+// group joined, the groups folded in order. It depends on a request's own length only, so its bits do not change with the
+// batch. A workgroup's waves take the four strands of a group, one each, and need each other only at its end; where that
+// leaves too few workgroups, a workgroup takes one strand and its waves one segment each: the same sums.
 //
 // Rounding. Scores, maxima, sums and accumulators are fp32. P is split into two 16-bit parts, hi + lo, with one
 // MFMA each: P keeps 16 bits (22 in fp16), as the 16-bit output is rounded once from an fp32 sum; the 8-bit
@@ -30,9 +32,12 @@
 namespace {
 
 constexpr int kSeg = 512;    // keys of a segment
+constexpr int kGroup = 4;    // segments that are folded one after the other
 constexpr int kTile = 32;    // keys of a wave's step
 constexpr int kWaves = 4;
+constexpr int kWaveKeys = kSeg / kWaves;
 constexpr int kMaxNodes = 64;
+constexpr int kManyWorkgroups = 1536;
 
 struct TreeParams {
   const uint16_t* q;
@@ -48,19 +53,25 @@ struct TreeParams {
   const int32_t* bt;
   int64_t sbt;
   int32_t cols, page;     // block-table entries of a request, tokens of a page
+  uint32_t page_mul, page_shift;  // key / page = (2 key * page_mul >> 32) >> page_shift for keys below 2^31
   int64_t blocks;
   const int32_t* sl;
   const int32_t* qsl;
   const int64_t* mask;
   float scale_log2;
   int32_t n, total, KV, G, ns, row_blocks, max_nodes, max_len;
-  float* mp;  // [total][H][ns]
+  bool strands;  // a workgroup for each strand of a group of segments, not for each group
+  int64_t parts;  // partial sums of a row: kWaves for each group
+  bool out_wide;  // the output has the query's type and its rows start on 8 bytes
+  float* mp;  // [total][H][parts]
   float* lp;
-  float* ap;  // [total][H][ns][D]
+  float* ap;  // [total][H][parts][D]
   void* out;
   int64_t sot, soh;
   int32_t out_dtype;
 };
+
+__device__ inline int page_of(const TreeParams& p, int key) { return (int)(__umulhi(2u * (uint32_t)key, p.page_mul) >> p.page_shift); }
 
 // The request's keys, nodes and first query row; `bad` where they do not fit the call (a length below its
 // nodes, more nodes or keys than the call's bounds): its rows become NaN.
@@ -122,38 +133,130 @@ __device__ inline Words<W> load_words(const char* p) {
   return r;
 }
 
+// What the wave's lanes have written to LDS is there for all of them: a wave's LDS operations end in order.
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The state (ma, la, sums a) of some segments followed by (mb, lb, sums b): a = a x + b y for every sum.
+template <typename F>
+__device__ inline void fold(float& ma, float& la, float mb, float lb, F&& sums) {
+  const float mn = fmaxf(ma, mb);
+  const float x = exp2_hw(ma - mn), y = exp2_hw(mb - mn);
+  la = fmaf(la, x, lb * y);
+  ma = mn;
+  sums(x, y);
+}
+
+// Maximum, sum and four dims' weighted values of a row over some keys; add: over those of b, which come after.
+struct State {
+  float m, l;
+  v4f a;
+  __device__ inline void add(const State& b) {
+    fold(m, l, b.m, b.l, [&](float x, float y) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[e] = fmaf(a[e], x, b.a[e] * y);
+    });
+  }
+};
+// The strands of a group, into s[0].
+__device__ inline void join(State (&s)[kWaves]) {
+  float m = s[0].m, l = 0.0f;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s[w].m);
+  v4f a = {0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float x = exp2_hw(s[w].m - m);
+    l = fmaf(s[w].l, x, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] = fmaf(s[w].a[e], x, a[e]);
+  }
+  s[0] = State{m, l, a};
+}
+
+// What row (node, head) attends to is nothing: its sum is 0 by definition, not by underflow.
+__device__ inline bool attends_to_nothing(const TreeParams& p, const Request& rq, int node) {
+  if (rq.L > rq.T || p.mask == nullptr) return false;
+  const uint64_t all = rq.T >= 64 ? ~0ull : (1ull << rq.T) - 1;
+  return ((uint64_t)p.mask[rq.q0 + node] & all) == 0;
+}
+
+template <typename T>
+__device__ inline void store_row(const TreeParams& p, const Request& rq, int node, int head, int dim, v4f a, float l) {
+  const float inv = 1.0f / l;
+  const bool nothing = l == 0.0f && attends_to_nothing(p, rq, node);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) a[e] = nothing ? 0.0f : a[e] * inv;
+  const int64_t to = (int64_t)(rq.q0 + node) * p.sot + (int64_t)head * p.soh + dim;
+  if (p.out_wide) {
+    *reinterpret_cast<v2u32*>(reinterpret_cast<uint16_t*>(p.out) + to) = v2u32{T::pack(a[0], a[1]), T::pack(a[2], a[3])};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) store_f32_as(p.out, p.out_dtype, to + e, a[e]);
+  }
+}
+
+// Registers of a lane that live through a tile: sums and queries, and one tile's keys and values. Two workgroups share a
+// CU where those leave room; the next tile is loaded ahead where its registers do not cost that.
+constexpr int lane_regs(int d, int nq, bool int8, int tiles) { return 3 * d * nq / 8 + tiles * d / (int8 ? 4 : 2); }
+constexpr bool shares_cu(int d, int nq, bool int8) { return lane_regs(d, nq, int8, 1) <= 180; }
+constexpr bool loads_ahead(int d, int nq, bool int8) {
+  return lane_regs(d, nq, int8, 2) <= (shares_cu(d, nq, int8) ? 180 : 300);
+}
+
 // T: the query's element type; INT8: the cache's; NQ: 16-row blocks of a workgroup.
 template <typename T, bool INT8, int D, int NQ>
-__global__ __launch_bounds__(64 * kWaves) void tree_partial_kernel(TreeParams p) {
+__global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void tree_partial_kernel(TreeParams p) {
   using PT = std::conditional_t<INT8, BF16, T>;  // the type of P and V
+  constexpr bool AHEAD = loads_ahead(D, NQ, INT8);
   constexpr int QS = D / 32;                     // MFMA steps over the head's dims
   constexpr int DPL = D / 16;                    // dims of a lane in V, and 16-dim blocks of O^T
   constexpr int KW = INT8 ? D / 16 : D / 8;      // dwords of a lane's share of a key
   constexpr int VW = INT8 ? DPL / 4 : DPL / 2;   // dwords of a lane's dims of one key's value
-  __shared__ int64_t s_koff[kSeg], s_voff[kSeg];
-  __shared__ float s_ks[INT8 ? kSeg : 1], s_vs[INT8 ? kSeg : 1];
-  __shared__ float s_m[2][16 * NQ], s_l[2][16 * NQ];
-  __shared__ float s_acc[2][DPL * NQ][4][64];
+  __shared__ int64_t s_koff[kWaves][kWaveKeys], s_voff[kWaves][kWaveKeys];
+  __shared__ __attribute__((aligned(16))) float s_ks[kWaves][INT8 ? kWaveKeys : 4], s_vs[kWaves][INT8 ? kWaveKeys : 4];
+  __shared__ float s_m[kWaves][16 * NQ], s_l[kWaves][16 * NQ];
+  __shared__ v4f s_acc[kWaves][16 * NQ][D / 4];  // [wave][row][4 dims ^ row]
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15;
   const int grp = lane >> 4;
 
-  int64_t id = blockIdx.x;
-  const int rb = (int)(id % p.row_blocks);
-  id /= p.row_blocks;
-  const int g = (int)(id % p.KV);
-  id /= p.KV;
-  const int b = (int)(id % p.n);
-  const int seg = (int)(id / p.n);
+  uint32_t id = blockIdx.x;
+  const int rb = (int)(id % (uint32_t)p.row_blocks);
+  id /= (uint32_t)p.row_blocks;
+  const int g = (int)(id % (uint32_t)p.KV);
+  id /= (uint32_t)p.KV;
+  const int b = (int)(id % (uint32_t)p.n);
+  id /= (uint32_t)p.n;
+  const int group = p.strands ? (int)id / kWaves : (int)id, strand = (int)id % kWaves;
+
+  // The pages of the wave's own keys of a segment, tile after tile. They are asked for before the request's length is
+  // known: past it, table entries are read and not used.
+  constexpr int kOwn = kWaveKeys / 64;
+  auto key_of = [&](int seg, int first, int i) { return seg * kSeg + ((64 * i + lane) / kTile * kWaves + first) * kTile + lane % kTile; };
+  auto find = [&](int seg, int first, int32_t (&pages)[kOwn]) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+      pages[i] = p.cols == 0 ? -1 : p.bt[(int64_t)b * p.sbt + min(page_of(p, key_of(seg, first, i)), p.cols - 1)];
+  };
+  // This wave's segments of the group and its tiles of them: strand `wave` of all four, or a strand of segment `wave`.
+  // The first tile of a short request may be its strand 0 all the same: that choice waits for its length.
+  int32_t pages[kOwn];
+  find(group * kGroup + (p.strands ? wave : 0), p.strands ? strand : wave, pages);
   const Request rq = request_of(p, b);
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) asm volatile("" : "+v"(pages[i]));
   const int rows = rq.T * p.G;
   const int row0 = rb * 16 * NQ;
   if (row0 >= rows) return;
   const int H = p.KV * p.G;
   if (rq.bad) {
-    if (seg == 0 && rb == 0)
+    if (group == 0 && rb == 0 && (!p.strands || strand == 0))
       for (int64_t i = threadIdx.x; i < (int64_t)rows * D; i += 64 * kWaves) {
         const int row = (int)(i / D);
         store_f32_as(p.out, p.out_dtype,
@@ -161,30 +264,42 @@ __global__ __launch_bounds__(64 * kWaves) void tree_partial_kernel(TreeParams p)
       }
     return;
   }
-  const int start = seg * kSeg;
-  const int end = min(start + kSeg, rq.L);
-  if (start >= end) return;
+  const int segs = (rq.L + kSeg - 1) / kSeg;
+  const bool alone = segs <= kGroup;             // one group: its workgroup takes all strands and writes the output
+  const bool whole = alone || !p.strands;
+  if (group * kGroup >= segs || (alone && p.strands && strand != 0)) return;
+  const int first = whole ? wave : strand;       // the wave's first tile of a segment
+  const int seg0 = group * kGroup + (whole ? 0 : wave);
+  const int seg_end = min(group * kGroup + kGroup, whole ? segs : min(seg0 + 1, segs));
+  if (alone && p.strands) find(seg0, first, pages);
   const int ctx = rq.L - rq.T;
 
-  // Row offsets (and scales) of the segment's keys; keys past its end repeat the last one. A page that the cache
-  // does not have makes the request's rows NaN.
+  // Row offsets and scales of the wave's own keys. Keys past the last one repeat the wave's first, masked. A page that the
+  // cache does not have makes the request's rows NaN.
   bool bad_page = false;
-  for (int i = threadIdx.x; i < kSeg; i += 64 * kWaves) {
-    const int key = min(start + i, end - 1);
-    const int pg = (int)((uint32_t)key / (uint32_t)p.page);
-    const int off = key - pg * p.page;
-    int64_t block = p.bt[(int64_t)b * p.sbt + pg];
-    if (block < 0 || block >= p.blocks) {
-      bad_page = true;
-      block = 0;
+  float scales[kOwn][2];
+  auto place = [&](int seg, const int32_t (&pages)[kOwn]) {
+    const int key0 = seg * kSeg + first * kTile;
+    const int32_t page0 = __builtin_amdgcn_readfirstlane(pages[0]);
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      int key = key_of(seg, first, i);
+      int64_t block = key < rq.L ? pages[i] : page0;
+      if (key >= rq.L) key = key0;
+      const int off = key - page_of(p, key) * p.page;
+      if (block < 0 || block >= p.blocks) {
+        bad_page |= key0 < rq.L;
+        block = 0;
+      }
+      s_koff[wave][64 * i + lane] = block * p.skb + (int64_t)off * p.skp;
+      s_voff[wave][64 * i + lane] = block * p.svb + (int64_t)off * p.svp;
+      if constexpr (INT8) {
+        scales[i][0] = p.ks[block * p.sksb + (int64_t)off * p.sksp + (int64_t)g * p.sksh];
+        scales[i][1] = p.vs[block * p.svsb + (int64_t)off * p.svsp + (int64_t)g * p.svsh];
+      }
     }
-    s_koff[i] = block * p.skb + (int64_t)off * p.skp;
-    s_voff[i] = block * p.svb + (int64_t)off * p.svp;
-    if constexpr (INT8) {
-      s_ks[i] = p.ks[block * p.sksb + (int64_t)off * p.sksp + (int64_t)g * p.sksh] * p.scale_log2;
-      s_vs[i] = p.vs[block * p.svsb + (int64_t)off * p.svsp + (int64_t)g * p.svsh];
-    }
-  }
+    wave_sync();
+  };
 
   // This lane's rows: their masks over the drafted keys, and q as the second operand.
   v4u32 qf[NQ][QS];
@@ -202,40 +317,47 @@ __global__ __launch_bounds__(64 * kWaves) void tree_partial_kernel(TreeParams p)
     const uint64_t all = rq.T >= 64 ? ~0ull : (1ull << rq.T) - 1;
     seen[t] = all & (p.mask != nullptr ? (uint64_t)p.mask[rq.q0 + node] : (2ull << node) - 1);
   }
-  bad_page = __syncthreads_or(bad_page);
-
   const char* kbase = p.kc + (int64_t)g * p.skh + 16 * grp;
   const char* vbase = p.vc + (int64_t)g * p.svh + VW * 4 * col;
-  Words<KW> kr[2];
-  Words<VW> vr[8];
-  auto load = [&](int tile) {  // key slots of a lane: 4 grp + j of each half tile
+  struct Loads {
+    Words<KW> k[2];
+    Words<VW> v[8];
+  };
+  auto load = [&](int j, Loads& r) {  // the wave's tile j; key slots of a lane: 4 grp + i of each half tile
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const char* k = kbase + s_koff[tile * kTile + 16 * h + col];
+      const char* k = kbase + s_koff[wave][j * kTile + 16 * h + col];
 #pragma unroll
       for (int c = 0; c < KW / 4; ++c) {
         const Words<4> w = load_words<4>(k + 64 * c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) kr[h].w[4 * c + i] = w.w[i];
+        for (int i = 0; i < 4; ++i) r.k[h].w[4 * c + i] = w.w[i];
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) vr[4 * h + j] = load_words<VW>(vbase + s_voff[tile * kTile + 16 * h + 4 * grp + j]);
+      for (int i = 0; i < 4; ++i) r.v[4 * h + i] = load_words<VW>(vbase + s_voff[wave][j * kTile + 16 * h + 4 * grp + i]);
     }
   };
 
   float m[NQ], l[NQ];
   v4f acc[NQ][DPL];
+  auto clear = [&] {
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    m[t] = kLowest;
-    l[t] = 0.0f;
+    for (int t = 0; t < NQ; ++t) {
+      m[t] = kLowest;
+      l[t] = 0.0f;
 #pragma unroll
-    for (int e = 0; e < DPL; ++e) acc[t][e] = v4f{0, 0, 0, 0};
-  }
+      for (int e = 0; e < DPL; ++e) acc[t][e] = v4f{0, 0, 0, 0};
+    }
+  };
 
-  const int tiles = (end - start + kTile - 1) / kTile;
-  for (int tile = wave; tile < tiles; tile += kWaves) {
-    load(tile);
+  // DRAFTED: the tile holds drafted keys, or ends past the last key. CAREFUL: values of keys that some rows do not attend
+  // to may be infinities or NaN, and 0 times those is NaN; here they enter the product as 0 and are added to the rows that
+  // attend to them. (8-bit values are finite.)
+  auto compute = [&](int start, int tile, const Loads& r, auto drafted_c, auto careful_c) {
+    constexpr bool drafted = decltype(drafted_c)::value, CAREFUL = decltype(careful_c)::value;
+    const Words<KW>(&kr)[2] = r.k;
+    const Words<VW>(&vr)[8] = r.v;
+    const int own = tile / kWaves * kTile;  // the tile's first key among the wave's
     v4f s[NQ][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -258,30 +380,27 @@ __global__ __launch_bounds__(64 * kWaves) void tree_partial_kernel(TreeParams p)
     }
 
     const int key0 = start + tile * kTile;
-    const bool drafted = key0 + kTile > ctx;  // the tile holds drafted keys, or ends past the last key
     uint32_t phi[NQ][4], plo[NQ][4], flag[NQ][4];
     const v4f one = {p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2};
     v4f ks[2] = {one, one}, vs[2];
     if constexpr (INT8) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        ks[h] = *reinterpret_cast<const v4f*>(&s_ks[tile * kTile + 16 * h + 4 * grp]);
-        vs[h] = *reinterpret_cast<const v4f*>(&s_vs[tile * kTile + 16 * h + 4 * grp]);
+        ks[h] = *reinterpret_cast<const v4f*>(&s_ks[wave][own + 16 * h + 4 * grp]);
+        vs[h] = *reinterpret_cast<const v4f*>(&s_vs[wave][own + 16 * h + 4 * grp]);
       }
     }
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
       uint32_t live = 0xFF;  // bit 4 h + j: this row attends to the key
-      if (drafted) {
+      if constexpr (drafted) {
         live = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int d = key0 + 16 * h + 4 * grp + j - ctx;
-            const bool on = d < 0 || (d < 64 && ((seen[t] >> (d & 63)) & 1));
-            live |= on ? 1u << (4 * h + j) : 0u;
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int d = key0 + 16 * h + 4 * grp - ctx;  // the first of the lane's four keys among the drafted ones
+          const uint64_t on = d >= 0 ? seen[t] >> min(d, 63) : seen[t] << min(-d, 63) | ((1ull << min(-d, 63)) - 1);
+          live |= d >= 64 ? 0u : ((uint32_t)on & 15u) << (4 * h);
+        }
       }
       float top = kLowest;
 #pragma unroll
@@ -293,7 +412,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_partial_kernel(TreeParams p)
           top = fmaxf(top, s[t][h][j]);
         }
       top = rows_max(top);
-      if (__any(top > m[t])) {
+      if (__any(top > m[t] + kSlack)) {
         const float mn = fmaxf(m[t], top);
         const float c = exp2_hw(m[t] - mn);
         l[t] *= c;
@@ -317,23 +436,11 @@ __global__ __launch_bounds__(64 * kWaves) void tree_partial_kernel(TreeParams p)
         phi[t][i] = PT::pack(pv[2 * i], pv[2 * i + 1]);
         const v2f back = PT::unpack(phi[t][i]);
         plo[t][i] = PT::pack(pv[2 * i] - back[0], pv[2 * i + 1] - back[1]);
-        if constexpr (!INT8)
+        if constexpr (CAREFUL)
           flag[t][i] = ((live >> (2 * i)) & 1 ? (uint32_t)PT::kOne : 0u) | ((live >> (2 * i + 1)) & 1 ? (uint32_t)PT::kOne << 16 : 0u);
       }
     }
 
-    // Values of keys that some rows do not attend to may be infinities or NaN, and 0 times those is NaN: where a
-    // tile with masked keys holds any, they enter the product as 0 and are added to the rows that attend to them.
-    bool special = false;
-    if constexpr (!INT8) {
-      if (drafted) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-          for (int i = 0; i < VW; ++i) special |= any_special<PT>(vr[k].w[i]);
-        special = __any(special);
-      }
-    }
     static_for<DPL>([&](auto ec) {
       constexpr int e = decltype(ec)::value;
       v4u32 a;
@@ -344,24 +451,22 @@ __global__ __launch_bounds__(64 * kWaves) void tree_partial_kernel(TreeParams p)
         else
           a[i] = __builtin_amdgcn_perm(vr[2 * i + 1].w[e / 2], vr[2 * i].w[e / 2], e % 2 ? 0x07060302u : 0x05040100u);
       }
-      if constexpr (!INT8) {
-        if (special) {
-          v4u32 plus, minus;
+      if constexpr (CAREFUL) {
+        v4u32 plus, minus;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            plus[i] = special_flags<PT, 0>(a[i]);
-            minus[i] = special_flags<PT, 1>(a[i]);
-            a[i] = only_finite<PT>(a[i]);
-          }
+        for (int i = 0; i < 4; ++i) {
+          plus[i] = special_flags<PT, 0>(a[i]);
+          minus[i] = special_flags<PT, 1>(a[i]);
+          a[i] = only_finite<PT>(a[i]);
+        }
 #pragma unroll
-          for (int t = 0; t < NQ; ++t) {
-            const v4u32 f = {flag[t][0], flag[t][1], flag[t][2], flag[t][3]};
-            const v4f up = PT::mfma16(plus, f, v4f{0, 0, 0, 0}), down = PT::mfma16(minus, f, v4f{0, 0, 0, 0});
+        for (int t = 0; t < NQ; ++t) {
+          const v4u32 f = {flag[t][0], flag[t][1], flag[t][2], flag[t][3]};
+          const v4f up = PT::mfma16(plus, f, v4f{0, 0, 0, 0}), down = PT::mfma16(minus, f, v4f{0, 0, 0, 0});
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              if (up[r] > 0.0f) acc[t][e][r] += __builtin_huge_valf();
-              if (down[r] > 0.0f) acc[t][e][r] += kNegInf;
-            }
+          for (int r = 0; r < 4; ++r) {
+            if (up[r] > 0.0f) acc[t][e][r] += __builtin_huge_valf();
+            if (down[r] > 0.0f) acc[t][e][r] += kNegInf;
           }
         }
       }
@@ -371,132 +476,199 @@ __global__ __launch_bounds__(64 * kWaves) void tree_partial_kernel(TreeParams p)
         acc[t][e] = PT::mfma16(a, v4u32{plo[t][0], plo[t][1], plo[t][2], plo[t][3]}, acc[t][e]);
       }
     });
+  };
+  // The wave's sums over its segments lie in LDS, folded as a segment ends; every lane reads what it wrote itself.
+  float jm[NQ], jl[NQ];
+  auto at_acc = [&](int t, int r, int e) -> v4f& { return s_acc[wave][16 * t + col][(((4 * grp + r) * DPL + e) / 4) ^ col]; };
+
+  Loads cur, next;
+  if (seg0 < seg_end) {
+    place(seg0, pages);
+    if constexpr (AHEAD) load(0, cur);
   }
+  for (int seg = seg0; seg < seg_end; ++seg) {
+    if constexpr (INT8) {
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) l[t] = rows_sum(l[t]);
-
-  // Merge the waves: 2 and 3 into 0 and 1, then 1 into 0.
-  auto give = [&](int slot) {
-#pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-      if (grp == 0) {
-        s_m[slot][16 * t + col] = m[t];
-        s_l[slot][16 * t + col] = l[t];
+      for (int i = 0; i < kOwn; ++i) {
+        s_ks[wave][64 * i + lane] = scales[i][0] * p.scale_log2;
+        s_vs[wave][64 * i + lane] = scales[i][1];
       }
-#pragma unroll
-      for (int e = 0; e < DPL; ++e)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s_acc[slot][t * DPL + e][r][lane] = acc[t][e][r];
+      wave_sync();
     }
-  };
-  auto take = [&](int slot) {
-#pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-      const float mo = s_m[slot][16 * t + col], lo = s_l[slot][16 * t + col];
-      const float mn = fmaxf(m[t], mo);
-      const float c0 = exp2_hw(m[t] - mn), c1 = exp2_hw(mo - mn);
-      l[t] = fmaf(l[t], c0, lo * c1);
-      m[t] = mn;
-#pragma unroll
-      for (int e = 0; e < DPL; ++e)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[t][e][r] = fmaf(acc[t][e][r], c0, s_acc[slot][t * DPL + e][r][lane] * c1);
+    const bool more = seg + 1 < seg_end;
+    if (more) find(seg + 1, first, pages);
+    // The next tile's loads are in flight while a tile is computed. Segments with drafted keys take the step that looks
+    // at the masks for all their tiles: one loop's instructions to fetch.
+    const int start = seg * kSeg, end = min(start + kSeg, rq.L);
+    const int tiles = (end - start + kTile - 1) / kTile;
+    const int plain = end > ctx ? 0 : tiles;
+    clear();
+    int tile = first;
+#pragma unroll 1
+    for (; tile < plain; tile += kWaves) {
+      if constexpr (AHEAD) {
+        if (tile + kWaves < tiles) load(tile / kWaves + 1, next);
+      } else {
+        load(tile / kWaves, cur);
+      }
+      compute(start, tile, cur, std::false_type{}, std::false_type{});
+      if constexpr (AHEAD) cur = next;
     }
-  };
-  if (wave >= 2) give(wave - 2);
-  __syncthreads();
-  if (wave < 2) take(wave);
-  __syncthreads();
-  if (wave == 1) give(0);
-  __syncthreads();
-  if (wave != 0) return;
-  take(0);
-
-  const bool alone = rq.L <= kSeg;
+#pragma unroll 1
+    for (; tile < tiles; tile += kWaves) {
+      if constexpr (AHEAD) {
+        if (tile + kWaves < tiles) load(tile / kWaves + 1, next);
+      } else {
+        load(tile / kWaves, cur);
+      }
+      compute(start, tile, cur, std::true_type{}, std::false_type{});
+      if constexpr (AHEAD) cur = next;
+    }
+    if constexpr (!INT8) {
+      float odd = 0.0f;  // 0 where all sums are finite, else NaN
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    const int row = row0 + 16 * t + col;
-    if (row >= rows) continue;
-    const int node = row / p.G, head = g * p.G + row % p.G;
-    if (bad_page) l[t] = __builtin_nanf("");
-    if (alone) {
-      const bool nothing = ctx == 0 && seen[t] == 0;
-      const int64_t at = (int64_t)(rq.q0 + node) * p.sot + (int64_t)head * p.soh;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int t = 0; t < NQ; ++t)
 #pragma unroll
         for (int e = 0; e < DPL; ++e)
-          store_f32_as(p.out, p.out_dtype, at + (4 * grp + r) * DPL + e, nothing && !bad_page ? 0.0f : acc[t][e][r] / l[t]);
-    } else {
-      const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.ns + seg;
-      if (grp == 0) {
-        p.mp[part] = m[t];
-        p.lp[part] = l[t];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) odd = fmaf(acc[t][e][r], 0.0f, odd);
+      if (plain == 0 && __any(odd != 0.0f)) {
+        clear();
+#pragma unroll 1
+        for (tile = first; tile < tiles; tile += kWaves) {
+          load(tile / kWaves, cur);
+          compute(start, tile, cur, std::true_type{}, std::true_type{});
+        }
       }
+    }
+    if (more) {
+      place(seg + 1, pages);
+      if constexpr (AHEAD) load(0, cur);
+    }
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+    for (int t = 0; t < NQ; ++t) {
+      const float sum = rows_sum(l[t]);
+      if (seg == seg0) {
+        jm[t] = m[t], jl[t] = sum;
 #pragma unroll
-        for (int e = 0; e < DPL; ++e) p.ap[part * D + (4 * grp + r) * DPL + e] = acc[t][e][r];
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < DPL; e += 4) at_acc(t, r, e) = v4f{acc[t][e][r], acc[t][e + 1][r], acc[t][e + 2][r], acc[t][e + 3][r]};
+      } else {
+        fold(jm[t], jl[t], m[t], sum, [&](float x, float y) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < DPL; e += 4) {
+              v4f a = at_acc(t, r, e);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) a[i] = fmaf(a[i], x, acc[t][e + i][r] * y);
+              at_acc(t, r, e) = a;
+            }
+        });
+      }
+    }
+  }
+  if (grp == 0 && seg0 < seg_end) {
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) s_m[wave][16 * t + col] = jm[t], s_l[wave][16 * t + col] = jl[t];
+  }
+  const bool bad = __syncthreads_or(bad_page);
+
+  // The workgroup's waves: strands of a group are joined, segments of a strand folded in order.
+  const int waves = whole ? kWaves : min(kWaves, segs - group * kGroup);
+#pragma unroll 1
+  for (int at = threadIdx.x; at < 16 * NQ * (D / 4); at += 64 * kWaves) {
+    const int in_block = at / (D / 4), c = at % (D / 4);
+    const int row = row0 + in_block;
+    if (row >= rows) break;
+    State s[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+      if (w < waves) s[w] = State{s_m[w][in_block], s_l[w][in_block], s_acc[w][in_block][c ^ (in_block & 15)]};
+    if (whole) {
+      join(s);
+    } else {
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w)
+        if (w < waves) s[0].add(s[w]);
+    }
+    if (bad) s[0].l = __builtin_nanf("");
+    const int node = row / p.G, head = g * p.G + row % p.G;
+    if (alone) {
+      store_row<T>(p, rq, node, head, 4 * c, s[0].a, s[0].l);
+    } else {
+      const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + group * kWaves + (whole ? 0 : strand);
+      if (c == 0) p.mp[part] = s[0].m, p.lp[part] = s[0].l;
+      reinterpret_cast<v4f*>(p.ap)[part * (D / 4) + c] = s[0].a;
     }
   }
 }
 
-// Joins a row's segments in order: a wave per (node, head). A row longer than a segment attends to its context, so
-// its sum is not empty.
-template <int D>
-__global__ __launch_bounds__(64 * kWaves) void tree_merge_kernel(TreeParams p) {
-  constexpr int DPW = D / 64;
-  const int lane = threadIdx.x & 63;
+// Joins a row's groups: the strands of a group where workgroups have left them apart, then the groups in order. A
+// workgroup joins one row, kMergeGroups groups at a time, 4 dims a lane: their partials are on their way together. A row
+// of several groups attends to its context, so its sum is not empty.
+constexpr int kMergeGroups = 4;
+template <typename T, int D>
+__global__ __launch_bounds__(D * kMergeGroups / 4) void tree_merge_kernel(TreeParams p) {
+  constexpr int kLanes = D / 4;
+  __shared__ float s_ml[kMergeGroups][2];
+  __shared__ v4f s_a[kMergeGroups][kLanes];
   const int H = p.KV * p.G;
-  const int64_t id = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  const int head = (int)(id % H);
-  const int64_t bn = id / H;
-  const int b = (int)(bn / p.max_nodes), node = (int)(bn % p.max_nodes);
-  if (b >= p.n) return;
+  const int mine = threadIdx.x / kLanes, c = threadIdx.x % kLanes;
+  const int head = (int)(blockIdx.x % (uint32_t)H);
+  const uint32_t bn = blockIdx.x / (uint32_t)H;
+  const int b = (int)(bn / (uint32_t)p.max_nodes), node = (int)(bn % (uint32_t)p.max_nodes);
   const Request rq = request_of(p, b);
-  if (rq.bad || node >= rq.T || rq.L <= kSeg) return;
-  const int segs = (rq.L + kSeg - 1) / kSeg;
-  const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.ns;
-  float top = kLowest;
-  for (int s = lane; s < segs; s += 64) top = fmaxf(top, p.mp[part + s]);
+  const int groups = (rq.L + kGroup * kSeg - 1) / (kGroup * kSeg);
+  if (rq.bad || node >= rq.T || groups <= 1) return;
+  const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts;
+  State sum;
+  for (int g0 = 0; g0 < groups; g0 += kMergeGroups) {
+    if (g0 + mine < groups) {
+      State s[kWaves];
+      const int64_t at = part + (g0 + mine) * kWaves;
 #pragma unroll
-  for (int x = 1; x < 64; x *= 2) top = fmaxf(top, shfl_xor_f32(top, x));
-  float l = 0.0f, a[DPW];
+      for (int w = 0; w < kWaves; ++w)
+        if (w == 0 || p.strands) s[w] = State{p.mp[at + w], p.lp[at + w], reinterpret_cast<const v4f*>(p.ap)[(at + w) * kLanes + c]};
+      if (p.strands) join(s);
+      if (c == 0) s_ml[mine][0] = s[0].m, s_ml[mine][1] = s[0].l;
+      s_a[mine][c] = s[0].a;
+    }
+    __syncthreads();
+    if (mine == 0) {
 #pragma unroll
-  for (int j = 0; j < DPW; ++j) a[j] = 0.0f;
-#pragma unroll 8
-  for (int s = 0; s < segs; ++s) {
-    const float c = exp2_hw(p.mp[part + s] - top);
-    l = fmaf(p.lp[part + s], c, l);
-#pragma unroll
-    for (int j = 0; j < DPW; ++j) a[j] = fmaf(p.ap[(part + s) * D + DPW * lane + j], c, a[j]);
+      for (int i = 0; i < kMergeGroups; ++i) {
+        if (g0 + i >= groups) break;
+        const State s{s_ml[i][0], s_ml[i][1], s_a[i][c]};
+        if (g0 + i == 0) sum = s; else sum.add(s);
+      }
+    }
+    __syncthreads();
   }
-  const int64_t at = (int64_t)(rq.q0 + node) * p.sot + (int64_t)head * p.soh;
-#pragma unroll
-  for (int j = 0; j < DPW; ++j) store_f32_as(p.out, p.out_dtype, at + DPW * lane + j, a[j] / l);
+  if (mine == 0) store_row<T>(p, rq, node, head, 4 * c, sum.a, sum.l);
 }
-
-int row_blocks16(int64_t rows, int64_t D) { return rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 4; }
 
 template <typename T, bool INT8, int D>
 hipError_t launch_tree(TreeParams p, hipStream_t st) {
   const int64_t rows = (int64_t)p.max_nodes * p.G;
-  const int nq = row_blocks16(rows, D);
+  const int nq = rows <= 16 ? 1 : 2;
   p.row_blocks = (int32_t)cdiv<int64_t>(rows, 16 * nq);
-  const int64_t blocks = (int64_t)p.row_blocks * p.KV * p.n * p.ns;
-  const int64_t merges = cdiv<int64_t>((int64_t)p.n * p.max_nodes * p.KV * p.G, kWaves);
+  // A workgroup for each group of segments, or for each of its strands where the former would not fill the GPU. The order
+  // of the sums, and so every bit, is the same.
+  const int64_t units = (int64_t)p.row_blocks * p.KV * p.n, groups = cdiv<int64_t>(p.ns, kGroup);
+  p.strands = groups > 1 && units * groups < kManyWorkgroups;
+  const int64_t blocks = units * groups * (p.strands ? kWaves : 1);
+  const int64_t merges = (int64_t)p.n * p.max_nodes * p.KV * p.G;
   if (blocks > 0x7FFFFFFFLL || merges > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)blocks), threads(64 * kWaves);
-  if (nq == 1) {
+  if (nq == 1)
     hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 1>), grid, threads, 0, st, p);
-  } else if (nq == 2) {
+  else
     hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 2>), grid, threads, 0, st, p);
-  } else {
-    if constexpr (D < 256) hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 4>), grid, threads, 0, st, p);
-  }
   hipError_t err = hipGetLastError();
-  if (err != hipSuccess || p.ns == 1) return err;
-  hipLaunchKernelGGL((tree_merge_kernel<D>), dim3((unsigned)merges), threads, 0, st, p);
+  if (err != hipSuccess || groups <= 1) return err;
+  hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3((unsigned)merges), dim3(D * kMergeGroups / 4), 0, st, p);
   return hipGetLastError();
 }
 
@@ -509,13 +681,20 @@ hipError_t dispatch_dim(int64_t D, const TreeParams& p, hipStream_t st) {
 
 int64_t num_segments(int64_t keys) { return std::max<int64_t>(1, cdiv<int64_t>(keys, kSeg)); }
 
+// Partial sums of a row of at most `keys` keys: one for each strand of each group of segments. A single group needs none,
+// but its segments are counted.
+int64_t part_count(int64_t keys) {
+  const int64_t ns = num_segments(keys);
+  return ns <= kGroup ? ns : cdiv<int64_t>(ns, kGroup) * kWaves;
+}
+
 }  // namespace
 
 extern "C" int vxa_tree_decode_workspace(int64_t tokens, int64_t num_heads, int64_t head_dim, int64_t max_seq_len,
                                          size_t* ws_bytes) {
   if (tokens < 0 || num_heads <= 0 || head_dim <= 0 || max_seq_len < 0 || !ws_bytes) return VXA_ERR_ARG;
-  const int64_t ns = num_segments(max_seq_len);
-  *ws_bytes = ns > 1 ? (size_t)tokens * num_heads * ns * (head_dim + 2) * sizeof(float) : 0;
+  const int64_t parts = part_count(max_seq_len);
+  *ws_bytes = parts > 1 ? (size_t)tokens * num_heads * parts * (head_dim + 2) * sizeof(float) : 0;
   return VXA_OK;
 }
 
@@ -551,6 +730,7 @@ extern "C" int vxa_tree_decode(const void* q, int64_t sqt, int64_t sqh, int q_dt
   size_t need = 0;
   vxa_tree_decode_workspace(tokens, num_heads, head_dim, max_seq_len, &need);
   if (need > 0 && (!ws || ws_bytes < need)) return VXA_ERR_WORKSPACE;
+  if (need > 0 && (uintptr_t)ws % 16) return VXA_ERR_UNSUPPORTED;
 
   TreeParams p;
   p.q = reinterpret_cast<const uint16_t*>(q);
@@ -566,10 +746,18 @@ extern "C" int vxa_tree_decode(const void* q, int64_t sqt, int64_t sqh, int q_dt
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
   p.n = (int32_t)n, p.total = (int32_t)tokens, p.KV = (int32_t)num_kv_heads, p.G = (int32_t)(num_heads / num_kv_heads);
   p.ns = (int32_t)ns, p.row_blocks = 1, p.max_nodes = (int32_t)max_nodes, p.max_len = (int32_t)max_seq_len;
-  const int64_t parts = tokens * num_heads * ns;
+  p.strands = false, p.parts = part_count(max_seq_len);
+  // The weighted values first, on 16 bytes as the workspace is.
+  const int64_t parts = tokens * num_heads * p.parts;
   float* w = reinterpret_cast<float*>(ws);
-  p.mp = w, p.lp = ns > 1 ? w + parts : nullptr, p.ap = ns > 1 ? w + 2 * parts : nullptr;
+  p.ap = w, p.mp = need > 0 ? w + parts * head_dim : nullptr, p.lp = need > 0 ? p.mp + parts : nullptr;
   p.out = out, p.sot = sot, p.soh = soh, p.out_dtype = out_dtype;
+  p.out_wide = out_dtype == q_dtype && (uintptr_t)out % 8 == 0 && sot % 4 == 0 && soh % 4 == 0;
+  // page_mul = 2^(31 + s) / page rounded up, with 2^s >= page: its excess over the quotient, below page / page, times a
+  // key stays below 2^(31 + s) / page, so the shifted product is exact.
+  p.page_shift = 0;
+  while ((1LL << p.page_shift) < block_size) ++p.page_shift;
+  p.page_mul = (uint32_t)(((1ULL << (31 + p.page_shift)) + (uint64_t)block_size - 1) / (uint64_t)block_size);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   hipError_t err;
   if (q_dtype == VXA_BF16)
