@@ -6,6 +6,9 @@
 
 #include "common.h"
 
+// copy_to_lds sets M0 and names it as clobbered; clang warns that M0 is a reserved register.
+#pragma clang diagnostic ignored "-Winline-asm"
+
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
@@ -115,3 +118,28 @@ __device__ inline uint32_t special_flags(uint32_t w) {
   const uint32_t lo = w & 0xFFFFu, hi = w >> 16;
   return ((lo & m) == m && lo != other ? T::kOne : 0u) | ((hi & m) == m && hi != other ? T::kOne << 16 : 0u);
 }
+
+// Four 16-bit elements of one column, from four rows that the 16 lanes of a group address together (8 bytes a lane,
+// four lanes a row): gfx950's transposing LDS read.
+__device__ inline v2u32 read_transposed(const char* lds) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4s lds_v4s;
+  return __builtin_bit_cast(v2u32, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)lds));
+}
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+// 16 bytes a lane straight from memory into LDS: lane i's land at dst + 16 i. From inline asm: with the builtin the
+// compiler, which cannot tell one buffer from another, waits for copies in flight before it reads any. Explicit waits order
+// them. M0 needs one wait state before the load that uses it; the build checks that only this code uses it.
+__device__ inline void copy_to_lds(const char* src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+}
+
+// Tiles of 16-bit keys and values in LDS, a key after the other in 16-byte chunks: chunk c of a key lies at
+// c ^ swizzle(key), so that 16 lanes that read one chunk of 16 keys (K), or four chunks of four keys (V, transposed), meet
+// 16 different 16-byte columns of the 256 bytes that the banks deliver.
+template <int D>
+__device__ inline int key_swizzle(int key) { return D == 64 ? (key >> 1) & 7 : key & 15; }
+template <int D>
+__device__ inline int value_swizzle(int key) { return D == 64 ? 4 * ((key >> 1) & 1) : 4 * (key & 3); }

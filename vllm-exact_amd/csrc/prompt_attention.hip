@@ -47,47 +47,73 @@ struct PromptParams {
   bool out_wide;  // the output has the input's type and its rows start on 8 bytes
 };
 
-// The sequence and rows of tile `tile`, counted over the sequences' tiles of p.rows rows in order.
+// Sums and maxima of values >= 0 over the wave.
+template <int CTRL, int ROWS>
+__device__ inline int from_row(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+template <typename F>
+__device__ inline int wave_reduce(int x, F&& f) {
+  x = f(x, from_row<0x111, 0xF>(x));  // the lanes 1, 2, 4 and 8 before, in rows of 16
+  x = f(x, from_row<0x112, 0xF>(x));
+  x = f(x, from_row<0x114, 0xF>(x));
+  x = f(x, from_row<0x118, 0xF>(x));
+  x = f(x, from_row<0x142, 0xA>(x));  // row 0's and 2's last lane to rows 1 and 3
+  x = f(x, from_row<0x143, 0xC>(x));  // row 1's last lane to rows 2 and 3
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// The sequence and rows of tile `tile`. Tiles of p.rows rows are counted from those furthest from their sequence's start,
+// which take longest, over all sequences (256 sequences at a time).
 struct Tile {
   int base, len, row0;  // first packed row of the sequence, its length (0: no such tile), the tile's first row in it
 };
 __device__ inline Tile find_tile(const PromptParams& p, int tile) {
+  if (p.n == 1) {
+    const int lo = max(p.cu[0], 0), len = max(min(p.cu[1], p.total) - lo, 0), count = (len + p.rows - 1) / p.rows;
+    return tile < count ? Tile{lo, len, (count - 1 - tile) * p.rows} : Tile{0, 0, 0};
+  }
   const int lane = threadIdx.x & 63;
-  int before = 0;
-  for (int j0 = 0; j0 < p.n; j0 += 64) {
-    const int j = j0 + lane;
-    int lo = 0, len = 0;
-    if (j < p.n) {
-      lo = max(p.cu[j], 0);
-      len = max(min(p.cu[j + 1], p.total) - lo, 0);
-    }
-    const int mine = (len + p.rows - 1) / p.rows;
-    int sum = mine;  // inclusive over the lanes
+  for (int j0 = 0; j0 < p.n; j0 += 256) {
+    int lo[4], len[4], count[4];
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) {
-      const int up = __shfl_up(sum, x);
-      if (lane >= x) sum += up;
+    for (int c = 0; c < 4; ++c) {
+      const int j = j0 + 64 * c + lane;
+      lo[c] = 0, len[c] = 0;
+      if (j < p.n) {
+        lo[c] = max(p.cu[j], 0);
+        len[c] = max(min(p.cu[j + 1], p.total) - lo[c], 0);
+      }
+      count[c] = (len[c] + p.rows - 1) / p.rows;
     }
-    const uint64_t hit = __ballot(before + sum > tile);
-    if (hit != 0) {
-      const int at = __builtin_ctzll(hit);
-      const int first = before + __shfl(sum - mine, at);
-      return Tile{__shfl(lo, at), __shfl(len, at), (tile - first) * p.rows};
+    // below(k) tiles are among their sequences' first k.
+    auto below = [&](int k) { return wave_reduce(min(count[0], k) + min(count[1], k) + min(count[2], k) + min(count[3], k), [](int a, int b) { return a + b; }); };
+    const int total = below(0x7FFFFFFF);
+    if (tile >= total) {
+      tile -= total;
+      continue;
     }
-    before += __shfl(sum, 63);
+    int left = total - 1 - tile, level = 0, under = 0;
+    const int most = wave_reduce(max(max(count[0], count[1]), max(count[2], count[3])), [](int a, int b) { return max(a, b); });
+    for (int step = 1 << (31 - __builtin_clz(most)); step > 0; step /= 2) {
+      const int s = below(level + step);
+      if (s <= left) level += step, under = s;
+    }
+    left -= under;  // the sequence is number `left` of those with more than `level` tiles
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint64_t more = __ballot(count[c] > level);
+      const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(more >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)more, 0));
+      const uint64_t hit = __ballot(count[c] > level && before == left);
+      if (hit != 0) {
+        const int at = __builtin_ctzll(hit);
+        return Tile{__builtin_amdgcn_readlane(lo[c], at), __builtin_amdgcn_readlane(len[c], at), level * p.rows};
+      }
+      left -= __popcll(more);
+    }
   }
   return Tile{0, 0, 0};
 }
-
-// Four 16-bit elements of one column, from four rows that the 16 lanes of a group address together (8 bytes a lane,
-// four lanes a row): gfx950's transposing LDS read.
-__device__ inline v2u32 read_transposed(const char* lds) {
-  typedef short v4s __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) v4s lds_v4s;
-  return __builtin_bit_cast(v2u32, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)lds));
-}
-
-typedef __attribute__((address_space(3))) void lds_void_t;
 
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_kernel(PromptParams p) {
@@ -102,10 +128,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
   constexpr int kCopies = kKeys / kRound;             // copies of a wave for a tile of K, and of V
   constexpr int kBases = kRound < 16 && D > 64 ? 16 / kRound : 1;  // copies after which K's swizzle repeats
   __shared__ __attribute__((aligned(1024))) char s_kv[2][2][kTileBytes];  // [buffer][K, V][key][16-byte chunk, swizzled]
-  // A key's chunk c lies at c ^ swizzle(key): 16 lanes that read one chunk of 16 keys (K), or four chunks of four keys
-  // (V, transposed), meet 16 different 16-byte columns of the 256 bytes that the banks deliver.
-  auto swk = [](int key) { return D == 64 ? (key >> 1) & 7 : key & 15; };
-  auto swv = [](int key) { return D == 64 ? 4 * ((key >> 1) & 1) : 4 * (key & 3); };
+  auto swk = [](int key) { return key_swizzle<D>(key); };
+  auto swv = [](int key) { return value_swizzle<D>(key); };
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -115,7 +139,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
   const int groups = p.H / p.heads;
   const int x = (int)(blockIdx.x % groups);
   const int head = (groups % 8 == 0 ? (x % 8) * (groups / 8) + x / 8 : x) * p.heads + wave % p.heads;
-  const Tile tile = find_tile(p, p.tiles - 1 - (int)(blockIdx.x / groups));
+  const Tile tile = find_tile(p, (int)(blockIdx.x / groups));
   if (tile.len == 0) return;
   const int base = __builtin_amdgcn_readfirstlane(tile.base);
   const int len = __builtin_amdgcn_readfirstlane(tile.len);
@@ -136,32 +160,27 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
   const int last = min(row0 + p.rows, len);  // keys of the workgroup
   const int tiles = (last + kKeys - 1) / kKeys;
 
-  // Tiles go straight from memory into LDS (global_load_lds_dwordx4: lane i's 16 bytes land at M0 + 16 i), from inline
-  // asm: with the builtin the compiler, which cannot tell the buffers apart, waits for the next tile's copies before it
-  // reads this one. Only the waits below order them. Copy i of a wave moves keys i * kRound + wave * kPer + [0, kPer).
+  // Tiles go straight from memory into LDS. Copy i of a wave moves keys i * kRound + wave * kPer + [0, kPer).
   const int key_l = wave * kPer + lane / (kRow / 16), chunk = lane % (kRow / 16);
   const char* ksrc[kBases];
 #pragma unroll
   for (int i = 0; i < kBases; ++i) ksrc[i] = kh + (key_l + i * kRound) * skt + 16 * (chunk ^ swk(key_l + i * kRound));
   const char* vsrc = vh + key_l * svt + 16 * (chunk ^ swv(key_l));
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t*)&s_kv[0][0][0]) + wave * 1024;
-  auto copy = [&](const char* src, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
-  };
   auto load = [&](int t, int buf) {
     const uint32_t dst = lds0 + buf * 2 * kTileBytes;
     if ((t + 1) * kKeys <= len) {
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
-        copy(ksrc[i % kBases] + (int64_t)(t * kKeys + i / kBases * kBases * kRound) * skt, dst + i * kWaves * 1024);
-        copy(vsrc + (int64_t)(t * kKeys + i * kRound) * svt, dst + kTileBytes + i * kWaves * 1024);
+        copy_to_lds(ksrc[i % kBases] + (int64_t)(t * kKeys + i / kBases * kBases * kRound) * skt, dst + i * kWaves * 1024);
+        copy_to_lds(vsrc + (int64_t)(t * kKeys + i * kRound) * svt, dst + kTileBytes + i * kWaves * 1024);
       }
     } else {  // keys past the sequence's end repeat its last one
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
         const int in_tile = i * kRound + key_l, key = min(t * kKeys + in_tile, len - 1);
-        copy(kh + key * skt + 16 * (chunk ^ swk(in_tile)), dst + i * kWaves * 1024);
-        copy(vh + key * svt + 16 * (chunk ^ swv(in_tile)), dst + kTileBytes + i * kWaves * 1024);
+        copy_to_lds(kh + key * skt + 16 * (chunk ^ swk(in_tile)), dst + i * kWaves * 1024);
+        copy_to_lds(vh + key * svt + 16 * (chunk ^ swv(in_tile)), dst + kTileBytes + i * kWaves * 1024);
       }
     }
   };

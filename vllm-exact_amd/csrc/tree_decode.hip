@@ -37,6 +37,8 @@ constexpr int kTile = 32;    // keys of a wave's step
 constexpr int kWaves = 4;
 constexpr int kWaveKeys = kSeg / kWaves;
 constexpr int kMaxNodes = 64;
+constexpr int kWideRows = 96;   // requests with more rows (nodes times heads of a group) take the wide kernel
+constexpr int kFill = 256;      // keys whose places the wide kernel looks up at a time
 constexpr int kManyWorkgroups = 1536;
 
 struct TreeParams {
@@ -161,14 +163,16 @@ struct State {
     });
   }
 };
-// The strands of a group, into s[0].
-__device__ inline void join(State (&s)[kWaves]) {
+// The first `count` strands of a group, into s[0].
+__device__ inline void join(State (&s)[kWaves], int count) {
   float m = s[0].m, l = 0.0f;
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s[w].m);
+  for (int w = 1; w < kWaves; ++w)
+    if (w < count) m = fmaxf(m, s[w].m);
   v4f a = {0, 0, 0, 0};
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
+    if (w >= count) break;
     const float x = exp2_hw(s[w].m - m);
     l = fmaf(s[w].l, x, l);
 #pragma unroll
@@ -199,6 +203,14 @@ __device__ inline void store_row(const TreeParams& p, const Request& rq, int nod
   }
 }
 
+// The row block of a workgroup, and what it shares with the other row blocks in `id`. Workgroups go to the 8 XCDs in turn:
+// the row blocks of the same keys are 8 apart, next to each other on one XCD and its L2.
+__device__ inline int row_block_of(const TreeParams& p, uint32_t& id) {
+  const uint32_t y = blockIdx.x / 8, rb = y % (uint32_t)p.row_blocks;
+  id = y / (uint32_t)p.row_blocks * 8 + blockIdx.x % 8;
+  return (int)rb;
+}
+
 // Registers of a lane that live through a tile: sums and queries, and one tile's keys and values. Two workgroups share a
 // CU where those leave room; the next tile is loaded ahead where its registers do not cost that.
 constexpr int lane_regs(int d, int nq, bool int8, int tiles) { return 3 * d * nq / 8 + tiles * d / (int8 ? 4 : 2); }
@@ -226,14 +238,13 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
   const int col = lane & 15;
   const int grp = lane >> 4;
 
-  uint32_t id = blockIdx.x;
-  const int rb = (int)(id % (uint32_t)p.row_blocks);
-  id /= (uint32_t)p.row_blocks;
+  uint32_t id;
+  const int rb = row_block_of(p, id);
   const int g = (int)(id % (uint32_t)p.KV);
   id /= (uint32_t)p.KV;
   const int b = (int)(id % (uint32_t)p.n);
   id /= (uint32_t)p.n;
-  const int group = p.strands ? (int)id / kWaves : (int)id, strand = (int)id % kWaves;
+  const int group = p.strands ? (int)id / kWaves : (int)id, strand = (int)id % kWaves;  // past the groups: nothing to do
 
   // The pages of the wave's own keys of a segment, tile after tile. They are asked for before the request's length is
   // known: past it, table entries are read and not used.
@@ -253,7 +264,7 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
   for (int i = 0; i < kOwn; ++i) asm volatile("" : "+v"(pages[i]));
   const int rows = rq.T * p.G;
   const int row0 = rb * 16 * NQ;
-  if (row0 >= rows) return;
+  if (row0 >= rows || (rows > kWideRows && !rq.bad)) return;
   const int H = p.KV * p.G;
   if (rq.bad) {
     if (group == 0 && rb == 0 && (!p.strands || strand == 0))
@@ -587,7 +598,7 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
     for (int w = 0; w < kWaves; ++w)
       if (w < waves) s[w] = State{s_m[w][in_block], s_l[w][in_block], s_acc[w][in_block][c ^ (in_block & 15)]};
     if (whole) {
-      join(s);
+      join(s, kWaves);
     } else {
 #pragma unroll
       for (int w = 1; w < kWaves; ++w)
@@ -605,8 +616,304 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
   }
 }
 
-// Joins a row's groups: the strands of a group where workgroups have left them apart, then the groups in order. A
-// workgroup joins one row, kMergeGroups groups at a time, 4 dims a lane: their partials are on their way together. A row
+// Keys of a workgroup of the wide kernel, by the request's own length: more of them halve the partial sums.
+__device__ __host__ inline int wide_chunk(int keys) { return keys <= 4096 ? kSeg : 2 * kSeg; }
+
+// Requests of more than kWideRows rows. A workgroup takes 128 rows of a (request, KV head), 32 a wave, and a chunk of
+// keys in tiles that its waves share through LDS, as 16-bit elements: a key is converted once for 128 rows. 32 x 32 x 16
+// MFMAs, otherwise as above: S^T = K Q^T, then O^T = V^T P^T with V transposed by the LDS read. Tiles of a 16-bit cache are
+// copied straight into LDS, those of an 8-bit one through registers, the next tile while one is computed.
+template <typename T, bool INT8, int D>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void tree_decode_kernel_wide(TreeParams p) {
+  using PT = std::conditional_t<INT8, BF16, T>;
+  constexpr int kKeys = D == 256 ? 32 : 64, KU = kKeys / 32;
+  constexpr int QS = D / 16, DB = D / 32;
+  constexpr int kRow = 2 * D, kTileBytes = kKeys * kRow;
+  constexpr int kPer = 1024 / kRow, kRound = kPer * kWaves, kCopies = kKeys / kRound;  // as copied: keys of a copy, of a round
+  constexpr int KL = kKeys * D / 16 / (64 * kWaves);                                   // as converted: 16-byte pieces a thread
+  __shared__ __attribute__((aligned(1024))) char s_kv[2][2][kTileBytes];
+  __shared__ int64_t s_koff[kFill], s_voff[kFill];
+  __shared__ __attribute__((aligned(16))) float s_ks[2][INT8 ? kFill : 4], s_vs[2][INT8 ? kFill : 4];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  uint32_t id;
+  const int rb = row_block_of(p, id);
+  const int g = (int)(id % (uint32_t)p.KV);
+  id /= (uint32_t)p.KV;
+  const int b = (int)(id % (uint32_t)p.n);
+  const int chunk = (int)(id / (uint32_t)p.n);
+  const Request rq = request_of(p, b);
+  const int rows = rq.T * p.G, row0 = rb * 32 * kWaves;
+  if (rq.bad || rows <= kWideRows || row0 >= rows) return;
+  const int keys = wide_chunk(rq.L);
+  const int start = chunk * keys, end = min(start + keys, rq.L);
+  if (start >= end) return;
+  const int ctx = rq.L - rq.T;
+  const int H = p.KV * p.G;
+
+  // Places of kFill keys; those past the last one repeat it.
+  bool bad_page = false;
+  auto page_at = [&](int fill) {
+    const int key = min(start + fill * kFill + (int)threadIdx.x, end - 1);
+    return p.bt[(int64_t)b * p.sbt + page_of(p, key)];
+  };
+  auto place = [&](int fill, int32_t page) {
+    const int key = min(start + fill * kFill + (int)threadIdx.x, end - 1);
+    const int off = key - page_of(p, key) * p.page;
+    int64_t block = page;
+    if (block < 0 || block >= p.blocks) {
+      bad_page = true;
+      block = 0;
+    }
+    s_koff[threadIdx.x] = block * p.skb + (int64_t)off * p.skp;
+    s_voff[threadIdx.x] = block * p.svb + (int64_t)off * p.svp;
+    if constexpr (INT8) {
+      s_ks[fill & 1][threadIdx.x] = p.ks[block * p.sksb + (int64_t)off * p.sksp + (int64_t)g * p.sksh] * p.scale_log2;
+      s_vs[fill & 1][threadIdx.x] = p.vs[block * p.svsb + (int64_t)off * p.svsp + (int64_t)g * p.svsh];
+    }
+    __syncthreads();
+  };
+  int32_t page = page_at(0);
+
+  const int row = min(row0 + 32 * wave + col, rows - 1), node = row / p.G, head = g * p.G + row - node * p.G;
+  v4u32 qf[QS];
+  {
+    const uint16_t* q = p.q + (int64_t)(rq.q0 + node) * p.sqt + (int64_t)head * p.sqh + 8 * half;
+#pragma unroll
+    for (int i = 0; i < QS; ++i) qf[i] = *reinterpret_cast<const v4u32*>(q + 16 * i);
+  }
+  const uint64_t all = rq.T >= 64 ? ~0ull : (1ull << rq.T) - 1;
+  const uint64_t seen = all & (p.mask != nullptr ? (uint64_t)p.mask[rq.q0 + node] : (2ull << node) - 1);
+
+  const int tiles = (end - start + kKeys - 1) / kKeys;
+  const int plain = min(max(ctx - start, 0) / kKeys, tiles);  // tiles of the context alone
+  const char* kh = p.kc + (int64_t)g * p.skh;
+  const char* vh = p.vc + (int64_t)g * p.svh;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t*)&s_kv[0][0][0]) + wave * 1024;
+  v4u32 kr[INT8 ? KL : 1], vr[INT8 ? KL : 1];
+  auto load = [&](int t) {
+    const int at = t * kKeys % kFill;
+    if constexpr (INT8) {
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        const int u = threadIdx.x + i * 64 * kWaves, key = u / (D / 16), c = u % (D / 16);
+        kr[i] = *reinterpret_cast<const v4u32*>(kh + s_koff[at + key] + 16 * c);
+        vr[i] = *reinterpret_cast<const v4u32*>(vh + s_voff[at + key] + 16 * c);
+      }
+    } else {
+      const uint32_t dst = lds0 + (t & 1) * 2 * kTileBytes;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int key = i * kRound + wave * kPer + lane / (kRow / 16), c = lane % (kRow / 16);
+        copy_to_lds(kh + s_koff[at + key] + 16 * (c ^ key_swizzle<D>(key)), dst + i * kWaves * 1024);
+        copy_to_lds(vh + s_voff[at + key] + 16 * (c ^ value_swizzle<D>(key)), dst + kTileBytes + i * kWaves * 1024);
+      }
+    }
+  };
+  auto store = [&](int t) {
+    if constexpr (INT8) {
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        const int u = threadIdx.x + i * 64 * kWaves, key = u / (D / 16), c = u % (D / 16);
+        char* kd = s_kv[t & 1][0] + key * kRow;
+        char* vd = s_kv[t & 1][1] + key * kRow;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t x[4], y[4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            bytes_as<T>(kr[i][2 * j + e], x[2 * e], x[2 * e + 1]);
+            bytes_as<PT>(vr[i][2 * j + e], y[2 * e], y[2 * e + 1]);
+          }
+          *reinterpret_cast<v4u32*>(kd + 16 * ((2 * c + j) ^ key_swizzle<D>(key))) = v4u32{x[0], x[1], x[2], x[3]};
+          *reinterpret_cast<v4u32*>(vd + 16 * ((2 * c + j) ^ value_swizzle<D>(key))) = v4u32{y[0], y[1], y[2], y[3]};
+        }
+      }
+    }
+  };
+
+  const int vkey = 4 * half + (lane & 15) / 4;
+  const int vdim = 2 * ((lane >> 4) & 1) + (lane & 3) / 2;  // chunk in a 32-dim block
+  const int vbyte = vkey * kRow + 8 * (lane & 1);
+  float m, l[4];
+  v16f acc[DB];
+  auto step = [&](int t, auto drafted_c, auto careful_c) {
+    constexpr bool DRAFTED = decltype(drafted_c)::value, CAREFUL = decltype(careful_c)::value;
+    // Tile t is there for every wave, and every wave has read tile t - 1: its buffer takes tile t + 1.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 1 < tiles) {
+      if ((t + 1) * kKeys % kFill == 0) {
+        place((t + 1) * kKeys / kFill, page);
+        if ((t + 1) * kKeys + kFill < keys) page = page_at((t + 1) * kKeys / kFill + 1);
+      }
+      load(t + 1);
+    }
+    const int key0 = start + t * kKeys, at = t * kKeys % kFill, fill = t * kKeys / kFill & 1;
+    const char* kt = s_kv[t & 1][0] + col * kRow;
+    const char* vt = s_kv[t & 1][1] + vbyte;
+    v16f s[KU];
+#pragma unroll
+    for (int u = 0; u < KU; ++u) s[u] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < QS; ++i)
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+        s[u] = T::mfma32(*reinterpret_cast<const v4u32*>(kt + 32 * u * kRow + 16 * ((2 * i + half) ^ key_swizzle<D>(col))), qf[i], s[u]);
+    uint32_t live[KU][4];  // bit j of [u][i]: this row attends to key 32 u + 8 i + 4 half + j of the tile
+    float top = kLowest;
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (DRAFTED) {
+          const int d = key0 + 32 * u + 8 * i + 4 * half - ctx;
+          const uint64_t on = d >= 0 ? seen >> min(d, 63) : seen << min(-d, 63) | ((1ull << min(-d, 63)) - 1);
+          live[u][i] = d >= 64 ? 0u : (uint32_t)on & 15u;
+        }
+        v4f ks = {p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2};
+        if constexpr (INT8) ks = *reinterpret_cast<const v4f*>(&s_ks[fill][at + 32 * u + 8 * i + 4 * half]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float x = s[u][4 * i + j] * ks[j];
+          if (DRAFTED && !((live[u][i] >> j) & 1)) x = kNegInf;
+          s[u][4 * i + j] = x;
+          top = fmaxf(top, x);
+        }
+      }
+    float ta = top, tb = top;
+    swap32(ta, tb);
+    top = fmaxf(ta, tb);
+    if (__any(top > m + kSlack)) {
+      const float mn = fmaxf(m, top);
+      const float c = exp2_hw(m - mn);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l[i] *= c;
+#pragma unroll
+      for (int i = 0; i < DB; ++i) acc[i] = acc[i] * c;
+      m = mn;
+    }
+    v4u32 phi[2 * KU], plo[2 * KU];
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float pv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          pv[j] = exp2_hw(s[u][4 * i + j] - m);
+          l[j] += pv[j];
+        }
+        if constexpr (INT8) {
+          const v4f vs = *reinterpret_cast<const v4f*>(&s_vs[fill][at + 32 * u + 8 * i + 4 * half]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) pv[j] = DRAFTED && !((live[u][i] >> j) & 1) ? 0.0f : pv[j] * vs[j];  // a masked key's scale may be NaN
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t hi = PT::pack(pv[2 * j], pv[2 * j + 1]);
+          const v2f back = PT::unpack(hi);
+          phi[2 * u + i / 2][2 * (i % 2) + j] = hi;
+          plo[2 * u + i / 2][2 * (i % 2) + j] = PT::pack(pv[2 * j] - back[0], pv[2 * j + 1] - back[1]);
+        }
+      }
+    if constexpr (INT8) __builtin_amdgcn_sched_barrier(0);  // no registers for values read ahead of the weights
+#pragma unroll
+    for (int c = 0; c < 2 * KU; ++c)
+#pragma unroll
+      for (int i = 0; i < DB; i += 2) {  // two sums in turn: neither waits for the other
+        v4u32 a[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const char* from = vt + 16 * c * kRow + 16 * ((4 * (i + k) + vdim) ^ value_swizzle<D>(vkey));
+          const v2u32 lo = read_transposed(from), hi = read_transposed(from + 8 * kRow);
+          a[k] = v4u32{lo.x, lo.y, hi.x, hi.y};
+          if constexpr (CAREFUL) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[k][j] = only_finite<PT>(a[k][j]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[i + k % 2] = PT::mfma32(a[k % 2], k < 2 ? phi[c] : plo[c], acc[i + k % 2]);
+      }
+    if (t + 1 < tiles) store(t + 1);
+  };
+  auto begin = [&] {
+    place(0, page);
+    if (kFill < keys) page = page_at(1);
+    m = kLowest;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l[i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DB; ++i) acc[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    load(0);
+    store(0);
+  };
+  begin();
+  int t = 0;
+#pragma unroll 1
+  for (; t < plain; ++t) step(t, std::false_type{}, std::false_type{});
+#pragma unroll 1
+  for (; t < tiles; ++t) step(t, std::true_type{}, std::false_type{});
+  // As in the narrow kernel: values of masked keys that are infinities or NaN have spoiled the sums; the tiles with
+  // drafted keys are computed without such values, which are added at the end to the rows that attend to them.
+  bool careful = false;
+  if constexpr (!INT8) {
+    if (plain < tiles) {
+      float odd = 0.0f;  // 0 where all sums are finite, else NaN
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) odd = fmaf(acc[i][r], 0.0f, odd);
+      careful = __syncthreads_or(odd != 0.0f);
+      if (careful) {
+        page = page_at(0);
+        begin();
+#pragma unroll 1
+        for (t = 0; t < plain; ++t) step(t, std::false_type{}, std::false_type{});
+#pragma unroll 1
+        for (; t < tiles; ++t) step(t, std::true_type{}, std::true_type{});
+      }
+    }
+  }
+  const bool bad = __syncthreads_or(bad_page);
+  float la = (l[0] + l[1]) + (l[2] + l[3]), lb = la;
+  swap32(la, lb);
+  const float sum = bad ? __builtin_nanf("") : la + lb;
+  if (row0 + 32 * wave + col >= rows) return;
+  const bool alone = rq.L <= keys;
+  const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + chunk;
+  if (!alone && half == 0) p.mp[part] = m, p.lp[part] = sum;
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int dim = 32 * i + 2 * r + 4 * half;
+      v4f o = {acc[i][r], acc[i][r + 1], acc[i][r + 2], acc[i][r + 3]};
+      if (careful) {
+#pragma unroll 1
+        for (int key = start + plain * kKeys; key < end; ++key) {
+          const int32_t block = p.bt[(int64_t)b * p.sbt + page_of(p, key)];
+          const bool on = (key < ctx || (seen >> (key - ctx)) & 1) && block >= 0 && block < p.blocks;
+          if (!on) continue;
+          const v2u32 w = *reinterpret_cast<const v2u32*>(vh + block * p.svb + (int64_t)(key - page_of(p, key) * p.page) * p.svp + 2 * dim);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float f = T::to_f32((uint16_t)(w[j / 2] >> (16 * (j % 2))));
+            if (!__builtin_isfinite(f)) o[j] += f;
+          }
+        }
+      }
+      if (alone)
+        store_row<T>(p, rq, node, head, dim, o, sum);
+      else
+        *reinterpret_cast<v4f*>(p.ap + part * D + dim) = o;
+    }
+}
+
+// Joins a row's groups: the strands of a group where workgroups have left them apart, then the groups in order; of the wide
+// kernel four chunks are a group. A workgroup joins one row, kMergeGroups groups at a time, 4 dims a lane: their partials are on their way together. A row
 // of several groups attends to its context, so its sum is not empty.
 constexpr int kMergeGroups = 4;
 template <typename T, int D>
@@ -620,8 +927,10 @@ __global__ __launch_bounds__(D * kMergeGroups / 4) void tree_merge_kernel(TreePa
   const uint32_t bn = blockIdx.x / (uint32_t)H;
   const int b = (int)(bn / (uint32_t)p.max_nodes), node = (int)(bn % (uint32_t)p.max_nodes);
   const Request rq = request_of(p, b);
-  const int groups = (rq.L + kGroup * kSeg - 1) / (kGroup * kSeg);
-  if (rq.bad || node >= rq.T || groups <= 1) return;
+  const bool wide = rq.T * p.G > kWideRows, apart = wide || p.strands;
+  const int keys = wide ? wide_chunk(rq.L) : kSeg;
+  const int chunks = (rq.L + keys - 1) / keys, groups = (chunks + kGroup - 1) / kGroup;
+  if (rq.bad || node >= rq.T || chunks <= (wide ? 1 : kGroup)) return;
   const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts;
   State sum;
   for (int g0 = 0; g0 < groups; g0 += kMergeGroups) {
@@ -630,8 +939,8 @@ __global__ __launch_bounds__(D * kMergeGroups / 4) void tree_merge_kernel(TreePa
       const int64_t at = part + (g0 + mine) * kWaves;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w)
-        if (w == 0 || p.strands) s[w] = State{p.mp[at + w], p.lp[at + w], reinterpret_cast<const v4f*>(p.ap)[(at + w) * kLanes + c]};
-      if (p.strands) join(s);
+        if (w == 0 || (apart && (!wide || (g0 + mine) * kGroup + w < chunks))) s[w] = State{p.mp[at + w], p.lp[at + w], reinterpret_cast<const v4f*>(p.ap)[(at + w) * kLanes + c]};
+      if (apart) join(s, wide ? chunks - (g0 + mine) * kGroup : kWaves);
       if (c == 0) s_ml[mine][0] = s[0].m, s_ml[mine][1] = s[0].l;
       s_a[mine][c] = s[0].a;
     }
@@ -649,25 +958,45 @@ __global__ __launch_bounds__(D * kMergeGroups / 4) void tree_merge_kernel(TreePa
   if (mine == 0) store_row<T>(p, rq, node, head, 4 * c, sum.a, sum.l);
 }
 
+// The most chunks of any request of at most `keys` keys.
+int64_t most_chunks(int64_t keys) {
+  const int64_t few = std::min<int64_t>(keys, 4096);
+  return std::max(cdiv<int64_t>(few, wide_chunk((int)few)), cdiv<int64_t>(keys, wide_chunk((int)keys)));
+}
+
 template <typename T, bool INT8, int D>
 hipError_t launch_tree(TreeParams p, hipStream_t st) {
-  const int64_t rows = (int64_t)p.max_nodes * p.G;
-  const int nq = rows <= 16 ? 1 : 2;
-  p.row_blocks = (int32_t)cdiv<int64_t>(rows, 16 * nq);
-  // A workgroup for each group of segments, or for each of its strands where the former would not fill the GPU. The order
-  // of the sums, and so every bit, is the same.
-  const int64_t units = (int64_t)p.row_blocks * p.KV * p.n, groups = cdiv<int64_t>(p.ns, kGroup);
-  p.strands = groups > 1 && units * groups < kManyWorkgroups;
-  const int64_t blocks = units * groups * (p.strands ? kWaves : 1);
+  // The narrow kernel covers the rows of requests that do not take the wide one.
+  const int64_t rows = (int64_t)p.max_nodes * p.G, narrow = std::min<int64_t>(rows, kWideRows / p.G * p.G);
   const int64_t merges = (int64_t)p.n * p.max_nodes * p.KV * p.G;
-  if (blocks > 0x7FFFFFFFLL || merges > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)blocks), threads(64 * kWaves);
-  if (nq == 1)
-    hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 1>), grid, threads, 0, st, p);
-  else
-    hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 2>), grid, threads, 0, st, p);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess || groups <= 1) return err;
+  if (merges > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+  const dim3 threads(64 * kWaves);
+  {
+    const int nq = narrow <= 16 ? 1 : 2;
+    p.row_blocks = (int32_t)std::max<int64_t>(1, cdiv<int64_t>(narrow, 16 * nq));
+    // A workgroup for each group of segments, or for each of its strands where the former would not fill the GPU. The
+    // order of the sums, and so every bit, is the same.
+    const int64_t units = (int64_t)p.KV * p.n, groups = cdiv<int64_t>(p.ns, kGroup);
+    p.strands = groups > 1 && units * p.row_blocks * groups < kManyWorkgroups;
+    const int64_t blocks = cdiv<int64_t>(units * groups * (p.strands ? kWaves : 1), 8) * 8 * p.row_blocks;
+    if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+    if (nq == 1)
+      hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 1>), dim3((unsigned)blocks), threads, 0, st, p);
+    else
+      hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 2>), dim3((unsigned)blocks), threads, 0, st, p);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  if (rows > kWideRows) {
+    TreeParams w = p;
+    w.row_blocks = (int32_t)cdiv<int64_t>(rows, 32 * kWaves);
+    const int64_t blocks = cdiv<int64_t>((int64_t)p.KV * p.n * most_chunks(p.max_len), 8) * 8 * w.row_blocks;
+    if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((tree_decode_kernel_wide<T, INT8, D>), dim3((unsigned)blocks), threads, 0, st, w);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  if (p.ns <= (rows > kWideRows ? 1 : kGroup)) return hipSuccess;
   hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3((unsigned)merges), dim3(D * kMergeGroups / 4), 0, st, p);
   return hipGetLastError();
 }
