@@ -24,6 +24,18 @@ constexpr float kLowest = -3.402823466e38f;  // -FLT_MAX
 // weights up to 1 in every type here, and a tile seldom passes it, so the accumulators are seldom rescaled.
 constexpr float kSlack = 8.0f;
 
+// x / d for 0 <= x < 2^31 and 1 <= d < 2^31: (2 x mul >> 32) >> shift with 2^shift >= d and mul = 2^(31 + shift) / d rounded
+// up. The excess of mul is below 1, so times 2 x it stays below 2^32 <= 2^(32 + shift) / d: the quotient is exact.
+struct Divisor {
+  uint32_t mul, shift;
+};
+inline Divisor make_divisor(int64_t d) {
+  uint32_t s = 0;
+  while ((1LL << s) < d) ++s;
+  return Divisor{(uint32_t)(((1ULL << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d), s};
+}
+__device__ inline int divide(int x, const Divisor& d) { return (int)(__umulhi(2u * (uint32_t)x, d.mul) >> d.shift); }
+
 __device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Exchanges between the four 16-lane rows of a wave on the vector ALU (gfx950 lane swaps), in

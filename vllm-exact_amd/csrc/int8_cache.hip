@@ -7,7 +7,11 @@
 // of the quotient itself. A row with an infinity or NaN gets q = 0 and the scale NaN: it reads back as NaN.
 // A row of zeros gets the scale 0.
 //
-// Both kernels move each byte once and are bound by HBM, and by launch latency at a decode step's sizes.
+// Both kernels move each byte once and are bound by HBM, and by the latency of a few dependent loads at a decode step's
+// sizes. Measured: 16 contexts of up to 8192 tokens (8 heads of 128 dims) read back as bf16 in 137 us, 4.5 TB/s, where a
+// large copy reaches 4.9; 64 tokens written and read back in 7 us.
+
+#include <algorithm>
 
 #include "attention_common.h"
 
@@ -23,27 +27,43 @@ struct CacheWrite {
   const int64_t* slots;
   int64_t tokens;
   int32_t KV, page;
+  Divisor by_token, by_page;  // by a token's units, by the tokens of a page
   int64_t rows_total;     // slots of the cache: blocks * page
+  int32_t per_group;      // tokens of a workgroup
 };
 
-// LPR lanes hold a row, 8 elements each; a workgroup's rows are consecutive (token, KV head, key or value).
+// The largest value of the LPR lanes of a row, in each of them.
+template <int CTRL>
+__device__ inline uint32_t max_with(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false));
+}
+template <int LPR>
+__device__ inline uint32_t row_max(uint32_t x) {
+  x = max_with<0xB1>(x);   // lane ^ 1
+  x = max_with<0x4E>(x);   // lane ^ 2
+  x = max_with<0x141>(x);  // the other end of 8 lanes
+  if constexpr (LPR >= 16) x = max_with<0x140>(x);  // ... of 16
+  if constexpr (LPR == 32) x = max(x, (uint32_t)__shfl_xor((int)x, 16));
+  return x;
+}
+
+// A unit is 8 elements of a row; a token's units are those of its heads in turn. The lanes of a row are neighbours in a wave.
+// A workgroup takes per_group tokens' keys or values, a unit for every thread where a token has no more than that: several
+// loads ahead in a thread were slower (10,000 tokens of 2 heads of 256 dims: 14 us with four, 11 with one).
 template <int DTYPE, int D, bool VEC>
 __global__ __launch_bounds__(256) void int8_write_kernel(CacheWrite p) {
   constexpr int LPR = D / 8;
+  const int per_token = p.KV * LPR, w = blockIdx.y;
+  const int64_t t0 = (int64_t)blockIdx.x * p.per_group;
+  const int units = (int)min((int64_t)p.per_group, p.tokens - t0) * per_token;
   const int lane = threadIdx.x & (LPR - 1);
-  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const int which = (int)(row & 1);
-  const int64_t th = row >> 1;
-  const int64_t t = th / p.KV;
-  const int h = (int)(th - t * p.KV);
-  const bool live = t < p.tokens;
-  float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  int64_t slot = -1;
-  if (live) {
-    slot = p.slots[t];
-    const int64_t at = t * p.sxt[which] + (int64_t)h * p.sxh[which] + 8 * lane;
+  for (int u = threadIdx.x; u < units; u += 256) {  // a row's lanes are all in or all out
+    const int tok = divide(u, p.by_token), h = (u - tok * per_token) / LPR;
+    const int64_t slot = p.slots[t0 + tok];
+    const int64_t at = (t0 + tok) * p.sxt[w] + (int64_t)h * p.sxh[w] + 8 * lane;
+    float x[8];
     if constexpr (DTYPE == VXA_F32) {
-      const float* src = reinterpret_cast<const float*>(p.x[which]) + at;
+      const float* src = reinterpret_cast<const float*>(p.x[w]) + at;
       if constexpr (VEC) {
         const v4f a = *reinterpret_cast<const v4f*>(src), b = *reinterpret_cast<const v4f*>(src + 4);
 #pragma unroll
@@ -54,7 +74,7 @@ __global__ __launch_bounds__(256) void int8_write_kernel(CacheWrite p) {
       }
     } else {
       using T = std::conditional_t<DTYPE == VXA_BF16, BF16, FP16>;
-      const uint16_t* src = reinterpret_cast<const uint16_t*>(p.x[which]) + at;
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(p.x[w]) + at;
       if constexpr (VEC) {
         const v4u32 a = *reinterpret_cast<const v4u32*>(src);
 #pragma unroll
@@ -67,33 +87,46 @@ __global__ __launch_bounds__(256) void int8_write_kernel(CacheWrite p) {
         for (int j = 0; j < 8; ++j) x[j] = T::to_f32(src[j]);
       }
     }
+    // The largest magnitude as bits: NaN and infinities order above every finite value.
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+    top = row_max<LPR>(top);
+    if (slot < 0 || slot >= p.rows_total) continue;
+    const float ftop = __uint_as_float(top);
+    const bool special = top >= 0x7F800000u;
+    const int32_t block = divide((int32_t)slot, p.by_page);
+    const int32_t off = (int32_t)slot - block * p.page;
+    if (lane == 0)
+      p.s[w][(int64_t)block * p.ssb[w] + (int64_t)off * p.ssp[w] + (int64_t)h * p.ssh[w]] = special ? __builtin_nanf("") : ftop / 127.0f;
+    // x times 127 / top is off by at most 2^-16; adding 1.5 2^23 rounds it to a whole number in the low byte. Next to a half,
+    // and where 127 / top overflows, the quotient decides.
+    constexpr float kWhole = 12582912.0f;
+    const float mul = 127.0f / ftop;
+    uint32_t q[8];
+    float away = 0.0f;  // from the whole numbers
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float r = x[j] * mul, a = r + kWhole;
+      q[j] = __float_as_uint(a);
+      away = fmaxf(away, fabsf(r - (a - kWhole)));
+    }
+    if (away > 0.4999f || ftop < 0x1p-110f || special) {
+      // Above 2^100 the products 127 x could overflow: both sides are scaled by 2^-32, which rounds nothing that counts.
+      const float down = ftop > 0x1p100f ? 0x1p-32f : 1.0f;
+      const float div = ftop * down;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = special || top == 0 ? 0u : (uint32_t)(int)rintf((x[j] * down) * 127.0f / div);
+    }
+    uint32_t out[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t lo = __builtin_amdgcn_perm(q[4 * j + 1], q[4 * j], 0x0C0C0400u);
+      out[j] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[4 * j + 3], q[4 * j + 2], 0x0C0C0400u), lo, 0x05040100u);
+    }
+    int8_t* dst = p.c[w] + (int64_t)block * p.scb[w] + (int64_t)off * p.scp[w] + (int64_t)h * p.sch[w] + 8 * lane;
+    *reinterpret_cast<v2u32*>(dst) = v2u32{out[0], out[1]};
   }
-  // The largest magnitude as bits: NaN and infinities order above every finite value.
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-#pragma unroll
-  for (int m = 1; m < LPR; m *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, m));
-  if (!live || slot < 0 || slot >= p.rows_total) return;
-  const float ftop = __uint_as_float(top);
-  const bool special = top >= 0x7F800000u;
-  const int32_t block = (int32_t)((uint32_t)slot / (uint32_t)p.page);
-  const int32_t off = (int32_t)slot - block * p.page;
-  if (lane == 0)
-    p.s[which][(int64_t)block * p.ssb[which] + (int64_t)off * p.ssp[which] + (int64_t)h * p.ssh[which]] =
-        special ? __builtin_nanf("") : ftop / 127.0f;
-  // Above 2^100 the products 127 x could overflow: both sides are scaled by 2^-32, which rounds nothing that counts.
-  const float down = ftop > 0x1p100f ? 0x1p-32f : 1.0f;
-  const float div = ftop * down;
-  const bool zero = special || top == 0;
-  uint32_t w[2] = {0, 0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int q = zero ? 0 : (int)rintf((x[j] * down) * 127.0f / div);
-    w[j / 4] |= ((uint32_t)q & 0xFFu) << (8 * (j % 4));
-  }
-  int8_t* dst = p.c[which] + (int64_t)block * p.scb[which] + (int64_t)off * p.scp[which] + (int64_t)h * p.sch[which] + 8 * lane;
-  *reinterpret_cast<v2u32*>(dst) = v2u32{w[0], w[1]};
 }
 
 struct CacheRead {
@@ -107,20 +140,25 @@ struct CacheRead {
   const int32_t* first;  // [n] or null: the first token read of each sequence
   int64_t n, total;      // sequences, packed rows
   int32_t KV, page, cols;  // cols: block-table entries of a sequence
+  Divisor by_token, by_page;  // by a token's units, by the tokens of a page
+  int32_t per_group;      // tokens of a workgroup
   int64_t blocks;
   void* o[2];
   int64_t sot[2], soh[2];
 };
 
-constexpr int kReadTokens = 16;  // tokens of a workgroup
+constexpr int kReadTokens = 16;  // tokens of a workgroup, at most
 
-// A workgroup reads 16 packed tokens, all heads, keys and values: whole lines of the cache's pages (a page's
-// tokens follow each other) and whole lines of the output (a token's heads do). A lane moves 16 elements.
+// A workgroup reads up to 16 packed tokens, all heads, keys and values: whole lines of the cache's pages (a page's tokens follow
+// each other) and whole lines of the output (a token's heads do). A unit is 16 bytes of output; a token's units are those
+// of its heads in turn, keys first, then values. A thread has kReadUnits units on their way together.
+constexpr int kReadUnits = 4;
+constexpr int64_t kNone = -0x7FFFFFFFFFFFFFFFLL;  // no place: a unit past the end or in no sequence
 template <int OUT, int D>
 __global__ __launch_bounds__(256) void int8_read_kernel(CacheRead p) {
-  constexpr int LPR = D / 16;
+  constexpr int EPU = OUT == VXA_F32 ? 4 : 8, LPR = D / EPU;  // elements of a unit, units of a row
   __shared__ int32_t s_block[kReadTokens], s_off[kReadTokens];
-  const int64_t t0 = (int64_t)blockIdx.x * kReadTokens;
+  const int64_t t0 = (int64_t)blockIdx.x * p.per_group;
   if (threadIdx.x < 64) {
     // A token's sequence is the number of sequences that end at or before it: lanes compare 64 ends at a time.
     const int lane = threadIdx.x;
@@ -128,20 +166,19 @@ __global__ __launch_bounds__(256) void int8_read_kernel(CacheRead p) {
     for (int64_t j0 = 0; j0 < p.n; j0 += 64) {
       const int64_t j = j0 + lane;
       const int32_t end = j < p.n ? p.cu[j + 1] : 0x7FFFFFFF;
-#pragma unroll
-      for (int i = 0; i < kReadTokens; ++i) {
+      for (int i = 0; i < p.per_group; ++i) {
         const int c = __popcll(__ballot((int64_t)end <= t0 + i));
         if (lane == i) seq += c;
       }
     }
-    if (lane < kReadTokens) {
+    if (lane < p.per_group) {
       int32_t block = -1, off = 0;  // -1: the row is in no sequence, -2: its page does not exist
       const int64_t in_seq = t0 + lane < p.total && seq < p.n ? t0 + lane - p.cu[seq] : -1;
       if (in_seq >= 0) {
         const int64_t pos = in_seq + (p.first != nullptr ? p.first[seq] : 0);
         block = -2;
         if (pos >= 0 && pos < (int64_t)p.cols * p.page) {
-          const int32_t pg = (int32_t)((uint32_t)pos / (uint32_t)p.page);
+          const int32_t pg = divide((int)pos, p.by_page);
           const int32_t id = p.bt[(int64_t)seq * p.sbt + pg];
           off = (int32_t)pos - pg * p.page;
           if (id >= 0 && id < p.blocks) block = id;
@@ -152,57 +189,76 @@ __global__ __launch_bounds__(256) void int8_read_kernel(CacheRead p) {
     }
   }
   __syncthreads();
-  const int units = kReadTokens * p.KV * 2 * LPR;
-  for (int u = threadIdx.x; u < units; u += 256) {
-    const int lane = u & (LPR - 1);
-    const int r = u / LPR;
-    const int which = r & 1;
-    const int i = (r >> 1) / p.KV;
-    const int h = (r >> 1) - i * p.KV;
-    const int32_t block = s_block[i], off = s_off[i];
-    if (block == -1) continue;
-    float scale = __builtin_nanf("");
-    v4u32 w = {0, 0, 0, 0};
-    if (block >= 0) {
-      scale = p.s[which][(int64_t)block * p.ssb[which] + (int64_t)off * p.ssp[which] + (int64_t)h * p.ssh[which]];
-      w = *reinterpret_cast<const v4u32*>(p.c[which] + (int64_t)block * p.scb[which] + (int64_t)off * p.scp[which] +
-                                          (int64_t)h * p.sch[which] + 16 * lane);
-    }
-    float f[16];
+  const int per_token = p.KV * LPR, units = p.per_group * per_token;
+  static_for<2>([&](auto wc) {
+    constexpr int wh = decltype(wc)::value;
+    for (int u0 = threadIdx.x; u0 < units; u0 += 256 * kReadUnits) {
+      uint32_t w[kReadUnits][EPU / 4];
+      float scale[kReadUnits];
+      int64_t at[kReadUnits];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) f[j] = (float)(int8_t)(w[j / 4] >> (8 * (j % 4))) * scale;
-    const int64_t at = (t0 + i) * p.sot[which] + (int64_t)h * p.soh[which] + 16 * lane;
-    if constexpr (OUT == VXA_F32) {
-      float* dst = reinterpret_cast<float*>(p.o[which]) + at;
+      for (int n = 0; n < kReadUnits; ++n) {
+        const int u = u0 + 256 * n;
+        at[n] = kNone;
+        if (u >= units) continue;
+        const int i = divide(u, p.by_token), rest = u - i * per_token;
+        const int lane = rest & (LPR - 1), h = rest / LPR;
+        const int32_t block = s_block[i], off = s_off[i];
+        if (block == -1) continue;
+        at[n] = (t0 + i) * p.sot[wh] + (int64_t)h * p.soh[wh] + EPU * lane;
+        scale[n] = __builtin_nanf("");
 #pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<v4f*>(dst + 4 * j) = v4f{f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]};
-    } else {
-      using T = std::conditional_t<OUT == VXA_BF16, BF16, FP16>;
-      uint32_t o[8];
+        for (int j = 0; j < EPU / 4; ++j) w[n][j] = 0;
+        if (block >= 0) {
+          scale[n] = p.s[wh][(int64_t)block * p.ssb[wh] + (int64_t)off * p.ssp[wh] + (int64_t)h * p.ssh[wh]];
+          const int8_t* src = p.c[wh] + (int64_t)block * p.scb[wh] + (int64_t)off * p.scp[wh] + (int64_t)h * p.sch[wh] + EPU * lane;
+          if constexpr (EPU == 8) {
+            const v2u32 x = *reinterpret_cast<const v2u32*>(src);
+            w[n][0] = x.x, w[n][1] = x.y;
+          } else {
+            w[n][0] = *reinterpret_cast<const uint32_t*>(src);
+          }
+        }
+      }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = T::pack(f[2 * j], f[2 * j + 1]);
-      uint16_t* dst = reinterpret_cast<uint16_t*>(p.o[which]) + at;
-      *reinterpret_cast<v4u32*>(dst) = v4u32{o[0], o[1], o[2], o[3]};
-      *reinterpret_cast<v4u32*>(dst + 8) = v4u32{o[4], o[5], o[6], o[7]};
-    }
+      for (int n = 0; n < kReadUnits; ++n) {
+        if (at[n] == kNone) continue;
+        float f[EPU];
+#pragma unroll
+        for (int j = 0; j < EPU; ++j) f[j] = (float)(int8_t)(w[n][j / 4] >> (8 * (j % 4))) * scale[n];
+        if constexpr (OUT == VXA_F32) {
+          *reinterpret_cast<v4f*>(reinterpret_cast<float*>(p.o[wh]) + at[n]) = v4f{f[0], f[1], f[2], f[3]};
+        } else {
+          using T = std::conditional_t<OUT == VXA_BF16, BF16, FP16>;
+          *reinterpret_cast<v4u32*>(reinterpret_cast<uint16_t*>(p.o[wh]) + at[n]) =
+              v4u32{T::pack(f[0], f[1]), T::pack(f[2], f[3]), T::pack(f[4], f[5]), T::pack(f[6], f[7])};
+        }
+      }
+    }  });
   }
-}
 
 template <int DTYPE, int D>
-hipError_t launch_write(const CacheWrite& p, bool vec, hipStream_t st) {
-  const int64_t blocks = cdiv<int64_t>(p.tokens * p.KV * 2, 256 / (D / 8));
+hipError_t launch_write(CacheWrite p, bool vec, hipStream_t st) {
+  const int64_t per_token = p.KV * (D / 8);
+  p.per_group = (int32_t)std::max<int64_t>(1, 256 / per_token);
+  p.by_token = make_divisor(per_token);
+  const int64_t blocks = cdiv<int64_t>(p.tokens, p.per_group);
   if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+  const dim3 grid((unsigned)blocks, 2), threads(256);
   if (vec)
-    hipLaunchKernelGGL((int8_write_kernel<DTYPE, D, true>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((int8_write_kernel<DTYPE, D, true>), grid, threads, 0, st, p);
   else
-    hipLaunchKernelGGL((int8_write_kernel<DTYPE, D, false>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((int8_write_kernel<DTYPE, D, false>), grid, threads, 0, st, p);
   return hipGetLastError();
 }
 
 template <int OUT, int D>
-hipError_t launch_read(const CacheRead& p, hipStream_t st) {
-  const int64_t blocks = cdiv<int64_t>(p.total, kReadTokens);
+hipError_t launch_read(CacheRead p, hipStream_t st) {
+  // Fewer tokens a workgroup where 16 would leave places on the GPU empty.
+  p.per_group = (int32_t)std::clamp<int64_t>(p.total / 2048, 1, kReadTokens);
+  const int64_t blocks = cdiv<int64_t>(p.total, p.per_group);
   if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+  p.by_token = make_divisor(p.KV * (D / (OUT == VXA_F32 ? 4 : 8)));
   hipLaunchKernelGGL((int8_read_kernel<OUT, D>), dim3((unsigned)blocks), dim3(256), 0, st, p);
   return hipGetLastError();
 }
@@ -226,7 +282,7 @@ bool known_dim(int64_t d) { return d == 64 || d == 128 || d == 256; }
 // Sizes both entry points take: 32-bit slot arithmetic, and 8-bit rows that start on 16 bytes.
 int check_cache(const void* kc, const void* vc, const int64_t* sk, const int64_t* sv, int64_t blocks, int64_t page,
                 int64_t KV, int64_t D) {
-  if (!known_dim(D) || KV > (1 << 20) || page > (1 << 30) || blocks > 0x7FFFFFFFLL / page) return VXA_ERR_UNSUPPORTED;
+  if (!known_dim(D) || KV > (1 << 16) || page > (1 << 30) || blocks > 0x7FFFFFFFLL / page) return VXA_ERR_UNSUPPORTED;
   if ((uintptr_t)kc % 16 || (uintptr_t)vc % 16) return VXA_ERR_UNSUPPORTED;
   for (int i = 0; i < 3; ++i)
     if (sk[i] % 16 || sv[i] % 16) return VXA_ERR_UNSUPPORTED;
@@ -255,7 +311,7 @@ extern "C" int vxa_int8_cache_write(const void* key, int64_t skt, int64_t skh, c
                    svt % piece == 0 && svh % piece == 0;
   const CacheWrite p{{key, value}, {skt, svt}, {skh, svh}, {k_cache, v_cache}, {skcb, svcb}, {skcp, svcp}, {skch, svch},
                      {k_scale, v_scale}, {sksb, svsb}, {sksp, svsp}, {sksh, svsh}, slots, tokens, (int32_t)num_kv_heads,
-                     (int32_t)block_size, num_blocks * block_size};
+                     (int32_t)block_size, Divisor{}, make_divisor(block_size), num_blocks * block_size, 1};
   const hipError_t err = dispatch(dtype, head_dim, [&](auto t, auto d) {
     return launch_write<decltype(t)::value, decltype(d)::value>(p, vec, reinterpret_cast<hipStream_t>(stream));
   });
@@ -285,7 +341,7 @@ extern "C" int vxa_int8_cache_read(const int8_t* k_cache, int64_t skcb, int64_t 
     return VXA_ERR_UNSUPPORTED;
   const CacheRead p{{k_cache, v_cache}, {skcb, svcb}, {skcp, svcp}, {skch, svch}, {k_scale, v_scale}, {sksb, svsb},
                     {sksp, svsp}, {sksh, svsh}, block_table, sbt, starts, first, n, tokens, (int32_t)num_kv_heads,
-                    (int32_t)block_size, (int32_t)bt_cols, num_blocks, {key, value}, {skt, svt}, {skh, svh}};
+                    (int32_t)block_size, (int32_t)bt_cols, Divisor{}, make_divisor(block_size), kReadTokens, num_blocks, {key, value}, {skt, svt}, {skh, svh}};
   const hipError_t err = dispatch(dtype, head_dim, [&](auto t, auto d) {
     return launch_read<decltype(t)::value, decltype(d)::value>(p, reinterpret_cast<hipStream_t>(stream));
   });

@@ -55,7 +55,7 @@ struct TreeParams {
   const int32_t* bt;
   int64_t sbt;
   int32_t cols, page;     // block-table entries of a request, tokens of a page
-  uint32_t page_mul, page_shift;  // key / page = (2 key * page_mul >> 32) >> page_shift for keys below 2^31
+  Divisor by_page;
   int64_t blocks;
   const int32_t* sl;
   const int32_t* qsl;
@@ -73,7 +73,7 @@ struct TreeParams {
   int32_t out_dtype;
 };
 
-__device__ inline int page_of(const TreeParams& p, int key) { return (int)(__umulhi(2u * (uint32_t)key, p.page_mul) >> p.page_shift); }
+__device__ inline int page_of(const TreeParams& p, int key) { return divide(key, p.by_page); }
 
 // The request's keys, nodes and first query row; `bad` where they do not fit the call (a length below its
 // nodes, more nodes or keys than the call's bounds): its rows become NaN.
@@ -1082,11 +1082,7 @@ extern "C" int vxa_tree_decode(const void* q, int64_t sqt, int64_t sqh, int q_dt
   p.ap = w, p.mp = need > 0 ? w + parts * head_dim : nullptr, p.lp = need > 0 ? p.mp + parts : nullptr;
   p.out = out, p.sot = sot, p.soh = soh, p.out_dtype = out_dtype;
   p.out_wide = out_dtype == q_dtype && (uintptr_t)out % 8 == 0 && sot % 4 == 0 && soh % 4 == 0;
-  // page_mul = 2^(31 + s) / page rounded up, with 2^s >= page: its excess over the quotient, below page / page, times a
-  // key stays below 2^(31 + s) / page, so the shifted product is exact.
-  p.page_shift = 0;
-  while ((1LL << p.page_shift) < block_size) ++p.page_shift;
-  p.page_mul = (uint32_t)(((1ULL << (31 + p.page_shift)) + (uint64_t)block_size - 1) / (uint64_t)block_size);
+  p.by_page = make_divisor(block_size);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   hipError_t err;
   if (q_dtype == VXA_BF16)

@@ -10,6 +10,9 @@ argument types, and turns status codes into Python exceptions:
 * VXA_ERR_TOO_LARGE   -> ValueError (a problem beyond vxa_exact_linear_op_noalloc's fixed scratch)
 * VXA_ERR_WORKSPACE / VXA_ERR_LAUNCH -> RuntimeError
 
+The serving operators (prompt_attn, int8_cache, tree_attn) reach the same entry points through calls(), a module that takes
+the tensors themselves.
+
 There is no fallback: if the library is missing, every GPU entry point raises.
 """
 import ctypes
@@ -199,6 +202,31 @@ def launch(device, fn, *args):
         return fn(*args, stream_handle(device))
 
 
+def stream_of(t):
+    """torch's current stream on the tensor's GPU, as an integer (0 for a CPU tensor)."""
+    if not t.is_cuda:
+        return 0
+    return stream_handle(t.device) if _raw_stream is None else _raw_stream(t.device.index)
+
+
+_calls = None
+_CALLED = ("vxa_prompt_attention", "vxa_int8_cache_write", "vxa_int8_cache_read", "vxa_tree_decode_workspace", "vxa_tree_decode")
+
+
+def calls():
+    """The module of the serving operators' calls on tensors (csrc/tensor_calls.cpp), bound to the loaded library."""
+    global _calls
+    if _calls is None:
+        L = lib()
+        try:
+            from . import _tensor_calls
+        except ImportError as e:
+            raise RuntimeError(f"vllm_exact: _tensor_calls.so is not available ({e}). Build it with `make -C vllm-exact_amd`.") from e
+        _tensor_calls.bind(*(ctypes.cast(getattr(L, name), _vp).value for name in _CALLED))
+        _calls = _tensor_calls
+    return _calls
+
+
 def dtype_enum(dtype):
     try:
         return DTYPE_ENUM[dtype]
@@ -256,11 +284,6 @@ def paged_units_workspace(n, H, KV, D, max_len, split, blk, waves):
     check(lib().vxa_paged_decode_units_workspace(n, H, KV, D, max_len, split, blk, waves, ctypes.byref(ws)),
           "paged_decode_units_workspace")
     return ws.value
-
-
-def strided(t, *axes):
-    """(pointer, strides of `axes`) as the entry points take a tensor; nulls and zeros for None."""
-    return (None,) + (0,) * len(axes) if t is None else (t.data_ptr(),) + tuple(t.stride(a) for a in axes)
 
 
 @functools.lru_cache(maxsize=1024)

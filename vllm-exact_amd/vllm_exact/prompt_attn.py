@@ -14,31 +14,7 @@ def prompt_attention(query, key, value, cu_seqlens, scale, out):
     [cu_seqlens[i], cu_seqlens[i + 1]) holds t; cu_seqlens (n + 1,) int32 on the GPU (vLLM's query_start_loc); out
     (tokens, H, D) fp32, bf16 or fp16. Row j of a sequence attends to its rows 0..j. Rows and heads may be strided (views of
     a fused projection), D is 64, 128 or 256 and contiguous. Rows after cu_seqlens[n] are left alone. Returns out."""
-    for t in (query, key, value, cu_seqlens, out):
-        if not t.is_cuda:
-            raise ValueError("prompt_attention runs the gfx950 HIP kernel and needs GPU tensors; "
-                             "use prompt_attention_torch for the CPU statement")
-    L = _nx.lib()
-    if query.dtype not in (torch.bfloat16, torch.float16) or key.dtype != query.dtype or value.dtype != query.dtype:
-        raise NotImplementedError("prompt_attention: query, key and value must be all bf16 or all fp16")
-    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or not cu_seqlens.is_contiguous() or not len(cu_seqlens):
-        raise ValueError("prompt_attention: cu_seqlens must be a contiguous int32 vector of the n + 1 starts")
-    if query.dim() != 3 or key.dim() != 3 or value.shape != key.shape or out.shape != query.shape:
-        raise ValueError("prompt_attention: inconsistent shapes")
-    T, H, D = query.shape
-    KV = key.shape[1]
-    if key.shape[0] != T or key.shape[2] != D or KV == 0 or H % KV:
-        raise ValueError("prompt_attention: inconsistent shapes")
-    if any(t.device != query.device for t in (key, value, cu_seqlens, out)):
-        raise ValueError("prompt_attention: all tensors must be on the query's GPU")
-    if D and any(t.stride(2) != 1 for t in (query, key, value, out)):
-        raise ValueError("prompt_attention: the head dimension must be contiguous")
-    if T == 0:
-        return out
-    st = _nx.strided
-    status = _nx.launch(query.device, L.vxa_prompt_attention, *st(query, 0, 1), *st(key, 0, 1), *st(value, 0, 1),
-                        _nx.dtype_enum(query.dtype), cu_seqlens.data_ptr(), len(cu_seqlens) - 1, T, float(scale),
-                        out.data_ptr(), _nx.dtype_enum(out.dtype), out.stride(0), out.stride(1), H, KV, D)
+    status = (_nx._calls or _nx.calls()).prompt_attention(query, key, value, cu_seqlens, scale, out, _nx.stream_of(query))
     if status:
         _nx.check(status, "prompt_attention")
     return out

@@ -8,9 +8,9 @@ of 512 keys and the order inside them are fixed, so a request's bits depend on i
 import torch
 
 from . import _native as _nx
-from . import int8_cache, paged_attn
+from . import paged_attn
 
-MAX_NODES = 64  # bits of a mask
+MAX_NODES = 64  # bits of a mask: the most nodes of a request
 
 
 def tree_decode(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, tree_mask, scale, out, max_nodes,
@@ -22,57 +22,9 @@ def tree_decode(query, key_cache, value_cache, block_table, seq_lens, query_star
     None: to the drafted tokens up to its own; out (tokens, H, D) fp32, bf16 or fp16. A node that attends to nothing
     gives zeros. max_nodes (at most 64) and max_seq_len (0 or None: paged_attn.MAX_LEN) bound the nodes and seq_lens of every
     request: one beyond them, or shorter than its nodes, or with a block outside the cache, gets NaN rows. Returns out."""
-    tensors = [query, key_cache, value_cache, block_table, seq_lens, query_start_loc, out]
-    tensors += [t for t in (tree_mask, key_scale, value_scale) if t is not None]
-    for t in tensors:
-        if not t.is_cuda:
-            raise ValueError("tree_decode runs the gfx950 HIP kernel and needs GPU tensors; "
-                             "use tree_decode_torch for the CPU statement")
-    L = _nx.lib()
-    if any(t.device != query.device for t in tensors):
-        raise ValueError("tree_decode: all tensors must be on the query's GPU")
-    if query.dtype not in (torch.bfloat16, torch.float16):
-        raise NotImplementedError("tree_decode: query must be bf16 or fp16")
-    if (key_scale is None) != (value_scale is None):
-        raise ValueError("tree_decode: key_scale and value_scale come together")
-    if key_scale is not None:
-        int8_cache.check_views("tree_decode", key_cache, value_cache, key_scale, value_scale)
-    elif key_cache.dtype != query.dtype or value_cache.dtype != query.dtype:
-        raise NotImplementedError("tree_decode: the cache must have the query's type, or be int8 with scales")
-    if query.dim() != 3 or key_cache.dim() != 4 or value_cache.shape != key_cache.shape or out.shape != query.shape:
-        raise ValueError("tree_decode: inconsistent shapes")
-    T, H, D = query.shape
-    blocks, page, KV, _ = key_cache.shape
-    if key_cache.shape[3] != D or KV == 0 or H % KV:
-        raise ValueError("tree_decode: inconsistent shapes")
-    if query.stride(2) != 1 or key_cache.stride(3) != 1 or value_cache.stride(3) != 1 or out.stride(2) != 1:
-        raise ValueError("tree_decode: the head dimension must be contiguous")
-    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or query_start_loc.dtype != torch.int32:
-        raise ValueError("tree_decode: block_table, seq_lens and query_start_loc must be int32")
-    n = len(seq_lens)
-    if block_table.dim() != 2 or len(block_table) != n or query_start_loc.shape != (n + 1,) or seq_lens.dim() != 1:
-        raise ValueError("tree_decode: one block-table row and length for each request, and n + 1 starts")
-    if (block_table.shape[1] > 1 and block_table.stride(1) != 1) or not seq_lens.is_contiguous() \
-            or not query_start_loc.is_contiguous():
-        raise ValueError("tree_decode: block_table rows, seq_lens and query_start_loc must be contiguous")
-    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tree_mask.shape != (T,) or not tree_mask.is_contiguous()):
-        raise ValueError("tree_decode: tree_mask must be a contiguous int64 vector, one mask for each node")
-    max_nodes, max_seq_len = int(max_nodes), int(max_seq_len or paged_attn.MAX_LEN)
-    if max_nodes < 0 or max_seq_len < 0:
-        raise ValueError("tree_decode: max_nodes and max_seq_len must be >= 0")
-    if max_nodes > MAX_NODES:
-        raise NotImplementedError(f"tree_decode: at most {MAX_NODES} nodes a request, got {max_nodes}")
-    if T == 0 or n == 0 or max_nodes == 0:
-        return out
-    ws_bytes = _nx.tree_workspace(T, H, D, max_seq_len)
-    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=query.device) if ws_bytes else None
-    st = _nx.strided
-    status = _nx.launch(query.device, L.vxa_tree_decode, *st(query, 0, 1), _nx.dtype_enum(query.dtype),
-                        *st(key_cache, 0, 1, 2), *st(value_cache, 0, 1, 2), *st(key_scale, 0, 1, 2), *st(value_scale, 0, 1, 2),
-                        blocks, page, *st(block_table, 0), block_table.shape[1], seq_lens.data_ptr(),
-                        query_start_loc.data_ptr(), _nx.ptr(tree_mask), float(scale), out.data_ptr(),
-                        _nx.dtype_enum(out.dtype), out.stride(0), out.stride(1), n, T, H, KV, D, max_nodes, max_seq_len,
-                        _nx.ptr(ws), ws_bytes)
+    status = (_nx._calls or _nx.calls()).tree_decode(
+        query, key_cache, value_cache, block_table, seq_lens, query_start_loc, tree_mask, scale, out, max_nodes,
+        max_seq_len or paged_attn.MAX_LEN, key_scale, value_scale, _nx.stream_of(query))
     if status:
         _nx.check(status, "tree_decode")
     return out
