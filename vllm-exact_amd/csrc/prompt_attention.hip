@@ -44,7 +44,7 @@ struct PromptParams {
   void* out;
   int64_t sot, soh;
   int32_t out_dtype;
-  bool out_wide;  // the output has the input's type and its rows start on 8 bytes
+  bool out_wide;  // the output has the input's type and its rows start on 16 bytes
 };
 
 // Sums and maxima of values >= 0 over the wave.
@@ -288,37 +288,50 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
   const bool careful = __syncthreads_or(odd != 0.0f);
   if (careful) {
     start();
-    for (t = 0; t < tiles; ++t) step(t, std::true_type{}, std::true_type{});
+    for (t = 0; t < full; ++t) step(t, std::false_type{}, std::false_type{});
+    for (; t < tiles; ++t) step(t, std::true_type{}, std::true_type{});
   }
   float la = (l[0] + l[1]) + (l[2] + l[3]), lb = la;
   swap32(la, lb);
   const float inv = 1.0f / (la + lb);
   if (row >= len) return;
-  const int64_t at = (int64_t)(base + row) * p.sot + (int64_t)head * p.soh + 4 * half;
+  const int64_t at = (int64_t)(base + row) * p.sot + (int64_t)head * p.soh;
 #pragma unroll
   for (int i = 0; i < DB; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      float o[4];
+    for (int r0 = 0; r0 < 16; r0 += 8) {
+      uint32_t w[2][2];  // dims 32 i + 2 r0 + 8 k + 4 half + 0..3
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = acc[i][r + j] * inv;
-      if (careful) {
+      for (int k = 0; k < 2; ++k) {
+        float o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = acc[i][r0 + 4 * k + j] * inv;
+        const int dim = 32 * i + 2 * r0 + 8 * k + 4 * half;
+        if (careful) {
 #pragma unroll 1
-        for (int key = 0; key <= row; ++key) {
-          const v2u32 w = *reinterpret_cast<const v2u32*>(vh + key * svt + 64 * i + 4 * r + 8 * half);
+          for (int key = full * kKeys; key <= row; ++key) {
+            const v2u32 x = *reinterpret_cast<const v2u32*>(vh + key * svt + 2 * dim);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float f = T::to_f32((uint16_t)(w[j / 2] >> (16 * (j % 2))));
-            if (!__builtin_isfinite(f)) o[j] += f;
+            for (int j = 0; j < 4; ++j) {
+              const float f = T::to_f32((uint16_t)(x[j / 2] >> (16 * (j % 2))));
+              if (!__builtin_isfinite(f)) o[j] += f;
+            }
           }
         }
-      }
-      const int64_t to = at + 32 * i + 2 * r;
-      if (p.out_wide) {
-        reinterpret_cast<v2u32*>(reinterpret_cast<uint16_t*>(p.out) + to)[0] = v2u32{T::pack(o[0], o[1]), T::pack(o[2], o[3])};
-      } else {
+        w[k][0] = T::pack(o[0], o[1]), w[k][1] = T::pack(o[2], o[3]);
+        if (!p.out_wide) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) store_f32_as(p.out, p.out_dtype, to + j, o[j]);
+          for (int j = 0; j < 4; ++j) store_f32_as(p.out, p.out_dtype, at + dim + j, o[j]);
+        }
+      }
+      if (p.out_wide) {  // 8 dims a lane: the halves exchange what the other stores
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const auto x = __builtin_amdgcn_permlane32_swap(w[0][j], w[1][j], false, false);
+          w[0][j] = x[0], w[1][j] = x[1];
+        }
+        *reinterpret_cast<v4u32*>(reinterpret_cast<uint16_t*>(p.out) + at + 32 * i + 2 * r0 + 8 * half) =
+            v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
       }
     }
 }
@@ -369,7 +382,7 @@ extern "C" int vxa_prompt_attention(const void* q, int64_t sqt, int64_t sqh, con
   // At most this many tiles: each sequence's last one may be part filled.
   p.tiles = (int32_t)std::min<int64_t>(cdiv<int64_t>(tokens, p.rows) + n, tokens);
   p.out = out, p.sot = sot, p.soh = soh, p.out_dtype = out_dtype;
-  p.out_wide = out_dtype == dtype && (uintptr_t)out % 8 == 0 && sot % 4 == 0 && soh % 4 == 0;
+  p.out_wide = out_dtype == dtype && (uintptr_t)out % 16 == 0 && sot % 8 == 0 && soh % 8 == 0;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const hipError_t err = dtype == VXA_BF16 ? launch_prompt<BF16>(head_dim, p, st) : launch_prompt<FP16>(head_dim, p, st);
   if (err == hipErrorInvalidConfiguration) return VXA_ERR_UNSUPPORTED;
