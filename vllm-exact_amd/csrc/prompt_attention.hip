@@ -150,13 +150,6 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
 
   const int wrow = row0 + wave / p.heads * 32;  // the wave's first row
   const int row = wrow + col;
-  v4u32 qf[QS];
-  {
-    const uint16_t* q = p.q + (int64_t)(base + min(row, len - 1)) * p.sqt + (int64_t)head * p.sqh + 8 * half;
-#pragma unroll
-    for (int i = 0; i < QS; ++i) qf[i] = (*reinterpret_cast<const v4u32*>(q + 16 * i) & p.q_and) ^ p.q_xor;
-  }
-
   const int last = min(row0 + p.rows, len);  // keys of the workgroup
   const int tiles = (last + kKeys - 1) / kKeys;
 
@@ -193,6 +186,22 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
   float m, l[4];
   v16f acc[DB];
 
+  const int full = min((wrow + 1) / kKeys, tiles);  // tiles without masked keys
+  auto start = [&] {
+    m = kLowest;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l[i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DB; ++i) acc[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    load(0, 0);
+  };
+  start();
+  v4u32 qf[QS];  // after the first tile has been asked for: changing their signs waits for them
+  {
+    const uint16_t* q = p.q + (int64_t)(base + min(row, len - 1)) * p.sqt + (int64_t)head * p.sqh + 8 * half;
+#pragma unroll
+    for (int i = 0; i < QS; ++i) qf[i] = (*reinterpret_cast<const v4u32*>(q + 16 * i) & p.q_and) ^ p.q_xor;
+  }
   // One tile. MASKED: some of its keys may come after some of the wave's rows.
   // CAREFUL: values of keys that some rows do not attend to may be infinities or NaN, and 0 times those is NaN; here they
   // enter the product as 0, and the rows that attend to them add them at the end. The pass that does not look ends with
@@ -267,16 +276,6 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
         acc[i] = T::mfma32(a, pf[c], acc[i]);
       }
   };
-  const int full = min((wrow + 1) / kKeys, tiles);  // tiles without masked keys
-  auto start = [&] {
-    m = kLowest;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) l[i] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < DB; ++i) acc[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-    load(0, 0);
-  };
-  start();
   int t = 0;
   for (; t < full; ++t) step(t, std::false_type{}, std::false_type{});
   for (; t < tiles; ++t) step(t, std::true_type{}, std::false_type{});
