@@ -4,20 +4,23 @@
 // for every row i of every sequence, with groups of G = H / KV query heads on one key/value head.
 //
 // Work split. A workgroup of 4 waves computes 32 rows of four heads of one KV head (64 rows of two, 128 of one where
-// the group has no more), 32 rows of one head a wave, and walks the keys up to its last row in tiles of 64 (32 at 256
-// dims) with one running maximum and sum: every score is computed once and kept in registers. A wave's rows are the
-// columns of S^T = K Q^T (32 x 32 x 16 MFMAs) and of O^T = V^T P^T, so a lane holds scores of one row only, and with the
-// keys of the second product taken in the order in which the first one leaves them in the lane, P goes from one product
-// to the other without leaving the lane. The tiles of K and V are copied straight into LDS, two in turn; V is transposed
-// as it is read from there. Two workgroups share a CU, so that one's softmax runs beside the other's products.
+// the group has no more), 32 rows of one head a wave, and walks the keys up to its last row in tiles of 64 with one running
+// maximum and sum: every score is computed once and kept in registers. A wave's rows are the columns of S^T = K Q^T
+// (32 x 32 x 16 MFMAs) and of O^T = V^T P^T, so a lane holds scores of one row only, and with the keys of the second
+// product taken in the order in which the first one leaves them in the lane, P goes from one product to the other
+// without leaving the lane. The tiles of K and V are copied straight into LDS, two in turn; V is transposed as it is read
+// from there. Two workgroups share a CU. At 256 dims a wave takes 16 rows (below). The workgroups furthest from their
+// sequence's start, which take longest, go first.
 // A row's order of operations depends on its place in its sequence alone, not on the batch.
 //
 // Rounding. Scores, maxima, sums and accumulators are fp32; P is rounded to the 16-bit element type for the second
 // product, an error of the size of the output's own rounding, while its sum takes the fp32 values.
 //
-// Measured (one prompt of 8192 tokens, 32 heads on 8, 128 dims, bf16): 525 us, 1048 TFLOP/s of the scores that count; a
-// large library matrix product reaches 1185 on the same card. The matrix pipes are busy 52 % of the cycles, the vector
-// ALU's softmax takes most of the others, and the clock falls below 2 GHz.
+// What bounds it. One prompt of 8192 tokens (32 heads on 8, 128 dims, bf16) takes 525 us, 1048 TFLOP/s of the scores that
+// count; a large library matrix product reaches 1185 on the same card, and both at a clock well below 2.4 GHz: power. The
+// matrix pipes are busy 52 % of the cycles; the next tile's scores among this one's softmax instructions, in one wave, gave
+// no time back (519 to 540 us). 16 prompts of up to 1024 tokens take 92 us, 577 TFLOP/s: 7 us of every workgroup's 20 go
+// to finding its rows, the first loads and the output.
 
 #include <algorithm>
 #include <cmath>
@@ -26,8 +29,8 @@
 
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kWaves = 4;     // of a workgroup
+constexpr int kWaves256 = 8;  // ... of the kernel for 256 dims
 
 struct PromptParams {
   const uint16_t* q;
@@ -40,7 +43,7 @@ struct PromptParams {
   float scale_log2;  // > 0: the sign and a zero of the scale are in q's elements,
   uint32_t q_and, q_xor;  // (q & q_and) ^ q_xor, so that scaled scores keep the order of the products
   int32_t n, total, H, G, tiles;
-  int32_t heads, rows;  // of a workgroup: heads of one KV head, and rows of each; 4 waves of 32 rows in all
+  int32_t heads, rows;  // of a workgroup: heads of one KV head, and rows of each: a wave's rows are of one head
   void* out;
   int64_t sot, soh;
   int32_t out_dtype;
@@ -116,9 +119,8 @@ __device__ inline Tile find_tile(const PromptParams& p, int tile) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_kernel(PromptParams p) {
-  constexpr int kKeys = D == 256 ? 32 : 64;  // keys of a tile: at 256 dims 64 keys' scores leave too few registers
-  constexpr int KU = kKeys / 32;
+__global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(PromptParams p) {
+  constexpr int kKeys = 64, KU = kKeys / 32;  // keys of a tile, in blocks of 32
   constexpr int QS = D / 16;       // MFMA steps over the head's dims
   constexpr int DB = D / 32;       // 32-dim blocks of O^T
   constexpr int kRow = 2 * D;      // bytes of a key in LDS
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
   constexpr int kPer = 1024 / kRow;                   // keys that one wave's copy moves
   constexpr int kRound = kPer * kWaves;               // ... that all waves' copies move
   constexpr int kCopies = kKeys / kRound;             // copies of a wave for a tile of K, and of V
-  constexpr int kBases = kRound < 16 && D > 64 ? 16 / kRound : 1;  // copies after which K's swizzle repeats
+  static_assert(kRound % 16 == 0);                    // K's swizzle is the same for every copy of a wave
   __shared__ __attribute__((aligned(1024))) char s_kv[2][2][kTileBytes];  // [buffer][K, V][key][16-byte chunk, swizzled]
   auto swk = [](int key) { return key_swizzle<D>(key); };
   auto swv = [](int key) { return value_swizzle<D>(key); };
@@ -155,9 +157,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
 
   // Tiles go straight from memory into LDS. Copy i of a wave moves keys i * kRound + wave * kPer + [0, kPer).
   const int key_l = wave * kPer + lane / (kRow / 16), chunk = lane % (kRow / 16);
-  const char* ksrc[kBases];
-#pragma unroll
-  for (int i = 0; i < kBases; ++i) ksrc[i] = kh + (key_l + i * kRound) * skt + 16 * (chunk ^ swk(key_l + i * kRound));
+  const char* ksrc = kh + key_l * skt + 16 * (chunk ^ swk(key_l));
   const char* vsrc = vh + key_l * svt + 16 * (chunk ^ swv(key_l));
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t*)&s_kv[0][0][0]) + wave * 1024;
   auto load = [&](int t, int buf) {
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
     if ((t + 1) * kKeys <= len) {
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
-        copy_to_lds(ksrc[i % kBases] + (int64_t)(t * kKeys + i / kBases * kBases * kRound) * skt, dst + i * kWaves * 1024);
+        copy_to_lds(ksrc + (int64_t)(t * kKeys + i * kRound) * skt, dst + i * kWaves * 1024);
         copy_to_lds(vsrc + (int64_t)(t * kKeys + i * kRound) * svt, dst + kTileBytes + i * kWaves * 1024);
       }
     } else {  // keys past the sequence's end repeat its last one
@@ -335,18 +335,218 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_attention_k
     }
 }
 
+// The same for 256 dims, with 8 waves of 16 rows and 16 x 16 x 32 MFMAs: 32 rows of a wave take 430 registers and leave one
+// wave a SIMD, whose softmax and products follow each other; 16 rows take 201 and leave two, though each reads K and V from
+// LDS for half as many rows. Three prompts of up to 2111 tokens: 119 us -> 90; one of 5000: 650 -> 466 (879 TFLOP/s). With
+// 64 or 128 dims, where two waves of 32 rows fit, they are faster (8192 tokens, 128 dims: 525 us against 575).
 template <typename T>
-hipError_t launch_prompt(int64_t D, const PromptParams& p, hipStream_t st) {
-  const int64_t blocks = (int64_t)p.tiles * (p.H / p.heads);
-  if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)blocks), threads(kThreads);
-  if (D == 64)
-    hipLaunchKernelGGL((prompt_attention_kernel<T, 64>), grid, threads, 0, st, p);
-  else if (D == 128)
-    hipLaunchKernelGGL((prompt_attention_kernel<T, 128>), grid, threads, 0, st, p);
-  else
-    hipLaunchKernelGGL((prompt_attention_kernel<T, 256>), grid, threads, 0, st, p);
-  return hipGetLastError();
+__global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256(PromptParams p) {
+  constexpr int D = 256, NW = kWaves256;
+  constexpr int kKeys = 32;
+  constexpr int KT = kKeys / 16;   // 16-key blocks of S^T
+  constexpr int QS = D / 32;       // MFMA steps over the head's dims
+  constexpr int DB = D / 16;       // 16-dim blocks of O^T
+  constexpr int kRow = 2 * D, kTileBytes = kKeys * kRow;
+  constexpr int kPer = 1024 / kRow, kRound = kPer * NW, kCopies = kKeys / kRound;
+  static_assert(kRound == 16);     // K's swizzle is the same for every copy of a wave
+  __shared__ __attribute__((aligned(1024))) char s_kv[2][2][kTileBytes];
+  auto swk = [](int key) { return key_swizzle<D>(key); };
+  // Here 16 lanes read two chunks of four keys, and 64 lanes of 16: eight keys meet the 256 bytes of the banks.
+  auto swv = [](int key) { return 2 * (key & 7); };
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int groups = p.H / p.heads;
+  const int x = (int)(blockIdx.x % groups);
+  const int head = (groups % 8 == 0 ? (x % 8) * (groups / 8) + x / 8 : x) * p.heads + wave % p.heads;
+  const Tile tile = find_tile(p, (int)(blockIdx.x / groups));
+  if (tile.len == 0) return;
+  const int base = __builtin_amdgcn_readfirstlane(tile.base);
+  const int len = __builtin_amdgcn_readfirstlane(tile.len);
+  const int row0 = __builtin_amdgcn_readfirstlane(tile.row0);
+  const char* kh = reinterpret_cast<const char*>(p.k + (int64_t)base * p.skt + (int64_t)(head / p.G) * p.skh);
+  const char* vh = reinterpret_cast<const char*>(p.v + (int64_t)base * p.svt + (int64_t)(head / p.G) * p.svh);
+  const int64_t skt = 2 * p.skt, svt = 2 * p.svt;
+  const int wrow = row0 + wave / p.heads * 16;  // the wave's first row
+  const int row = wrow + col;
+  const int last = min(row0 + p.rows, len);  // keys of the workgroup
+  const int tiles = (last + kKeys - 1) / kKeys;
+
+  const int key_l = wave * kPer + lane / (kRow / 16), chunk = lane % (kRow / 16);
+  const char* ksrc = kh + key_l * skt + 16 * (chunk ^ swk(key_l));
+  const char* vsrc = vh + key_l * svt + 16 * (chunk ^ swv(key_l));
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t*)&s_kv[0][0][0]) + wave * 1024;
+  auto load = [&](int t, int buf) {
+    const uint32_t dst = lds0 + buf * 2 * kTileBytes;
+    if ((t + 1) * kKeys <= len) {
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        copy_to_lds(ksrc + (int64_t)(t * kKeys + i * kRound) * skt, dst + i * NW * 1024);
+        copy_to_lds(vsrc + (int64_t)(t * kKeys + i * kRound) * svt, dst + kTileBytes + i * NW * 1024);
+      }
+    } else {  // keys past the sequence's end repeat its last one
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int in_tile = i * kRound + key_l, key = min(t * kKeys + in_tile, len - 1);
+        copy_to_lds(kh + key * skt + 16 * (chunk ^ swk(in_tile)), dst + i * NW * 1024);
+        copy_to_lds(vh + key * svt + 16 * (chunk ^ swv(in_tile)), dst + kTileBytes + i * NW * 1024);
+      }
+    }
+  };
+
+  // Where this lane reads: K's row `col` of a 16-key block, V's rows 4 grp + col / 4 and 16 further.
+  const int vkey = 4 * grp + col / 4;
+  const int vbyte = vkey * kRow + 8 * (lane & 1);
+  const int full = min((wrow + 1) / kKeys, tiles);  // tiles without masked keys
+  float m, l;
+  v4f acc[DB];
+  auto start = [&] {
+    m = kLowest, l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < DB; ++e) acc[e] = v4f{0, 0, 0, 0};
+    load(0, 0);
+  };
+  start();
+  v4u32 qf[QS];
+  {
+    const uint16_t* q = p.q + (int64_t)(base + min(row, len - 1)) * p.sqt + (int64_t)head * p.sqh + 8 * grp;
+#pragma unroll
+    for (int i = 0; i < QS; ++i) qf[i] = (*reinterpret_cast<const v4u32*>(q + 32 * i) & p.q_and) ^ p.q_xor;
+  }
+  auto step = [&](int t, auto masked_c, auto careful_c) {
+    constexpr bool MASKED = decltype(masked_c)::value, CAREFUL = decltype(careful_c)::value;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int buf = t & 1;
+    if (t + 1 < tiles) load(t + 1, buf ^ 1);
+    const int key0 = t * kKeys;
+    if (MASKED && key0 > wrow + 15) return;
+    const char* kt = s_kv[buf][0] + col * kRow;
+    const char* vt = s_kv[buf][1] + vbyte;
+    v4f s[KT];
+#pragma unroll
+    for (int u = 0; u < KT; ++u) s[u] = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < QS; ++i)
+#pragma unroll
+      for (int u = 0; u < KT; ++u)
+        s[u] = T::mfma16(*reinterpret_cast<const v4u32*>(kt + 16 * u * kRow + 16 * ((4 * i + grp) ^ swk(col))), qf[i], s[u]);
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int u = 0; u < KT; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (key0 + 16 * u + 4 * grp + r > row) s[u][r] = kNegInf;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int u = 0; u < KT; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, s[u][r]);
+    top = rows_max(top) * p.scale_log2;
+    if (__any(top > m + kSlack)) {
+      const float mn = fmaxf(m, top);
+      const float c = exp2_hw(m - mn);
+      l *= c;
+#pragma unroll
+      for (int e = 0; e < DB; ++e) acc[e] = acc[e] * c;
+      m = mn;
+    }
+    v4u32 pf[KT / 2];
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < KT; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const float a = exp2_hw(fmaf(s[u][r], p.scale_log2, -m)), b = exp2_hw(fmaf(s[u][r + 1], p.scale_log2, -m));
+        sum[0] += a;
+        sum[1] += b;
+        pf[u / 2][2 * (u % 2) + r / 2] = T::pack(a, b);
+      }
+    l += sum[0] + sum[1];
+#pragma unroll
+    for (int c = 0; c < KT / 2; ++c)
+#pragma unroll
+      for (int e = 0; e < DB; ++e) {
+        const char* at = vt + 32 * c * kRow + 16 * ((2 * e + (lane & 3) / 2) ^ swv(vkey));
+        const v2u32 lo = read_transposed(at), hi = read_transposed(at + 16 * kRow);
+        v4u32 a = {lo.x, lo.y, hi.x, hi.y};
+        if constexpr (CAREFUL) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) a[j] = only_finite<T>(a[j]);
+        }
+        acc[e] = T::mfma16(a, pf[c], acc[e]);
+      }
+  };
+  int t = 0;
+  for (; t < full; ++t) step(t, std::false_type{}, std::false_type{});
+  for (; t < tiles; ++t) step(t, std::true_type{}, std::false_type{});
+  float odd = 0.0f;  // 0 where all sums are finite, else NaN
+#pragma unroll
+  for (int e = 0; e < DB; ++e)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) odd = fmaf(acc[e][r], 0.0f, odd);
+  const bool careful = __syncthreads_or(odd != 0.0f);
+  if (careful) {
+    start();
+    for (t = 0; t < full; ++t) step(t, std::false_type{}, std::false_type{});
+    for (; t < tiles; ++t) step(t, std::true_type{}, std::true_type{});
+  }
+  const float inv = 1.0f / rows_sum(l);
+  if (row >= len) return;
+  const int64_t at = (int64_t)(base + row) * p.sot + (int64_t)head * p.soh;
+#pragma unroll
+  for (int e0 = 0; e0 < DB; e0 += 2) {
+    uint32_t w[2][2];  // dims 16 (e0 + k) + 4 grp + 0..3
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = acc[e0 + k][j] * inv;
+      const int dim = 16 * (e0 + k) + 4 * grp;
+      if (careful) {
+#pragma unroll 1
+        for (int key = full * kKeys; key <= row; ++key) {
+          const v2u32 v = *reinterpret_cast<const v2u32*>(vh + key * svt + 2 * dim);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float f = T::to_f32((uint16_t)(v[j / 2] >> (16 * (j % 2))));
+            if (!__builtin_isfinite(f)) o[j] += f;
+          }
+        }
+      }
+      w[k][0] = T::pack(o[0], o[1]), w[k][1] = T::pack(o[2], o[3]);
+      if (!p.out_wide) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) store_f32_as(p.out, p.out_dtype, at + dim + j, o[j]);
+      }
+    }
+    if (p.out_wide) {  // 8 dims a lane: neighbouring groups exchange what the other stores
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const auto y = __builtin_amdgcn_permlane16_swap(w[0][j], w[1][j], false, false);
+        w[0][j] = y[0], w[1][j] = y[1];
+      }
+      *reinterpret_cast<v4u32*>(reinterpret_cast<uint16_t*>(p.out) + at + 16 * (e0 + (grp & 1)) + 4 * (grp & 2)) =
+          v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
+    }
+  }
+}
+
+template <typename T>
+hipError_t launch_prompt(int64_t D, PromptParams p, hipStream_t st) {
+  auto launch = [&](auto kernel, int waves, int rows) {
+    p.rows = rows * waves / p.heads;
+    // At most this many tiles: each sequence's last one may be part filled.
+    p.tiles = (int32_t)std::min<int64_t>(cdiv<int64_t>(p.total, p.rows) + p.n, p.total);
+    const int64_t blocks = (int64_t)p.tiles * (p.H / p.heads);
+    if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * waves), 0, st, p);
+    return hipGetLastError();
+  };
+  if (D == 64) return launch(prompt_attention_kernel<T, 64>, kWaves, 32);
+  if (D == 128) return launch(prompt_attention_kernel<T, 128>, kWaves, 32);
+  return launch(prompt_attention_kernel_256<T>, kWaves256, 16);
 }
 
 }  // namespace
@@ -377,9 +577,6 @@ extern "C" int vxa_prompt_attention(const void* q, int64_t sqt, int64_t sqh, con
   p.q_xor = scale < 0.0f ? 0x80008000u : 0u;
   p.n = (int32_t)n, p.total = (int32_t)tokens, p.H = (int32_t)num_heads, p.G = (int32_t)(num_heads / num_kv_heads);
   p.heads = p.G % 4 == 0 ? 4 : p.G % 2 == 0 ? 2 : 1;
-  p.rows = 32 * kWaves / p.heads;
-  // At most this many tiles: each sequence's last one may be part filled.
-  p.tiles = (int32_t)std::min<int64_t>(cdiv<int64_t>(tokens, p.rows) + n, tokens);
   p.out = out, p.sot = sot, p.soh = soh, p.out_dtype = out_dtype;
   p.out_wide = out_dtype == dtype && (uintptr_t)out % 16 == 0 && sot % 8 == 0 && soh % 8 == 0;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
