@@ -1,7 +1,7 @@
 """Causal attention over whole prompts with a fixed reduction order on MI355X.
 
 Kernel (libvllm_exact_amd.so, prompt_attention.hip): sequences of different lengths, their rows packed one after the
-other as vLLM passes them, grouped heads, bf16 or fp16. Scores, the softmax and all sums are fp32 and every score is
+other as vLLM passes them, grouped heads, bf16 or fp16, heads of 64, 128 or 256 dims. Scores, the softmax and all sums are fp32 and every score is
 computed once, on the matrix cores. A row's bits depend on its own sequence only, never on the rest of the batch.
 """
 import torch
