@@ -62,6 +62,25 @@ def test_one_strand_or_a_group_a_workgroup(int8, length):
     assert torch.equal(trees.run(many), out.repeat(n, 1, 1))
 
 
+@pytest.mark.parametrize("n", [60, 130, 260, 300])
+def test_large_batches_of_every_kind_of_request(n):
+    """Requests of one to four segments past whole groups, empty ones, misfits and requests of many rows, in batches whose
+    workgroups go by size (up to 256 requests) and beyond: each as it is alone."""
+    kinds = [(2600, 1), (6000, 2), (0, 0), (5, 3), (2047, 1), (2048, 1), (4096, 64), (8191, 1), (3000, 30), (700, 4)]
+    ctx, nodes = [k[0] for k in kinds], [k[1] for k in kinds]
+    s = trees.make(ctx, nodes, 16, 4, 64, 16, torch.bfloat16, True, seed=11)
+    longest = 8000  # the eighth is beyond it
+    want = trees.run(s, longest=longest)
+    starts = s["qsl"].tolist()
+    assert torch.isnan(want[starts[7]:starts[8]]).all() and torch.isfinite(want[:starts[7]]).all()
+    pick = torch.randint(0, len(kinds), (n,), generator=torch.Generator().manual_seed(n)).tolist()
+    rows = torch.cat([torch.arange(starts[i], starts[i + 1]) for i in pick]).to(DEV)
+    many = dict(s, q=s["q"][rows], bt=s["bt"][pick], sl=s["sl"][pick], mask=s["mask"][rows],
+                qsl=torch.tensor([0] + [nodes[i] for i in pick]).cumsum(0).to(torch.int32).to(DEV))
+    out = trees.run(many, longest=longest, max_nodes=64)
+    assert torch.equal(out.nan_to_num(7.0), want[rows].nan_to_num(7.0)) and torch.equal(torch.isnan(out), torch.isnan(want[rows]))
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_specials_of_masked_drafts_among_many_rows(D, dtype):

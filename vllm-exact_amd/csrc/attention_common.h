@@ -67,6 +67,25 @@ __device__ inline float rows_sum(float v) {
   swap32(a, b);
   return a + b;
 }
+// Running sums or maxima of values >= 0 over the lanes of a wave, this lane's included; wave_reduce: over all of them.
+template <int CTRL, int ROWS>
+__device__ inline int from_row(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+template <typename F>
+__device__ inline int wave_scan(int x, F&& f) {
+  x = f(x, from_row<0x111, 0xF>(x));  // the lanes 1, 2, 4 and 8 before, in rows of 16
+  x = f(x, from_row<0x112, 0xF>(x));
+  x = f(x, from_row<0x114, 0xF>(x));
+  x = f(x, from_row<0x118, 0xF>(x));
+  x = f(x, from_row<0x142, 0xA>(x));  // row 0's and 2's last lane to rows 1 and 3
+  return f(x, from_row<0x143, 0xC>(x));  // row 1's last lane to rows 2 and 3
+}
+template <typename F>
+__device__ inline int wave_reduce(int x, F&& f) {
+  return __builtin_amdgcn_readlane(wave_scan(x, f), 63);
+}
+
 template <int N, typename F, int I = 0>
 __device__ inline void static_for(F&& f) {
   if constexpr (I < N) {

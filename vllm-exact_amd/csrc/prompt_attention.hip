@@ -50,22 +50,6 @@ struct PromptParams {
   bool out_wide;  // the output has the input's type and its rows start on 16 bytes
 };
 
-// Sums and maxima of values >= 0 over the wave.
-template <int CTRL, int ROWS>
-__device__ inline int from_row(int x) {
-  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
-}
-template <typename F>
-__device__ inline int wave_reduce(int x, F&& f) {
-  x = f(x, from_row<0x111, 0xF>(x));  // the lanes 1, 2, 4 and 8 before, in rows of 16
-  x = f(x, from_row<0x112, 0xF>(x));
-  x = f(x, from_row<0x114, 0xF>(x));
-  x = f(x, from_row<0x118, 0xF>(x));
-  x = f(x, from_row<0x142, 0xA>(x));  // row 0's and 2's last lane to rows 1 and 3
-  x = f(x, from_row<0x143, 0xC>(x));  // row 1's last lane to rows 2 and 3
-  return __builtin_amdgcn_readlane(x, 63);
-}
-
 // The sequence and rows of tile `tile`. Tiles of p.rows rows are counted from those furthest from their sequence's start,
 // which take longest, over all sequences (256 sequences at a time).
 struct Tile {

@@ -1,5 +1,6 @@
-// The serving operators' calls on torch tensors: argument checks, pointers and strides, and the C entry point, without a Python object per stride. A call of 9 tensors spends 2 us here, where the same checks in Python
-// and a ctypes call of 50 arguments took 15: a decode step makes such calls for every layer.
+// The serving operators' calls on torch tensors: argument checks, pointers and strides, torch's current stream, and the C
+// entry point, without a Python object for every stride. A call of 9 tensors spends 2 us here, where the same checks in
+// Python and a ctypes call of 50 arguments took 15: a decode step makes such calls for every layer.
 //
 // The module holds no code of the kernels: bind() is given the addresses of the loaded library's entry points.
 // Every function returns the entry point's status; what an argument check refuses is raised here.
@@ -7,6 +8,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
 
 #include <string>
 
@@ -51,15 +53,6 @@ int64_t integer(const char* what, PyObject* o) {
   return v;
 }
 
-vxa_stream_t stream_of(PyObject* o) {  // 0: the default stream
-  vxa_stream_t s = PyLong_AsVoidPtr(o);
-  if (!s && PyErr_Occurred()) {
-    PyErr_Clear();
-    refuse("stream", ": expected an address", PyExc_TypeError);
-  }
-  return s;
-}
-
 void check_gpu(const char* what, std::initializer_list<const at::Tensor*> tensors, const char* statement) {
   const at::Tensor* first = *tensors.begin();
   for (const at::Tensor* t : tensors)
@@ -86,12 +79,13 @@ T* ptr(const at::Tensor* t) {
 }
 int64_t stride(const at::Tensor* t, int i) { return t ? t->stride(i) : 0; }
 
-// status = call() with the tensors' device current.
+// status = call(stream) with the tensors' device current and torch's current stream there.
 template <typename F>
 int on_device(const at::Tensor& t, F&& call) {
   const c10::DeviceGuard guard(t.device());
+  const vxa_stream_t stream = c10::hip::getCurrentHIPStream(t.device().index()).stream();
   int status;
-  Py_BEGIN_ALLOW_THREADS status = call();
+  Py_BEGIN_ALLOW_THREADS status = call(stream);
   Py_END_ALLOW_THREADS
   return status;
 }
@@ -121,7 +115,6 @@ void check_table(const char* what, const at::Tensor& t) {
 }
 
 int prompt_attention(PyObject* const* a) {
-  const vxa_stream_t stream = stream_of(a[6]);
   const char* what = "prompt_attention";
   const at::Tensor &q = *tensor(what, a[0]), &k = *tensor(what, a[1]), &v = *tensor(what, a[2]), &cu = *tensor(what, a[3]);
   const double scale = number(what, a[4]);
@@ -138,7 +131,7 @@ int prompt_attention(PyObject* const* a) {
     if (t->size(2) && t->stride(2) != 1) refuse(what, ": the head dimension must be contiguous");
   const int out_dtype = dtype_enum(out);
   if (q.size(0) == 0) return VXA_OK;
-  return on_device(q, [&] {
+  return on_device(q, [&](vxa_stream_t stream) {
     return prompt_attention_fn(ptr(&q), q.stride(0), q.stride(1), ptr(&k), k.stride(0), k.stride(1), ptr(&v), v.stride(0), v.stride(1),
                                dtype_enum(q), ptr<int32_t>(&cu), cu.size(0) - 1, q.size(0), (float)scale, ptr(&out), out_dtype,
                                out.stride(0), out.stride(1), q.size(1), k.size(1), q.size(2), stream);
@@ -146,7 +139,6 @@ int prompt_attention(PyObject* const* a) {
 }
 
 int write_cache(PyObject* const* a) {
-  const vxa_stream_t stream = stream_of(a[7]);
   const char* what = "write_cache";
   const at::Tensor &k = *tensor(what, a[0]), &v = *tensor(what, a[1]);
   const Cache c{tensor(what, a[2]), tensor(what, a[3]), tensor(what, a[4]), tensor(what, a[5])};
@@ -158,7 +150,7 @@ int write_cache(PyObject* const* a) {
   const int dtype = dtype_enum(k);
   if (k.size(0) == 0) return VXA_OK;
   const at::Tensor &kc = *c.key, &vc = *c.value, &ks = *c.key_scale, &vs = *c.value_scale;
-  return on_device(k, [&] {
+  return on_device(k, [&](vxa_stream_t stream) {
     return cache_write_fn(ptr(&k), k.stride(0), k.stride(1), ptr(&v), v.stride(0), v.stride(1), dtype, k.size(0), k.size(1), k.size(2),
                           ptr<int8_t>(&kc), kc.stride(0), kc.stride(1), kc.stride(2), ptr<int8_t>(&vc), vc.stride(0), vc.stride(1),
                           vc.stride(2), ptr<float>(&ks), ks.stride(0), ks.stride(1), ks.stride(2), ptr<float>(&vs), vs.stride(0),
@@ -167,7 +159,6 @@ int write_cache(PyObject* const* a) {
 }
 
 int read_cache(PyObject* const* a) {
-  const vxa_stream_t stream = stream_of(a[9]);
   const char* what = "read_cache";
   const Cache c{tensor(what, a[0]), tensor(what, a[1]), tensor(what, a[2]), tensor(what, a[3])};
   const at::Tensor &bt = *tensor(what, a[4]), &cu = *tensor(what, a[5]), &k = *tensor(what, a[6]), &v = *tensor(what, a[7]);
@@ -182,7 +173,7 @@ int read_cache(PyObject* const* a) {
   const int dtype = dtype_enum(k);
   if (k.size(0) == 0 || n == 0) return VXA_OK;
   const at::Tensor &kc = *c.key, &vc = *c.value, &ks = *c.key_scale, &vs = *c.value_scale;
-  return on_device(k, [&] {
+  return on_device(k, [&](vxa_stream_t stream) {
     return cache_read_fn(ptr<int8_t>(&kc), kc.stride(0), kc.stride(1), kc.stride(2), ptr<int8_t>(&vc), vc.stride(0), vc.stride(1),
                          vc.stride(2), ptr<float>(&ks), ks.stride(0), ks.stride(1), ks.stride(2), ptr<float>(&vs), vs.stride(0),
                          vs.stride(1), vs.stride(2), kc.size(0), kc.size(1), ptr<int32_t>(&bt), bt.stride(0), bt.size(1),
@@ -192,7 +183,6 @@ int read_cache(PyObject* const* a) {
 }
 
 int tree_decode(PyObject* const* a) {
-  const vxa_stream_t stream = stream_of(a[13]);
   const char* what = "tree_decode";
   const at::Tensor& q = *tensor(what, a[0]);
   const Cache c{tensor(what, a[1]), tensor(what, a[2]), tensor(what, a[11], true), tensor(what, a[12], true)};
@@ -229,7 +219,7 @@ int tree_decode(PyObject* const* a) {
   if (rc != VXA_OK) return rc;
   at::Tensor ws;
   if (bytes) ws = at::empty({(int64_t)bytes / 4}, q.options().dtype(at::kFloat));
-  return on_device(q, [&] {
+  return on_device(q, [&](vxa_stream_t stream) {
     const at::Tensor *ks = c.key_scale, *vs = c.value_scale;
     return tree_decode_fn(ptr(&q), q.stride(0), q.stride(1), dtype_enum(q), ptr(&kc), kc.stride(0), kc.stride(1), kc.stride(2), ptr(&vc),
                           vc.stride(0), vc.stride(1), vc.stride(2), ptr<float>(ks), stride(ks, 0), stride(ks, 1), stride(ks, 2),
@@ -240,8 +230,7 @@ int tree_decode(PyObject* const* a) {
   });
 }
 
-// fn(arguments) as a Python function of `count` positional arguments, the last one torch's current stream on the tensors'
-// device; C++ exceptions end here.
+// fn(arguments) as a Python function of `count` positional arguments; C++ exceptions end here.
 template <int (*fn)(PyObject* const*), int count>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t given) {
   if (given != count || !tree_decode_fn) {
@@ -282,10 +271,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t given) {
 
 #define VXA_METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {VXA_METHOD("bind", bind),
-                         VXA_METHOD("prompt_attention", (call<prompt_attention, 7>)),
-                         VXA_METHOD("write_cache", (call<write_cache, 8>)),
-                         VXA_METHOD("read_cache", (call<read_cache, 10>)),
-                         VXA_METHOD("tree_decode", (call<tree_decode, 14>)),
+                         VXA_METHOD("prompt_attention", (call<prompt_attention, 6>)),
+                         VXA_METHOD("write_cache", (call<write_cache, 7>)),
+                         VXA_METHOD("read_cache", (call<read_cache, 9>)),
+                         VXA_METHOD("tree_decode", (call<tree_decode, 13>)),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

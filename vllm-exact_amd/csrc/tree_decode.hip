@@ -47,6 +47,7 @@ constexpr int kMaxNodes = 64;
 constexpr int kWideRows = 96;   // requests with more rows (nodes times heads of a group) take the wide kernel
 constexpr int kFill = 256;      // keys whose places the wide kernel looks up at a time
 constexpr int kManyWorkgroups = 1536;
+constexpr int kSearched = 256;  // requests
 
 struct TreeParams {
   const uint16_t* q;
@@ -69,6 +70,7 @@ struct TreeParams {
   const int64_t* mask;
   float scale_log2;
   int32_t n, total, KV, G, ns, row_blocks, max_nodes, max_len;
+  bool by_size;  // workgroups of whole groups go by their work, the largest first
   bool strands;  // a workgroup for each strand of a group of segments, not for each group
   int64_t parts;  // partial sums of a row: kWaves for each group
   bool out_wide;  // the output has the query's type and its rows start on 8 bytes
@@ -218,6 +220,39 @@ __device__ inline int row_block_of(const TreeParams& p, uint32_t& id) {
   return (int)rb;
 }
 
+// Unit `unit` of the requests' groups, those of four segments first, then those of three, two and one. A request that does
+// not fit the call is one small unit: its rows become NaN.
+struct GroupOf {
+  int request, group;  // request < 0: no such unit
+};
+__device__ inline GroupOf find_group(const TreeParams& p, int unit) {
+  const int lane = threadIdx.x & 63;
+  for (int left = kGroup; left > 0; --left) {
+    for (int j0 = 0; j0 < p.n; j0 += 64) {
+      int count = 0, rest = 0;
+      if (j0 + lane < p.n) {
+        const Request rq = request_of(p, j0 + lane);
+        const int segs = (rq.L + kSeg - 1) / kSeg;
+        rest = rq.bad ? 0 : segs / kGroup;
+        if (rq.T > 0 && rq.bad)
+          count = left == 1;
+        else if (rq.T > 0 && rq.T * p.G <= kWideRows)
+          count = left == kGroup ? segs / kGroup : segs % kGroup == left;
+      }
+      const int sum = wave_scan(count, [](int a, int b) { return a + b; });
+      const int total = __builtin_amdgcn_readlane(sum, 63);
+      if (unit < total) {
+        const int at = __builtin_ctzll(__ballot(sum > unit));
+        // A whole group is counted from its request's first; a part comes after them; a misfit has group 0.
+        const int before = __builtin_amdgcn_readlane(sum - count, at);
+        return GroupOf{j0 + at, left == kGroup ? unit - before : __builtin_amdgcn_readlane(rest, at)};
+      }
+      unit -= total;
+    }
+  }
+  return GroupOf{-1, 0};
+}
+
 // Registers of a lane that live through a tile: sums and queries, and one tile's keys and values. Two workgroups share a
 // CU where those leave room; the next tile is loaded ahead where its registers do not cost that.
 constexpr int lane_regs(int d, int nq, bool int8, int tiles) { return 3 * d * nq / 8 + tiles * d / (int8 ? 4 : 2); }
@@ -249,9 +284,16 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
   const int rb = row_block_of(p, id);
   const int g = (int)(id % (uint32_t)p.KV);
   id /= (uint32_t)p.KV;
-  const int b = (int)(id % (uint32_t)p.n);
-  id /= (uint32_t)p.n;
-  const int group = p.strands ? (int)id / kWaves : (int)id, strand = (int)id % kWaves;  // past the groups: nothing to do
+  int b, group, strand = 0;
+  if (p.by_size) {
+    const GroupOf at = find_group(p, (int)id);
+    if (at.request < 0) return;
+    b = __builtin_amdgcn_readfirstlane(at.request), group = __builtin_amdgcn_readfirstlane(at.group);
+  } else {
+    b = (int)(id % (uint32_t)p.n);
+    id /= (uint32_t)p.n;
+    group = p.strands ? (int)id / kWaves : (int)id, strand = (int)id % kWaves;  // past the groups: nothing to do
+  }
 
   // The pages of the wave's own keys of a segment, tile after tile. They are asked for before the request's length is
   // known: past it, table entries are read and not used.
@@ -296,7 +338,20 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
   // cache does not have makes the request's rows NaN.
   bool bad_page = false;
   float scales[kOwn][2];
+  struct Strides {
+    int64_t kb, kp, vb, vp, ksb, ksp, ksh, vsb, vsp, vsh;
+  };
   auto place = [&](int seg, const int32_t (&pages)[kOwn]) {
+    Strides a;
+    if constexpr (NQ == 2 && D < 256) {
+      // Read again from the arguments: kept through the tiles of 32 rows, they cost more registers than there are.
+      typedef const __attribute__((address_space(4))) TreeParams Args;
+      Args* args = (Args*)__builtin_amdgcn_kernarg_segment_ptr();
+      asm volatile("" : "+s"(args));
+      a = Strides{args->skb, args->skp, args->svb, args->svp, args->sksb, args->sksp, args->sksh, args->svsb, args->svsp, args->svsh};
+    } else {
+      a = Strides{p.skb, p.skp, p.svb, p.svp, p.sksb, p.sksp, p.sksh, p.svsb, p.svsp, p.svsh};
+    }
     const int key0 = seg * kSeg + first * kTile;
     const int32_t page0 = __builtin_amdgcn_readfirstlane(pages[0]);
 #pragma unroll
@@ -309,11 +364,11 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
         bad_page |= key0 < rq.L;
         block = 0;
       }
-      s_koff[wave][64 * i + lane] = block * p.skb + (int64_t)off * p.skp;
-      s_voff[wave][64 * i + lane] = block * p.svb + (int64_t)off * p.svp;
+      s_koff[wave][64 * i + lane] = block * a.kb + (int64_t)off * a.kp;
+      s_voff[wave][64 * i + lane] = block * a.vb + (int64_t)off * a.vp;
       if constexpr (INT8) {
-        scales[i][0] = p.ks[block * p.sksb + (int64_t)off * p.sksp + (int64_t)g * p.sksh];
-        scales[i][1] = p.vs[block * p.svsb + (int64_t)off * p.svsp + (int64_t)g * p.svsh];
+        scales[i][0] = p.ks[block * a.ksb + (int64_t)off * a.ksp + (int64_t)g * a.ksh];
+        scales[i][1] = p.vs[block * a.vsb + (int64_t)off * a.vsp + (int64_t)g * a.vsh];
       }
     }
     wave_sync();
@@ -997,6 +1052,9 @@ hipError_t launch_tree(TreeParams p, hipStream_t st) {
     // order of the sums, and so every bit, is the same.
     const int64_t units = (int64_t)p.KV * p.n, groups = cdiv<int64_t>(p.ns, kGroup);
     p.strands = groups > 1 && units * p.row_blocks * groups < kManyWorkgroups;
+    // The last rounds of workgroups end together where the large ones have gone first. The search takes a turn for every 64
+    // requests, and there are many rounds where they are many.
+    p.by_size = !p.strands && groups > 1 && p.n <= kSearched;
     const int64_t blocks = cdiv<int64_t>(units * groups * (p.strands ? kWaves : 1), 8) * 8 * p.row_blocks;
     if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
     if (nq == 1)
@@ -1100,7 +1158,7 @@ extern "C" int vxa_tree_decode(const void* q, int64_t sqt, int64_t sqh, int q_dt
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
   p.n = (int32_t)n, p.total = (int32_t)tokens, p.KV = (int32_t)num_kv_heads, p.G = (int32_t)(num_heads / num_kv_heads);
   p.ns = (int32_t)ns, p.row_blocks = 1, p.max_nodes = (int32_t)max_nodes, p.max_len = (int32_t)max_seq_len;
-  p.strands = false, p.parts = part_count(max_seq_len);
+  p.strands = false, p.by_size = false, p.parts = part_count(max_seq_len);
   // The weighted values first, on 16 bytes as the workspace is.
   const int64_t parts = tokens * num_heads * p.parts;
   float* w = reinterpret_cast<float*>(ws);

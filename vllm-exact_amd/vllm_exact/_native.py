@@ -202,13 +202,6 @@ def launch(device, fn, *args):
         return fn(*args, stream_handle(device))
 
 
-def stream_of(t):
-    """torch's current stream on the tensor's GPU, as an integer (0 for a CPU tensor)."""
-    if not t.is_cuda:
-        return 0
-    return stream_handle(t.device) if _raw_stream is None else _raw_stream(t.device.index)
-
-
 _calls = None
 _CALLED = ("vxa_prompt_attention", "vxa_int8_cache_write", "vxa_int8_cache_read", "vxa_tree_decode_workspace", "vxa_tree_decode")
 

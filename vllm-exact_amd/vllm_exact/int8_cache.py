@@ -25,8 +25,7 @@ def write_cache(key, value, key_cache, value_cache, key_scale, value_scale, slot
     """Quantise key and value (tokens, KV, D; fp32, bf16 or fp16) into the slots slot_mapping (tokens,) int64, a slot
     being block * block_size + place (vLLM's slot mapping). Slots outside the cache (-1: padding) are skipped; two tokens
     of one call never share a slot."""
-    status = (_nx._calls or _nx.calls()).write_cache(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping,
-                                                     _nx.stream_of(key))
+    status = (_nx._calls or _nx.calls()).write_cache(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
     if status:
         _nx.check(status, "write_cache")
 
@@ -37,7 +36,7 @@ def read_cache(key_cache, value_cache, key_scale, value_scale, block_table, cu_s
     from its start), whose blocks are block_table[i]. A row past the block table or on a block outside the cache is NaN;
     rows of no sequence are left alone. cu_seqlens (n + 1,) and first (n,) are int32 on the GPU."""
     status = (_nx._calls or _nx.calls()).read_cache(key_cache, value_cache, key_scale, value_scale, block_table, cu_seqlens, key,
-                                                    value, first, _nx.stream_of(key))
+                                                    value, first)
     if status:
         _nx.check(status, "read_cache")
     return key, value

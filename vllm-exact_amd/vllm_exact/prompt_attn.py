@@ -14,7 +14,7 @@ def prompt_attention(query, key, value, cu_seqlens, scale, out):
     [cu_seqlens[i], cu_seqlens[i + 1]) holds t; cu_seqlens (n + 1,) int32 on the GPU (vLLM's query_start_loc); out
     (tokens, H, D) fp32, bf16 or fp16. Row j of a sequence attends to its rows 0..j. Rows and heads may be strided (views of
     a fused projection), D is 64, 128 or 256 and contiguous. Rows after cu_seqlens[n] are left alone. Returns out."""
-    status = (_nx._calls or _nx.calls()).prompt_attention(query, key, value, cu_seqlens, scale, out, _nx.stream_of(query))
+    status = (_nx._calls or _nx.calls()).prompt_attention(query, key, value, cu_seqlens, scale, out)
     if status:
         _nx.check(status, "prompt_attention")
     return out

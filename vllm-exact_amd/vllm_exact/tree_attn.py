@@ -24,7 +24,7 @@ def tree_decode(query, key_cache, value_cache, block_table, seq_lens, query_star
     request: one beyond them, or shorter than its nodes, or with a block outside the cache, gets NaN rows. Returns out."""
     status = (_nx._calls or _nx.calls()).tree_decode(
         query, key_cache, value_cache, block_table, seq_lens, query_start_loc, tree_mask, scale, out, max_nodes,
-        max_seq_len or paged_attn.MAX_LEN, key_scale, value_scale, _nx.stream_of(query))
+        max_seq_len or paged_attn.MAX_LEN, key_scale, value_scale)
     if status:
         _nx.check(status, "tree_decode")
     return out
