@@ -27,10 +27,10 @@
 // cache always takes bf16 parts there, because P vscale can leave the fp16 range.
 //
 // What bounds it (32 heads on 8, 128 dims). 64 requests of up to 8192 keys with one token, 16-bit cache: 330 us, 6.5 TB/s,
-// the rate of reading. With 8 tokens and the 8-bit cache: 216 us, 3.9 TB/s of half the bytes. There a tile of 32 keys costs a
-// wave some 430 vector instructions, 192 of them to make 16-bit operands of its bytes, and 48 MFMAs; 242 registers leave
-// two waves a SIMD. With loads alone the same kernel takes 186 us. One request of 16384 keys and one token: 15.6 us, a
-// chain of dependent loads and four tiles (10) and a second launch for the merge (4.7).
+// the rate of reading. With 8 tokens and the 8-bit cache: 195 us, 4.3 TB/s of half the bytes. There a tile of 32 keys costs a
+// wave some 430 vector instructions, 192 of them to make 16-bit operands of its bytes, and 48 MFMAs; 245 registers leave
+// two waves a SIMD. One request of 16384 keys and one token: 14.5 us, a chain of dependent loads and four tiles (10) and a
+// second launch for the merge (4).
 
 #include <algorithm>
 
@@ -46,7 +46,7 @@ constexpr int kWaveKeys = kSeg / kWaves;
 constexpr int kMaxNodes = 64;
 constexpr int kWideRows = 96;   // requests with more rows (nodes times heads of a group) take the wide kernel
 constexpr int kFill = 256;      // keys whose places the wide kernel looks up at a time
-constexpr int kManyWorkgroups = 1536;
+constexpr int kManyWorkgroups = 256;  // of whole groups: one a CU
 constexpr int kSearched = 256;  // requests
 
 struct TreeParams {
@@ -1048,8 +1048,9 @@ hipError_t launch_tree(TreeParams p, hipStream_t st) {
   {
     const int nq = narrow <= 16 ? 1 : 2;
     p.row_blocks = (int32_t)std::max<int64_t>(1, cdiv<int64_t>(narrow, 16 * nq));
-    // A workgroup for each group of segments, or for each of its strands where the former would not fill the GPU. The
-    // order of the sums, and so every bit, is the same.
+    // A workgroup for each group of segments, or for each of its strands where the former would leave CUs without one. The
+    // order of the sums, and so every bit, is the same. (10 requests of up to 8000 keys, 8 tokens, 320 groups: 54 us in
+    // strands, 45 in groups; 20 of up to 16384, 2 tokens, 1440 groups: 118 and 98; with 256 the same.)
     const int64_t units = (int64_t)p.KV * p.n, groups = cdiv<int64_t>(p.ns, kGroup);
     p.strands = groups > 1 && units * p.row_blocks * groups < kManyWorkgroups;
     // The last rounds of workgroups end together where the large ones have gone first. The search takes a turn for every 64
