@@ -14,7 +14,7 @@
 // second product is chosen so that the lane's own scores are its operand: P is never exchanged between lanes.
 // V is loaded by rows, each lane 8 keys of the same D / 16 dims, and transposed in registers, one byte permute
 // for every two elements. K and V go from HBM to registers; LDS holds the places and scales of a segment's keys and the
-// sums that are folded. Requests of more than kWideRows rows take a kernel that shares tiles of K and V through LDS (below).
+// sums that are folded. Requests of more than wide_rows(D) rows take a kernel that shares tiles of K and V through LDS (below).
 //
 // Order. Keys are cut into segments of kSeg and groups of kGroup segments. Strand w of a segment, its 32-key tiles w,
 // w + 4, ..., is summed with one running maximum; the segments of a strand are folded in order, the four strands of a
@@ -44,7 +44,12 @@ constexpr int kTile = 32;    // keys of a wave's step
 constexpr int kWaves = 4;
 constexpr int kWaveKeys = kSeg / kWaves;
 constexpr int kMaxNodes = 64;
-constexpr int kWideRows = 96;   // requests with more rows (nodes times heads of a group) take the wide kernel
+// Requests with more rows (nodes times heads of a group) take the wide kernel. 128 dims: 96 and 64 are alike from 97 rows on,
+// 80 rows of 16 requests took 50 us in the narrow kernel and 64 in the wide one. 256 dims, where the narrow kernel has one
+// wave a SIMD for 32 rows: 107 requests of 72 to 144 rows 150 us wide from 33 rows on, 196 from 97 on; 8 of 24 rows
+// 70 us narrow, 104 wide.
+constexpr int wide_rows(int d) { return d == 256 ? 32 : 96; }
+constexpr int kWaves256 = 8;    // of its workgroups at 256 dims
 constexpr int kFill = 256;      // keys whose places the wide kernel looks up at a time
 constexpr int kManyWorkgroups = 256;  // of whole groups: one a CU
 constexpr int kSearched = 256;  // requests
@@ -69,7 +74,7 @@ struct TreeParams {
   const int32_t* qsl;
   const int64_t* mask;
   float scale_log2;
-  int32_t n, total, KV, G, ns, row_blocks, max_nodes, max_len;
+  int32_t n, total, KV, G, ns, row_blocks, max_nodes, max_len, wide_rows;
   bool by_size;  // workgroups of whole groups go by their work, the largest first
   bool strands;  // a workgroup for each strand of a group of segments, not for each group
   int64_t parts;  // partial sums of a row: kWaves for each group
@@ -236,7 +241,7 @@ __device__ inline GroupOf find_group(const TreeParams& p, int unit) {
         rest = rq.bad ? 0 : segs / kGroup;
         if (rq.T > 0 && rq.bad)
           count = left == 1;
-        else if (rq.T > 0 && rq.T * p.G <= kWideRows)
+        else if (rq.T > 0 && rq.T * p.G <= p.wide_rows)
           count = left == kGroup ? segs / kGroup : segs % kGroup == left;
       }
       const int sum = wave_scan(count, [](int a, int b) { return a + b; });
@@ -313,7 +318,7 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
   for (int i = 0; i < kOwn; ++i) asm volatile("" : "+v"(pages[i]));
   const int rows = rq.T * p.G;
   const int row0 = rb * 16 * NQ;
-  if (row0 >= rows || (rows > kWideRows && !rq.bad)) return;
+  if (row0 >= rows || (rows > p.wide_rows && !rq.bad)) return;
   const int H = p.KV * p.G;
   if (rq.bad) {
     if (group == 0 && rb == 0 && (!p.strands || strand == 0))
@@ -694,14 +699,14 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
 // Keys of a workgroup of the wide kernel, by the request's own length: more of them halve the partial sums.
 __device__ __host__ inline int wide_chunk(int keys) { return keys <= 4096 ? kSeg : 2 * kSeg; }
 
-// Requests of more than kWideRows rows. A workgroup takes 128 rows of a (request, KV head), 32 a wave, and a chunk of
+// Requests of more than wide_rows(D) rows. A workgroup takes 128 rows of a (request, KV head), 32 a wave, and a chunk of
 // keys in tiles that its waves share through LDS, as 16-bit elements: a key is converted once for 128 rows. 32 x 32 x 16
 // MFMAs, otherwise as above: S^T = K Q^T, then O^T = V^T P^T with V transposed by the LDS read. Tiles of a 16-bit cache are
 // copied straight into LDS, those of an 8-bit one through registers, the next tile while one is computed.
 template <typename T, bool INT8, int D>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void tree_decode_kernel_wide(TreeParams p) {
+__global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel_wide(TreeParams p) {
   using PT = std::conditional_t<INT8, BF16, T>;
-  constexpr int kKeys = D == 256 ? 32 : 64, KU = kKeys / 32;
+  constexpr int kKeys = 64, KU = kKeys / 32;
   constexpr int QS = D / 16, DB = D / 32;
   constexpr int kRow = 2 * D, kTileBytes = kKeys * kRow;
   constexpr int kPer = 1024 / kRow, kRound = kPer * kWaves, kCopies = kKeys / kRound;  // as copied: keys of a copy, of a round
@@ -721,7 +726,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void tree_decode_ker
   const int chunk = (int)(id / (uint32_t)p.n);
   const Request rq = request_of(p, b);
   const int rows = rq.T * p.G, row0 = rb * 32 * kWaves;
-  if (rq.bad || rows <= kWideRows || row0 >= rows) return;
+  if (rq.bad || rows <= p.wide_rows || row0 >= rows) return;
   const int keys = wide_chunk(rq.L);
   const int start = chunk * keys, end = min(start + keys, rq.L);
   if (start >= end) return;
@@ -987,6 +992,281 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void tree_decode_ker
     }
 }
 
+// The same for 256 dims, with 8 waves of 16 rows and 16 x 16 x 32 MFMAs: two waves a SIMD, where 32 rows leave one. Six
+// trees of 61 nodes, 488 rows: 45 us where that took 52. (8-bit keys of 128 dims: 199 us this way, 133 with 32 rows.)
+template <typename T, bool INT8>
+__global__ __launch_bounds__(64 * kWaves256, 2) void tree_decode_kernel_wide_256(TreeParams p) {
+  constexpr int D = 256, kThreads = 64 * kWaves256;
+  using PT = std::conditional_t<INT8, BF16, T>;
+  constexpr int kKeys = 32, KT = kKeys / 16;  // keys of a tile, in blocks of 16
+  constexpr int QS = D / 32, DB = D / 16;
+  constexpr int kRow = 2 * D, kTileBytes = kKeys * kRow;
+  constexpr int kPer = 1024 / kRow, kRound = kPer * kWaves256, kCopies = kKeys / kRound;  // as copied: keys of a copy, of a round
+  static_assert(kKeys * D / 16 == kThreads && kFill <= kThreads);  // as converted: a 16-byte piece a thread
+  __shared__ __attribute__((aligned(1024))) char s_kv[2][2][kTileBytes];
+  __shared__ int64_t s_koff[kFill], s_voff[kFill];
+  __shared__ __attribute__((aligned(16))) float s_ks[2][INT8 ? kFill : 4], s_vs[2][INT8 ? kFill : 4];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  uint32_t id;
+  const int rb = row_block_of(p, id);
+  const int g = (int)(id % (uint32_t)p.KV);
+  id /= (uint32_t)p.KV;
+  const int b = (int)(id % (uint32_t)p.n);
+  const int chunk = (int)(id / (uint32_t)p.n);
+  const Request rq = request_of(p, b);
+  const int rows = rq.T * p.G, row0 = rb * 16 * kWaves256;
+  if (rq.bad || rows <= p.wide_rows || row0 >= rows) return;
+  const int keys = wide_chunk(rq.L);
+  const int start = chunk * keys, end = min(start + keys, rq.L);
+  if (start >= end) return;
+  const int ctx = rq.L - rq.T;
+  const int H = p.KV * p.G;
+
+  // Places of kFill keys; those past the last one repeat it.
+  bool bad_page = false;
+  auto page_at = [&](int fill) {
+    const int key = min(start + fill * kFill + (int)threadIdx.x % kFill, end - 1);
+    return p.bt[(int64_t)b * p.sbt + page_of(p, key)];
+  };
+  auto place = [&](int fill, int32_t page) {
+    const int key = min(start + fill * kFill + (int)threadIdx.x % kFill, end - 1);
+    const int off = key - page_of(p, key) * p.page;
+    int64_t block = page;
+    if (block < 0 || block >= p.blocks) {
+      bad_page = true;
+      block = 0;
+    }
+    if (threadIdx.x < kFill) {
+      s_koff[threadIdx.x] = block * p.skb + (int64_t)off * p.skp;
+      s_voff[threadIdx.x] = block * p.svb + (int64_t)off * p.svp;
+      if constexpr (INT8) {
+        s_ks[fill & 1][threadIdx.x] = p.ks[block * p.sksb + (int64_t)off * p.sksp + (int64_t)g * p.sksh] * p.scale_log2;
+        s_vs[fill & 1][threadIdx.x] = p.vs[block * p.svsb + (int64_t)off * p.svsp + (int64_t)g * p.svsh];
+      }
+    }
+    __syncthreads();
+  };
+  int32_t page = page_at(0);
+
+  const int row = min(row0 + 16 * wave + col, rows - 1), node = row / p.G, head = g * p.G + row - node * p.G;
+  v4u32 qf[QS];
+  {
+    const uint16_t* q = p.q + (int64_t)(rq.q0 + node) * p.sqt + (int64_t)head * p.sqh + 8 * grp;
+#pragma unroll
+    for (int i = 0; i < QS; ++i) qf[i] = *reinterpret_cast<const v4u32*>(q + 32 * i);
+  }
+  const uint64_t all = rq.T >= 64 ? ~0ull : (1ull << rq.T) - 1;
+  const uint64_t seen = all & (p.mask != nullptr ? (uint64_t)p.mask[rq.q0 + node] : (2ull << node) - 1);
+
+  const int tiles = (end - start + kKeys - 1) / kKeys;
+  const int plain = min(max(ctx - start, 0) / kKeys, tiles);  // tiles of the context alone
+  const char* kh = p.kc + (int64_t)g * p.skh;
+  const char* vh = p.vc + (int64_t)g * p.svh;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t*)&s_kv[0][0][0]) + wave * 1024;
+  v4u32 kr, vr;
+  const int piece_key = threadIdx.x / (D / 16), piece = threadIdx.x % (D / 16);
+  // 16 lanes read two chunks of four keys of V, 64 lanes of 16: eight keys meet the 256 bytes of the banks.
+  auto swv = [](int key) { return 2 * (key & 7); };
+  auto load = [&](int t) {
+    const int at = t * kKeys % kFill;
+    if constexpr (INT8) {
+      kr = *reinterpret_cast<const v4u32*>(kh + s_koff[at + piece_key] + 16 * piece);
+      vr = *reinterpret_cast<const v4u32*>(vh + s_voff[at + piece_key] + 16 * piece);
+    } else {
+      const uint32_t dst = lds0 + (t & 1) * 2 * kTileBytes;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int key = i * kRound + wave * kPer + lane / (kRow / 16), c = lane % (kRow / 16);
+        copy_to_lds(kh + s_koff[at + key] + 16 * (c ^ key_swizzle<D>(key)), dst + i * kThreads * 16);
+        copy_to_lds(vh + s_voff[at + key] + 16 * (c ^ swv(key)), dst + kTileBytes + i * kThreads * 16);
+      }
+    }
+  };
+  auto store = [&](int t) {
+    if constexpr (INT8) {
+      char* kd = s_kv[t & 1][0] + piece_key * kRow;
+      char* vd = s_kv[t & 1][1] + piece_key * kRow;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          bytes_as<T>(kr[2 * j + e], x[2 * e], x[2 * e + 1]);
+          bytes_as<PT>(vr[2 * j + e], y[2 * e], y[2 * e + 1]);
+        }
+        *reinterpret_cast<v4u32*>(kd + 16 * ((2 * piece + j) ^ key_swizzle<D>(piece_key))) = v4u32{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<v4u32*>(vd + 16 * ((2 * piece + j) ^ swv(piece_key))) = v4u32{y[0], y[1], y[2], y[3]};
+      }
+    }
+  };
+
+  const int vkey = 4 * grp + col / 4;
+  const int vbyte = vkey * kRow + 8 * (lane & 1);
+  float m, l;
+  v4f acc[DB];
+  auto step = [&](int t, auto drafted_c, auto careful_c) {
+    constexpr bool DRAFTED = decltype(drafted_c)::value, CAREFUL = decltype(careful_c)::value;
+    // Tile t is there for every wave, and every wave has read tile t - 1: its buffer takes tile t + 1.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 1 < tiles) {
+      if ((t + 1) * kKeys % kFill == 0) {
+        place((t + 1) * kKeys / kFill, page);
+        if ((t + 1) * kKeys + kFill < keys) page = page_at((t + 1) * kKeys / kFill + 1);
+      }
+      load(t + 1);
+    }
+    const int key0 = start + t * kKeys, at = t * kKeys % kFill, fill = t * kKeys / kFill & 1;
+    const char* kt = s_kv[t & 1][0] + col * kRow;
+    const char* vt = s_kv[t & 1][1] + vbyte;
+    v4f s[KT];
+#pragma unroll
+    for (int u = 0; u < KT; ++u) s[u] = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < QS; ++i)
+#pragma unroll
+      for (int u = 0; u < KT; ++u)
+        s[u] = T::mfma16(*reinterpret_cast<const v4u32*>(kt + 16 * u * kRow + 16 * ((4 * i + grp) ^ key_swizzle<D>(col))), qf[i], s[u]);
+    uint32_t live[KT];  // bit j of [u]: this row attends to key 16 u + 4 grp + j of the tile
+    float top = kLowest;
+#pragma unroll
+    for (int u = 0; u < KT; ++u) {
+      if constexpr (DRAFTED) {
+        const int d = key0 + 16 * u + 4 * grp - ctx;
+        const uint64_t on = d >= 0 ? seen >> min(d, 63) : seen << min(-d, 63) | ((1ull << min(-d, 63)) - 1);
+        live[u] = d >= 64 ? 0u : (uint32_t)on & 15u;
+      }
+      v4f ks = {p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2};
+      if constexpr (INT8) ks = *reinterpret_cast<const v4f*>(&s_ks[fill][at + 16 * u + 4 * grp]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x = s[u][j] * ks[j];
+        if (DRAFTED && !((live[u] >> j) & 1)) x = kNegInf;
+        s[u][j] = x;
+        top = fmaxf(top, x);
+      }
+    }
+    top = rows_max(top);
+    if (__any(top > m + kSlack)) {
+      const float mn = fmaxf(m, top);
+      const float c = exp2_hw(m - mn);
+      l *= c;
+#pragma unroll
+      for (int e = 0; e < DB; ++e) acc[e] = acc[e] * c;
+      m = mn;
+    }
+    v4u32 phi, plo;
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < KT; ++u) {
+      float pv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pv[j] = exp2_hw(s[u][j] - m);
+        sum[j % 2] += pv[j];
+      }
+      if constexpr (INT8) {
+        const v4f vs = *reinterpret_cast<const v4f*>(&s_vs[fill][at + 16 * u + 4 * grp]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pv[j] = DRAFTED && !((live[u] >> j) & 1) ? 0.0f : pv[j] * vs[j];  // a masked key's scale may be NaN
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t hi = PT::pack(pv[2 * j], pv[2 * j + 1]);
+        const v2f back = PT::unpack(hi);
+        phi[2 * u + j] = hi;
+        plo[2 * u + j] = PT::pack(pv[2 * j] - back[0], pv[2 * j + 1] - back[1]);
+      }
+    }
+    l += sum[0] + sum[1];
+#pragma unroll
+    for (int e = 0; e < DB; e += 2) {  // two sums in turn: neither waits for the other
+      v4u32 a[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const char* from = vt + 16 * ((2 * (e + k) + (lane & 3) / 2) ^ swv(vkey));
+        const v2u32 lo = read_transposed(from), hi = read_transposed(from + 16 * kRow);
+        a[k] = v4u32{lo.x, lo.y, hi.x, hi.y};
+        if constexpr (CAREFUL) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) a[k][j] = only_finite<PT>(a[k][j]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[e + k % 2] = PT::mfma16(a[k % 2], k < 2 ? phi : plo, acc[e + k % 2]);
+    }
+    if (t + 1 < tiles) store(t + 1);
+  };
+  auto begin = [&] {
+    place(0, page);
+    if (kFill < keys) page = page_at(1);
+    m = kLowest, l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < DB; ++e) acc[e] = v4f{0, 0, 0, 0};
+    load(0);
+    store(0);
+  };
+  begin();
+  int t = 0;
+#pragma unroll 1
+  for (; t < plain; ++t) step(t, std::false_type{}, std::false_type{});
+#pragma unroll 1
+  for (; t < tiles; ++t) step(t, std::true_type{}, std::false_type{});
+  // As in the narrow kernel: values of masked keys that are infinities or NaN have spoiled the sums; the tiles with
+  // drafted keys are computed without such values, which are added at the end to the rows that attend to them.
+  bool careful = false;
+  if constexpr (!INT8) {
+    if (plain < tiles) {
+      float odd = 0.0f;  // 0 where all sums are finite, else NaN
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) odd = fmaf(acc[i][r], 0.0f, odd);
+      careful = __syncthreads_or(odd != 0.0f);
+      if (careful) {
+        page = page_at(0);
+        begin();
+#pragma unroll 1
+        for (t = 0; t < plain; ++t) step(t, std::false_type{}, std::false_type{});
+#pragma unroll 1
+        for (; t < tiles; ++t) step(t, std::true_type{}, std::true_type{});
+      }
+    }
+  }
+  const bool bad = __syncthreads_or(bad_page);
+  l = rows_sum(l);
+  if (bad) l = __builtin_nanf("");
+  if (row0 + 16 * wave + col >= rows) return;
+  const bool alone = rq.L <= keys;
+  const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + chunk;
+  if (!alone && grp == 0) p.mp[part] = m, p.lp[part] = l;
+#pragma unroll
+  for (int e = 0; e < DB; ++e) {
+    const int dim = 16 * e + 4 * grp;
+    v4f o = acc[e];
+    if (careful) {
+#pragma unroll 1
+      for (int key = start + plain * kKeys; key < end; ++key) {
+        const int32_t block = p.bt[(int64_t)b * p.sbt + page_of(p, key)];
+        const bool on = (key < ctx || (seen >> (key - ctx)) & 1) && block >= 0 && block < p.blocks;
+        if (!on) continue;
+        const v2u32 w = *reinterpret_cast<const v2u32*>(vh + block * p.svb + (int64_t)(key - page_of(p, key) * p.page) * p.svp + 2 * dim);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float f = T::to_f32((uint16_t)(w[j / 2] >> (16 * (j % 2))));
+          if (!__builtin_isfinite(f)) o[j] += f;
+        }
+      }
+    }
+    if (alone)
+      store_row<T>(p, rq, node, head, dim, o, l);
+    else
+      *reinterpret_cast<v4f*>(p.ap + part * D + dim) = o;
+  }
+}
+
 // Joins a row's groups: the strands of a group where workgroups have left them apart, then the groups in order; of the wide
 // kernel four chunks are a group. A workgroup joins one row, GROUPS groups at a time, 4 dims a lane: their partials are on
 // their way together. A row of several groups attends to its context, so its sum is not empty.
@@ -1001,7 +1281,7 @@ __global__ __launch_bounds__(D * GROUPS / 4) void tree_merge_kernel(TreeParams p
   const uint32_t bn = blockIdx.x / (uint32_t)H;
   const int b = (int)(bn / (uint32_t)p.max_nodes), node = (int)(bn % (uint32_t)p.max_nodes);
   const Request rq = request_of(p, b);
-  const bool wide = rq.T * p.G > kWideRows, apart = wide || p.strands;
+  const bool wide = rq.T * p.G > p.wide_rows, apart = wide || p.strands;
   const int keys = wide ? wide_chunk(rq.L) : kSeg;
   const int chunks = (rq.L + keys - 1) / keys, groups = (chunks + kGroup - 1) / kGroup;
   if (rq.bad || node >= rq.T || chunks <= (wide ? 1 : kGroup)) return;
@@ -1041,7 +1321,8 @@ int64_t most_chunks(int64_t keys) {
 template <typename T, bool INT8, int D>
 hipError_t launch_tree(TreeParams p, hipStream_t st) {
   // The narrow kernel covers the rows of requests that do not take the wide one.
-  const int64_t rows = (int64_t)p.max_nodes * p.G, narrow = std::min<int64_t>(rows, kWideRows / p.G * p.G);
+  const int64_t rows = (int64_t)p.max_nodes * p.G, narrow = std::min<int64_t>(rows, wide_rows(D) / p.G * p.G);
+  p.wide_rows = wide_rows(D);
   const int64_t merges = (int64_t)p.n * p.max_nodes * p.KV * p.G;
   if (merges > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
   const dim3 threads(64 * kWaves);
@@ -1065,16 +1346,19 @@ hipError_t launch_tree(TreeParams p, hipStream_t st) {
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
-  if (rows > kWideRows) {
+  if (rows > wide_rows(D)) {
     TreeParams w = p;
-    w.row_blocks = (int32_t)cdiv<int64_t>(rows, 32 * kWaves);
+    w.row_blocks = (int32_t)cdiv<int64_t>(rows, 128);
     const int64_t blocks = cdiv<int64_t>((int64_t)p.KV * p.n * most_chunks(p.max_len), 8) * 8 * w.row_blocks;
     if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((tree_decode_kernel_wide<T, INT8, D>), dim3((unsigned)blocks), threads, 0, st, w);
+    if constexpr (D == 256)
+      hipLaunchKernelGGL((tree_decode_kernel_wide_256<T, INT8>), dim3((unsigned)blocks), dim3(64 * kWaves256), 0, st, w);
+    else
+      hipLaunchKernelGGL((tree_decode_kernel_wide<T, INT8, D>), dim3((unsigned)blocks), threads, 0, st, w);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
-  if (p.ns <= (rows > kWideRows ? 1 : kGroup)) return hipSuccess;
+  if (p.ns <= (rows > wide_rows(D) ? 1 : kGroup)) return hipSuccess;
   // Few rows: latency counts, and all their groups are read at once (one row over 16384 keys: 15.7 us -> 14.6). Many rows: the
   // fewer threads that wait for others, the better (16384 rows of 3 groups: 237 us with 16 groups at a time, 219 with 4, 216
   // with 2).
