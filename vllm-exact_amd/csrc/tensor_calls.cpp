@@ -79,15 +79,22 @@ T* ptr(const at::Tensor* t) {
 }
 int64_t stride(const at::Tensor* t, int i) { return t ? t->stride(i) : 0; }
 
-// status = call(stream) with the tensors' device current and torch's current stream there.
-template <typename F>
-int on_device(const at::Tensor& t, F&& call) {
+// The interpreter lock, given back while this lives: also where an exception ends the scope.
+struct Unlocked {
+  PyThreadState* const state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
+// fn(arguments, stream) with the tensors' device current and torch's current stream there. The arguments are pointers, strides and
+// sizes, taken from the tensors by the caller while it holds the lock: a tensor without memory (torch.vmap's) throws there.
+template <typename F, typename... A>
+int on_device(const at::Tensor& t, F fn, A... arguments) {
   const c10::DeviceGuard guard(t.device());
   const vxa_stream_t stream = c10::hip::getCurrentHIPStream(t.device().index()).stream();
-  int status;
-  Py_BEGIN_ALLOW_THREADS status = call(stream);
-  Py_END_ALLOW_THREADS
-  return status;
+  const Unlocked unlocked;
+  return fn(arguments..., stream);
 }
 
 struct Cache {
@@ -131,11 +138,9 @@ int prompt_attention(PyObject* const* a) {
     if (t->size(2) && t->stride(2) != 1) refuse(what, ": the head dimension must be contiguous");
   const int out_dtype = dtype_enum(out);
   if (q.size(0) == 0) return VXA_OK;
-  return on_device(q, [&](vxa_stream_t stream) {
-    return prompt_attention_fn(ptr(&q), q.stride(0), q.stride(1), ptr(&k), k.stride(0), k.stride(1), ptr(&v), v.stride(0), v.stride(1),
-                               dtype_enum(q), ptr<int32_t>(&cu), cu.size(0) - 1, q.size(0), (float)scale, ptr(&out), out_dtype,
-                               out.stride(0), out.stride(1), q.size(1), k.size(1), q.size(2), stream);
-  });
+  return on_device(q, prompt_attention_fn, ptr(&q), q.stride(0), q.stride(1), ptr(&k), k.stride(0), k.stride(1), ptr(&v), v.stride(0),
+                   v.stride(1), dtype_enum(q), ptr<int32_t>(&cu), cu.size(0) - 1, q.size(0), (float)scale, ptr(&out), out_dtype,
+                   out.stride(0), out.stride(1), q.size(1), k.size(1), q.size(2));
 }
 
 int write_cache(PyObject* const* a) {
@@ -150,12 +155,10 @@ int write_cache(PyObject* const* a) {
   const int dtype = dtype_enum(k);
   if (k.size(0) == 0) return VXA_OK;
   const at::Tensor &kc = *c.key, &vc = *c.value, &ks = *c.key_scale, &vs = *c.value_scale;
-  return on_device(k, [&](vxa_stream_t stream) {
-    return cache_write_fn(ptr(&k), k.stride(0), k.stride(1), ptr(&v), v.stride(0), v.stride(1), dtype, k.size(0), k.size(1), k.size(2),
-                          ptr<int8_t>(&kc), kc.stride(0), kc.stride(1), kc.stride(2), ptr<int8_t>(&vc), vc.stride(0), vc.stride(1),
-                          vc.stride(2), ptr<float>(&ks), ks.stride(0), ks.stride(1), ks.stride(2), ptr<float>(&vs), vs.stride(0),
-                          vs.stride(1), vs.stride(2), kc.size(0), kc.size(1), ptr<int64_t>(&slots), stream);
-  });
+  return on_device(k, cache_write_fn, ptr(&k), k.stride(0), k.stride(1), ptr(&v), v.stride(0), v.stride(1), dtype, k.size(0), k.size(1),
+                   k.size(2), ptr<int8_t>(&kc), kc.stride(0), kc.stride(1), kc.stride(2), ptr<int8_t>(&vc), vc.stride(0), vc.stride(1),
+                   vc.stride(2), ptr<float>(&ks), ks.stride(0), ks.stride(1), ks.stride(2), ptr<float>(&vs), vs.stride(0), vs.stride(1),
+                   vs.stride(2), kc.size(0), kc.size(1), ptr<int64_t>(&slots));
 }
 
 int read_cache(PyObject* const* a) {
@@ -173,13 +176,11 @@ int read_cache(PyObject* const* a) {
   const int dtype = dtype_enum(k);
   if (k.size(0) == 0 || n == 0) return VXA_OK;
   const at::Tensor &kc = *c.key, &vc = *c.value, &ks = *c.key_scale, &vs = *c.value_scale;
-  return on_device(k, [&](vxa_stream_t stream) {
-    return cache_read_fn(ptr<int8_t>(&kc), kc.stride(0), kc.stride(1), kc.stride(2), ptr<int8_t>(&vc), vc.stride(0), vc.stride(1),
-                         vc.stride(2), ptr<float>(&ks), ks.stride(0), ks.stride(1), ks.stride(2), ptr<float>(&vs), vs.stride(0),
-                         vs.stride(1), vs.stride(2), kc.size(0), kc.size(1), ptr<int32_t>(&bt), bt.stride(0), bt.size(1),
-                         ptr<int32_t>(&cu), ptr<int32_t>(first), n, k.size(0), k.size(1), k.size(2), ptr(&k), k.stride(0), k.stride(1),
-                         ptr(&v), v.stride(0), v.stride(1), dtype, stream);
-  });
+  return on_device(k, cache_read_fn, ptr<int8_t>(&kc), kc.stride(0), kc.stride(1), kc.stride(2), ptr<int8_t>(&vc), vc.stride(0),
+                   vc.stride(1), vc.stride(2), ptr<float>(&ks), ks.stride(0), ks.stride(1), ks.stride(2), ptr<float>(&vs), vs.stride(0),
+                   vs.stride(1), vs.stride(2), kc.size(0), kc.size(1), ptr<int32_t>(&bt), bt.stride(0), bt.size(1), ptr<int32_t>(&cu),
+                   ptr<int32_t>(first), n, k.size(0), k.size(1), k.size(2), ptr(&k), k.stride(0), k.stride(1), ptr(&v), v.stride(0),
+                   v.stride(1), dtype);
 }
 
 int tree_decode(PyObject* const* a) {
@@ -219,15 +220,12 @@ int tree_decode(PyObject* const* a) {
   if (rc != VXA_OK) return rc;
   at::Tensor ws;
   if (bytes) ws = at::empty({(int64_t)bytes / 4}, q.options().dtype(at::kFloat));
-  return on_device(q, [&](vxa_stream_t stream) {
-    const at::Tensor *ks = c.key_scale, *vs = c.value_scale;
-    return tree_decode_fn(ptr(&q), q.stride(0), q.stride(1), dtype_enum(q), ptr(&kc), kc.stride(0), kc.stride(1), kc.stride(2), ptr(&vc),
-                          vc.stride(0), vc.stride(1), vc.stride(2), ptr<float>(ks), stride(ks, 0), stride(ks, 1), stride(ks, 2),
-                          ptr<float>(vs), stride(vs, 0), stride(vs, 1), stride(vs, 2), kc.size(0), kc.size(1), ptr<int32_t>(&bt),
-                          bt.stride(0), bt.size(1), ptr<int32_t>(&sl), ptr<int32_t>(&qsl), ptr<int64_t>(mask), (float)scale, ptr(&out),
-                          out_dtype, out.stride(0), out.stride(1), n, T, H, KV, D, max_nodes, max_len, bytes ? ptr(&ws) : nullptr,
-                          bytes, stream);
-  });
+  const at::Tensor *ks = c.key_scale, *vs = c.value_scale;
+  return on_device(q, tree_decode_fn, ptr(&q), q.stride(0), q.stride(1), dtype_enum(q), ptr(&kc), kc.stride(0), kc.stride(1),
+                   kc.stride(2), ptr(&vc), vc.stride(0), vc.stride(1), vc.stride(2), ptr<float>(ks), stride(ks, 0), stride(ks, 1),
+                   stride(ks, 2), ptr<float>(vs), stride(vs, 0), stride(vs, 1), stride(vs, 2), kc.size(0), kc.size(1), ptr<int32_t>(&bt),
+                   bt.stride(0), bt.size(1), ptr<int32_t>(&sl), ptr<int32_t>(&qsl), ptr<int64_t>(mask), (float)scale, ptr(&out),
+                   out_dtype, out.stride(0), out.stride(1), n, T, H, KV, D, max_nodes, max_len, bytes ? ptr(&ws) : nullptr, bytes);
 }
 
 // fn(arguments) as a Python function of `count` positional arguments; C++ exceptions end here.
