@@ -11,7 +11,8 @@
 // without leaving the lane. The tiles of K and V are copied straight into LDS, two in turn; V is transposed as it is read
 // from there. Two workgroups share a CU. At 256 dims a wave takes 16 rows (below). The workgroups furthest from their
 // sequence's start, which take longest, go first.
-// A row's order of operations depends on its place in its sequence alone, not on the batch.
+// A row's order of operations depends on its place in its sequence and its own scores, so its bits depend on its query and on
+// the keys and values up to its own, not on other rows or the batch.
 //
 // Rounding. Scores, maxima, sums and accumulators are fp32; P is rounded to the 16-bit element type for the second
 // product, an error of the size of the output's own rounding, while its sum takes the fp32 values.
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
     swap32(ta, tb);
     top = fmaxf(ta, tb) * p.scale_log2;
     if (__any(top > m + kSlack)) {
-      const float mn = fmaxf(m, top);
+      const float mn = top > m + kSlack ? top : m;
       const float c = exp2_hw(m - mn);
 #pragma unroll
       for (int i = 0; i < 4; ++i) l[i] *= c;
@@ -429,7 +430,7 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
       for (int r = 0; r < 4; ++r) top = fmaxf(top, s[u][r]);
     top = rows_max(top) * p.scale_log2;
     if (__any(top > m + kSlack)) {
-      const float mn = fmaxf(m, top);
+      const float mn = top > m + kSlack ? top : m;
       const float c = exp2_hw(m - mn);
       l *= c;
 #pragma unroll

@@ -18,8 +18,9 @@
 //
 // Order. Keys are cut into segments of kSeg and groups of kGroup segments. Strand w of a segment, its 32-key tiles w,
 // w + 4, ..., is summed with one running maximum; the segments of a strand are folded in order, the four strands of a
-// group joined, the groups folded in order. It depends on a request's own length only, so its bits do not change with the
-// batch. A workgroup's waves take the four strands of a group, one each, and need each other only at its end; where that
+// group joined, the groups folded in order. It depends on a request's own length and number of rows, and the running maxima
+// on a row's own scores: a row's bits do not change with the batch, nor with the queries of the request's other nodes. A
+// workgroup's waves take the four strands of a group, one each, and need each other only at its end; where that
 // leaves too few workgroups, a workgroup takes one strand and its waves one segment each: the same sums.
 //
 // Rounding. Scores, maxima, sums and accumulators are fp32. P is split into two 16-bit parts, hi + lo, with one
@@ -491,7 +492,7 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
         }
       top = rows_max(top);
       if (__any(top > m[t] + kSlack)) {
-        const float mn = fmaxf(m[t], top);
+        const float mn = top > m[t] + kSlack ? top : m[t];
         const float c = exp2_hw(m[t] - mn);
         l[t] *= c;
 #pragma unroll
@@ -866,7 +867,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel_wide(TreePa
     swap32(ta, tb);
     top = fmaxf(ta, tb);
     if (__any(top > m + kSlack)) {
-      const float mn = fmaxf(m, top);
+      const float mn = top > m + kSlack ? top : m;
       const float c = exp2_hw(m - mn);
 #pragma unroll
       for (int i = 0; i < 4; ++i) l[i] *= c;
@@ -1150,7 +1151,7 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void tree_decode_kernel_wide_256
     }
     top = rows_max(top);
     if (__any(top > m + kSlack)) {
-      const float mn = fmaxf(m, top);
+      const float mn = top > m + kSlack ? top : m;
       const float c = exp2_hw(m - mn);
       l *= c;
 #pragma unroll
