@@ -136,6 +136,22 @@ __device__ inline bool any_special(uint32_t w) {
   constexpr uint32_t m = T::kExpMask;
   return (w & m) == m || ((w >> 16) & m) == m;
 }
+// Four elements' infinities and NaN, added to `sum`.
+template <typename T>
+__device__ inline void add_specials(v4f& sum, v2u32 w) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float f = T::to_f32((uint16_t)(w[e / 2] >> (16 * (e % 2))));
+    if (!__builtin_isfinite(f)) sum[e] += f;
+  }
+}
+// The elements of four dims whose values hold an infinity or NaN that the row attends to, in place of what was stored there. Such
+// a value counts however small its weight; in the sums it has met weights of 0, or negative second parts of one, and become NaN.
+__device__ inline void store_specials(void* out, int dtype, int64_t at, v4f special) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (!__builtin_isfinite(special[e])) store_f32_as(out, dtype, at + e, special[e]);
+}
 // The dword with its infinities and NaN replaced by 0, and which of its elements add +inf (SIGN = 0: +inf
 // and NaN) or -inf (SIGN = 1: -inf and NaN), as elements 1 and 0.
 template <typename T>

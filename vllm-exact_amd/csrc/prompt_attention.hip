@@ -103,6 +103,22 @@ __device__ inline Tile find_tile(const PromptParams& p, int tile) {
   return Tile{0, 0, 0};
 }
 
+// A row after a careful pass, its dims dim0 + 0..3, dim0 + STEP + 0..3, ...: values of its keys from `first` on that are infinities or
+// NaN take the place of what was stored. first is 0 where the row's sums are not finite: infinities met weights of 0 in tiles
+// that were not looked at, too.
+template <typename T, int D, int STEP>
+__device__ inline void find_specials(const PromptParams& p, int64_t at, int dim0, float sum, const char* values, int64_t stride, int first, int row) {
+  if (__builtin_isnan(sum)) return;  // a score is +inf or NaN: so is the row
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the wave's other lanes have stored there
+#pragma unroll 1
+  for (int dim = dim0; dim < D; dim += STEP) {
+    v4f special = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int key = first; key <= row; ++key) add_specials<T>(special, *reinterpret_cast<const v2u32*>(values + key * stride + 2 * dim));
+    store_specials(p.out, p.out_dtype, at + dim, special);
+  }
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(PromptParams p) {
   constexpr int kKeys = 64, KU = kKeys / 32;  // keys of a tile, in blocks of 32
@@ -189,7 +205,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
   }
   // One tile. MASKED: some of its keys may come after some of the wave's rows.
   // CAREFUL: values of keys that some rows do not attend to may be infinities or NaN, and 0 times those is NaN; here they
-  // enter the product as 0, and the rows that attend to them add them at the end. The pass that does not look ends with
+  // enter the product as 0, and the rows that attend to them find them at the end. The pass that does not look ends with
   // NaN wherever that mattered.
   auto step = [&](int t, auto masked_c, auto careful_c) {
     constexpr bool MASKED = decltype(masked_c)::value, CAREFUL = decltype(careful_c)::value;
@@ -277,7 +293,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
   }
   float la = (l[0] + l[1]) + (l[2] + l[3]), lb = la;
   swap32(la, lb);
-  const float inv = 1.0f / (la + lb);
+  const float sum = la + lb, inv = 1.0f / sum;
   if (row >= len) return;
   const int64_t at = (int64_t)(base + row) * p.sot + (int64_t)head * p.soh;
 #pragma unroll
@@ -291,17 +307,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] = acc[i][r0 + 4 * k + j] * inv;
         const int dim = 32 * i + 2 * r0 + 8 * k + 4 * half;
-        if (careful) {
-#pragma unroll 1
-          for (int key = full * kKeys; key <= row; ++key) {
-            const v2u32 x = *reinterpret_cast<const v2u32*>(vh + key * svt + 2 * dim);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float f = T::to_f32((uint16_t)(x[j / 2] >> (16 * (j % 2))));
-              if (!__builtin_isfinite(f)) o[j] += f;
-            }
-          }
-        }
         w[k][0] = T::pack(o[0], o[1]), w[k][1] = T::pack(o[2], o[3]);
         if (!p.out_wide) {
 #pragma unroll
@@ -318,6 +323,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
             v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
       }
     }
+  if (careful) {
+    odd = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) odd = fmaf(acc[i][r], 0.0f, odd);
+    find_specials<T, D, 8>(p, at, 4 * half, sum, vh, svt, odd == 0.0f ? full * kKeys : 0, row);
+  }
 }
 
 // The same for 256 dims, with 8 waves of 16 rows and 16 x 16 x 32 MFMAs: 32 rows of a wave take 430 registers and leave one
@@ -477,7 +490,7 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
     for (t = 0; t < full; ++t) step(t, std::false_type{}, std::false_type{});
     for (; t < tiles; ++t) step(t, std::true_type{}, std::true_type{});
   }
-  const float inv = 1.0f / rows_sum(l);
+  const float sum = rows_sum(l), inv = 1.0f / sum;
   if (row >= len) return;
   const int64_t at = (int64_t)(base + row) * p.sot + (int64_t)head * p.soh;
 #pragma unroll
@@ -489,17 +502,6 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = acc[e0 + k][j] * inv;
       const int dim = 16 * (e0 + k) + 4 * grp;
-      if (careful) {
-#pragma unroll 1
-        for (int key = full * kKeys; key <= row; ++key) {
-          const v2u32 v = *reinterpret_cast<const v2u32*>(vh + key * svt + 2 * dim);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float f = T::to_f32((uint16_t)(v[j / 2] >> (16 * (j % 2))));
-            if (!__builtin_isfinite(f)) o[j] += f;
-          }
-        }
-      }
       w[k][0] = T::pack(o[0], o[1]), w[k][1] = T::pack(o[2], o[3]);
       if (!p.out_wide) {
 #pragma unroll
@@ -515,6 +517,14 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
       *reinterpret_cast<v4u32*>(reinterpret_cast<uint16_t*>(p.out) + at + 16 * (e0 + (grp & 1)) + 4 * (grp & 2)) =
           v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
     }
+  }
+  if (careful) {
+    odd = 0.0f;
+#pragma unroll
+    for (int e = 0; e < DB; ++e)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) odd = fmaf(acc[e][r], 0.0f, odd);
+    find_specials<T, D, 16>(p, at, 4 * grp, sum, vh, svt, odd == 0.0f ? full * kKeys : 0, row);
   }
 }
 

@@ -203,12 +203,17 @@ __device__ inline bool attends_to_nothing(const TreeParams& p, const Request& rq
   return ((uint64_t)p.mask[rq.q0 + node] & all) == 0;
 }
 
+// Gives whether there are sums that are not finite, though the scores are.
 template <typename T>
-__device__ inline void store_row(const TreeParams& p, const Request& rq, int node, int head, int dim, v4f a, float l) {
+__device__ inline bool store_row(const TreeParams& p, const Request& rq, int node, int head, int dim, v4f a, float l) {
   const float inv = 1.0f / l;
   const bool nothing = l == 0.0f && attends_to_nothing(p, rq, node);
+  float odd = 0.0f;  // 0 where all four are finite, else NaN
 #pragma unroll
-  for (int e = 0; e < 4; ++e) a[e] = nothing ? 0.0f : a[e] * inv;
+  for (int e = 0; e < 4; ++e) {
+    odd = fmaf(a[e], 0.0f, odd);
+    a[e] = nothing ? 0.0f : a[e] * inv;
+  }
   const int64_t to = (int64_t)(rq.q0 + node) * p.sot + (int64_t)head * p.soh + dim;
   if (p.out_wide) {
     *reinterpret_cast<v2u32*>(reinterpret_cast<uint16_t*>(p.out) + to) = v2u32{T::pack(a[0], a[1]), T::pack(a[2], a[3])};
@@ -216,6 +221,38 @@ __device__ inline void store_row(const TreeParams& p, const Request& rq, int nod
 #pragma unroll
     for (int e = 0; e < 4; ++e) store_f32_as(p.out, p.out_dtype, to + e, a[e]);
   }
+  return odd != 0.0f && l > 0.0f;  // l is NaN where a score is +inf or NaN, or a page is missing
+}
+// For those: values that are infinities or NaN, of keys that the row attends to, take the place of what was stored.
+template <typename T, bool INT8>
+__device__ inline void find_specials(const TreeParams& p, const Request& rq, int b, int node, int head, int dim) {
+  const int g = head / p.G, ctx = rq.L - rq.T;
+  const uint64_t seen = p.mask != nullptr ? (uint64_t)p.mask[rq.q0 + node] : (2ull << node) - 1;
+  v4f special = {0, 0, 0, 0};
+#pragma unroll 1
+  for (int first = 0, page = 0; first < rq.L; first += p.page, ++page) {
+    const int64_t block = p.bt[(int64_t)b * p.sbt + page];
+    if (block < 0 || block >= p.blocks) continue;
+    const char* values = p.vc + block * p.svb + (int64_t)g * p.svh + (INT8 ? 1 : 2) * dim;
+    const int count = min(p.page, rq.L - first);
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+      const int draft = first + i - ctx;
+      if (draft >= 0 && !((seen >> draft) & 1)) continue;
+      if constexpr (INT8) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(values + i * p.svp);
+        const float scale = p.vs[block * p.svsb + i * p.svsp + (int64_t)g * p.svsh];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float f = (float)(int8_t)(w >> (8 * e)) * scale;
+          if (!__builtin_isfinite(f)) special[e] += f;
+        }
+      } else {
+        add_specials<T>(special, *reinterpret_cast<const v2u32*>(values + i * p.svp));
+      }
+    }
+  }
+  store_specials(p.out, p.out_dtype, (int64_t)(rq.q0 + node) * p.sot + (int64_t)head * p.soh + dim, special);
 }
 
 // The row block of a workgroup, and what it shares with the other row blocks in `id`. Workgroups go to the 8 XCDs in turn:
@@ -688,7 +725,8 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
     if (bad) s[0].l = __builtin_nanf("");
     const int node = row / p.G, head = g * p.G + row % p.G;
     if (alone) {
-      store_row<T>(p, rq, node, head, 4 * c, s[0].a, s[0].l);
+      const bool spoiled = store_row<T>(p, rq, node, head, 4 * c, s[0].a, s[0].l);
+      if (__builtin_expect(spoiled, 0)) find_specials<T, INT8>(p, rq, b, node, head, 4 * c);
     } else {
       const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + group * kWaves + (whole ? 0 : strand);
       if (c == 0) p.mp[part] = s[0].m, p.lp[part] = s[0].l;
@@ -964,6 +1002,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel_wide(TreePa
   const float sum = bad ? __builtin_nanf("") : la + lb;
   if (row0 + 32 * wave + col >= rows) return;
   const bool alone = rq.L <= keys;
+  bool spoiled = false;
   const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + chunk;
   if (!alone && half == 0) p.mp[part] = m, p.lp[part] = sum;
 #pragma unroll
@@ -987,10 +1026,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel_wide(TreePa
         }
       }
       if (alone)
-        store_row<T>(p, rq, node, head, dim, o, sum);
+        spoiled |= store_row<T>(p, rq, node, head, dim, o, sum);
       else
         *reinterpret_cast<v4f*>(p.ap + part * D + dim) = o;
     }
+  if (__builtin_expect(spoiled, 0))
+#pragma unroll 1
+    for (int dim = 4 * half; dim < D; dim += 8) find_specials<T, INT8>(p, rq, b, node, head, dim);
 }
 
 // The same for 256 dims, with 8 waves of 16 rows and 16 x 16 x 32 MFMAs: two waves a SIMD, where 32 rows leave one. Six
@@ -1241,6 +1283,7 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void tree_decode_kernel_wide_256
   if (bad) l = __builtin_nanf("");
   if (row0 + 16 * wave + col >= rows) return;
   const bool alone = rq.L <= keys;
+  bool spoiled = false;
   const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + chunk;
   if (!alone && grp == 0) p.mp[part] = m, p.lp[part] = l;
 #pragma unroll
@@ -1262,16 +1305,19 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void tree_decode_kernel_wide_256
       }
     }
     if (alone)
-      store_row<T>(p, rq, node, head, dim, o, l);
+      spoiled |= store_row<T>(p, rq, node, head, dim, o, l);
     else
       *reinterpret_cast<v4f*>(p.ap + part * D + dim) = o;
   }
+  if (__builtin_expect(spoiled, 0))
+#pragma unroll 1
+    for (int dim = 4 * grp; dim < D; dim += 16) find_specials<T, INT8>(p, rq, b, node, head, dim);
 }
 
 // Joins a row's groups: the strands of a group where workgroups have left them apart, then the groups in order; of the wide
 // kernel four chunks are a group. A workgroup joins one row, GROUPS groups at a time, 4 dims a lane: their partials are on
 // their way together. A row of several groups attends to its context, so its sum is not empty.
-template <typename T, int D, int GROUPS>
+template <typename T, bool INT8, int D, int GROUPS>
 __global__ __launch_bounds__(D * GROUPS / 4) void tree_merge_kernel(TreeParams p) {
   constexpr int kLanes = D / 4;
   __shared__ float s_ml[GROUPS][2];
@@ -1310,7 +1356,9 @@ __global__ __launch_bounds__(D * GROUPS / 4) void tree_merge_kernel(TreeParams p
     }
     __syncthreads();
   }
-  if (mine == 0) store_row<T>(p, rq, node, head, 4 * c, sum.a, sum.l);
+  if (mine != 0) return;
+  const bool spoiled = store_row<T>(p, rq, node, head, 4 * c, sum.a, sum.l);
+  if (__builtin_expect(spoiled, 0)) find_specials<T, INT8>(p, rq, b, node, head, 4 * c);
 }
 
 // The most chunks of any request of at most `keys` keys.
@@ -1364,9 +1412,9 @@ hipError_t launch_tree(TreeParams p, hipStream_t st) {
   // fewer threads that wait for others, the better (16384 rows of 3 groups: 237 us with 16 groups at a time, 219 with 4, 216
   // with 2).
   if (merges <= 2048)
-    hipLaunchKernelGGL((tree_merge_kernel<T, D, 16>), dim3((unsigned)merges), dim3(D * 16 / 4), 0, st, p);
+    hipLaunchKernelGGL((tree_merge_kernel<T, INT8, D, 16>), dim3((unsigned)merges), dim3(D * 16 / 4), 0, st, p);
   else
-    hipLaunchKernelGGL((tree_merge_kernel<T, D, 2>), dim3((unsigned)merges), dim3(D * 2 / 4), 0, st, p);
+    hipLaunchKernelGGL((tree_merge_kernel<T, INT8, D, 2>), dim3((unsigned)merges), dim3(D * 2 / 4), 0, st, p);
   return hipGetLastError();
 }
 
