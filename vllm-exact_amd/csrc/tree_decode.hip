@@ -223,6 +223,13 @@ __device__ inline bool store_row(const TreeParams& p, const Request& rq, int nod
   }
   return odd != 0.0f && l > 0.0f;  // l is NaN where a score is +inf or NaN, or a page is missing
 }
+// The arguments, read again: for code that is seldom reached and would keep registers through all that comes before.
+__device__ inline TreeParams arguments_again() {
+  typedef const __attribute__((address_space(4))) TreeParams Args;
+  Args* args = (Args*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  return *(const TreeParams*)args;
+}
 // For those: values that are infinities or NaN, of keys that the row attends to, take the place of what was stored.
 template <typename T, bool INT8>
 __device__ inline void find_specials(const TreeParams& p, const Request& rq, int b, int node, int head, int dim) {
@@ -726,7 +733,7 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
     const int node = row / p.G, head = g * p.G + row % p.G;
     if (alone) {
       const bool spoiled = store_row<T>(p, rq, node, head, 4 * c, s[0].a, s[0].l);
-      if (__builtin_expect(spoiled, 0)) find_specials<T, INT8>(p, rq, b, node, head, 4 * c);
+      if (__builtin_expect(spoiled, 0)) find_specials<T, INT8>(arguments_again(), rq, b, node, head, 4 * c);
     } else {
       const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + group * kWaves + (whole ? 0 : strand);
       if (c == 0) p.mp[part] = s[0].m, p.lp[part] = s[0].l;
@@ -1032,7 +1039,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel_wide(TreePa
     }
   if (__builtin_expect(spoiled, 0))
 #pragma unroll 1
-    for (int dim = 4 * half; dim < D; dim += 8) find_specials<T, INT8>(p, rq, b, node, head, dim);
+    for (int dim = 4 * half; dim < D; dim += 8) find_specials<T, INT8>(arguments_again(), rq, b, node, head, dim);
 }
 
 // The same for 256 dims, with 8 waves of 16 rows and 16 x 16 x 32 MFMAs: two waves a SIMD, where 32 rows leave one. Six
@@ -1311,7 +1318,7 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void tree_decode_kernel_wide_256
   }
   if (__builtin_expect(spoiled, 0))
 #pragma unroll 1
-    for (int dim = 4 * grp; dim < D; dim += 16) find_specials<T, INT8>(p, rq, b, node, head, dim);
+    for (int dim = 4 * grp; dim < D; dim += 16) find_specials<T, INT8>(arguments_again(), rq, b, node, head, dim);
 }
 
 // Joins a row's groups: the strands of a group where workgroups have left them apart, then the groups in order; of the wide
@@ -1358,7 +1365,7 @@ __global__ __launch_bounds__(D * GROUPS / 4) void tree_merge_kernel(TreeParams p
   }
   if (mine != 0) return;
   const bool spoiled = store_row<T>(p, rq, node, head, 4 * c, sum.a, sum.l);
-  if (__builtin_expect(spoiled, 0)) find_specials<T, INT8>(p, rq, b, node, head, 4 * c);
+  if (__builtin_expect(spoiled, 0)) find_specials<T, INT8>(arguments_again(), rq, b, node, head, 4 * c);
 }
 
 // The most chunks of any request of at most `keys` keys.
