@@ -20,8 +20,10 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // and finite, so that keys scoring -inf weigh exp2(-inf - m) = 0 also where nothing else has been seen
 // (-inf - -inf would be NaN). Such a unit's state is (kLowest, 0, 0), which adds 0 to any merge.
 constexpr float kLowest = -3.402823466e38f;  // -FLT_MAX
-// A running maximum stays until a score passes it by this much (in powers of two): weights up to 2^8 are as precise as
-// weights up to 1 in every type here, and a tile seldom passes it, so the accumulators are seldom rescaled.
+// Weights are 2^(score - m) with a reference m near the running maximum. m stays until a weight would pass 2^reach, and is then
+// set so that the weight of that score is 2^(reach - kSlack): a tile seldom asks for it, so the accumulators are seldom
+// rescaled. A wave rescales where any of its rows' scores pass, but only those rows move: a row's bits do not depend on its
+// neighbours. The reach is the element type's (BF16, FP16 below).
 constexpr float kSlack = 8.0f;
 
 // x / d for 0 <= x < 2^31 and 1 <= d < 2^31: (2 x mul >> 32) >> shift with 2^shift >= d and mul = 2^(31 + shift) / d rounded
@@ -100,6 +102,9 @@ __device__ inline void static_for(F&& f) {
 struct BF16 {
   static constexpr uint32_t kExpMask = 0x7F80u, kOne = 0x3F80u;
   static constexpr int kDtype = VXA_BF16;
+  // Values may be as large as floats are: a row's weights stay below one over the number of its keys, so that its sums stay below
+  // the largest value. (Values below some 2^-100 lose bits in turn.)
+  static __device__ inline float reach(int keys) { return keys <= 1 << 12 ? -12.0f : keys <= 1 << 18 ? -18.0f : -30.0f; }
   static __device__ inline float to_f32(uint16_t b) { return bf16_to_f32(b); }
   static __device__ inline uint32_t pack(float a, float b) {  // round to nearest even
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
@@ -117,6 +122,7 @@ struct BF16 {
 struct FP16 {
   static constexpr uint32_t kExpMask = 0x7C00u, kOne = 0x3C00u;
   static constexpr int kDtype = VXA_F16;
+  static __device__ inline float reach(int) { return kSlack; }
   static __device__ inline float to_f32(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
   static __device__ inline uint32_t pack(float a, float b) {  // round to nearest even
     return __builtin_bit_cast(uint32_t, v2h{(_Float16)a, (_Float16)b});

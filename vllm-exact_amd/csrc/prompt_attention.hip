@@ -153,6 +153,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
 
   const int wrow = row0 + wave / p.heads * 32;  // the wave's first row
   const int row = wrow + col;
+  const float reach = T::reach(row + 1);
   const int last = min(row0 + p.rows, len);  // keys of the workgroup
   const int tiles = (last + kKeys - 1) / kKeys;
 
@@ -240,8 +241,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
     float ta = top, tb = top;
     swap32(ta, tb);
     top = fmaxf(ta, tb) * p.scale_log2;
-    if (__any(top > m + kSlack)) {
-      const float mn = top > m + kSlack ? top : m;
+    if (__any(top > m + reach)) {
+      const float mn = top > m + reach ? (top - reach) + kSlack : m;
       const float c = exp2_hw(m - mn);
 #pragma unroll
       for (int i = 0; i < 4; ++i) l[i] *= c;
@@ -368,6 +369,7 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
   const int64_t skt = 2 * p.skt, svt = 2 * p.svt;
   const int wrow = row0 + wave / p.heads * 16;  // the wave's first row
   const int row = wrow + col;
+  const float reach = T::reach(row + 1);
   const int last = min(row0 + p.rows, len);  // keys of the workgroup
   const int tiles = (last + kKeys - 1) / kKeys;
 
@@ -442,8 +444,8 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
 #pragma unroll
       for (int r = 0; r < 4; ++r) top = fmaxf(top, s[u][r]);
     top = rows_max(top) * p.scale_log2;
-    if (__any(top > m + kSlack)) {
-      const float mn = top > m + kSlack ? top : m;
+    if (__any(top > m + reach)) {
+      const float mn = top > m + reach ? (top - reach) + kSlack : m;
       const float c = exp2_hw(m - mn);
       l *= c;
 #pragma unroll

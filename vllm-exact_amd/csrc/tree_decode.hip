@@ -383,6 +383,7 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
   const int seg_end = min(group * kGroup + kGroup, whole ? segs : min(seg0 + 1, segs));
   if (alone && p.strands) find(seg0, first, pages);
   const int ctx = rq.L - rq.T;
+  const float reach = PT::reach(rq.L);
 
   // Row offsets and scales of the wave's own keys. Keys past the last one repeat the wave's first, masked. A page that the
   // cache does not have makes the request's rows NaN.
@@ -535,8 +536,8 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
           top = fmaxf(top, s[t][h][j]);
         }
       top = rows_max(top);
-      if (__any(top > m[t] + kSlack)) {
-        const float mn = top > m[t] + kSlack ? top : m[t];
+      if (__any(top > m[t] + reach)) {
+        const float mn = top > m[t] + reach ? (top - reach) + kSlack : m[t];
         const float c = exp2_hw(m[t] - mn);
         l[t] *= c;
 #pragma unroll
@@ -777,6 +778,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel_wide(TreePa
   const int start = chunk * keys, end = min(start + keys, rq.L);
   if (start >= end) return;
   const int ctx = rq.L - rq.T;
+  const float reach = PT::reach(rq.L);
   const int H = p.KV * p.G;
 
   // Places of kFill keys; those past the last one repeat it.
@@ -911,8 +913,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel_wide(TreePa
     float ta = top, tb = top;
     swap32(ta, tb);
     top = fmaxf(ta, tb);
-    if (__any(top > m + kSlack)) {
-      const float mn = top > m + kSlack ? top : m;
+    if (__any(top > m + reach)) {
+      const float mn = top > m + reach ? (top - reach) + kSlack : m;
       const float c = exp2_hw(m - mn);
 #pragma unroll
       for (int i = 0; i < 4; ++i) l[i] *= c;
@@ -1073,6 +1075,7 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void tree_decode_kernel_wide_256
   const int start = chunk * keys, end = min(start + keys, rq.L);
   if (start >= end) return;
   const int ctx = rq.L - rq.T;
+  const float reach = PT::reach(rq.L);
   const int H = p.KV * p.G;
 
   // Places of kFill keys; those past the last one repeat it.
@@ -1199,8 +1202,8 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void tree_decode_kernel_wide_256
       }
     }
     top = rows_max(top);
-    if (__any(top > m + kSlack)) {
-      const float mn = top > m + kSlack ? top : m;
+    if (__any(top > m + reach)) {
+      const float mn = top > m + reach ? (top - reach) + kSlack : m;
       const float c = exp2_hw(m - mn);
       l *= c;
 #pragma unroll
