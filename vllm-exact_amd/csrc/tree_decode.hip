@@ -24,8 +24,8 @@
 // leaves too few workgroups, a workgroup takes one strand and its waves one segment each: the same sums.
 //
 // Rounding. Scores, maxima, sums and accumulators are fp32. P is split into two 16-bit parts, hi + lo, with one
-// MFMA each: P keeps 16 bits (22 in fp16), as the 16-bit output is rounded once from an fp32 sum; the 8-bit
-// cache always takes bf16 parts there, because P vscale can leave the fp16 range.
+// MFMA each: P keeps 16 bits (in fp16 22, or what counts to 2^-32 of the row's largest weight), as the 16-bit output is rounded
+// once from an fp32 sum; the 8-bit cache always takes bf16 parts there, because P vscale can leave the fp16 range.
 //
 // What bounds it (32 heads on 8, 128 dims). 64 requests of up to 8192 keys with one token, 16-bit cache: 330 us, 6.5 TB/s,
 // the rate of reading. With 8 tokens and the 8-bit cache: 195 us, 4.3 TB/s of half the bytes. There a tile of 32 keys costs a
