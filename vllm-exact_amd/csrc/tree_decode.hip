@@ -223,7 +223,7 @@ __device__ inline bool store_row(const TreeParams& p, const Request& rq, int nod
   }
   return odd != 0.0f && l > 0.0f;  // l is NaN where a score is +inf or NaN, or a page is missing
 }
-// The arguments, read again: for code that is seldom reached and would keep registers through all that comes before.
+// The arguments, read again: for code at the end or seldom reached, which would keep registers through all that comes before.
 __device__ inline TreeParams arguments_again() {
   typedef const __attribute__((address_space(4))) TreeParams Args;
   Args* args = (Args*)__builtin_amdgcn_kernarg_segment_ptr();
@@ -1009,11 +1009,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel_wide(TreePa
   float la = (l[0] + l[1]) + (l[2] + l[3]), lb = la;
   swap32(la, lb);
   const float sum = bad ? __builtin_nanf("") : la + lb;
-  if (row0 + 32 * wave + col >= rows) return;
+  const TreeParams q = arguments_again();
+  int own = col;  // the row's node and head are found again, too
+  asm volatile("" : "+v"(own));
+  own += row0 + 32 * wave;
+  if (own >= rows) return;
+  const int out_node = own / q.G, out_head = g * q.G + own - out_node * q.G;
   const bool alone = rq.L <= keys;
   bool spoiled = false;
-  const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + chunk;
-  if (!alone && half == 0) p.mp[part] = m, p.lp[part] = sum;
+  const int64_t part = ((int64_t)(rq.q0 + out_node) * H + out_head) * q.parts + chunk;
+  if (!alone && half == 0) q.mp[part] = m, q.lp[part] = sum;
 #pragma unroll
   for (int i = 0; i < DB; ++i)
 #pragma unroll
@@ -1035,13 +1040,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_decode_kernel_wide(TreePa
         }
       }
       if (alone)
-        spoiled |= store_row<T>(p, rq, node, head, dim, o, sum);
+        spoiled |= store_row<T>(q, rq, out_node, out_head, dim, o, sum);
       else
-        *reinterpret_cast<v4f*>(p.ap + part * D + dim) = o;
+        *reinterpret_cast<v4f*>(q.ap + part * D + dim) = o;
     }
   if (__builtin_expect(spoiled, 0))
 #pragma unroll 1
-    for (int dim = 4 * half; dim < D; dim += 8) find_specials<T, INT8>(arguments_again(), rq, b, node, head, dim);
+    for (int dim = 4 * half; dim < D; dim += 8) find_specials<T, INT8>(q, rq, b, out_node, out_head, dim);
 }
 
 // The same for 256 dims, with 8 waves of 16 rows and 16 x 16 x 32 MFMAs: two waves a SIMD, where 32 rows leave one. Six
@@ -1291,11 +1296,16 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void tree_decode_kernel_wide_256
   const bool bad = __syncthreads_or(bad_page);
   l = rows_sum(l);
   if (bad) l = __builtin_nanf("");
-  if (row0 + 16 * wave + col >= rows) return;
+  const TreeParams q = arguments_again();
+  int own = col;  // the row's node and head are found again, too
+  asm volatile("" : "+v"(own));
+  own += row0 + 16 * wave;
+  if (own >= rows) return;
+  const int out_node = own / q.G, out_head = g * q.G + own - out_node * q.G;
   const bool alone = rq.L <= keys;
   bool spoiled = false;
-  const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + chunk;
-  if (!alone && grp == 0) p.mp[part] = m, p.lp[part] = l;
+  const int64_t part = ((int64_t)(rq.q0 + out_node) * H + out_head) * q.parts + chunk;
+  if (!alone && grp == 0) q.mp[part] = m, q.lp[part] = l;
 #pragma unroll
   for (int e = 0; e < DB; ++e) {
     const int dim = 16 * e + 4 * grp;
@@ -1315,13 +1325,13 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void tree_decode_kernel_wide_256
       }
     }
     if (alone)
-      spoiled |= store_row<T>(p, rq, node, head, dim, o, l);
+      spoiled |= store_row<T>(q, rq, out_node, out_head, dim, o, l);
     else
-      *reinterpret_cast<v4f*>(p.ap + part * D + dim) = o;
+      *reinterpret_cast<v4f*>(q.ap + part * D + dim) = o;
   }
   if (__builtin_expect(spoiled, 0))
 #pragma unroll 1
-    for (int dim = 4 * grp; dim < D; dim += 16) find_specials<T, INT8>(arguments_again(), rq, b, node, head, dim);
+    for (int dim = 4 * grp; dim < D; dim += 16) find_specials<T, INT8>(q, rq, b, out_node, out_head, dim);
 }
 
 // Joins a row's groups: the strands of a group where workgroups have left them apart, then the groups in order; of the wide
