@@ -317,11 +317,14 @@ int vxa_int8_cache_read(const int8_t* k_cache, int64_t stride_kcb, int64_t strid
  * where bit j of its tree_mask [tokens] is set (null: to the drafted keys up to its own). A node that attends to
  * nothing gives zeros. The cache: the query's type, or int8 with k_scale and v_scale as above (both null: not int8).
  * max_nodes <= 64 and max_seq_len bound T and seq_lens; a request beyond them, shorter than its nodes, or with a block
- * that the cache does not have gets NaN rows. The workspace (on 16 bytes) holds the partial sums of groups of
- * four 512-key segments, four for each group.
+ * that the cache does not have gets NaN rows. max_nodes 0: nothing is done. The workspace (on 16 bytes) holds partial sums:
+ * vxa_tree_decode_call_workspace gives the bytes of a call of n requests, vxa_tree_decode_workspace bytes that are enough
+ * for any n, num_kv_heads and max_nodes (four times as many for a large call).
  */
 int vxa_tree_decode_workspace(int64_t tokens, int64_t num_heads, int64_t head_dim, int64_t max_seq_len,
                               size_t* ws_bytes);
+int vxa_tree_decode_call_workspace(int64_t n, int64_t tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                                   int64_t max_nodes, int64_t max_seq_len, size_t* ws_bytes);
 int vxa_tree_decode(const void* q, int64_t stride_qt, int64_t stride_qh, int q_dtype, const void* k_cache,
                     int64_t stride_kcb, int64_t stride_kcp, int64_t stride_kch, const void* v_cache,
                     int64_t stride_vcb, int64_t stride_vcp, int64_t stride_vch, const float* k_scale,

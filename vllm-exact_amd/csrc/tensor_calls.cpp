@@ -19,7 +19,7 @@ namespace {
 decltype(&vxa_prompt_attention) prompt_attention_fn;
 decltype(&vxa_int8_cache_write) cache_write_fn;
 decltype(&vxa_int8_cache_read) cache_read_fn;
-decltype(&vxa_tree_decode_workspace) tree_workspace_fn;
+decltype(&vxa_tree_decode_call_workspace) tree_workspace_fn;
 decltype(&vxa_tree_decode) tree_decode_fn;
 
 struct Refused {
@@ -216,7 +216,7 @@ int tree_decode(PyObject* const* a) {
   const int out_dtype = dtype_enum(out);
   if (T == 0 || n == 0 || max_nodes == 0) return VXA_OK;
   size_t bytes = 0;
-  const int rc = tree_workspace_fn(T, H, D, max_len, &bytes);
+  const int rc = tree_workspace_fn(n, T, H, KV, D, max_nodes, max_len, &bytes);
   if (rc != VXA_OK) return rc;
   at::Tensor ws;
   if (bytes) ws = at::empty({(int64_t)bytes / 4}, q.options().dtype(at::kFloat));

@@ -78,7 +78,7 @@ struct TreeParams {
   int32_t n, total, KV, G, ns, row_blocks, max_nodes, max_len, wide_rows;
   bool by_size;  // workgroups of whole groups go by their work, the largest first
   bool strands;  // a workgroup for each strand of a group of segments, not for each group
-  int64_t parts;  // partial sums of a row: kWaves for each group
+  int64_t parts;  // partial sums that a row has place for
   bool out_wide;  // the output has the query's type and its rows start on 8 bytes
   float* mp;  // [total][H][parts]
   float* lp;
@@ -736,7 +736,7 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
       const bool spoiled = store_row<T>(p, rq, node, head, 4 * c, s[0].a, s[0].l);
       if (__builtin_expect(spoiled, 0)) find_specials<T, INT8>(arguments_again(), rq, b, node, head, 4 * c);
     } else {
-      const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + group * kWaves + (whole ? 0 : strand);
+      const int64_t part = ((int64_t)(rq.q0 + node) * H + head) * p.parts + (whole ? group : group * kWaves + strand);
       if (c == 0) p.mp[part] = s[0].m, p.lp[part] = s[0].l;
       reinterpret_cast<v4f*>(p.ap)[part * (D / 4) + c] = s[0].a;
     }
@@ -1357,7 +1357,7 @@ __global__ __launch_bounds__(D * GROUPS / 4) void tree_merge_kernel(TreeParams p
   for (int g0 = 0; g0 < groups; g0 += GROUPS) {
     if (g0 + mine < groups) {
       State s[kWaves];
-      const int64_t at = part + (g0 + mine) * kWaves;
+      const int64_t at = part + (g0 + mine) * (apart ? kWaves : 1);
 #pragma unroll
       for (int w = 0; w < kWaves; ++w)
         if (w == 0 || (apart && (!wide || (g0 + mine) * kGroup + w < chunks))) s[w] = State{p.mp[at + w], p.lp[at + w], reinterpret_cast<const v4f*>(p.ap)[(at + w) * kLanes + c]};
@@ -1387,37 +1387,55 @@ int64_t most_chunks(int64_t keys) {
   return std::max(cdiv<int64_t>(few, wide_chunk((int)few)), cdiv<int64_t>(keys, wide_chunk((int)keys)));
 }
 
+int64_t num_segments(int64_t keys) { return std::max<int64_t>(1, cdiv<int64_t>(keys, kSeg)); }
+
+// How a call's rows and keys are split, and the partial sums that a row has place for.
+struct Plan {
+  int64_t narrow, row_blocks, groups, parts;  // narrow: rows that the narrow kernel covers, of requests that do not take the wide one
+  int nq;
+  bool strands, by_size, wide;
+};
+Plan plan_of(int64_t n, int64_t KV, int64_t G, int64_t D, int64_t max_nodes, int64_t max_len) {
+  Plan p;
+  const int64_t rows = max_nodes * G, most = wide_rows((int)D), ns = num_segments(max_len);
+  p.narrow = std::min<int64_t>(rows, most / G * G);
+  p.nq = p.narrow <= 16 ? 1 : 2;
+  p.row_blocks = std::max<int64_t>(1, cdiv<int64_t>(p.narrow, 16 * p.nq));
+  p.wide = rows > most;
+  // A workgroup for each group of segments, or for each of its strands where the former would leave CUs without one. The
+  // order of the sums, and so every bit, is the same. (10 requests of up to 8000 keys, 8 tokens, 320 groups: 54 us in
+  // strands, 45 in groups; 20 of up to 16384, 2 tokens, 1440 groups: 118 and 98; with 256 the same.)
+  p.groups = cdiv<int64_t>(ns, kGroup);
+  p.strands = p.groups > 1 && n * KV * p.row_blocks * p.groups < kManyWorkgroups;
+  // The last rounds of workgroups end together where the large ones have gone first. The search takes a turn for every 64
+  // requests, and there are many rounds where they are many.
+  p.by_size = !p.strands && p.groups > 1 && n <= kSearched;
+  // A single group of segments has no partial sums, but they are few and counted for its chunks in the wide kernel.
+  p.parts = ns <= kGroup ? ns : p.strands ? p.groups * kWaves : std::max(p.groups, p.wide ? most_chunks(max_len) : 0);
+  return p;
+}
+
 template <typename T, bool INT8, int D>
-hipError_t launch_tree(TreeParams p, hipStream_t st) {
-  // The narrow kernel covers the rows of requests that do not take the wide one.
-  const int64_t rows = (int64_t)p.max_nodes * p.G, narrow = std::min<int64_t>(rows, wide_rows(D) / p.G * p.G);
+hipError_t launch_tree(TreeParams p, const Plan& plan, hipStream_t st) {
   p.wide_rows = wide_rows(D);
   const int64_t merges = (int64_t)p.n * p.max_nodes * p.KV * p.G;
   if (merges > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
   const dim3 threads(64 * kWaves);
   {
-    const int nq = narrow <= 16 ? 1 : 2;
-    p.row_blocks = (int32_t)std::max<int64_t>(1, cdiv<int64_t>(narrow, 16 * nq));
-    // A workgroup for each group of segments, or for each of its strands where the former would leave CUs without one. The
-    // order of the sums, and so every bit, is the same. (10 requests of up to 8000 keys, 8 tokens, 320 groups: 54 us in
-    // strands, 45 in groups; 20 of up to 16384, 2 tokens, 1440 groups: 118 and 98; with 256 the same.)
-    const int64_t units = (int64_t)p.KV * p.n, groups = cdiv<int64_t>(p.ns, kGroup);
-    p.strands = groups > 1 && units * p.row_blocks * groups < kManyWorkgroups;
-    // The last rounds of workgroups end together where the large ones have gone first. The search takes a turn for every 64
-    // requests, and there are many rounds where they are many.
-    p.by_size = !p.strands && groups > 1 && p.n <= kSearched;
-    const int64_t blocks = cdiv<int64_t>(units * groups * (p.strands ? kWaves : 1), 8) * 8 * p.row_blocks;
+    p.row_blocks = (int32_t)plan.row_blocks;
+    p.strands = plan.strands, p.by_size = plan.by_size;
+    const int64_t blocks = cdiv<int64_t>((int64_t)p.KV * p.n * plan.groups * (plan.strands ? kWaves : 1), 8) * 8 * p.row_blocks;
     if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
-    if (nq == 1)
+    if (plan.nq == 1)
       hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 1>), dim3((unsigned)blocks), threads, 0, st, p);
     else
       hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 2>), dim3((unsigned)blocks), threads, 0, st, p);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
-  if (rows > wide_rows(D)) {
+  if (plan.wide) {
     TreeParams w = p;
-    w.row_blocks = (int32_t)cdiv<int64_t>(rows, 128);
+    w.row_blocks = (int32_t)cdiv<int64_t>((int64_t)p.max_nodes * p.G, 128);
     const int64_t blocks = cdiv<int64_t>((int64_t)p.KV * p.n * most_chunks(p.max_len), 8) * 8 * w.row_blocks;
     if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
     if constexpr (D == 256)
@@ -1427,7 +1445,7 @@ hipError_t launch_tree(TreeParams p, hipStream_t st) {
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
-  if (p.ns <= (rows > wide_rows(D) ? 1 : kGroup)) return hipSuccess;
+  if (p.ns <= (plan.wide ? 1 : kGroup)) return hipSuccess;
   // Few rows: latency counts, and all their groups are read at once (one row over 16384 keys: 15.7 us -> 14.6). Many rows: the
   // fewer threads that wait for others, the better (16384 rows of 3 groups: 237 us with 16 groups at a time, 219 with 4, 216
   // with 2).
@@ -1439,19 +1457,19 @@ hipError_t launch_tree(TreeParams p, hipStream_t st) {
 }
 
 template <typename T, bool INT8>
-hipError_t dispatch_dim(int64_t D, const TreeParams& p, hipStream_t st) {
-  if (D == 64) return launch_tree<T, INT8, 64>(p, st);
-  if (D == 128) return launch_tree<T, INT8, 128>(p, st);
-  return launch_tree<T, INT8, 256>(p, st);
+hipError_t dispatch_dim(int64_t D, const TreeParams& p, const Plan& plan, hipStream_t st) {
+  if (D == 64) return launch_tree<T, INT8, 64>(p, plan, st);
+  if (D == 128) return launch_tree<T, INT8, 128>(p, plan, st);
+  return launch_tree<T, INT8, 256>(p, plan, st);
 }
 
-int64_t num_segments(int64_t keys) { return std::max<int64_t>(1, cdiv<int64_t>(keys, kSeg)); }
-
-// Partial sums of a row of at most `keys` keys: one for each strand of each group of segments. A single group needs none,
-// but its segments are counted.
-int64_t part_count(int64_t keys) {
-  const int64_t ns = num_segments(keys);
-  return ns <= kGroup ? ns : cdiv<int64_t>(ns, kGroup) * kWaves;
+// Bytes of `parts` partial sums for each row, 0 for one; less than 0 where that is no size of anything.
+int64_t workspace_bytes(int64_t tokens, int64_t H, int64_t D, int64_t parts) {
+  if (parts <= 1) return 0;
+  int64_t bytes;
+  const bool over = __builtin_mul_overflow(tokens, H, &bytes) || __builtin_mul_overflow(bytes, parts, &bytes) ||
+                    __builtin_mul_overflow(bytes, (D + 2) * (int64_t)sizeof(float), &bytes);
+  return over ? -1 : bytes;
 }
 
 }  // namespace
@@ -1459,8 +1477,26 @@ int64_t part_count(int64_t keys) {
 extern "C" int vxa_tree_decode_workspace(int64_t tokens, int64_t num_heads, int64_t head_dim, int64_t max_seq_len,
                                          size_t* ws_bytes) {
   if (tokens < 0 || num_heads <= 0 || head_dim <= 0 || max_seq_len < 0 || !ws_bytes) return VXA_ERR_ARG;
-  const int64_t parts = part_count(max_seq_len);
-  *ws_bytes = parts > 1 ? (size_t)tokens * num_heads * parts * (head_dim + 2) * sizeof(float) : 0;
+  // The most of any plan: a partial sum for each strand of each group of segments.
+  const int64_t ns = num_segments(max_seq_len);
+  const int64_t bytes = workspace_bytes(tokens, num_heads, head_dim, ns <= kGroup ? ns : cdiv<int64_t>(ns, kGroup) * kWaves);
+  if (bytes < 0) return VXA_ERR_UNSUPPORTED;
+  *ws_bytes = (size_t)bytes;
+  return VXA_OK;
+}
+
+extern "C" int vxa_tree_decode_call_workspace(int64_t n, int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                                              int64_t head_dim, int64_t max_nodes, int64_t max_seq_len, size_t* ws_bytes) {
+  if (n < 0 || tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_nodes < 0 || max_seq_len < 0 || !ws_bytes ||
+      num_heads % num_kv_heads != 0)
+    return VXA_ERR_ARG;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return VXA_ERR_UNSUPPORTED;
+  if (n > 0x7FFFFFFFLL || tokens > 0x7FFFFFFFLL || num_heads > (1 << 16) || max_nodes > kMaxNodes || max_seq_len > (1 << 30))
+    return VXA_ERR_UNSUPPORTED;
+  const int64_t bytes = workspace_bytes(tokens, num_heads, head_dim,
+                                        plan_of(n, num_kv_heads, num_heads / num_kv_heads, head_dim, max_nodes, max_seq_len).parts);
+  if (bytes < 0) return VXA_ERR_UNSUPPORTED;
+  *ws_bytes = (size_t)bytes;
   return VXA_OK;
 }
 
@@ -1492,9 +1528,9 @@ extern "C" int vxa_tree_decode(const void* q, int64_t sqt, int64_t sqh, int q_dt
   if ((uintptr_t)q % 16 || (uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || sqt % 8 || sqh % 8 || skb % piece ||
       skp % piece || skh % piece || svb % piece || svp % piece || svh % piece)
     return VXA_ERR_UNSUPPORTED;
-  const int64_t ns = num_segments(max_seq_len);
   size_t need = 0;
-  vxa_tree_decode_workspace(tokens, num_heads, head_dim, max_seq_len, &need);
+  const int rc = vxa_tree_decode_call_workspace(n, tokens, num_heads, num_kv_heads, head_dim, max_nodes, max_seq_len, &need);
+  if (rc != VXA_OK) return rc;
   if (need > 0 && (!ws || ws_bytes < need)) return VXA_ERR_WORKSPACE;
   if (need > 0 && (uintptr_t)ws % 16) return VXA_ERR_UNSUPPORTED;
 
@@ -1511,8 +1547,9 @@ extern "C" int vxa_tree_decode(const void* q, int64_t sqt, int64_t sqh, int q_dt
   p.sl = seq_lens, p.qsl = query_starts, p.mask = tree_mask;
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
   p.n = (int32_t)n, p.total = (int32_t)tokens, p.KV = (int32_t)num_kv_heads, p.G = (int32_t)(num_heads / num_kv_heads);
-  p.ns = (int32_t)ns, p.row_blocks = 1, p.max_nodes = (int32_t)max_nodes, p.max_len = (int32_t)max_seq_len;
-  p.strands = false, p.by_size = false, p.parts = part_count(max_seq_len);
+  const Plan plan = plan_of(n, p.KV, p.G, head_dim, max_nodes, max_seq_len);
+  p.ns = (int32_t)num_segments(max_seq_len), p.row_blocks = 1, p.max_nodes = (int32_t)max_nodes, p.max_len = (int32_t)max_seq_len;
+  p.strands = false, p.by_size = false, p.parts = plan.parts;
   // The weighted values first, on 16 bytes as the workspace is.
   const int64_t parts = tokens * num_heads * p.parts;
   float* w = reinterpret_cast<float*>(ws);
@@ -1523,9 +1560,9 @@ extern "C" int vxa_tree_decode(const void* q, int64_t sqt, int64_t sqh, int q_dt
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   hipError_t err;
   if (q_dtype == VXA_BF16)
-    err = int8 ? dispatch_dim<BF16, true>(head_dim, p, st) : dispatch_dim<BF16, false>(head_dim, p, st);
+    err = int8 ? dispatch_dim<BF16, true>(head_dim, p, plan, st) : dispatch_dim<BF16, false>(head_dim, p, plan, st);
   else
-    err = int8 ? dispatch_dim<FP16, true>(head_dim, p, st) : dispatch_dim<FP16, false>(head_dim, p, st);
+    err = int8 ? dispatch_dim<FP16, true>(head_dim, p, plan, st) : dispatch_dim<FP16, false>(head_dim, p, plan, st);
   if (err == hipErrorInvalidConfiguration) return VXA_ERR_UNSUPPORTED;
   return err == hipSuccess ? VXA_OK : VXA_ERR_LAUNCH;
 }

@@ -54,6 +54,7 @@ EXPORTED = (
     "vxa_int8_cache_write",
     "vxa_int8_cache_read",
     "vxa_tree_decode_workspace",
+    "vxa_tree_decode_call_workspace",
     "vxa_tree_decode",
 )
 
@@ -126,6 +127,7 @@ _SIGNATURES = {
         + [_vp, _i64, _i64] * 2 + [_int, _vp],
     ),
     "vxa_tree_decode_workspace": (_int, [_i64, _i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "vxa_tree_decode_call_workspace": (_int, [_i64] * 7 + [ctypes.POINTER(_sz)]),
     "vxa_tree_decode": (
         _int,
         [_vp, _i64, _i64, _int] + [_vp, _i64, _i64, _i64] * 4 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
@@ -203,7 +205,7 @@ def launch(device, fn, *args):
 
 
 _calls = None
-_CALLED = ("vxa_prompt_attention", "vxa_int8_cache_write", "vxa_int8_cache_read", "vxa_tree_decode_workspace", "vxa_tree_decode")
+_CALLED = ("vxa_prompt_attention", "vxa_int8_cache_write", "vxa_int8_cache_read", "vxa_tree_decode_call_workspace", "vxa_tree_decode")
 
 
 def calls():
