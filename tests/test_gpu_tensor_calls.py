@@ -26,3 +26,17 @@ def test_vmap_is_an_error():
                 torch.vmap(call)(over)
     out = torch.empty(3, 2, 64, device=DEV)
     assert torch.equal(prompt_attention(q[0], k[0], k[0], cu, 1.0, out), torch.zeros_like(out))
+
+
+def test_a_workspace_that_does_not_fit():
+    """Lengths up to 2^30 of many nodes: more than any memory. torch's own exception, as from a tensor of that size."""
+    n, nodes, H, D = 300, 64, 64, 64
+    q = torch.zeros(n * nodes, H, D, dtype=torch.bfloat16, device=DEV)
+    cache = make_cache(2, 16, H, D, DEV)
+    bt, sl = torch.zeros(n, 4, dtype=torch.int32, device=DEV), torch.full((n,), nodes, dtype=torch.int32, device=DEV)
+    qsl, out = torch.arange(0, n * nodes + 1, nodes, dtype=torch.int32, device=DEV), torch.empty_like(q)
+    call = lambda longest: tree_decode(q, *cache[:2], bt, sl, qsl, None, 1.0, out, nodes, longest, *cache[2:])
+    with pytest.raises(torch.OutOfMemoryError):
+        call(1 << 30)
+    call(64)
+    assert (out == 0).all()

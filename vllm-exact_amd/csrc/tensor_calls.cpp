@@ -4,6 +4,7 @@
 //
 // The module holds no code of the kernels: bind() is given the addresses of the loaded library's entry points.
 // Every function returns the entry point's status; what an argument check refuses is raised here.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
@@ -228,21 +229,22 @@ int tree_decode(PyObject* const* a) {
                    out_dtype, out.stride(0), out.stride(1), n, T, H, KV, D, max_nodes, max_len, bytes ? ptr(&ws) : nullptr, bytes);
 }
 
-// fn(arguments) as a Python function of `count` positional arguments; C++ exceptions end here.
+// fn(arguments) as a Python function of `count` positional arguments; C++ exceptions end here, torch's as the Python exceptions
+// that torch makes of them (OutOfMemoryError for a workspace that does not fit).
 template <int (*fn)(PyObject* const*), int count>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t given) {
   if (given != count || !tree_decode_fn) {
     PyErr_SetString(PyExc_TypeError, given != count ? "wrong number of arguments" : "bind() has not been called");
     return nullptr;
   }
+  HANDLE_TH_ERRORS
   try {
     return PyLong_FromLong(fn(args));
   } catch (const Refused& r) {
     PyErr_SetString(r.kind, r.text.c_str());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
   }
-  return nullptr;
+  END_HANDLE_TH_ERRORS
 }
 
 // bind(prompt_attention, cache_write, cache_read, tree_workspace, tree_decode): the entry points' addresses.
