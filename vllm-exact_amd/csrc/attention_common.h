@@ -96,12 +96,10 @@ __device__ inline void static_for(F&& f) {
   }
 }
 
-
 // The two 16-bit element types. Operands of the matrix instructions are held as four dwords of
 // two elements each; products of two such elements are exact in fp32.
 struct BF16 {
   static constexpr uint32_t kExpMask = 0x7F80u, kOne = 0x3F80u;
-  static constexpr int kDtype = VXA_BF16;
   // Values may be as large as floats are: a row's weights stay below one over the number of its keys, so that its sums stay below
   // the largest value. (Values below some 2^-100 lose bits in turn.)
   static __device__ inline float reach(int keys) { return keys <= 1 << 12 ? -12.0f : keys <= 1 << 18 ? -18.0f : -30.0f; }
@@ -121,7 +119,6 @@ struct BF16 {
 };
 struct FP16 {
   static constexpr uint32_t kExpMask = 0x7C00u, kOne = 0x3C00u;
-  static constexpr int kDtype = VXA_F16;
   // Values end at 65504, so weights may be as large as the type holds: many small ones count down to 2^-32 of a row's largest.
   static __device__ inline float reach(int) { return 15.0f; }
   static __device__ inline float to_f32(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
@@ -137,12 +134,6 @@ struct FP16 {
   }
 };
 
-// Whether one of a dword's two elements is an infinity or NaN.
-template <typename T>
-__device__ inline bool any_special(uint32_t w) {
-  constexpr uint32_t m = T::kExpMask;
-  return (w & m) == m || ((w >> 16) & m) == m;
-}
 // Four elements' infinities and NaN, added to `sum`.
 template <typename T>
 __device__ inline void add_specials(v4f& sum, v2u32 w) {

@@ -234,8 +234,9 @@ __global__ __launch_bounds__(256) void int8_read_kernel(CacheRead p) {
               v4u32{T::pack(f[0], f[1]), T::pack(f[2], f[3]), T::pack(f[4], f[5]), T::pack(f[6], f[7])};
         }
       }
-    }  });
-  }
+    }
+  });
+}
 
 template <int DTYPE, int D>
 hipError_t launch_write(CacheWrite p, bool vec, hipStream_t st) {

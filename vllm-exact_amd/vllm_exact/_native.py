@@ -283,6 +283,7 @@ def paged_units_workspace(n, H, KV, D, max_len, split, blk, waves):
 
 @functools.lru_cache(maxsize=1024)
 def tree_workspace(tokens, H, D, max_seq_len):
+    """Bytes that are enough for any vxa_tree_decode of these sizes, for callers of the C entry point."""
     ws = _sz()
     check(lib().vxa_tree_decode_workspace(tokens, H, D, max_seq_len, ctypes.byref(ws)), "tree_decode_workspace")
     return ws.value
