@@ -2,6 +2,7 @@
 // between the lane rows of a wave, and the 16-bit element types with their matrix instructions.
 #pragma once
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.h"
@@ -25,6 +26,16 @@ constexpr float kLowest = -3.402823466e38f;  // -FLT_MAX
 // rescaled. A wave rescales where any of its rows' scores pass, but only those rows move: a row's bits do not depend on its
 // neighbours. The reach is the element type's (BF16, FP16 below).
 constexpr float kSlack = 8.0f;
+
+// The product of sizes, or 2^62 where it would be beyond that.
+inline int64_t product(std::initializer_list<int64_t> sizes) {
+  int64_t n = 1;
+  for (int64_t s : sizes)
+    if (__builtin_mul_overflow(n, s, &n) || n > 1LL << 62) return 1LL << 62;
+  return n;
+}
+// Whether a launch may have so many workgroups of `threads`: the threads of all are a 32-bit number.
+inline bool launchable(int64_t blocks, int threads) { return blocks <= 0xFFFFFFFFLL / threads; }
 
 // x / d for 0 <= x < 2^31 and 1 <= d < 2^31: (2 x mul >> 32) >> shift with 2^shift >= d and mul = 2^(31 + shift) / d rounded
 // up. The excess of mul is below 1, so times 2 x it stays below 2^32 <= 2^(32 + shift) / d: the quotient is exact.

@@ -244,7 +244,7 @@ hipError_t launch_write(CacheWrite p, bool vec, hipStream_t st) {
   p.per_group = (int32_t)std::max<int64_t>(1, 256 / per_token);
   p.by_token = make_divisor(per_token);
   const int64_t blocks = cdiv<int64_t>(p.tokens, p.per_group);
-  if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+  if (!launchable(blocks, 256)) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)blocks, 2), threads(256);
   if (vec)
     hipLaunchKernelGGL((int8_write_kernel<DTYPE, D, true>), grid, threads, 0, st, p);
@@ -258,7 +258,7 @@ hipError_t launch_read(CacheRead p, hipStream_t st) {
   // Fewer tokens a workgroup where 16 would leave places on the GPU empty.
   p.per_group = (int32_t)std::clamp<int64_t>(p.total / 2048, 1, kReadTokens);
   const int64_t blocks = cdiv<int64_t>(p.total, p.per_group);
-  if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+  if (!launchable(blocks, 256)) return hipErrorInvalidConfiguration;
   p.by_token = make_divisor(p.KV * (D / (OUT == VXA_F32 ? 4 : 8)));
   hipLaunchKernelGGL((int8_read_kernel<OUT, D>), dim3((unsigned)blocks), dim3(256), 0, st, p);
   return hipGetLastError();

@@ -538,7 +538,7 @@ hipError_t launch_prompt(int64_t D, PromptParams p, hipStream_t st) {
     // At most this many tiles: each sequence's last one may be part filled.
     p.tiles = (int32_t)std::min<int64_t>(cdiv<int64_t>(p.total, p.rows) + p.n, p.total);
     const int64_t blocks = (int64_t)p.tiles * (p.H / p.heads);
-    if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+    if (!launchable(blocks, 64 * waves)) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * waves), 0, st, p);
     return hipGetLastError();
   };

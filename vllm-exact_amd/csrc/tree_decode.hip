@@ -1406,7 +1406,7 @@ Plan plan_of(int64_t n, int64_t KV, int64_t G, int64_t D, int64_t max_nodes, int
   // order of the sums, and so every bit, is the same. (10 requests of up to 8000 keys, 8 tokens, 320 groups: 54 us in
   // strands, 45 in groups; 20 of up to 16384, 2 tokens, 1440 groups: 118 and 98; with 256 the same.)
   p.groups = cdiv<int64_t>(ns, kGroup);
-  p.strands = p.groups > 1 && n * KV * p.row_blocks * p.groups < kManyWorkgroups;
+  p.strands = p.groups > 1 && product({n, KV, p.row_blocks, p.groups}) < kManyWorkgroups;
   // The last rounds of workgroups end together where the large ones have gone first. The search takes a turn for every 64
   // requests, and there are many rounds where they are many.
   p.by_size = !p.strands && p.groups > 1 && n <= kSearched;
@@ -1418,38 +1418,37 @@ Plan plan_of(int64_t n, int64_t KV, int64_t G, int64_t D, int64_t max_nodes, int
 template <typename T, bool INT8, int D>
 hipError_t launch_tree(TreeParams p, const Plan& plan, hipStream_t st) {
   p.wide_rows = wide_rows(D);
-  const int64_t merges = (int64_t)p.n * p.max_nodes * p.KV * p.G;
-  if (merges > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
-  const dim3 threads(64 * kWaves);
-  {
-    p.row_blocks = (int32_t)plan.row_blocks;
-    p.strands = plan.strands, p.by_size = plan.by_size;
-    const int64_t blocks = cdiv<int64_t>((int64_t)p.KV * p.n * plan.groups * (plan.strands ? kWaves : 1), 8) * 8 * p.row_blocks;
-    if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
-    if (plan.nq == 1)
-      hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 1>), dim3((unsigned)blocks), threads, 0, st, p);
-    else
-      hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 2>), dim3((unsigned)blocks), threads, 0, st, p);
-    const hipError_t err = hipGetLastError();
-    if (err != hipSuccess) return err;
-  }
+  p.row_blocks = (int32_t)plan.row_blocks;
+  p.strands = plan.strands, p.by_size = plan.by_size;
+  TreeParams w = p;
+  w.row_blocks = (int32_t)cdiv<int64_t>((int64_t)p.max_nodes * p.G, 128);
+  // Every launch is looked at before the first.
+  const int64_t blocks = product({cdiv<int64_t>(product({p.KV, p.n, plan.groups, plan.strands ? kWaves : 1}), 8), 8, p.row_blocks});
+  const int64_t wide = product({cdiv<int64_t>(product({p.KV, p.n, most_chunks(p.max_len)}), 8), 8, w.row_blocks});
+  const int64_t merges = product({p.n, p.max_nodes, p.KV, p.G});
+  const int threads = 64 * kWaves, wide_threads = D == 256 ? 64 * kWaves256 : threads;
+  const bool merged = p.ns > (plan.wide ? 1 : kGroup), few = merges <= 2048;
+  if (!launchable(blocks, threads) || (plan.wide && !launchable(wide, wide_threads)) || (merged && !launchable(merges, D * (few ? 16 : 2) / 4)))
+    return hipErrorInvalidConfiguration;
+  if (plan.nq == 1)
+    hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 1>), dim3((unsigned)blocks), dim3(threads), 0, st, p);
+  else
+    hipLaunchKernelGGL((tree_partial_kernel<T, INT8, D, 2>), dim3((unsigned)blocks), dim3(threads), 0, st, p);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
   if (plan.wide) {
-    TreeParams w = p;
-    w.row_blocks = (int32_t)cdiv<int64_t>((int64_t)p.max_nodes * p.G, 128);
-    const int64_t blocks = cdiv<int64_t>((int64_t)p.KV * p.n * most_chunks(p.max_len), 8) * 8 * w.row_blocks;
-    if (blocks > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
     if constexpr (D == 256)
-      hipLaunchKernelGGL((tree_decode_kernel_wide_256<T, INT8>), dim3((unsigned)blocks), dim3(64 * kWaves256), 0, st, w);
+      hipLaunchKernelGGL((tree_decode_kernel_wide_256<T, INT8>), dim3((unsigned)wide), dim3(wide_threads), 0, st, w);
     else
-      hipLaunchKernelGGL((tree_decode_kernel_wide<T, INT8, D>), dim3((unsigned)blocks), threads, 0, st, w);
-    const hipError_t err = hipGetLastError();
+      hipLaunchKernelGGL((tree_decode_kernel_wide<T, INT8, D>), dim3((unsigned)wide), dim3(wide_threads), 0, st, w);
+    err = hipGetLastError();
     if (err != hipSuccess) return err;
   }
-  if (p.ns <= (plan.wide ? 1 : kGroup)) return hipSuccess;
+  if (!merged) return hipSuccess;
   // Few rows: latency counts, and all their groups are read at once (one row over 16384 keys: 15.7 us -> 14.6). Many rows: the
   // fewer threads that wait for others, the better (16384 rows of 3 groups: 237 us with 16 groups at a time, 219 with 4, 216
   // with 2).
-  if (merges <= 2048)
+  if (few)
     hipLaunchKernelGGL((tree_merge_kernel<T, INT8, D, 16>), dim3((unsigned)merges), dim3(D * 16 / 4), 0, st, p);
   else
     hipLaunchKernelGGL((tree_merge_kernel<T, INT8, D, 2>), dim3((unsigned)merges), dim3(D * 2 / 4), 0, st, p);

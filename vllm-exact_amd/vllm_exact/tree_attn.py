@@ -21,7 +21,8 @@ def tree_decode(query, key_cache, value_cache, block_table, seq_lens, query_star
     tree_mask (tokens,) int64, bit j set where the node attends to the request's drafted token j (its own bit included), or
     None: to the drafted tokens up to its own; out (tokens, H, D) fp32, bf16 or fp16. A node that attends to nothing
     gives zeros. max_nodes (at most 64) and max_seq_len (0 or None: paged_attn.MAX_LEN) bound the nodes and seq_lens of every
-    request: one beyond them, or shorter than its nodes, or with a block outside the cache, gets NaN rows. Returns out."""
+    request: one beyond them, or shorter than its nodes, or with a block outside the cache, gets NaN rows; max_nodes 0 does
+    nothing. Returns out."""
     status = (_nx._calls or _nx.calls()).tree_decode(
         query, key_cache, value_cache, block_table, seq_lens, query_start_loc, tree_mask, scale, out, max_nodes,
         max_seq_len or paged_attn.MAX_LEN, key_scale, value_scale)
