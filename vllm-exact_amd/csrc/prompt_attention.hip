@@ -18,10 +18,10 @@
 // product, an error of the size of the output's own rounding (in fp16, weights below 2^-21 of a row's largest are off by up to
 // 2^-32 of it), while its sum takes the fp32 values.
 //
-// What bounds it. One prompt of 8192 tokens (32 heads on 8, 128 dims, bf16) takes 525 us, 1048 TFLOP/s of the scores that
-// count; a large library matrix product reaches 1185 on the same card, and both at a clock well below 2.4 GHz: power. The
-// matrix pipes are busy 52 % of the cycles; the next tile's scores among this one's softmax instructions, in one wave, gave
-// no time back (519 to 540 us). 16 prompts of up to 1024 tokens take 92 us, 577 TFLOP/s: 7 us of every workgroup's 20 go
+// What bounds it. One prompt of 8192 tokens (32 heads on 8, 128 dims, bf16) takes 521 to 545 us on different cards, 1010 to
+// 1055 TFLOP/s of the scores that count; a large library matrix product reaches 1189, and this kernel runs at 1.9 GHz: power.
+// The matrix pipes are busy 52 % of the cycles; the next tile's scores among this one's softmax instructions, in one wave, gave
+// no time back (519 to 540 us). 16 prompts of up to 1024 tokens take 93 us, 570 TFLOP/s: 7 us of every workgroup's 20 go
 // to finding its rows, the first loads and the output.
 
 #include <algorithm>
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
 
 // The same for 256 dims, with 8 waves of 16 rows and 16 x 16 x 32 MFMAs: 32 rows of a wave take 430 registers and leave one
 // wave a SIMD, whose softmax and products follow each other; 16 rows take 201 and leave two, though each reads K and V from
-// LDS for half as many rows. Three prompts of up to 2111 tokens: 119 us -> 90; one of 5000: 650 -> 466 (879 TFLOP/s). With
+// LDS for half as many rows. Three prompts of up to 2111 tokens: 119 us -> 90; one of 5000: 650 -> 470 (870 TFLOP/s). With
 // 64 or 128 dims, where two waves of 32 rows fit, they are faster (8192 tokens, 128 dims: 525 us against 575).
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256(PromptParams p) {

@@ -27,10 +27,11 @@
 // MFMA each: P keeps 16 bits (in fp16 22, or what counts to 2^-32 of the row's largest weight), as the 16-bit output is rounded
 // once from an fp32 sum; the 8-bit cache always takes bf16 parts there, because P vscale can leave the fp16 range.
 //
-// What bounds it (32 heads on 8, 128 dims). 64 requests of up to 8192 keys with one token, 16-bit cache: 330 us, 6.5 TB/s,
-// the rate of reading. With 8 tokens and the 8-bit cache: 195 us, 4.3 TB/s of half the bytes. There a tile of 32 keys costs a
-// wave some 430 vector instructions, 192 of them to make 16-bit operands of its bytes, and 48 MFMAs; 245 registers leave
-// two waves a SIMD. One request of 16384 keys and one token: 14.5 us, a chain of dependent loads and four tiles (10) and a
+// What bounds it (32 heads on 8, 128 dims). 64 requests of 8192 keys with one token, 16-bit cache: 330 us, 6.5 TB/s, the rate
+// at which pages are read. With 8 tokens and the 8-bit cache: 262 us, 4.3 TB/s of half the bytes, two thirds of that rate
+// (4096 to 8192 keys: 197 us, the same). There a tile of 32 keys costs a wave some 430 vector instructions, 192 of them to
+// make 16-bit operands of its bytes, and 48 MFMAs; 245 registers leave two waves a SIMD. The vector instructions alone are
+// half of the cycles, and the waves wait for 36 % of theirs. One request of 16384 keys and one token: 14.5 us, a chain of dependent loads and four tiles (10) and a
 // second launch for the merge (4).
 
 #include <algorithm>
@@ -46,9 +47,9 @@ constexpr int kWaves = 4;
 constexpr int kWaveKeys = kSeg / kWaves;
 constexpr int kMaxNodes = 64;
 // Requests with more rows (nodes times heads of a group) take the wide kernel. 128 dims: 96 and 64 are alike from 97 rows on,
-// 80 rows of 16 requests took 50 us in the narrow kernel and 64 in the wide one. 256 dims, where the narrow kernel has one
-// wave a SIMD for 32 rows: 107 requests of 72 to 144 rows 150 us wide from 33 rows on, 196 from 97 on; 8 of 24 rows
-// 70 us narrow, 104 wide.
+// 80 rows of 16 requests took 50 us in the narrow kernel and 61 in the wide one. 256 dims, where the narrow kernel has one
+// wave a SIMD for 32 rows: 107 requests of 72 to 144 rows 152 us wide from 33 rows on, 198 from 97 on; 8 of 24 rows
+// 70 us narrow, 105 wide.
 constexpr int wide_rows(int d) { return d == 256 ? 32 : 96; }
 constexpr int kWaves256 = 8;    // of its workgroups at 256 dims
 constexpr int kFill = 256;      // keys whose places the wide kernel looks up at a time
@@ -629,7 +630,7 @@ __global__ __launch_bounds__(64 * kWaves, shares_cu(D, NQ, INT8) ? 2 : 1) void t
     clear();
     int tile = first;
     if constexpr (AHEAD && NQ == 1) {
-      // Two tiles a turn, so that no registers are moved (16.4 us -> 15.6 for one row over 16384 keys; with 32 rows the
+      // Two tiles a turn, so that no registers are moved (15.5 us -> 14.6 for one row over 16384 keys; with 32 rows the
       // second copy of the step costs more registers than there are: 216 us -> 233).
       static_assert(kWaveKeys / kTile % 2 == 0);  // a segment of the context alone is whole: an even number of tiles
 #pragma unroll 1
@@ -1445,9 +1446,8 @@ hipError_t launch_tree(TreeParams p, const Plan& plan, hipStream_t st) {
     if (err != hipSuccess) return err;
   }
   if (!merged) return hipSuccess;
-  // Few rows: latency counts, and all their groups are read at once (one row over 16384 keys: 15.7 us -> 14.6). Many rows: the
-  // fewer threads that wait for others, the better (16384 rows of 3 groups: 237 us with 16 groups at a time, 219 with 4, 216
-  // with 2).
+  // Few rows: latency counts, and all their groups are read at once (one row over 16384 keys: 16.7 us -> 14.6). Many rows: the
+  // fewer threads that wait for others, the better (16384 rows of 2 to 5 groups: 218 us with 16 groups at a time, 198 with 2).
   if (few)
     hipLaunchKernelGGL((tree_merge_kernel<T, INT8, D, 16>), dim3((unsigned)merges), dim3(D * 16 / 4), 0, st, p);
   else
