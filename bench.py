@@ -439,17 +439,26 @@ TRAFFIC_SUMMARY = ROOT / "profiles" / "exact_gemm_m256_gate_up_hbm_traffic.md"
 COUNTERS_SUMMARY = ROOT / "profiles" / "exact_gemm_and_attention_counters.md"
 
 
+# The library's sources that no linear is built from: attention, the 8-bit cache and their calls.
+OTHER_SOURCES = {"attention_common.h", "int8_cache.hip", "paged_decode.hip", "prompt_attention.hip", "tensor_calls.cpp",
+                 "tree_decode.hip"}
+
+
+def kernel_sources():
+    """The csrc/ files that the linears' kernels are built from."""
+    files = (ROOT / "vllm-exact_amd" / "csrc").glob("*")
+    return sorted(f for f in files if f.is_file() and f.name not in OTHER_SOURCES)
+
+
 def kernel_sources_sha16():
-    """Hash of every source the HIP library is built from (its csrc/ files and the C header):
-    a traffic figure measured on one build is only reported for a library built from the
-    same sources."""
+    """Hash of the sources that the linears' kernels are built from: a traffic figure measured on
+    one build is only reported for a library whose linears are built from the same sources. Another
+    operator beside them changes nothing here."""
     import hashlib
 
     h = hashlib.sha256()
-    files = sorted((ROOT / "vllm-exact_amd" / "csrc").glob("*")) + [ROOT / "include" / "vllm_exact_amd.h"]
-    for f in files:
-        if f.is_file():
-            h.update(f.name.encode() + b"\0" + f.read_bytes())
+    for f in kernel_sources():
+        h.update(f.name.encode() + b"\0" + f.read_bytes())
     return h.hexdigest()[:16]
 
 
