@@ -102,3 +102,18 @@ def test_an_infinite_scale(nodes, at):
     want = (s["cache"][1][place][0].float() * INF).expand(nodes, 4, 64)
     out = trees.run(s)
     assert torch.equal(as_numbers(out[:, :4]), as_numbers(want)) and torch.equal(out[:, 4:], clean[:, 4:])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_no_score_above_minus_infinity(D):
+    """Where every score is -inf the formula gives no number, infinite values or not."""
+    q, k, v, cu = prompts.make((90,), 2, 1, D, torch.bfloat16)
+    q, k = q.abs() + 0.1, torch.full_like(k, -INF)
+    v[0, 0, 3] = INF
+    assert torch.isnan(prompts.run(q, k, v, cu)).all()
+    for nodes in (2, 40):
+        s = trees.make((600,), (nodes,), 4, 1, D, 16, torch.bfloat16, False)
+        s["q"].abs_().add_(0.1)
+        s["cache"][0][:] = -INF
+        s["cache"][1][int(s["bt"][0, 0]), 3, 0, 5] = INF
+        assert torch.isnan(trees.run(s)).all()

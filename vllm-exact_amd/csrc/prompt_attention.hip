@@ -109,7 +109,7 @@ __device__ inline Tile find_tile(const PromptParams& p, int tile) {
 // that were not looked at, too.
 template <typename T, int D, int STEP>
 __device__ inline void find_specials(const PromptParams& p, int64_t at, int dim0, float sum, const char* values, int64_t stride, int first, int row) {
-  if (__builtin_isnan(sum)) return;  // a score is +inf or NaN: so is the row
+  if (!(sum > 0.0f)) return;  // a score is +inf or NaN, or all are -inf: the row is NaN
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the wave's other lanes have stored there
 #pragma unroll 1
   for (int dim = dim0; dim < D; dim += STEP) {
