@@ -145,6 +145,8 @@ struct FP16 {
   }
 };
 
+// a * x of a sum a that may be an infinity or NaN and then stays what it is, also times 0: a value counts however small its weight.
+__device__ inline float scaled(float a, float x) { return __builtin_isfinite(a) ? a * x : a; }
 // Four elements' infinities and NaN, added to `sum`.
 template <typename T>
 __device__ inline void add_specials(v4f& sum, v2u32 w) {
@@ -167,6 +169,10 @@ template <typename T>
 __device__ inline uint32_t only_finite(uint32_t w) {
   constexpr uint32_t m = T::kExpMask;
   return ((w & m) == m ? 0u : w & 0xFFFFu) | (((w >> 16) & m) == m ? 0u : w & 0xFFFF0000u);
+}
+template <typename T>
+__device__ inline uint32_t only_special(uint32_t w) {  // the infinities and NaN, 0 elsewhere
+  return w ^ only_finite<T>(w);
 }
 template <typename T, int SIGN>
 __device__ inline uint32_t special_flags(uint32_t w) {

@@ -104,20 +104,14 @@ __device__ inline Tile find_tile(const PromptParams& p, int tile) {
   return Tile{0, 0, 0};
 }
 
-// A row after a careful pass, its dims dim0 + 0..3, dim0 + STEP + 0..3, ...: values of its keys from `first` on that are infinities or
-// NaN take the place of what was stored. first is 0 where the row's sums are not finite: infinities met weights of 0 in tiles
-// that were not looked at, too.
-template <typename T, int D, int STEP>
-__device__ inline void find_specials(const PromptParams& p, int64_t at, int dim0, float sum, const char* values, int64_t stride, int first, int row) {
-  if (!(sum > 0.0f)) return;  // a score is +inf or NaN, or all are -inf: the row is NaN
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the wave's other lanes have stored there
+// Four dims of a row after a careful pass: the infinities and NaN among the values of its keys from `masked` on, 8 bytes a key.
+template <typename T>
+__device__ inline void add_masked_specials(float (&o)[4], const char* values, int64_t stride, int masked, int row) {
+  v4f special = {0, 0, 0, 0};
 #pragma unroll 1
-  for (int dim = dim0; dim < D; dim += STEP) {
-    v4f special = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int key = first; key <= row; ++key) add_specials<T>(special, *reinterpret_cast<const v2u32*>(values + key * stride + 2 * dim));
-    store_specials(p.out, p.out_dtype, at + dim, special);
-  }
+  for (int key = masked; key <= row; ++key) add_specials<T>(special, *reinterpret_cast<const v2u32*>(values + key * stride));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] += special[j];
 }
 
 template <typename T, int D>
@@ -206,11 +200,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
     for (int i = 0; i < QS; ++i) qf[i] = (*reinterpret_cast<const v4u32*>(q + 16 * i) & p.q_and) ^ p.q_xor;
   }
   // One tile. MASKED: some of its keys may come after some of the wave's rows.
-  // CAREFUL: values of keys that some rows do not attend to may be infinities or NaN, and 0 times those is NaN; here they
-  // enter the product as 0, and the rows that attend to them find them at the end. The pass that does not look ends with
-  // NaN wherever that mattered.
+  // CAREFUL: values may be infinities or NaN, and 0 times those is NaN, for a key that a row does not attend to as for a weight
+  // that is too small for its type. Here they enter the product as 0. Rows that attend to all of the tile add them with
+  // weights of 1, the others add those that they attend to at the end. The pass that does not look ends with sums that are
+  // not finite wherever that mattered.
   auto step = [&](int t, auto masked_c, auto careful_c) {
     constexpr bool MASKED = decltype(masked_c)::value, CAREFUL = decltype(careful_c)::value;
+    constexpr uint32_t kOnes = T::kOne | T::kOne << 16;
     // Tile t has landed, for every wave, and every wave has read tile t - 1: its buffer takes tile t + 1.
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int buf = t & 1;
@@ -248,7 +244,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
 #pragma unroll
       for (int i = 0; i < 4; ++i) l[i] *= c;
 #pragma unroll
-      for (int i = 0; i < DB; ++i) acc[i] = acc[i] * c;
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = CAREFUL ? scaled(acc[i][r], c) : acc[i][r] * c;
       m = mn;
     }
     v4u32 pf[2 * KU];
@@ -273,8 +271,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
       for (int i = 0; i < DB; ++i) {
         v4u32 a = values(c, i);
         if constexpr (CAREFUL) {
+          v4u32 special;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) a[j] = only_finite<T>(a[j]);
+          for (int j = 0; j < 4; ++j) special[j] = only_special<T>(a[j]), a[j] ^= special[j];
+          if constexpr (!MASKED) acc[i] = T::mfma32(special, v4u32{kOnes, kOnes, kOnes, kOnes}, acc[i]);
         }
         acc[i] = T::mfma32(a, pf[c], acc[i]);
       }
@@ -290,12 +290,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
   const bool careful = __syncthreads_or(odd != 0.0f);
   if (careful) {
     start();
-    for (t = 0; t < full; ++t) step(t, std::false_type{}, std::false_type{});
+    for (t = 0; t < full; ++t) step(t, std::false_type{}, std::true_type{});
     for (; t < tiles; ++t) step(t, std::true_type{}, std::true_type{});
   }
   float la = (l[0] + l[1]) + (l[2] + l[3]), lb = la;
   swap32(la, lb);
-  const float sum = la + lb, inv = 1.0f / sum;
+  const float sum = la + lb, inv = sum > 0.0f ? 1.0f / sum : __builtin_nanf("");  // 0: every score is -inf
   if (row >= len) return;
   const int64_t at = (int64_t)(base + row) * p.sot + (int64_t)head * p.soh;
 #pragma unroll
@@ -309,6 +309,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] = acc[i][r0 + 4 * k + j] * inv;
         const int dim = 32 * i + 2 * r0 + 8 * k + 4 * half;
+        if (careful) add_masked_specials<T>(o, vh + 2 * dim, svt, full * kKeys, row);
         w[k][0] = T::pack(o[0], o[1]), w[k][1] = T::pack(o[2], o[3]);
         if (!p.out_wide) {
 #pragma unroll
@@ -325,14 +326,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prompt_attention_kernel(Prompt
             v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
       }
     }
-  if (careful) {
-    odd = 0.0f;
-#pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) odd = fmaf(acc[i][r], 0.0f, odd);
-    find_specials<T, D, 8>(p, at, 4 * half, sum, vh, svt, odd == 0.0f ? full * kKeys : 0, row);
-  }
 }
 
 // The same for 256 dims, with 8 waves of 16 rows and 16 x 16 x 32 MFMAs: 32 rows of a wave take 430 registers and leave one
@@ -417,6 +410,7 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
   }
   auto step = [&](int t, auto masked_c, auto careful_c) {
     constexpr bool MASKED = decltype(masked_c)::value, CAREFUL = decltype(careful_c)::value;
+    constexpr uint32_t kOnes = T::kOne | T::kOne << 16;
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int buf = t & 1;
     if (t + 1 < tiles) load(t + 1, buf ^ 1);
@@ -450,7 +444,9 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
       const float c = exp2_hw(m - mn);
       l *= c;
 #pragma unroll
-      for (int e = 0; e < DB; ++e) acc[e] = acc[e] * c;
+      for (int e = 0; e < DB; ++e)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[e][r] = CAREFUL ? scaled(acc[e][r], c) : acc[e][r] * c;
       m = mn;
     }
     v4u32 pf[KT / 2];
@@ -473,8 +469,10 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
         const v2u32 lo = read_transposed(at), hi = read_transposed(at + 16 * kRow);
         v4u32 a = {lo.x, lo.y, hi.x, hi.y};
         if constexpr (CAREFUL) {
+          v4u32 special;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) a[j] = only_finite<T>(a[j]);
+          for (int j = 0; j < 4; ++j) special[j] = only_special<T>(a[j]), a[j] ^= special[j];
+          if constexpr (!MASKED) acc[e] = T::mfma16(special, v4u32{kOnes, kOnes, kOnes, kOnes}, acc[e]);
         }
         acc[e] = T::mfma16(a, pf[c], acc[e]);
       }
@@ -490,10 +488,10 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
   const bool careful = __syncthreads_or(odd != 0.0f);
   if (careful) {
     start();
-    for (t = 0; t < full; ++t) step(t, std::false_type{}, std::false_type{});
+    for (t = 0; t < full; ++t) step(t, std::false_type{}, std::true_type{});
     for (; t < tiles; ++t) step(t, std::true_type{}, std::true_type{});
   }
-  const float sum = rows_sum(l), inv = 1.0f / sum;
+  const float sum = rows_sum(l), inv = sum > 0.0f ? 1.0f / sum : __builtin_nanf("");
   if (row >= len) return;
   const int64_t at = (int64_t)(base + row) * p.sot + (int64_t)head * p.soh;
 #pragma unroll
@@ -505,6 +503,7 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = acc[e0 + k][j] * inv;
       const int dim = 16 * (e0 + k) + 4 * grp;
+      if (careful) add_masked_specials<T>(o, vh + 2 * dim, svt, full * kKeys, row);
       w[k][0] = T::pack(o[0], o[1]), w[k][1] = T::pack(o[2], o[3]);
       if (!p.out_wide) {
 #pragma unroll
@@ -520,14 +519,6 @@ __global__ __launch_bounds__(64 * kWaves256, 2) void prompt_attention_kernel_256
       *reinterpret_cast<v4u32*>(reinterpret_cast<uint16_t*>(p.out) + at + 16 * (e0 + (grp & 1)) + 4 * (grp & 2)) =
           v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
     }
-  }
-  if (careful) {
-    odd = 0.0f;
-#pragma unroll
-    for (int e = 0; e < DB; ++e)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) odd = fmaf(acc[e][r], 0.0f, odd);
-    find_specials<T, D, 16>(p, at, 4 * grp, sum, vh, svt, odd == 0.0f ? full * kKeys : 0, row);
   }
 }
 

@@ -237,26 +237,44 @@ __device__ inline void find_specials(const TreeParams& p, const Request& rq, int
   const int g = head / p.G, ctx = rq.L - rq.T;
   const uint64_t seen = p.mask != nullptr ? (uint64_t)p.mask[rq.q0 + node] : (2ull << node) - 1;
   v4f special = {0, 0, 0, 0};
+  constexpr int kAhead = 8;  // keys on their way together
 #pragma unroll 1
   for (int first = 0, page = 0; first < rq.L; first += p.page, ++page) {
     const int64_t block = p.bt[(int64_t)b * p.sbt + page];
     if (block < 0 || block >= p.blocks) continue;
     const char* values = p.vc + block * p.svb + (int64_t)g * p.svh + (INT8 ? 1 : 2) * dim;
+    const float* scales = INT8 ? p.vs + block * p.svsb + (int64_t)g * p.svsh : nullptr;
     const int count = min(p.page, rq.L - first);
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-      const int draft = first + i - ctx;
-      if (draft >= 0 && !((seen >> draft) & 1)) continue;
-      if constexpr (INT8) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(values + i * p.svp);
-        const float scale = p.vs[block * p.svsb + i * p.svsp + (int64_t)g * p.svsh];
+#pragma unroll 1
+    for (int i0 = 0; i0 < count; i0 += kAhead) {
+      v2u32 w[kAhead];  // 16-bit values, or a scale
+      bool any = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float f = (float)(int8_t)(w >> (8 * e)) * scale;
-          if (!__builtin_isfinite(f)) special[e] += f;
+      for (int i = 0; i < kAhead; ++i) {
+        const int at = min(i0 + i, count - 1);
+        if constexpr (INT8)
+          w[i] = v2u32{__float_as_uint(scales[at * p.svsp]), 0};
+        else
+          w[i] = *reinterpret_cast<const v2u32*>(values + at * p.svp);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        any |= INT8 ? !__builtin_isfinite(__uint_as_float(w[i].x)) : (only_special<T>(w[i].x) | only_special<T>(w[i].y)) != 0;
+      if (!any) continue;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int draft = first + i0 + i - ctx;
+        if (i0 + i >= count || (draft >= 0 && !((seen >> draft) & 1))) continue;
+        if constexpr (INT8) {
+          const uint32_t q = *reinterpret_cast<const uint32_t*>(values + (i0 + i) * p.svp);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = (float)(int8_t)(q >> (8 * e)) * __uint_as_float(w[i].x);
+            if (!__builtin_isfinite(f)) special[e] += f;
+          }
+        } else {
+          add_specials<T>(special, w[i]);
         }
-      } else {
-        add_specials<T>(special, *reinterpret_cast<const v2u32*>(values + i * p.svp));
       }
     }
   }
