@@ -274,7 +274,7 @@ int vxa_exact_linear_op_noalloc(const void* x, int x_dtype, int64_t ldx, const i
  * (bf16 or fp16) with element strides of rows and heads; starts [n + 1] int32 on the GPU, the packed rows where the
  * sequences begin and the last one ends. Row i of a sequence attends to its rows 0 .. i. out may be fp32, bf16 or
  * fp16. Rows outside the sequences are not written; starts outside [0, tokens] are clamped to it. head_dim 64, 128 or
- * 256, rows aligned to 16 bytes, else VXA_ERR_UNSUPPORTED. A row's bits depend on its own sequence only.
+ * 256, rows aligned to 16 bytes, else VXA_ERR_UNSUPPORTED. A row's bits depend on its query and the keys and values up to its own.
  */
 int vxa_prompt_attention(const void* q, int64_t stride_qt, int64_t stride_qh, const void* k, int64_t stride_kt,
                          int64_t stride_kh, const void* v, int64_t stride_vt, int64_t stride_vh, int dtype,

@@ -2,7 +2,9 @@
 
 Kernel (libvllm_exact_amd.so, prompt_attention.hip): sequences of different lengths, their rows packed one after the
 other as vLLM passes them, grouped heads, bf16 or fp16, heads of 64, 128 or 256 dims. Scores, the softmax and all sums are fp32 and every score is
-computed once, on the matrix cores. A row's bits depend on its own sequence only, never on the rest of the batch.
+computed once, on the matrix cores. A row's bits depend on its query and on the keys and values up to its own, never on later
+rows or the rest of the batch. Finite values give finite rows; an infinity or NaN among the values that a row attends to is
+what it gets in that dim.
 """
 import torch
 

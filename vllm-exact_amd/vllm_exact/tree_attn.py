@@ -3,7 +3,9 @@
 Kernel (libvllm_exact_amd.so, tree_decode.hip): each request drafts a tree of up to 64 tokens, whose keys and values are
 already in the cache behind its context; every node attends to the context and to those drafted tokens that its mask
 names. One node is plain decoding. The cache holds the query's 16-bit type, or 8 bits with scales (int8_cache). How a
-request's keys are cut and in which order they are summed is fixed by its own length and nodes, and so are its bits.
+request's keys are cut and in which order they are summed is fixed by its own length and number of nodes, and a node's bits do
+not depend on the other nodes' queries. Finite values give finite rows; an infinity or NaN among the values that a node attends
+to is what it gets in that dim.
 """
 import torch
 
