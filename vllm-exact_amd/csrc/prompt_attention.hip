@@ -18,7 +18,7 @@
 // product, an error of the size of the output's own rounding (in fp16, weights below 2^-21 of a row's largest are off by up to
 // 2^-32 of it), while its sum takes the fp32 values.
 //
-// What bounds it. One prompt of 8192 tokens (32 heads on 8, 128 dims, bf16) takes 521 to 545 us on different cards, 1010 to
+// What bounds it. One prompt of 8192 tokens (32 heads on 8, 128 dims, bf16) takes 521 to 555 us on different cards, 990 to
 // 1055 TFLOP/s of the scores that count; a large library matrix product reaches 1189, and this kernel runs at 1.9 GHz: power.
 // The matrix pipes are busy 52 % of the cycles; the next tile's scores among this one's softmax instructions, in one wave, gave
 // no time back (519 to 540 us). 16 prompts of up to 1024 tokens take 93 us, 570 TFLOP/s: 7 us of every workgroup's 20 go
