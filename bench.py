@@ -440,8 +440,8 @@ COUNTERS_SUMMARY = ROOT / "profiles" / "exact_gemm_and_attention_counters.md"
 
 
 # The library's sources that no linear is built from: attention, the 8-bit cache and their calls.
-OTHER_SOURCES = {"attention_common.h", "int8_cache.hip", "paged_decode.hip", "prompt_attention.hip", "tensor_calls.cpp",
-                 "tree_decode.hip"}
+OTHER_SOURCES = {"attention_common.h", "beam_select.hip", "int8_cache.hip", "linear_attention.hip", "paged_decode.hip", "pages.hip",
+                 "prompt_attention.hip", "tensor_calls.cpp", "tree_decode.hip"}
 
 
 def kernel_sources():

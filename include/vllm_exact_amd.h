@@ -336,6 +336,84 @@ int vxa_tree_decode(const void* q, int64_t stride_qt, int64_t stride_qh, int q_d
                     int64_t num_kv_heads, int64_t head_dim, int64_t max_nodes, int64_t max_seq_len, void* ws,
                     size_t ws_bytes, vxa_stream_t stream);
 
+/*
+ * Linear attention with a decay for each head (linear_attn): S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T in fp32,
+ * out_t = scale q_t S_t, heads and strides as in vxa_prompt_attention. States [slots, num_heads, head_dim (k), head_dim (v)]
+ * fp32 by strides of slot and head (elements, multiples of 4); a sequence starts from slot read_slots[i] (null, or a
+ * negative slot: zeros) and ends in write_slots[i] (null, negative: not kept), which may be the slot that it reads. A sequence
+ * with a slot that the pool does not have, or one of whose slots another sequence writes, or that writes a slot which another
+ * reads, gets NaN rows and writes no state.
+ * prompt: sequence i is rows starts[i] .. starts[i + 1]; the workspace (on 16 bytes) holds states between parts of long sequences.
+ * step: sequence i is row i.
+ */
+int vxa_linear_prompt_workspace(int64_t tokens, int64_t num_heads, int64_t head_dim, size_t* ws_bytes);
+int vxa_linear_prompt(const void* q, int64_t stride_qt, int64_t stride_qh, const void* k, int64_t stride_kt,
+                      int64_t stride_kh, const void* v, int64_t stride_vt, int64_t stride_vh, int dtype,
+                      const int32_t* starts, int64_t n, int64_t tokens, const float* log_decay, float scale, void* out,
+                      int out_dtype, int64_t stride_ot, int64_t stride_oh, float* state, int64_t slots,
+                      int64_t stride_ss, int64_t stride_sh, const int32_t* read_slots, const int32_t* write_slots,
+                      int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, void* ws, size_t ws_bytes,
+                      vxa_stream_t stream);
+int vxa_linear_step(const void* q, int64_t stride_qt, int64_t stride_qh, const void* k, int64_t stride_kt,
+                    int64_t stride_kh, const void* v, int64_t stride_vt, int64_t stride_vh, int dtype, int64_t n,
+                    const float* log_decay, float scale, void* out, int out_dtype, int64_t stride_ot,
+                    int64_t stride_oh, float* state, int64_t slots, int64_t stride_ss, int64_t stride_sh,
+                    const int32_t* read_slots, const int32_t* write_slots, int64_t num_heads, int64_t num_kv_heads,
+                    int64_t head_dim, vxa_stream_t stream);
+
+/*
+ * Beam search's selection (beam.beam_select): of all continuations (beam b, token v) of a request, with the score
+ * scores[b] + x_bv - log sum_u exp(x_bu) in more than 32 bits, the `count` (<= 64) best in order; equal scores by (b, v).
+ * logits [n * beams, vocab] with row stride stride_row (fp32, bf16 or fp16), scores [n * beams]; out_scores, out_parents (the
+ * logits' row) and out_tokens [n, count]. A beam of score -inf has no continuations, nor a token of logit -inf; where a request
+ * has fewer than `count`, the rest is -inf, -1, -1. A request with a NaN or +inf among the logits or scores of its other beams
+ * gets NaN, -1, -1. The workspace is on 16 bytes.
+ */
+int vxa_beam_select_workspace(int64_t n, int64_t beams, int64_t vocab, int64_t count, size_t* ws_bytes);
+int vxa_beam_select(const void* logits, int64_t stride_row, int dtype, const float* scores, int64_t n, int64_t beams,
+                    int64_t vocab, int64_t count, float* out_scores, int32_t* out_parents, int64_t* out_tokens,
+                    void* ws, size_t ws_bytes, vxa_stream_t stream);
+
+/*
+ * Pages of caches (pages). A cache is given as vxa_cache_view's, rows of row_bytes bytes of each token and head found by
+ * strides in bytes from a block, a place in it and a head: as many views as there are tensors and layers. ref_count
+ * [num_blocks] says how many hold a page, 0: it is free. Rows of a block table name the pages of seq_lens tokens.
+ *
+ * copy: page source[i] to target[i] in every view. Pairs with a page that the cache does not have are skipped; of pairs with
+ * one target the last counts. No page is the source of one pair and the target of another.
+ * fork: row r of out_table takes the pages of row parents[r] (negative, or no row: an empty one) and its length. Whole pages are
+ * shared; a page that the length ends in is copied to the lowest free page, but for the first row of a parent where nobody else
+ * holds that page. Rows r without children let go of their pages. Entries past a row's pages are -1.
+ * out_table and out_lens are not block_table and seq_lens.
+ * resize: rows that get longer take the lowest free pages (by ref_count as it was), in the order of rows and places, shorter ones
+ * let go of theirs. Rows have at most `cols` pages. out_table may be block_table.
+ * In both, out_ref_count may be ref_count, and `missing` [1] is the number of places that found no free page: they are -1.
+ * keep: of the request's last T = starts[i + 1] - starts[i] <= 64 cached tokens those with bit j of keep[i] set move to
+ * the places behind the others, in order, and out_lens is the length with them alone (not seq_lens itself). A request with
+ * more tokens than that, or fewer cached ones, stays as it is. No other request holds the pages of these tokens.
+ */
+typedef struct {
+  void* data;
+  int64_t stride_block, stride_token, stride_head; /* bytes */
+  int64_t heads, row_bytes;
+} vxa_cache_view;
+int vxa_pages_copy(const vxa_cache_view* caches, int64_t count, int64_t num_blocks, int64_t block_size,
+                   const int32_t* source, const int32_t* target, int64_t n, vxa_stream_t stream);
+int vxa_pages_fork_workspace(int64_t rows, int64_t new_rows, size_t* ws_bytes);
+int vxa_pages_fork(const vxa_cache_view* caches, int64_t count, const int32_t* block_table, int64_t stride_bt,
+                   int64_t cols, const int32_t* seq_lens, int64_t rows, const int32_t* parents, int64_t new_rows,
+                   const int32_t* ref_count, int64_t num_blocks, int64_t block_size, int32_t* out_table,
+                   int64_t stride_ot, int32_t* out_lens, int32_t* out_ref_count, int32_t* missing, void* ws,
+                   size_t ws_bytes, vxa_stream_t stream);
+int vxa_pages_resize_workspace(int64_t rows, int64_t num_blocks, size_t* ws_bytes);
+int vxa_pages_resize(const int32_t* block_table, int64_t stride_bt, int64_t cols, const int32_t* seq_lens,
+                     const int32_t* new_lens, int64_t rows, const int32_t* ref_count, int64_t num_blocks,
+                     int64_t block_size, int32_t* out_table, int64_t stride_ot, int32_t* out_ref_count,
+                     int32_t* missing, void* ws, size_t ws_bytes, vxa_stream_t stream);
+int vxa_pages_keep(const vxa_cache_view* caches, int64_t count, const int32_t* block_table, int64_t stride_bt,
+                   int64_t cols, const int32_t* seq_lens, const int32_t* starts, const int64_t* keep, int64_t n,
+                   int64_t num_blocks, int64_t block_size, int32_t* out_lens, vxa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,325 @@
+// Beam search's selection over beams and vocabulary (gfx950).
+//
+//   score(b, v) = scores[b] + x_bv - log sum_u exp(x_bu)
+// for the beams b of a request; the `count` largest, in order, equal scores by (b, v). An fp64 score of a beam's log-sum, whose
+// terms are fp32 and whose sums are fp64, orders beams against each other; within a beam the logits themselves do.
+//
+// A row of logits is cut into slices, a workgroup each. A thread holds its values in registers, so the logits are read
+// once: maximum, sum of exponentials, and the slice's `count` largest. Those are among the values that are at least the
+// count-th largest of a wave's 64 lane maxima, a handful more than `count`. A second kernel, a workgroup for each request,
+// joins the slices' sums and picks from their candidates in the same way.
+// A slice's place goes by the vocabulary alone, so a row's sums are the same bits in any batch and at any alignment.
+
+#include "attention_common.h"
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kEach = 32;                  // values of a thread, in runs of 8
+constexpr int kSlice = kThreads * kEach;   // values of a workgroup
+constexpr int kMost = 64;                  // of `count`: a wave has so many lane maxima
+constexpr int kWaveList = 128;             // candidates that a wave may list; more (many equal values) are picked one by one
+constexpr int kMostSlices = 4096;          // of a request
+
+typedef unsigned long long u64;
+
+struct BeamParams {
+  const void* logits;
+  int64_t stride;
+  const float* scores;
+  int32_t n, beams, vocab, count, slices;
+  double* sums;   // [n * beams][slices][waves]: of exp(x - top)
+  float* tops;    // [n * beams][slices][waves]: the largest value, -inf: none
+  u64* keys;      // [n * beams][slices][count], the largest first, 0: none
+  float* out_scores;
+  int32_t* out_parents;
+  int64_t* out_tokens;
+};
+
+// Order of floats as whole numbers; -inf is 0, which is no candidate. Keys order by value, then the lower place first.
+__device__ inline uint32_t order_of(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);  // -0 is 0
+  return x == -__builtin_huge_valf() ? 0u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ inline float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+__device__ inline u64 key_of(uint32_t order, uint32_t place) { return order ? (u64)order << 32 | (uint32_t)~place : 0; }
+
+__device__ inline u64 shfl_u64(u64 x, int lane) {
+  return (u64)(uint32_t)__builtin_amdgcn_ds_bpermute(lane << 2, (int)(x >> 32)) << 32 |
+         (uint32_t)__builtin_amdgcn_ds_bpermute(lane << 2, (int)(uint32_t)x);
+}
+__device__ inline u64 wave_max(u64 x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) {
+    const u64 y = shfl_u64(x, lane ^ m);
+    x = y > x ? y : x;
+  }
+  return x;
+}
+__device__ inline double wave_sum(double x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) x += __builtin_bit_cast(double, shfl_u64(__builtin_bit_cast(u64, x), lane ^ m));
+  return x;
+}
+
+// exp(d) for d <= 0, off by a few 2^-25: the product with log2(e) is split into a whole part and a rest that keeps its bits.
+__device__ inline float exp_of(float d) {
+  constexpr float kLog2e = 1.44269504f, kRest = 1.92596303e-8f;  // their sum: log2(e) to 48 bits
+  d = d < -200.0f ? -200.0f : d;  // 0, also of -inf; a NaN stays one
+  const float whole = __builtin_rintf(d * kLog2e);
+  return __builtin_amdgcn_ldexpf(exp2_hw(fmaf(d, kRest, fmaf(d, kLog2e, -whole))), (int)whole);
+}
+
+template <int DTYPE>
+__global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamParams p) {
+  __shared__ u64 s_list[kWaves * kWaveList];
+  __shared__ int s_count;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int slice = blockIdx.x % p.slices, row = blockIdx.x / p.slices;
+  if (threadIdx.x == 0) s_count = 0;
+  __syncthreads();
+
+  // Run r of a thread: places slice * kSlice + r * 8 * kThreads + 8 * thread + 0..7.
+  float x[kEach];
+  const int64_t base = (int64_t)row * p.stride;
+#pragma unroll
+  for (int r = 0; r < kEach / 8; ++r) {
+    const int place = slice * kSlice + (r * kThreads + (int)threadIdx.x) * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float v = kNegInf;
+      if (place + j < p.vocab) {
+        if (DTYPE == VXA_F32)
+          v = reinterpret_cast<const float*>(p.logits)[base + place + j];
+        else if (DTYPE == VXA_BF16)
+          v = bf16_to_f32(reinterpret_cast<const uint16_t*>(p.logits)[base + place + j]);
+        else
+          v = (float)reinterpret_cast<const _Float16*>(p.logits)[base + place + j];
+      }
+      x[8 * r + j] = v;
+    }
+  }
+  auto place_of = [&](int i) { return (uint32_t)(slice * kSlice + (i / 8 * kThreads + (int)threadIdx.x) * 8 + i % 8); };
+
+  float top = kNegInf;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) top = fmaxf(top, x[i]);
+  const uint32_t mine = order_of(top);
+  const float most = value_of((uint32_t)(wave_max((u64)mine << 32 | 1) >> 32));  // of order 0: a NaN, and then nothing is summed
+  const float ref = __any(mine != 0) ? most : 0.0f;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kEach; i += 4) {
+    float part = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part += exp_of(x[i + j] - ref);
+    sum += (double)part;
+  }
+  sum = wave_sum(sum);
+  const bool any = __any(mine != 0);
+  if (lane == 0) p.tops[(int64_t)blockIdx.x * kWaves + wave] = any ? most : kNegInf, p.sums[(int64_t)blockIdx.x * kWaves + wave] = sum;
+
+  // The count-th largest order among the lanes' maxima, bit by bit; at least 1.
+  uint32_t bar = 0;
+#pragma unroll
+  for (int b = 31; b >= (DTYPE == VXA_F32 ? 0 : 12); --b)
+    if (__popcll(__ballot(mine >= (bar | 1u << b))) >= p.count) bar |= 1u << b;
+  if (bar == 0) bar = 1;
+  int many = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) many += order_of(x[i]) >= bar;
+  const int before = wave_scan(many, [](int a, int b) { return a + b; });
+  const int all = __builtin_amdgcn_readlane(before, 63);
+  if (all <= kWaveList) {
+    int at = 0;
+    if (lane == 0 && all) at = atomicAdd(&s_count, all);
+    at = __builtin_amdgcn_readfirstlane(at) + before - many;
+    if (many) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (order_of(x[i]) >= bar) s_list[at++] = key_of(order_of(x[i]), place_of(i));
+    }
+  } else {  // many values equal the bar: one after the other, each the largest below the last
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&s_count, p.count);
+    at = __builtin_amdgcn_readfirstlane(at);
+    u64 last = ~0ull;
+    for (int c = 0; c < p.count; ++c) {
+      u64 best = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const u64 key = key_of(order_of(x[i]), place_of(i));
+        if (key < last && key > best) best = key;
+      }
+      last = wave_max(best);
+      if (lane == 0) s_list[at + c] = last;
+    }
+  }
+  __syncthreads();
+
+  // A candidate's rank is how many are larger.
+  const int listed = s_count;
+  u64* keys = p.keys + (int64_t)blockIdx.x * p.count;
+  for (int i = threadIdx.x; i < listed; i += kThreads) {
+    const u64 key = s_list[i];
+    int rank = 0;
+    for (int j = 0; j < listed; ++j) rank += s_list[j] > key;
+    if (key != 0 && rank < p.count) keys[rank] = key;
+  }
+  int valid = 0;
+  for (int i = threadIdx.x; i < listed; i += kThreads) valid += s_list[i] != 0;
+  valid = __syncthreads_count(valid > 0) + __syncthreads_count(valid > 1);
+  for (int i = valid + (int)threadIdx.x; i < p.count; i += kThreads) keys[i] = 0;
+}
+
+// Order of fp64 scores as whole numbers; -inf is 0.
+__device__ inline u64 order_of(double x) {
+  const u64 u = __builtin_bit_cast(u64, x + 0.0);
+  return x == -__builtin_huge_val() ? 0 : u ^ ((u64)((int64_t)u >> 63) | 0x8000000000000000ull);
+}
+__device__ inline double score_of(u64 o) { return __builtin_bit_cast(double, o >> 63 ? o ^ 0x8000000000000000ull : ~o); }
+
+constexpr int kJoin = 1024;
+
+__global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamParams p) {
+  // Of beam b: its largest logit, the log of its sum of exp(x - largest), its score (-inf: no continuations).
+  __shared__ float s_top[kMost * 16];
+  __shared__ double s_log[kMost * 16], s_score[kMost * 16];
+  __shared__ u64 s_order[kMostSlices];        // of the slices' best, then of the candidates
+  __shared__ uint32_t s_place[kMostSlices];   // beam * vocab + token
+  __shared__ int s_count, s_bar, s_nan;
+  const int request = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row0 = (int64_t)request * p.beams;
+  if (threadIdx.x == 0) s_count = 0, s_bar = -1, s_nan = 0;
+  __syncthreads();
+  for (int b = wave; b < p.beams; b += kJoin / 64) {
+    const int parts = p.slices * kWaves;
+    const float* tops = p.tops + (row0 + b) * parts;
+    const double* sums = p.sums + (row0 + b) * parts;
+    float m = kNegInf;
+    for (int i = lane; i < parts; i += 64) m = fmaxf(m, tops[i]);
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) m = fmaxf(m, shfl_xor_f32(m, k));
+    double s = 0.0;
+    for (int i = lane; i < parts; i += 64) s += tops[i] == kNegInf ? sums[i] : sums[i] * exp((double)tops[i] - (double)m);
+    s = wave_sum(s);
+    const double score = s == 0.0 ? -__builtin_huge_val() : (double)p.scores[row0 + b];  // no token, or a beam that has ended
+    const double l = log(s);
+    if (lane == 0) {
+      s_top[b] = m, s_log[b] = l, s_score[b] = score;
+      if (score != -__builtin_huge_val() && !(score - l - (double)m < __builtin_huge_val() && l == l)) s_nan = 1;
+    }
+  }
+  __syncthreads();
+  const int64_t out = (int64_t)request * p.count;
+  if (s_nan) {
+    for (int i = threadIdx.x; i < p.count; i += kJoin) p.out_scores[out + i] = __builtin_nanf(""), p.out_parents[out + i] = -1, p.out_tokens[out + i] = -1;
+    return;
+  }
+  const int groups = p.beams * p.slices;
+  const u64* keys = p.keys + row0 * p.slices * p.count;
+  auto score = [&](int group, int rank, u64& order, uint32_t& place) {
+    const u64 key = keys[(int64_t)group * p.count + rank];
+    const int b = group / p.slices;
+    // the differences first: they are exact, or nearly, where logits are large
+    order = key && s_score[b] != -__builtin_huge_val() ? order_of(s_score[b] + (((double)value_of((uint32_t)(key >> 32)) - (double)s_top[b]) - s_log[b])) : 0;
+    place = (uint32_t)b * (uint32_t)p.vocab + ~(uint32_t)key;
+  };
+  auto above = [](u64 o, uint32_t q, u64 order, uint32_t place) { return o > order || (o == order && q < place); };
+  for (int g = threadIdx.x; g < groups; g += kJoin) score(g, 0, s_order[g], s_place[g]);
+  __syncthreads();
+  // The slice whose best is the count-th: no candidate below it is among the best.
+  for (int g = threadIdx.x; g < groups; g += kJoin) {
+    const u64 order = s_order[g];
+    const uint32_t place = s_place[g];
+    int rank = 0;
+    if (order)
+      for (int j = 0; j < groups; ++j) rank += above(s_order[j], s_place[j], order, place);
+    if (order && rank == p.count - 1) s_bar = g;
+  }
+  __syncthreads();
+  const int bar = s_bar;
+  const u64 least = bar >= 0 ? s_order[bar] : 1;
+  const uint32_t least_place = bar >= 0 ? s_place[bar] : ~0u;
+  __syncthreads();
+  // At most count slices have candidates from there on, of count each.
+  for (int i = threadIdx.x; i < groups * p.count; i += kJoin) {
+    u64 order;
+    uint32_t place;
+    score(i / p.count, i % p.count, order, place);
+    if (order && !above(least, least_place, order, place)) {
+      const int at = atomicAdd(&s_count, 1);
+      s_order[at] = order, s_place[at] = place;
+    }
+  }
+  __syncthreads();
+  const int listed = s_count;
+  for (int i = threadIdx.x; i < listed; i += kJoin) {
+    const u64 order = s_order[i];
+    const uint32_t place = s_place[i];
+    int rank = 0;
+    for (int j = 0; j < listed; ++j) rank += above(s_order[j], s_place[j], order, place);
+    if (rank < p.count) {
+      p.out_scores[out + rank] = (float)score_of(order);
+      p.out_parents[out + rank] = (int32_t)(row0 + place / p.vocab);
+      p.out_tokens[out + rank] = place % p.vocab;
+    }
+  }
+  for (int i = listed + (int)threadIdx.x; i < p.count; i += kJoin)
+    p.out_scores[out + i] = kNegInf, p.out_parents[out + i] = -1, p.out_tokens[out + i] = -1;
+}
+
+int64_t slices_of(int64_t vocab) { return cdiv<int64_t>(vocab, kSlice); }
+
+int check_sizes(int64_t n, int64_t beams, int64_t vocab, int64_t count) {
+  if (n < 0 || beams <= 0 || vocab <= 0 || count <= 0) return VXA_ERR_ARG;
+  if (count > kMost || beams > kMost * 16 || vocab > (1LL << 31) - kSlice || beams * vocab >= 1LL << 31 || beams * slices_of(vocab) > kMostSlices ||
+      n > (1 << 30) || n * beams > (1LL << 31) - 1)
+    return VXA_ERR_UNSUPPORTED;
+  return VXA_OK;
+}
+
+}  // namespace
+
+extern "C" int vxa_beam_select_workspace(int64_t n, int64_t beams, int64_t vocab, int64_t count, size_t* ws_bytes) {
+  const int rc = check_sizes(n, beams, vocab, count);
+  if (rc != VXA_OK || !ws_bytes) return rc != VXA_OK ? rc : VXA_ERR_ARG;
+  const int64_t slices = product({n, beams, slices_of(vocab)});
+  *ws_bytes = (size_t)product({slices, 8 * count + 12 * kWaves});
+  return VXA_OK;
+}
+
+extern "C" int vxa_beam_select(const void* logits, int64_t stride_row, int dtype, const float* scores, int64_t n, int64_t beams,
+                               int64_t vocab, int64_t count, float* out_scores, int32_t* out_parents, int64_t* out_tokens, void* ws,
+                               size_t ws_bytes, vxa_stream_t stream) {
+  size_t bytes = 0;
+  const int rc = vxa_beam_select_workspace(n, beams, vocab, count, &bytes);
+  if (rc != VXA_OK) return rc;
+  if (dtype != VXA_F32 && dtype != VXA_BF16 && dtype != VXA_F16) return VXA_ERR_ARG;
+  if (n == 0) return VXA_OK;
+  if (!logits || !scores || !out_scores || !out_parents || !out_tokens) return VXA_ERR_ARG;
+  if (!ws || (uintptr_t)ws % 16 || ws_bytes < bytes) return VXA_ERR_WORKSPACE;
+  BeamParams p;
+  p.logits = logits, p.stride = stride_row, p.scores = scores;
+  p.n = (int32_t)n, p.beams = (int32_t)beams, p.vocab = (int32_t)vocab, p.count = (int32_t)count, p.slices = (int32_t)slices_of(vocab);
+  const int64_t blocks = n * beams * p.slices;
+  if (!launchable(blocks, kThreads) || !launchable(n, kJoin)) return VXA_ERR_UNSUPPORTED;
+  p.sums = reinterpret_cast<double*>(ws);
+  p.keys = reinterpret_cast<u64*>(p.sums + blocks * kWaves);
+  p.tops = reinterpret_cast<float*>(p.keys + blocks * count);
+  p.out_scores = out_scores, p.out_parents = out_parents, p.out_tokens = out_tokens;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)blocks), threads(kThreads);
+  if (dtype == VXA_F32)
+    hipLaunchKernelGGL(beam_slice_kernel<VXA_F32>, grid, threads, 0, st, p);
+  else if (dtype == VXA_BF16)
+    hipLaunchKernelGGL(beam_slice_kernel<VXA_BF16>, grid, threads, 0, st, p);
+  else
+    hipLaunchKernelGGL(beam_slice_kernel<VXA_F16>, grid, threads, 0, st, p);
+  VXA_CHECK_LAUNCH();
+  hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)n), dim3(kJoin), 0, st, p);
+  VXA_CHECK_LAUNCH();
+  return VXA_OK;
+}

@@ -6,12 +6,15 @@
 // Every function returns the entry point's status; what an argument check refuses is raised here.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <string>
+#include <vector>
 
 #include "../../include/vllm_exact_amd.h"
 
@@ -22,6 +25,17 @@ decltype(&vxa_int8_cache_write) cache_write_fn;
 decltype(&vxa_int8_cache_read) cache_read_fn;
 decltype(&vxa_tree_decode_call_workspace) tree_workspace_fn;
 decltype(&vxa_tree_decode) tree_decode_fn;
+decltype(&vxa_linear_prompt_workspace) linear_workspace_fn;
+decltype(&vxa_linear_prompt) linear_prompt_fn;
+decltype(&vxa_linear_step) linear_step_fn;
+decltype(&vxa_beam_select_workspace) beam_workspace_fn;
+decltype(&vxa_beam_select) beam_select_fn;
+decltype(&vxa_pages_copy) pages_copy_fn;
+decltype(&vxa_pages_fork_workspace) fork_workspace_fn;
+decltype(&vxa_pages_fork) pages_fork_fn;
+decltype(&vxa_pages_resize_workspace) resize_workspace_fn;
+decltype(&vxa_pages_resize) pages_resize_fn;
+decltype(&vxa_pages_keep) pages_keep_fn;
 
 struct Refused {
   PyObject* kind;
@@ -229,6 +243,212 @@ int tree_decode(PyObject* const* a) {
                    out_dtype, out.stride(0), out.stride(1), n, T, H, KV, D, max_nodes, max_len, bytes ? ptr(&ws) : nullptr, bytes);
 }
 
+// What linear_prompt and linear_step share; `states` may be null.
+struct Linear {
+  const at::Tensor &q, &k, &v, &decay, &out;
+  double scale;
+  const at::Tensor *state, *read, *write;
+};
+void check_linear(const char* what, const Linear& x, int64_t n, const at::Tensor* cu) {
+  check_gpu(what, {&x.q, &x.k, &x.v, cu, &x.decay, &x.out, x.state, x.read, x.write}, "linear_attention_torch");
+  if (!is16(x.q) || x.k.scalar_type() != x.q.scalar_type() || x.v.scalar_type() != x.q.scalar_type())
+    refuse(what, ": query, key and value must be all bf16 or all fp16", PyExc_NotImplementedError);
+  if (x.q.dim() != 3 || x.k.dim() != 3 || x.v.sizes() != x.k.sizes() || x.out.sizes() != x.q.sizes() || x.k.size(0) != x.q.size(0) ||
+      x.k.size(2) != x.q.size(2) || x.k.size(1) == 0 || x.q.size(1) == 0 || x.q.size(1) % x.k.size(1) != 0)
+    refuse(what, ": inconsistent shapes");
+  for (const at::Tensor* t : {&x.q, &x.k, &x.v, &x.out})
+    if (t->size(2) && t->stride(2) != 1) refuse(what, ": the head dimension must be contiguous");
+  const int64_t H = x.q.size(1), D = x.q.size(2);
+  if (!vector_of(x.decay, at::kFloat, H)) refuse(what, ": log_decay must be a contiguous fp32 vector, one number for each head");
+  if ((x.read || x.write) && !x.state) refuse(what, ": slots need a pool of states");
+  if (x.state) {
+    const at::Tensor& s = *x.state;
+    if (s.scalar_type() != at::kFloat) refuse(what, ": states must be fp32", PyExc_NotImplementedError);
+    if (s.dim() != 4 || s.size(1) != H || s.size(2) != D || s.size(3) != D || s.stride(3) != 1 || s.stride(2) != D)
+      refuse(what, ": states are (slots, H, D, D), each matrix contiguous");
+  }
+  for (const at::Tensor* t : {x.read, x.write})
+    if (t && !vector_of(*t, at::kInt, n)) refuse(what, ": slots must be contiguous int32 vectors, one for each sequence");
+}
+
+int linear_prompt(PyObject* const* a) {
+  const char* what = "linear_prompt";
+  const at::Tensor& cu = *tensor(what, a[3]);
+  const Linear x{*tensor(what, a[0]),   *tensor(what, a[1]),       *tensor(what, a[2]),       *tensor(what, a[4]),      *tensor(what, a[6]),
+                 number(what, a[5]), tensor(what, a[7], true), tensor(what, a[8], true), tensor(what, a[9], true)};
+  if (cu.scalar_type() != at::kInt || cu.dim() != 1 || !cu.is_contiguous() || cu.size(0) == 0)
+    refuse(what, ": cu_seqlens must be a contiguous int32 vector of the n + 1 starts");
+  const int64_t n = cu.size(0) - 1;
+  check_linear(what, x, n, &cu);
+  const int out_dtype = dtype_enum(x.out);
+  const int64_t T = x.q.size(0), H = x.q.size(1), D = x.q.size(2);
+  if (n == 0) return VXA_OK;
+  size_t bytes = 0;
+  const int rc = linear_workspace_fn(T, H, D, &bytes);
+  if (rc != VXA_OK) return rc;
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes / 4}, x.q.options().dtype(at::kFloat));
+  return on_device(x.q, linear_prompt_fn, ptr(&x.q), x.q.stride(0), x.q.stride(1), ptr(&x.k), x.k.stride(0), x.k.stride(1), ptr(&x.v),
+                   x.v.stride(0), x.v.stride(1), dtype_enum(x.q), ptr<int32_t>(&cu), n, T, ptr<float>(&x.decay), (float)x.scale, ptr(&x.out),
+                   out_dtype, x.out.stride(0), x.out.stride(1), ptr<float>(x.state), x.state ? x.state->size(0) : 0, stride(x.state, 0),
+                   stride(x.state, 1), ptr<int32_t>(x.read), ptr<int32_t>(x.write), H, x.k.size(1), D, bytes ? ptr(&ws) : nullptr, bytes);
+}
+
+int linear_step(PyObject* const* a) {
+  const char* what = "linear_step";
+  const Linear x{*tensor(what, a[0]),   *tensor(what, a[1]), *tensor(what, a[2]),       *tensor(what, a[3]),      *tensor(what, a[5]),
+                 number(what, a[4]), tensor(what, a[6]),  tensor(what, a[7], true), tensor(what, a[8], true)};
+  check_linear(what, x, x.q.dim() ? x.q.size(0) : 0, nullptr);
+  const int out_dtype = dtype_enum(x.out);
+  const int64_t n = x.q.size(0);
+  if (n == 0) return VXA_OK;
+  return on_device(x.q, linear_step_fn, ptr(&x.q), x.q.stride(0), x.q.stride(1), ptr(&x.k), x.k.stride(0), x.k.stride(1), ptr(&x.v),
+                   x.v.stride(0), x.v.stride(1), dtype_enum(x.q), n, ptr<float>(&x.decay), (float)x.scale, ptr(&x.out), out_dtype,
+                   x.out.stride(0), x.out.stride(1), ptr<float>(x.state), x.state->size(0), x.state->stride(0), x.state->stride(1),
+                   ptr<int32_t>(x.read), ptr<int32_t>(x.write), x.q.size(1), x.k.size(1), x.q.size(2));
+}
+
+int beam_select(PyObject* const* a) {
+  const char* what = "beam_select";
+  const at::Tensor &x = *tensor(what, a[0]), &scores = *tensor(what, a[1]);
+  const int64_t beams = integer(what, a[2]);
+  const at::Tensor &best = *tensor(what, a[3]), &parents = *tensor(what, a[4]), &tokens = *tensor(what, a[5]);
+  check_gpu(what, {&x, &scores, &best, &parents, &tokens}, "beam_select_torch");
+  const int dtype = dtype_enum(x);
+  if (beams <= 0 || x.dim() != 2 || x.size(0) % beams != 0) refuse(what, ": logits are (requests * beams, vocabulary)");
+  if (x.size(1) > 1 && x.stride(1) != 1) refuse(what, ": the vocabulary must be contiguous");
+  const int64_t n = x.size(0) / beams, V = x.size(1);
+  if (!vector_of(scores, at::kFloat, x.size(0))) refuse(what, ": scores must be a contiguous fp32 vector, one for each row of logits");
+  if (best.scalar_type() != at::kFloat || parents.scalar_type() != at::kInt || tokens.scalar_type() != at::kLong || best.dim() != 2 ||
+      best.size(0) != n || best.size(1) == 0 || parents.sizes() != best.sizes() || tokens.sizes() != best.sizes() || !best.is_contiguous() ||
+      !parents.is_contiguous() || !tokens.is_contiguous())
+    refuse(what, ": out_scores (fp32), out_parents (int32) and out_tokens (int64) are contiguous (requests, count)");
+  if (n == 0) return VXA_OK;
+  size_t bytes = 0;
+  const int rc = beam_workspace_fn(n, beams, V, best.size(1), &bytes);
+  if (rc != VXA_OK) return rc;
+  const at::Tensor ws = at::empty({(int64_t)bytes / 4}, x.options().dtype(at::kFloat));
+  return on_device(x, beam_select_fn, ptr(&x), x.stride(0), dtype, ptr<float>(&scores), n, beams, V, best.size(1), ptr<float>(&best),
+                   ptr<int32_t>(&parents), ptr<int64_t>(&tokens), ptr(&ws), bytes);
+}
+
+// The tensors of a cache, views (num_blocks, block_size, KV, D) or (num_blocks, block_size, KV), as the library takes them.
+struct Caches {
+  std::vector<vxa_cache_view> views;
+  int64_t num_blocks = 0;
+};
+Caches caches_of(const char* what, PyObject* o, int64_t page, const at::Tensor& beside) {
+  PyObject* const list = PySequence_Fast(o, "");
+  if (!list) {
+    PyErr_Clear();
+    refuse(what, ": caches must be a list of tensors", PyExc_TypeError);
+  }
+  const THPObjectPtr kept(list);
+  Caches c;
+  c.num_blocks = -1;
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(list); ++i) {
+    const at::Tensor& t = *tensor(what, PySequence_Fast_GET_ITEM(list, i));
+    check_gpu(what, {&beside, &t}, "the torch statements of pages.py");
+    if ((t.dim() != 3 && t.dim() != 4) || t.size(1) != page || (t.dim() == 4 && t.size(3) > 1 && t.stride(3) != 1))
+      refuse(what, ": caches are views (num_blocks, block_size, KV, D) or (num_blocks, block_size, KV), D contiguous");
+    if (c.num_blocks >= 0 && t.size(0) != c.num_blocks) refuse(what, ": all caches must have the same blocks");
+    c.num_blocks = t.size(0);
+    const int64_t size = t.element_size();
+    if (t.numel())
+      c.views.push_back({t.data_ptr(), t.stride(0) * size, t.stride(1) * size, t.stride(2) * size, t.size(2), (t.dim() == 4 ? t.size(3) : 1) * size});
+  }
+  return c;
+}
+int64_t block_size(const char* what, PyObject* o) {
+  const int64_t page = integer(what, o);
+  if (page <= 0) refuse(what, ": block_size must be positive");
+  return page;
+}
+void check_counts(const char* what, const at::Tensor& refs, const at::Tensor& out) {
+  for (const at::Tensor* t : {&refs, &out})
+    if (!vector_of(*t, at::kInt, refs.dim() ? refs.size(0) : 0)) refuse(what, ": ref_count must be a contiguous int32 vector, one count for each block");
+}
+void check_tables(const char* what, const at::Tensor& table, const at::Tensor& out) {
+  check_table(what, table);
+  check_table(what, out);
+  if (out.size(1) != table.size(1)) refuse(what, ": the tables must have the same columns");
+}
+
+int copy_pages(PyObject* const* a) {
+  const char* what = "copy_pages";
+  const int64_t page = block_size(what, a[1]);
+  const at::Tensor &source = *tensor(what, a[2]), &target = *tensor(what, a[3]);
+  check_gpu(what, {&source, &target}, "the torch statements of pages.py");
+  const Caches c = caches_of(what, a[0], page, source);
+  const int64_t n = source.dim() == 1 ? source.size(0) : -1;
+  if (!vector_of(source, at::kInt, n) || !vector_of(target, at::kInt, n)) refuse(what, ": source and target must be contiguous int32 vectors of one length");
+  if (n == 0 || c.views.empty()) return VXA_OK;
+  return on_device(source, pages_copy_fn, c.views.data(), (int64_t)c.views.size(), c.num_blocks, page, ptr<int32_t>(&source), ptr<int32_t>(&target), n);
+}
+
+int fork_pages(PyObject* const* a) {
+  const char* what = "fork_pages";
+  const at::Tensor &bt = *tensor(what, a[1]), &sl = *tensor(what, a[2]), &parents = *tensor(what, a[3]), &refs = *tensor(what, a[4]);
+  const int64_t page = block_size(what, a[5]);
+  const at::Tensor &out = *tensor(what, a[6]), &out_lens = *tensor(what, a[7]), &out_refs = *tensor(what, a[8]), &missing = *tensor(what, a[9]);
+  check_gpu(what, {&bt, &sl, &parents, &refs, &out, &out_lens, &out_refs, &missing}, "fork_pages_torch");
+  const Caches c = caches_of(what, a[0], page, bt);
+  check_tables(what, bt, out);
+  check_counts(what, refs, out_refs);
+  if (c.num_blocks >= 0 && c.num_blocks != refs.size(0)) refuse(what, ": ref_count must have a count for each block of the caches");
+  const int64_t rows = bt.size(0), many = out.size(0);
+  if (!vector_of(sl, at::kInt, rows) || !vector_of(parents, at::kInt, many) || !vector_of(out_lens, at::kInt, many))
+    refuse(what, ": seq_lens, parents and out_lens must be contiguous int32 vectors, one number for each row of their table");
+  if (!vector_of(missing, at::kInt, 1)) refuse(what, ": missing must be one int32 number");
+  size_t bytes = 0;
+  const int rc = fork_workspace_fn(rows, many, &bytes);
+  if (rc != VXA_OK) return rc;
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes / 4}, bt.options());
+  return on_device(bt, pages_fork_fn, c.views.data(), (int64_t)c.views.size(), ptr<int32_t>(&bt), bt.stride(0), bt.size(1), ptr<int32_t>(&sl), rows,
+                   ptr<int32_t>(&parents), many, ptr<int32_t>(&refs), refs.size(0), page, ptr<int32_t>(&out), out.stride(0),
+                   ptr<int32_t>(&out_lens), ptr<int32_t>(&out_refs), ptr<int32_t>(&missing), bytes ? ptr(&ws) : nullptr, bytes);
+}
+
+int resize_pages(PyObject* const* a) {
+  const char* what = "resize_pages";
+  const at::Tensor &bt = *tensor(what, a[0]), &sl = *tensor(what, a[1]), &lens = *tensor(what, a[2]), &refs = *tensor(what, a[3]);
+  const int64_t page = block_size(what, a[4]);
+  const at::Tensor &out = *tensor(what, a[5]), &out_refs = *tensor(what, a[6]), &missing = *tensor(what, a[7]);
+  check_gpu(what, {&bt, &sl, &lens, &refs, &out, &out_refs, &missing}, "resize_pages_torch");
+  check_tables(what, bt, out);
+  check_counts(what, refs, out_refs);
+  const int64_t rows = bt.size(0);
+  if (out.size(0) != rows) refuse(what, ": the tables must have the same rows");
+  if (!vector_of(sl, at::kInt, rows) || !vector_of(lens, at::kInt, rows))
+    refuse(what, ": seq_lens and new_lens must be contiguous int32 vectors, one length for each row");
+  if (!vector_of(missing, at::kInt, 1)) refuse(what, ": missing must be one int32 number");
+  size_t bytes = 0;
+  const int rc = resize_workspace_fn(rows, refs.size(0), &bytes);
+  if (rc != VXA_OK) return rc;
+  const at::Tensor ws = at::empty({(int64_t)bytes / 4}, bt.options());
+  return on_device(bt, pages_resize_fn, ptr<int32_t>(&bt), bt.stride(0), bt.size(1), ptr<int32_t>(&sl), ptr<int32_t>(&lens), rows,
+                   ptr<int32_t>(&refs), refs.size(0), page, ptr<int32_t>(&out), out.stride(0), ptr<int32_t>(&out_refs), ptr<int32_t>(&missing),
+                   ptr(&ws), bytes);
+}
+
+int keep_drafted(PyObject* const* a) {
+  const char* what = "keep_drafted";
+  const at::Tensor &bt = *tensor(what, a[1]), &sl = *tensor(what, a[2]), &qsl = *tensor(what, a[3]), &keep = *tensor(what, a[4]);
+  const int64_t page = block_size(what, a[5]);
+  const at::Tensor& out_lens = *tensor(what, a[6]);
+  check_gpu(what, {&bt, &sl, &qsl, &keep, &out_lens}, "keep_drafted_torch");
+  const Caches c = caches_of(what, a[0], page, bt);
+  check_table(what, bt);
+  const int64_t n = bt.size(0);
+  if (!vector_of(sl, at::kInt, n) || !vector_of(qsl, at::kInt, n + 1) || !vector_of(out_lens, at::kInt, n))
+    refuse(what, ": seq_lens, query_start_loc and out_lens must be contiguous int32 vectors, one length for each block-table row and the n + 1 starts");
+  if (!vector_of(keep, at::kLong, n)) refuse(what, ": keep must be a contiguous int64 vector, one mask for each request");
+  if (n == 0) return VXA_OK;
+  return on_device(bt, pages_keep_fn, c.views.data(), (int64_t)c.views.size(), ptr<int32_t>(&bt), bt.stride(0), bt.size(1), ptr<int32_t>(&sl),
+                   ptr<int32_t>(&qsl), ptr<int64_t>(&keep), n, std::max<int64_t>(c.num_blocks, 0), page, ptr<int32_t>(&out_lens));
+}
+
 // fn(arguments) as a Python function of `count` positional arguments; C++ exceptions end here, torch's as the Python exceptions
 // that torch makes of them (OutOfMemoryError for a workspace that does not fit).
 template <int (*fn)(PyObject* const*), int count>
@@ -247,25 +467,27 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t given) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(prompt_attention, cache_write, cache_read, tree_workspace, tree_decode): the entry points' addresses.
+// bind(addresses): the entry points', in the order of _native.py's _CALLED.
+template <typename F>
+void take(F& fn, PyObject* address) {
+  fn = reinterpret_cast<F>(PyLong_AsVoidPtr(address));
+}
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t given) {
-  void* at[5];
-  if (given != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind() takes five addresses");
+  constexpr int kEntries = 16;
+  if (given != kEntries) {
+    PyErr_SetString(PyExc_TypeError, "bind() takes sixteen addresses");
     return nullptr;
   }
-  for (int i = 0; i < 5; ++i) {
-    at[i] = PyLong_AsVoidPtr(args[i]);
-    if (!at[i]) {
+  for (int i = 0; i < kEntries; ++i)
+    if (!PyLong_AsVoidPtr(args[i])) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind(): null address");
       return nullptr;
     }
-  }
-  prompt_attention_fn = reinterpret_cast<decltype(prompt_attention_fn)>(at[0]);
-  cache_write_fn = reinterpret_cast<decltype(cache_write_fn)>(at[1]);
-  cache_read_fn = reinterpret_cast<decltype(cache_read_fn)>(at[2]);
-  tree_workspace_fn = reinterpret_cast<decltype(tree_workspace_fn)>(at[3]);
-  tree_decode_fn = reinterpret_cast<decltype(tree_decode_fn)>(at[4]);
+  PyObject* const* next = args;
+  take(prompt_attention_fn, *next++), take(cache_write_fn, *next++), take(cache_read_fn, *next++), take(tree_workspace_fn, *next++);
+  take(tree_decode_fn, *next++), take(linear_workspace_fn, *next++), take(linear_prompt_fn, *next++), take(linear_step_fn, *next++);
+  take(beam_workspace_fn, *next++), take(beam_select_fn, *next++), take(pages_copy_fn, *next++), take(fork_workspace_fn, *next++);
+  take(pages_fork_fn, *next++), take(resize_workspace_fn, *next++), take(pages_resize_fn, *next++), take(pages_keep_fn, *next++);
   Py_RETURN_NONE;
 }
 
@@ -275,6 +497,13 @@ PyMethodDef methods[] = {VXA_METHOD("bind", bind),
                          VXA_METHOD("write_cache", (call<write_cache, 7>)),
                          VXA_METHOD("read_cache", (call<read_cache, 9>)),
                          VXA_METHOD("tree_decode", (call<tree_decode, 13>)),
+                         VXA_METHOD("linear_prompt", (call<linear_prompt, 10>)),
+                         VXA_METHOD("linear_step", (call<linear_step, 9>)),
+                         VXA_METHOD("beam_select", (call<beam_select, 6>)),
+                         VXA_METHOD("copy_pages", (call<copy_pages, 4>)),
+                         VXA_METHOD("fork_pages", (call<fork_pages, 10>)),
+                         VXA_METHOD("resize_pages", (call<resize_pages, 8>)),
+                         VXA_METHOD("keep_drafted", (call<keep_drafted, 7>)),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

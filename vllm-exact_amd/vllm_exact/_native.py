@@ -10,7 +10,7 @@ argument types, and turns status codes into Python exceptions:
 * VXA_ERR_TOO_LARGE   -> ValueError (a problem beyond vxa_exact_linear_op_noalloc's fixed scratch)
 * VXA_ERR_WORKSPACE / VXA_ERR_LAUNCH -> RuntimeError
 
-The serving operators (prompt_attn, int8_cache, tree_attn) reach the same entry points through calls(), a module that takes
+The serving operators (prompt_attn, int8_cache, tree_attn, linear_attn, beam, pages) reach the same entry points through calls(), a module that takes
 the tensors themselves.
 
 There is no fallback: if the library is missing, every GPU entry point raises.
@@ -56,9 +56,27 @@ EXPORTED = (
     "vxa_tree_decode_workspace",
     "vxa_tree_decode_call_workspace",
     "vxa_tree_decode",
+    "vxa_linear_prompt_workspace",
+    "vxa_linear_prompt",
+    "vxa_linear_step",
+    "vxa_beam_select_workspace",
+    "vxa_beam_select",
+    "vxa_pages_copy",
+    "vxa_pages_fork_workspace",
+    "vxa_pages_fork",
+    "vxa_pages_resize_workspace",
+    "vxa_pages_resize",
+    "vxa_pages_keep",
 )
 
 _i64, _i32, _int, _vp, _sz = ctypes.c_int64, ctypes.c_int32, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
+
+
+class CacheView(ctypes.Structure):
+    """vxa_cache_view"""
+    _fields_ = [("data", _vp)] + [(name, _i64) for name in ("stride_block", "stride_token", "stride_head", "heads", "row_bytes")]
+
+
 _SIGNATURES = {
     "vxa_version": (ctypes.c_char_p, []),
     "vxa_status_string": (ctypes.c_char_p, [_int]),
@@ -133,6 +151,28 @@ _SIGNATURES = {
         [_vp, _i64, _i64, _int] + [_vp, _i64, _i64, _i64] * 4 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
          ctypes.c_float, _vp, _int] + [_i64] * 9 + [_vp, _sz, _vp],
     ),
+    "vxa_linear_prompt_workspace": (_int, [_i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "vxa_linear_prompt": (
+        _int,
+        [_vp, _i64, _i64] * 3 + [_int, _vp, _i64, _i64, _vp, ctypes.c_float, _vp, _int, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp,
+                                 _i64, _i64, _i64, _vp, _sz, _vp],
+    ),
+    "vxa_linear_step": (
+        _int,
+        [_vp, _i64, _i64] * 3 + [_int, _i64, _vp, ctypes.c_float, _vp, _int, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64,
+                                 _i64, _vp],
+    ),
+    "vxa_beam_select_workspace": (_int, [_i64] * 4 + [ctypes.POINTER(_sz)]),
+    "vxa_beam_select": (_int, [_vp, _i64, _int, _vp] + [_i64] * 4 + [_vp, _vp, _vp, _vp, _sz, _vp]),
+    "vxa_pages_copy": (_int, [ctypes.POINTER(CacheView), _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "vxa_pages_fork_workspace": (_int, [_i64, _i64, ctypes.POINTER(_sz)]),
+    "vxa_pages_fork": (
+        _int,
+        [ctypes.POINTER(CacheView), _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "vxa_pages_resize_workspace": (_int, [_i64, _i64, ctypes.POINTER(_sz)]),
+    "vxa_pages_resize": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _sz, _vp]),
+    "vxa_pages_keep": (_int, [ctypes.POINTER(CacheView), _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
 }
 
 _lib = None
@@ -205,7 +245,9 @@ def launch(device, fn, *args):
 
 
 _calls = None
-_CALLED = ("vxa_prompt_attention", "vxa_int8_cache_write", "vxa_int8_cache_read", "vxa_tree_decode_call_workspace", "vxa_tree_decode")
+_CALLED = ("vxa_prompt_attention", "vxa_int8_cache_write", "vxa_int8_cache_read", "vxa_tree_decode_call_workspace", "vxa_tree_decode",
+           "vxa_linear_prompt_workspace", "vxa_linear_prompt", "vxa_linear_step", "vxa_beam_select_workspace", "vxa_beam_select",
+           "vxa_pages_copy", "vxa_pages_fork_workspace", "vxa_pages_fork", "vxa_pages_resize_workspace", "vxa_pages_resize", "vxa_pages_keep")
 
 
 def calls():
