@@ -22,6 +22,7 @@ struct LinearParams {
   void* out;
   int64_t sot, soh;
   int32_t out_dtype;
+  bool out_wide;  // the output has the input's type and its rows start on 16 bytes
   float* state;
   int64_t sss, ssh;
   int32_t slots;
@@ -108,6 +109,401 @@ __global__ __launch_bounds__(256) void linear_recurrent_kernel(LinearParams p) {
   }
 }
 
+
+// ---------------------------------------------------------------------------------- prompts
+// Rows go in chunks of kChunk: with S the state before a chunk and i, j the rows in it,
+//   o_i = scale (exp(g (i + 1)) q_i S + sum_{j <= i} exp(g (i - j)) (q_i . k_j) v_j)
+//   S'  = exp(g n) S + sum_j exp(g (n - 1 - j)) k_j v_j^T
+constexpr int kChunk = 32;
+constexpr int kPart = 512;  // rows of a part: long sequences are cut into parts whose states are computed first
+
+__device__ inline float power(float g, int e) { return e == 0 ? 1.0f : expf(g * (float)e); }  // exp(-inf * 0) is 1 here
+
+// Eight fp32 values as bf16 operands whose sum they are, N parts: off by 2^-9 of a value for one part, 2^-18 for two, 2^-27 for three.
+template <int N>
+__device__ inline void split(const float (&x)[8], v4u32 (&part)[N]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    float a = x[j], b = x[j + 1];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const uint32_t w = BF16::pack(a, b);
+      part[n][j / 2] = w;
+      if (n + 1 < N) {
+        const v2f f = BF16::unpack(w);
+        a -= f.x, b -= f.y;
+      }
+    }
+  }
+}
+template <typename T>
+__device__ inline void floats(v4u32 w, float (&x)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const v2f f = T::unpack(w[j]);
+    x[2 * j] = f.x, x[2 * j + 1] = f.y;
+  }
+}
+
+// Part `part` of sequence seq, for workgroup `index` of the grid's floor(tokens / kPart) + n: sequence i has the places from
+// floor(cu[i] / kPart) + i on, at least as many as it has parts.
+struct Part {
+  int seq, lo, len, part, parts;  // parts: of the sequence, at least 1
+};
+__device__ inline Part find_part(const LinearParams& p, int index) {
+  const int lane = threadIdx.x & 63;
+  auto start = [&](int i) { return min(max(p.cu[i], 0), p.total); };
+  int seq = 0;
+  for (int j0 = 0; j0 < p.n; j0 += 64) {
+    const int j = j0 + lane;
+    const uint64_t past = __ballot(j < p.n && start(j) / kPart + j > index);
+    if (past) {
+      seq = j0 + __builtin_ctzll(past) - 1;
+      break;
+    }
+    seq = min(j0 + 63, p.n - 1);
+  }
+  seq = __builtin_amdgcn_readfirstlane(max(seq, 0));
+  const int lo = start(seq), hi = max(start(seq + 1), lo);
+  return Part{seq, lo, hi - lo, index - (lo / kPart + seq), max(1, (hi - lo + kPart - 1) / kPart)};
+}
+// Where the state before part `part` of a sequence of several parts is kept: 2 floor(lo / kPart) + part. (The parts of a
+// sequence longer than kPart are at most twice its whole ones.)
+__device__ inline int64_t kept_at(const LinearParams& p, const Part& x, int part, int head, int size) {
+  return ((int64_t)(2 * (x.lo / kPart) + part) * p.H + head) * size;
+}
+
+// A workgroup of D / 32 waves takes one head of a part. A wave keeps 32 columns of the state in the accumulators of 32 x 32 x 16
+// MFMAs, where they are the operand of the next product as they lie.
+// OUT: the rows' outputs from the state that the part starts from, and the sequence's end state. Else: the state that a
+// part leaves when it starts from zeros, for all parts but a sequence's last.
+template <typename T, int D, bool OUT>
+__global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, float* kept) {
+  constexpr bool F16 = std::is_same_v<T, FP16>;
+  constexpr int kRow = 2 * D, kTile = kChunk * kRow;
+  constexpr int DT = D / 32;
+  constexpr int NV = F16 ? 2 : 1;  // parts of a value or query as bf16
+  constexpr bool kLate = OUT && D == 256;  // the next rows are asked for when the state's registers are nearly all that is held
+  __shared__ __attribute__((aligned(1024))) char s_q[OUT ? kTile : 16], s_k[OUT ? kTile : 16], s_qs[OUT && F16 ? 2 : 1][OUT && F16 ? kTile : 16];
+  __shared__ __attribute__((aligned(1024))) char s_kd[3][kTile], s_v[NV][kTile], s_p[OUT ? 4 : 1][OUT ? 1024 : 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int x = (int)(blockIdx.x % p.H);
+  const int head = p.H % 8 == 0 ? (x % 8) * (p.H / 8) + x / 8 : x;  // heads of one KV head on one XCD
+  const Part part = find_part(p, (int)(blockIdx.x / p.H));
+  if (part.part < 0 || part.part >= part.parts - (OUT ? 0 : 1)) return;
+  const Slots slots = find_slots(p, part.seq);
+  const int row0 = part.part * kPart, rows = min(kPart, part.len - row0);
+  const int64_t base = part.lo + row0;
+  char* const out = reinterpret_cast<char*>(p.out);
+  if (slots.bad) {
+    if (OUT)
+      for (int i = threadIdx.x; i < rows * D; i += 2 * D) store_f32_as(out, p.out_dtype, (base + i / D) * p.sot + head * p.soh + i % D, __builtin_nanf(""));
+    return;
+  }
+  const float g = p.log_decay[head];
+  const uint16_t* const qh = p.q + head * p.sqh;
+  const uint16_t* const kh = p.k + head / p.G * p.skh;
+  const uint16_t* const vh = p.v + head / p.G * p.svh;
+
+  // Places that go by the thread alone are found again for every chunk: kept, they would take more registers than there are.
+  auto again = [](int id) {
+    asm volatile("" : "+v"(id));
+    return id;
+  };
+  // Staging: this thread's 16-byte pieces are chunk `piece` of rows srow and srow + 16.
+  v4u32 gq[2], gk[2], gv[2];
+  auto fetch = [&](int t0) {
+    const int id = again(threadIdx.x), srow = id / (D / 8), piece = id % (D / 8);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = t0 + srow + 16 * r;
+      gq[r] = gk[r] = gv[r] = v4u32{0, 0, 0, 0};
+      if (row < rows) {
+        if (OUT) gq[r] = *reinterpret_cast<const v4u32*>(qh + (base + row) * p.sqt + 8 * piece);
+        gk[r] = *reinterpret_cast<const v4u32*>(kh + (base + row) * p.skt + 8 * piece);
+        gv[r] = *reinterpret_cast<const v4u32*>(vh + (base + row) * p.svt + 8 * piece);
+      }
+    }
+  };
+  // Queries and keys lie with the dims of each 16 in the order 0-3, 8-11, 4-7, 12-15: the order in which a lane holds the state's
+  // rows, 16 bytes of it for one half of the lanes.
+  auto stage_row = [&](char* tile, int row, int piece, v4u32 w) {
+    char* at = tile + row * kRow + 8 * (piece & 1);
+    const int c = piece & ~1;
+    *reinterpret_cast<v2u32*>(at + 16 * (c ^ key_swizzle<D>(row))) = v2u32{w.x, w.y};
+    *reinterpret_cast<v2u32*>(at + 16 * ((c + 1) ^ key_swizzle<D>(row))) = v2u32{w.z, w.w};
+  };
+  auto stage = [&](int count) {
+    const int id = again(threadIdx.x), srow = id / (D / 8), piece = id % (D / 8);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = srow + 16 * r;
+      const int wide = row * kRow + 16 * (piece ^ value_swizzle<D>(row));
+      float f[8];
+      if constexpr (OUT) {
+        stage_row(s_q, row, piece, gq[r]);
+        stage_row(s_k, row, piece, gk[r]);
+        if constexpr (F16) {
+          v4u32 two[2];
+          floats<T>(gq[r], f);
+          split(f, two);
+          stage_row(s_qs[0], row, piece, two[0]);
+          stage_row(s_qs[1], row, piece, two[1]);
+        }
+      }
+      if constexpr (F16) {
+        v4u32 two[2];
+        floats<T>(gv[r], f);
+        split(f, two);
+        *reinterpret_cast<v4u32*>(s_v[0] + wide) = two[0];
+        *reinterpret_cast<v4u32*>(s_v[1] + wide) = two[1];
+      } else {
+        *reinterpret_cast<v4u32*>(s_v[0] + wide) = gv[r];
+      }
+      const float w = row < count ? power(g, count - 1 - row) : 0.0f;
+      v4u32 three[3];
+      floats<T>(gk[r], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= w;
+      split(f, three);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) *reinterpret_cast<v4u32*>(s_kd[n] + wide) = three[n];
+    }
+  };
+
+  // The state: rows 32 t + 8 (r / 4) + 4 half + r % 4 of column 32 wave + col.
+  v16f s[DT];
+  const int64_t corner = (int64_t)4 * half * D + 32 * wave + col;
+  auto state_rows = [&](auto f) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) f(t, r, (int64_t)(32 * t + 8 * (r / 4) + r % 4) * D + corner);
+  };
+  fetch(0);
+  const float* from = nullptr;
+  if (OUT && part.parts > 1)
+    from = kept + kept_at(p, part, part.part, head, D * D);
+  else if (OUT && slots.read >= 0)
+    from = p.state + slots.read * p.sss + head * p.ssh;
+  if (from)
+    state_rows([&](int t, int r, int64_t at) { s[t][r] = from[at]; });
+  else
+    state_rows([&](int t, int r, int64_t) { s[t][r] = 0.0f; });
+
+  // Transposed reads of a tile of 32 rows: block b of 32 columns, step c of 16 rows; the rows 16 c + 4 half + 0..3 and 8 further.
+  auto transposed = [&](int now, const char* tile, int c, int b) {
+    const int trow = 4 * (now >> 5) + (now & 15) / 4, tchunk = 2 * ((now >> 4) & 1) + (now & 3) / 2;
+    const char* at = tile + (16 * c + trow) * kRow + 8 * (now & 1) + 16 * ((4 * b + tchunk) ^ value_swizzle<D>(trow));
+    const v2u32 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
+    return v4u32{lo.x, lo.y, hi.x, hi.y};
+  };
+  // 16 x 16 blocks of the scores, transposed: keys 16 (b % 2) + 4 (lane / 16) + r, query 16 (b / 2) + lane % 16.
+  constexpr int kBlocks = DT < 4 ? 2 : 1;  // of a wave; with 8 waves the first 4 have one
+  const float grow = OUT ? power(g, col + 1) : 0.0f;
+  const float full = power(g, kChunk);
+
+  for (int t0 = 0; t0 < rows; t0 += kChunk) {
+    const int count = min(kChunk, rows - t0);
+    __syncthreads();  // the last chunk's tiles have been read
+    stage(count);
+    if (!kLate && t0 + kChunk < rows) fetch(t0 + kChunk);
+    __syncthreads();
+    const int now = again(lane);
+    v16f from_start, o;  // the state's part of the outputs, and all of them
+    if constexpr (OUT) {
+      if (DT <= 4 || wave < 4) {
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) {
+          const int b = wave + n * 2, jt = b & 1, it = b >> 1, l16 = now & 15, l4 = now >> 4;
+          const int krow = 16 * jt + l16, qrow = 16 * it + l16;
+          v4f sc = {0, 0, 0, 0};
+#pragma unroll
+          for (int u = 0; u < D / 32; ++u)
+            sc = T::mfma16(*reinterpret_cast<const v4u32*>(s_k + krow * kRow + 16 * ((4 * u + l4) ^ key_swizzle<D>(krow))),
+                           *reinterpret_cast<const v4u32*>(s_q + qrow * kRow + 16 * ((4 * u + l4) ^ key_swizzle<D>(qrow))), sc);
+          float w[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int e = qrow - (16 * jt + 4 * l4 + r);
+            w[r] = e >= 0 ? sc[r] * power(g, e) : 0.0f;
+          }
+          const v2u32 hi = {BF16::pack(w[0], w[1]), BF16::pack(w[2], w[3])};
+          const v2f h0 = BF16::unpack(hi.x), h1 = BF16::unpack(hi.y);
+          const v2u32 lo = {BF16::pack(w[0] - h0.x, w[1] - h0.y), BF16::pack(w[2] - h1.x, w[3] - h1.y)};
+          const int at = (32 * (l4 & 1) + qrow) * 16 + 8 * (l4 >> 1);
+          *reinterpret_cast<v2u32*>(s_p[2 * jt] + at) = hi;
+          *reinterpret_cast<v2u32*>(s_p[2 * jt + 1] + at) = lo;
+        }
+      }
+    }
+    // q S, transposed: columns of the state as rows, queries as columns.
+    if constexpr (OUT) {
+      v16f acc = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = s[u / 2][8 * (u % 2) + j];
+        v4u32 two[2];
+        split(f, two);
+        const int at = (now & 31) * kRow + 16 * ((2 * u + (now >> 5)) ^ key_swizzle<D>(now & 31));
+        if constexpr (F16) {
+          const v4u32 qhi = *reinterpret_cast<const v4u32*>(s_qs[0] + at), qlo = *reinterpret_cast<const v4u32*>(s_qs[1] + at);
+          acc = BF16::mfma32(two[0], qhi, acc);
+          acc = BF16::mfma32(two[1], qhi, acc);
+          acc = BF16::mfma32(two[0], qlo, acc);
+        } else {
+          const v4u32 q = *reinterpret_cast<const v4u32*>(s_q + at);
+          acc = BF16::mfma32(two[0], q, acc);
+          acc = BF16::mfma32(two[1], q, acc);
+        }
+        if (u % 2) __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[r] *= grow;
+      from_start = acc;
+    }
+    v4u32 v[NV][2];
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) v[n][c] = transposed(now, s_v[n], c, wave);
+    if constexpr (OUT) {
+      __syncthreads();  // the scores
+      auto add_rows = [&](const v4u32 (&vs)[NV][2]) {
+        o = from_start;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const v4u32 hi = *reinterpret_cast<const v4u32*>(s_p[2 * c] + 16 * lane), lo = *reinterpret_cast<const v4u32*>(s_p[2 * c + 1] + 16 * lane);
+          o = BF16::mfma32(vs[0][c], hi, o);
+          o = BF16::mfma32(vs[0][c], lo, o);
+          if constexpr (F16) o = BF16::mfma32(vs[1][c], hi, o);
+        }
+      };
+      add_rows(v);
+      // 0 times an infinity or NaN of a later row is NaN. Where sums end up not finite, the rows are added again without such values,
+      // which then count for the rows from theirs on.
+      float odd = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) odd = fmaf(o[r], 0.0f, odd);
+      if (__any(odd != 0.0f)) {
+        v4u32 fine[NV][2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            fine[0][c][j] = only_finite<BF16>(v[0][c][j]);
+            if constexpr (F16) fine[1][c][j] = only_finite<BF16>(v[1][c][j]);
+          }
+        add_rows(fine);
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll 1
+          for (int j = 0; j <= col; ++j) {
+            const v2u32 w = *reinterpret_cast<const v2u32*>(s_v[0] + j * kRow + 16 * ((4 * wave + a) ^ value_swizzle<D>(j)) + 8 * half);
+            v4f special = {0, 0, 0, 0};
+            add_specials<BF16>(special, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[4 * a + e] += special[e];
+          }
+      }
+      // Row `col`, dims 32 wave + 8 a + 4 half + 0..3 for a = 0..3: with 16-bit outputs the halves exchange what the other stores.
+      const int64_t at = (base + t0 + col) * p.sot + head * p.soh + 32 * wave;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[r] *= p.scale;
+      if (p.out_wide) {
+#pragma unroll
+        for (int a = 0; a < 4; a += 2) {
+          uint32_t w[2][2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            w[0][j] = T::pack(o[4 * a + 2 * j], o[4 * a + 2 * j + 1]), w[1][j] = T::pack(o[4 * a + 4 + 2 * j], o[4 * a + 5 + 2 * j]);
+            const auto x = __builtin_amdgcn_permlane32_swap(w[0][j], w[1][j], false, false);
+            w[0][j] = x[0], w[1][j] = x[1];
+          }
+          if (col < count) *reinterpret_cast<v4u32*>(reinterpret_cast<uint16_t*>(out) + at + 8 * a + 8 * half) = v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
+        }
+      } else if (col < count) {
+        if (p.out_dtype == VXA_F32) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) reinterpret_cast<float*>(out)[at + 8 * (r / 4) + 4 * half + r % 4] = o[r];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) store_f32_as(out, p.out_dtype, at + 8 * (r / 4) + 4 * half + r % 4, o[r]);
+        }
+      }
+    }
+    if (kLate && t0 + kChunk < rows) fetch(t0 + kChunk);
+    const float decay = count == kChunk ? full : power(g, count);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] *= decay;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+          const v4u32 k = transposed(now, s_kd[n], c, t);
+          s[t] = BF16::mfma32(k, v[0][c], s[t]);
+          if constexpr (F16)
+            if (n < 2) s[t] = BF16::mfma32(k, v[1][c], s[t]);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  float* to = nullptr;
+  if (!OUT)
+    to = kept + kept_at(p, part, part.part + 1, head, D * D);
+  else if (part.part == part.parts - 1 && slots.write >= 0)
+    to = p.state + slots.write * p.sss + head * p.ssh;
+  if (to) state_rows([&](int t, int r, int64_t at) { to[at] = s[t][r]; });
+}
+
+// The states before a long sequence's parts, from what each part adds: 4 values of one head a thread.
+__global__ __launch_bounds__(256) void linear_parts_kernel(LinearParams p, float* kept, int size) {
+  const int pieces = size / 1024, head = (int)(blockIdx.x / pieces) % p.H, seq = (int)(blockIdx.x / pieces) / p.H;
+  const int lo = min(max(p.cu[seq], 0), p.total), len = min(max(p.cu[seq + 1], lo), p.total) - lo;
+  if (len <= kPart) return;
+  const Part part{seq, lo, len, 0, (len + kPart - 1) / kPart};
+  const int at = 4 * ((int)(blockIdx.x % pieces) * 256 + (int)threadIdx.x);
+  const int read = p.read ? p.read[seq] : -1;
+  v4f s = {0, 0, 0, 0};
+  if (read >= 0 && read < p.slots) s = *reinterpret_cast<const v4f*>(p.state + read * p.sss + head * p.ssh + at);
+  const float decay = power(p.log_decay[head], kPart);
+  for (int i = 0; i < part.parts; ++i) {
+    v4f* x = reinterpret_cast<v4f*>(kept + kept_at(p, part, i, head, size) + at);
+    if (i > 0) {
+      const v4f add = *x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] = fmaf(s[e], decay, add[e]);
+    }
+    *x = s;
+  }
+}
+
+int64_t kept_states(int64_t tokens) { return tokens > kPart ? 2 * (tokens / kPart) + 2 : 0; }
+
+template <typename T, int D>
+hipError_t launch_prompt(const LinearParams& p, float* kept, hipStream_t st) {
+  const int64_t blocks = (int64_t)p.H * (p.total / kPart + p.n);
+  const int64_t pieces = (int64_t)p.n * p.H * (D * D / 1024);
+  if (!launchable(blocks, 2 * D) || !launchable(pieces, 256)) return hipErrorInvalidConfiguration;
+  if (p.total > kPart) {  // some sequence may have several parts
+    hipLaunchKernelGGL((linear_chunk_kernel<T, D, false>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
+    hipLaunchKernelGGL(linear_parts_kernel, dim3((unsigned)pieces), dim3(256), 0, st, p, kept, D * D);
+  }
+  hipLaunchKernelGGL((linear_chunk_kernel<T, D, true>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
+  return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_prompt(int64_t D, const LinearParams& p, float* kept, hipStream_t st) {
+  if (D == 64) return launch_prompt<T, 64>(p, kept, st);
+  if (D == 128) return launch_prompt<T, 128>(p, kept, st);
+  return launch_prompt<T, 256>(p, kept, st);
+}
+
 template <typename T>
 hipError_t launch_recurrent(int64_t D, const LinearParams& p, hipStream_t st) {
   const int64_t blocks = (int64_t)p.n * p.H * (D / kCols);
@@ -146,6 +542,7 @@ int linear_params(LinearParams& p, const void* q, int64_t sqt, int64_t sqh, cons
   p.n = (int32_t)n, p.total = (int32_t)tokens, p.H = (int32_t)H, p.G = (int32_t)(H / KV);
   p.log_decay = log_decay, p.scale = scale;
   p.out = out, p.sot = sot, p.soh = soh, p.out_dtype = out_dtype;
+  p.out_wide = out_dtype == dtype && (uintptr_t)out % 16 == 0 && sot % 8 == 0 && soh % 8 == 0;
   p.state = state, p.sss = sss, p.ssh = ssh, p.slots = (int32_t)slots, p.read = read_slots, p.write = write_slots;
   return VXA_OK;
 }
@@ -159,7 +556,7 @@ int status_of(hipError_t err) {
 
 extern "C" int vxa_linear_prompt_workspace(int64_t tokens, int64_t num_heads, int64_t head_dim, size_t* ws_bytes) {
   if (tokens < 0 || num_heads <= 0 || head_dim <= 0 || !ws_bytes) return VXA_ERR_ARG;
-  *ws_bytes = 0;
+  *ws_bytes = (size_t)product({kept_states(tokens), num_heads, head_dim, head_dim, 4});
   return VXA_OK;
 }
 
@@ -174,9 +571,13 @@ extern "C" int vxa_linear_prompt(const void* q, int64_t sqt, int64_t sqh, const 
                                state, slots, sss, ssh, read_slots, write_slots, num_heads, num_kv_heads, head_dim);
   if (rc != VXA_OK || n == 0) return rc;
   if (!starts) return VXA_ERR_ARG;
+  size_t bytes = 0;
+  vxa_linear_prompt_workspace(tokens, num_heads, head_dim, &bytes);
+  if (bytes && (!ws || (uintptr_t)ws % 16 || ws_bytes < bytes)) return VXA_ERR_WORKSPACE;
   p.cu = starts;
+  float* kept = reinterpret_cast<float*>(ws);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  return status_of(dtype == VXA_BF16 ? launch_recurrent<BF16>(head_dim, p, st) : launch_recurrent<FP16>(head_dim, p, st));
+  return status_of(dtype == VXA_BF16 ? launch_prompt<BF16>(head_dim, p, kept, st) : launch_prompt<FP16>(head_dim, p, kept, st));
 }
 
 extern "C" int vxa_linear_step(const void* q, int64_t sqt, int64_t sqh, const void* k, int64_t skt, int64_t skh, const void* v,
