@@ -111,10 +111,9 @@ __global__ __launch_bounds__(256) void linear_recurrent_kernel(LinearParams p) {
 
 
 // ---------------------------------------------------------------------------------- prompts
-// Rows go in chunks of kChunk: with S the state before a chunk and i, j the rows in it,
+// Rows go in chunks: with S the state before a chunk of n rows and i, j the rows in it,
 //   o_i = scale (exp(g (i + 1)) q_i S + sum_{j <= i} exp(g (i - j)) (q_i . k_j) v_j)
-//   S'  = exp(g n) S + sum_j exp(g (n - 1 - j)) k_j v_j^T
-constexpr int kChunk = 32;
+//   S'  = exp(g n) S + sum_j k_j (exp(g (n - 1 - j)) v_j)^T
 constexpr int kPart = 512;  // rows of a part: long sequences are cut into parts whose states are computed first
 
 __device__ inline float power(float g, int e) { return e == 0 ? 1.0f : expf(g * (float)e); }  // exp(-inf * 0) is 1 here
@@ -144,6 +143,12 @@ __device__ inline void floats(v4u32 w, float (&x)[8]) {
     x[2 * j] = f.x, x[2 * j + 1] = f.y;
   }
 }
+// A lane's id, whose uses the compiler does not move across this: places that go by it alone are found again for every
+// chunk. Kept, they would take more registers than there are.
+__device__ inline int again(int id) {
+  asm volatile("" : "+v"(id));
+  return id;
+}
 
 // Part `part` of sequence seq, for workgroup `index` of the grid's floor(tokens / kPart) + n: sequence i has the places from
 // floor(cu[i] / kPart) + i on, at least as many as it has parts.
@@ -169,23 +174,37 @@ __device__ inline Part find_part(const LinearParams& p, int index) {
 }
 // Where the state before part `part` of a sequence of several parts is kept: 2 floor(lo / kPart) + part. (The parts of a
 // sequence longer than kPart are at most twice its whole ones.)
-__device__ inline int64_t kept_at(const LinearParams& p, const Part& x, int part, int head, int size) {
-  return ((int64_t)(2 * (x.lo / kPart) + part) * p.H + head) * size;
+__device__ inline int64_t kept_at(const LinearParams& p, int lo, int part, int head, int size) {
+  return ((int64_t)(2 * (lo / kPart) + part) * p.H + head) * size;
 }
+
+// A tile's 16-byte chunks lie at chunk ^ swizzle(row): 16 rows that are read at one chunk meet 16 different ones.
+template <typename T, int D, bool OUT>
+struct Shared {
+  static constexpr bool F16 = std::is_same_v<T, FP16>;
+  static constexpr int C = !F16 && D <= 128 ? 64 : 32;  // rows of a chunk
+  static constexpr int kTile = C * 2 * D;
+  char q[OUT ? kTile : 16], k[OUT ? kTile : 16];                       // for the scores
+  char qs[OUT && F16 ? 2 : 1][OUT && F16 ? kTile : 16];                // fp16: queries as two bf16 parts
+  char kt[F16 ? 2 : 1][kTile], v[kTile];                               // for transposed reads; fp16: keys as two bf16 parts
+  char scores[OUT ? (C == 64 ? 6 : 2) : 1][2][OUT ? 1024 : 16];        // operands of 16 keys and 32 queries, two parts
+  float power[C];                                                      // exp(g (C - 1 - x))
+  float left[C];                                                       // exp(g (n - 1 - j)) of row j of the chunk, 0 past its end
+};
 
 // A workgroup of D / 32 waves takes one head of a part. A wave keeps 32 columns of the state in the accumulators of 32 x 32 x 16
 // MFMAs, where they are the operand of the next product as they lie.
 // OUT: the rows' outputs from the state that the part starts from, and the sequence's end state. Else: the state that a
-// part leaves when it starts from zeros, for all parts but a sequence's last.
+// part leaves, for all parts but a sequence's last; the first starts from the sequence's state, the others from zeros.
 template <typename T, int D, bool OUT>
 __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, float* kept) {
-  constexpr bool F16 = std::is_same_v<T, FP16>;
-  constexpr int kRow = 2 * D, kTile = kChunk * kRow;
-  constexpr int DT = D / 32;
-  constexpr int NV = F16 ? 2 : 1;  // parts of a value or query as bf16
-  constexpr bool kLate = OUT && D == 256;  // the next rows are asked for when the state's registers are nearly all that is held
-  __shared__ __attribute__((aligned(1024))) char s_q[OUT ? kTile : 16], s_k[OUT ? kTile : 16], s_qs[OUT && F16 ? 2 : 1][OUT && F16 ? kTile : 16];
-  __shared__ __attribute__((aligned(1024))) char s_kd[3][kTile], s_v[NV][kTile], s_p[OUT ? 4 : 1][OUT ? 1024 : 16];
+  using S = Shared<T, D, OUT>;
+  constexpr bool F16 = S::F16;
+  constexpr int C = S::C, kRow = 2 * D;
+  constexpr int DT = D / 32, IT = C / 32, CT = C / 16;  // blocks of the state's rows, of queries, of keys
+  constexpr int kPieces = C / 16;                       // of a row tile, 16 bytes each, of a thread
+  constexpr bool kLate = OUT && D == 256;               // the next rows are asked for when little but the state is held
+  __shared__ __attribute__((aligned(1024))) S sh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int x = (int)(blockIdx.x % p.H);
@@ -206,17 +225,12 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   const uint16_t* const kh = p.k + head / p.G * p.skh;
   const uint16_t* const vh = p.v + head / p.G * p.svh;
 
-  // Places that go by the thread alone are found again for every chunk: kept, they would take more registers than there are.
-  auto again = [](int id) {
-    asm volatile("" : "+v"(id));
-    return id;
-  };
-  // Staging: this thread's 16-byte pieces are chunk `piece` of rows srow and srow + 16.
-  v4u32 gq[2], gk[2], gv[2];
+  // Staging: this thread's 16-byte pieces are chunk `piece` of rows srow + 16 r.
+  v4u32 gq[kPieces], gk[kPieces], gv[kPieces];
   auto fetch = [&](int t0) {
     const int id = again(threadIdx.x), srow = id / (D / 8), piece = id % (D / 8);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < kPieces; ++r) {
       const int row = t0 + srow + 16 * r;
       gq[r] = gk[r] = gv[r] = v4u32{0, 0, 0, 0};
       if (row < rows) {
@@ -226,8 +240,8 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
       }
     }
   };
-  // Queries and keys lie with the dims of each 16 in the order 0-3, 8-11, 4-7, 12-15: the order in which a lane holds the state's
-  // rows, 16 bytes of it for one half of the lanes.
+  // For the scores, queries and keys lie with the dims of each 16 in the order 0-3, 8-11, 4-7, 12-15: the order in which a lane holds
+  // the state's rows, 16 bytes of it for one half of the lanes.
   auto stage_row = [&](char* tile, int row, int piece, v4u32 w) {
     char* at = tile + row * kRow + 8 * (piece & 1);
     const int c = piece & ~1;
@@ -237,39 +251,32 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   auto stage = [&](int count) {
     const int id = again(threadIdx.x), srow = id / (D / 8), piece = id % (D / 8);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < kPieces; ++r) {
       const int row = srow + 16 * r;
       const int wide = row * kRow + 16 * (piece ^ value_swizzle<D>(row));
-      float f[8];
       if constexpr (OUT) {
-        stage_row(s_q, row, piece, gq[r]);
-        stage_row(s_k, row, piece, gk[r]);
-        if constexpr (F16) {
-          v4u32 two[2];
+        stage_row(sh.q, row, piece, gq[r]);
+        stage_row(sh.k, row, piece, gk[r]);
+      }
+      *reinterpret_cast<v4u32*>(sh.v + wide) = gv[r];
+      if constexpr (F16) {
+        float f[8];
+        v4u32 two[2];
+        if constexpr (OUT) {
           floats<T>(gq[r], f);
           split(f, two);
-          stage_row(s_qs[0], row, piece, two[0]);
-          stage_row(s_qs[1], row, piece, two[1]);
+          stage_row(sh.qs[0], row, piece, two[0]);
+          stage_row(sh.qs[1], row, piece, two[1]);
         }
-      }
-      if constexpr (F16) {
-        v4u32 two[2];
-        floats<T>(gv[r], f);
+        floats<T>(gk[r], f);
         split(f, two);
-        *reinterpret_cast<v4u32*>(s_v[0] + wide) = two[0];
-        *reinterpret_cast<v4u32*>(s_v[1] + wide) = two[1];
+        *reinterpret_cast<v4u32*>(sh.kt[0] + wide) = two[0];
+        *reinterpret_cast<v4u32*>(sh.kt[1] + wide) = two[1];
       } else {
-        *reinterpret_cast<v4u32*>(s_v[0] + wide) = gv[r];
+        *reinterpret_cast<v4u32*>(sh.kt[0] + wide) = gk[r];
       }
-      const float w = row < count ? power(g, count - 1 - row) : 0.0f;
-      v4u32 three[3];
-      floats<T>(gk[r], f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= w;
-      split(f, three);
-#pragma unroll
-      for (int n = 0; n < 3; ++n) *reinterpret_cast<v4u32*>(s_kd[n] + wide) = three[n];
     }
+    if (count < C && (int)threadIdx.x < C) sh.left[threadIdx.x] = (int)threadIdx.x < count ? power(g, count - 1 - (int)threadIdx.x) : 0.0f;
   };
 
   // The state: rows 32 t + 8 (r / 4) + 4 half + r % 4 of column 32 wave + col.
@@ -282,65 +289,76 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
       for (int r = 0; r < 16; ++r) f(t, r, (int64_t)(32 * t + 8 * (r / 4) + r % 4) * D + corner);
   };
   fetch(0);
+  if ((int)threadIdx.x < C) sh.power[threadIdx.x] = sh.left[threadIdx.x] = power(g, C - 1 - (int)threadIdx.x);
+  // A sequence of several parts that writes the slot that it reads keeps its first state apart: its last part may end before the first
+  // begins.
+  const bool apart = part.parts > 1 && slots.read == slots.write;
   const float* from = nullptr;
-  if (OUT && part.parts > 1)
-    from = kept + kept_at(p, part, part.part, head, D * D);
-  else if (OUT && slots.read >= 0)
+  if (part.part > 0 ? OUT : OUT && apart && slots.read >= 0)
+    from = kept + kept_at(p, part.lo, part.part, head, D * D);
+  else if (part.part == 0 && slots.read >= 0)
     from = p.state + slots.read * p.sss + head * p.ssh;
   if (from)
     state_rows([&](int t, int r, int64_t at) { s[t][r] = from[at]; });
   else
     state_rows([&](int t, int r, int64_t) { s[t][r] = 0.0f; });
+  if (!OUT && apart && part.part == 0 && slots.read >= 0) {
+    float* to = kept + kept_at(p, part.lo, 0, head, D * D);
+    state_rows([&](int t, int r, int64_t at) { to[at] = s[t][r]; });
+  }
 
-  // Transposed reads of a tile of 32 rows: block b of 32 columns, step c of 16 rows; the rows 16 c + 4 half + 0..3 and 8 further.
+  // Transposed reads of a tile: block b of 32 columns, step c of 16 rows; the rows 16 c + 4 half + 0..3 and 8 further.
   auto transposed = [&](int now, const char* tile, int c, int b) {
     const int trow = 4 * (now >> 5) + (now & 15) / 4, tchunk = 2 * ((now >> 4) & 1) + (now & 3) / 2;
     const char* at = tile + (16 * c + trow) * kRow + 8 * (now & 1) + 16 * ((4 * b + tchunk) ^ value_swizzle<D>(trow));
     const v2u32 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
     return v4u32{lo.x, lo.y, hi.x, hi.y};
   };
-  // 16 x 16 blocks of the scores, transposed: keys 16 (b % 2) + 4 (lane / 16) + r, query 16 (b / 2) + lane % 16.
-  constexpr int kBlocks = DT < 4 ? 2 : 1;  // of a wave; with 8 waves the first 4 have one
-  const float grow = OUT ? power(g, col + 1) : 0.0f;
-  const float full = power(g, kChunk);
+  float grow[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i) grow[i] = OUT ? power(g, 32 * i + col + 1) : 0.0f;
+  const float full = power(g, C);
 
-  for (int t0 = 0; t0 < rows; t0 += kChunk) {
-    const int count = min(kChunk, rows - t0);
+  for (int t0 = 0; t0 < rows; t0 += C) {
+    const int count = min(C, rows - t0);
     __syncthreads();  // the last chunk's tiles have been read
     stage(count);
-    if (!kLate && t0 + kChunk < rows) fetch(t0 + kChunk);
+    if (!kLate && t0 + C < rows) fetch(t0 + C);
     __syncthreads();
     const int now = again(lane);
-    v16f from_start, o;  // the state's part of the outputs, and all of them
+    v16f o[IT];
     if constexpr (OUT) {
-      if (DT <= 4 || wave < 4) {
+      // Scores in blocks of 16 keys 16 jt + 4 (lane / 16) + r and 16 queries 16 it + lane % 16, those that some query sees and the
+      // ones beside them that complete an operand.
+      constexpr int kBlocks = C == 64 ? 12 : 4;
 #pragma unroll
-        for (int n = 0; n < kBlocks; ++n) {
-          const int b = wave + n * 2, jt = b & 1, it = b >> 1, l16 = now & 15, l4 = now >> 4;
-          const int krow = 16 * jt + l16, qrow = 16 * it + l16;
+      for (int n = 0; n < (kBlocks + DT - 1) / DT; ++n) {
+        const int b = wave + n * DT;
+        if (b < kBlocks) {
+          const int it = b < 4 ? b >> 1 : 2 + ((b - 4) >> 2), jt = b < 4 ? b & 1 : (b - 4) & 3, l16 = now & 15, l4 = now >> 4;
+          const int krow = 16 * jt + l16, qrow = 16 * it + l16, key = 16 * jt + 4 * l4;
           v4f sc = {0, 0, 0, 0};
 #pragma unroll
           for (int u = 0; u < D / 32; ++u)
-            sc = T::mfma16(*reinterpret_cast<const v4u32*>(s_k + krow * kRow + 16 * ((4 * u + l4) ^ key_swizzle<D>(krow))),
-                           *reinterpret_cast<const v4u32*>(s_q + qrow * kRow + 16 * ((4 * u + l4) ^ key_swizzle<D>(qrow))), sc);
+            sc = T::mfma16(*reinterpret_cast<const v4u32*>(sh.k + krow * kRow + 16 * ((4 * u + l4) ^ key_swizzle<D>(krow))),
+                           *reinterpret_cast<const v4u32*>(sh.q + qrow * kRow + 16 * ((4 * u + l4) ^ key_swizzle<D>(qrow))), sc);
           float w[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int e = qrow - (16 * jt + 4 * l4 + r);
-            w[r] = e >= 0 ? sc[r] * power(g, e) : 0.0f;
-          }
+          for (int r = 0; r < 4; ++r)  // a later key's score may be an infinity
+            w[r] = qrow >= key + r ? sc[r] * sh.power[min(C - 1 - qrow + key + r, C - 1)] : 0.0f;
           const v2u32 hi = {BF16::pack(w[0], w[1]), BF16::pack(w[2], w[3])};
           const v2f h0 = BF16::unpack(hi.x), h1 = BF16::unpack(hi.y);
           const v2u32 lo = {BF16::pack(w[0] - h0.x, w[1] - h0.y), BF16::pack(w[2] - h1.x, w[3] - h1.y)};
-          const int at = (32 * (l4 & 1) + qrow) * 16 + 8 * (l4 >> 1);
-          *reinterpret_cast<v2u32*>(s_p[2 * jt] + at) = hi;
-          *reinterpret_cast<v2u32*>(s_p[2 * jt + 1] + at) = lo;
+          const int at = (32 * (l4 & 1) + (qrow & 31)) * 16 + 8 * (l4 >> 1), operand = (it < 2 ? 0 : 2) + jt;
+          *reinterpret_cast<v2u32*>(sh.scores[operand][0] + at) = hi;
+          *reinterpret_cast<v2u32*>(sh.scores[operand][1] + at) = lo;
         }
       }
     }
     // q S, transposed: columns of the state as rows, queries as columns.
-    if constexpr (OUT) {
-      v16f acc = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    auto from_state = [&] {
+#pragma unroll
+      for (int i = 0; i < IT; ++i) o[i] = v16f{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
       for (int u = 0; u < D / 16; ++u) {
         float f[8];
@@ -348,38 +366,50 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
         for (int j = 0; j < 8; ++j) f[j] = s[u / 2][8 * (u % 2) + j];
         v4u32 two[2];
         split(f, two);
-        const int at = (now & 31) * kRow + 16 * ((2 * u + (now >> 5)) ^ key_swizzle<D>(now & 31));
-        if constexpr (F16) {
-          const v4u32 qhi = *reinterpret_cast<const v4u32*>(s_qs[0] + at), qlo = *reinterpret_cast<const v4u32*>(s_qs[1] + at);
-          acc = BF16::mfma32(two[0], qhi, acc);
-          acc = BF16::mfma32(two[1], qhi, acc);
-          acc = BF16::mfma32(two[0], qlo, acc);
-        } else {
-          const v4u32 q = *reinterpret_cast<const v4u32*>(s_q + at);
-          acc = BF16::mfma32(two[0], q, acc);
-          acc = BF16::mfma32(two[1], q, acc);
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+          const int row = 32 * i + (now & 31), at = row * kRow + 16 * ((2 * u + (now >> 5)) ^ key_swizzle<D>(row));
+          if constexpr (F16) {
+            const v4u32 qhi = *reinterpret_cast<const v4u32*>(sh.qs[0] + at), qlo = *reinterpret_cast<const v4u32*>(sh.qs[1] + at);
+            o[i] = BF16::mfma32(two[0], qhi, o[i]);
+            o[i] = BF16::mfma32(two[1], qhi, o[i]);
+            o[i] = BF16::mfma32(two[0], qlo, o[i]);
+          } else {
+            const v4u32 q = *reinterpret_cast<const v4u32*>(sh.q + at);
+            o[i] = BF16::mfma32(two[0], q, o[i]);
+            o[i] = BF16::mfma32(two[1], q, o[i]);
+          }
         }
-        if (u % 2) __builtin_amdgcn_sched_barrier(0);
+        if (D == 256 && u % 2) __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[r] *= grow;
-      from_start = acc;
-    }
-    v4u32 v[NV][2];
+      for (int i = 0; i < IT; ++i)
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
+        for (int r = 0; r < 16; ++r) o[i][r] *= grow[i];
+    };
+    if constexpr (OUT) from_state();
+    v4u32 v[CT];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) v[n][c] = transposed(now, s_v[n], c, wave);
+    for (int c = 0; c < CT; ++c) v[c] = transposed(now, sh.v, c, wave);
     if constexpr (OUT) {
       __syncthreads();  // the scores
-      auto add_rows = [&](const v4u32 (&vs)[NV][2]) {
-        o = from_start;
+      auto add_rows = [&](const v4u32 (&vs)[CT]) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const v4u32 hi = *reinterpret_cast<const v4u32*>(s_p[2 * c] + 16 * lane), lo = *reinterpret_cast<const v4u32*>(s_p[2 * c + 1] + 16 * lane);
-          o = BF16::mfma32(vs[0][c], hi, o);
-          o = BF16::mfma32(vs[0][c], lo, o);
-          if constexpr (F16) o = BF16::mfma32(vs[1][c], hi, o);
+        for (int c = 0; c < CT; ++c) {
+          v4u32 two[2] = {vs[c], vs[c]};
+          if constexpr (F16) {
+            float f[8];
+            floats<T>(vs[c], f);
+            split(f, two);
+          }
+#pragma unroll
+          for (int i = c / 2; i < IT; ++i) {
+            const char* operand = sh.scores[(i ? 2 : 0) + c][0] + 16 * lane;
+            const v4u32 hi = *reinterpret_cast<const v4u32*>(operand), lo = *reinterpret_cast<const v4u32*>(operand + 1024);
+            o[i] = BF16::mfma32(two[0], hi, o[i]);
+            o[i] = BF16::mfma32(two[0], lo, o[i]);
+            if constexpr (F16) o[i] = BF16::mfma32(two[1], hi, o[i]);
+          }
         }
       };
       add_rows(v);
@@ -387,99 +417,119 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
       // which then count for the rows from theirs on.
       float odd = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) odd = fmaf(o[r], 0.0f, odd);
+      for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) odd = fmaf(o[i][r], 0.0f, odd);
       if (__any(odd != 0.0f)) {
-        v4u32 fine[NV][2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int t = 0; t < DT; ++t) asm volatile("" : "+v"(s[t]));  // computed again, not kept from above
+        from_state();
+        v4u32 fine[CT];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            fine[0][c][j] = only_finite<BF16>(v[0][c][j]);
-            if constexpr (F16) fine[1][c][j] = only_finite<BF16>(v[1][c][j]);
-          }
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) fine[c][j] = only_finite<T>(v[c][j]);
         add_rows(fine);
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+          for (int a = 0; a < 4; ++a)
 #pragma unroll 1
-          for (int j = 0; j <= col; ++j) {
-            const v2u32 w = *reinterpret_cast<const v2u32*>(s_v[0] + j * kRow + 16 * ((4 * wave + a) ^ value_swizzle<D>(j)) + 8 * half);
-            v4f special = {0, 0, 0, 0};
-            add_specials<BF16>(special, w);
+            for (int j = 0; j <= 32 * i + col; ++j) {
+              const v2u32 w = *reinterpret_cast<const v2u32*>(sh.v + j * kRow + 16 * ((4 * wave + a) ^ value_swizzle<D>(j)) + 8 * half);
+              v4f special = {0, 0, 0, 0};
+              add_specials<T>(special, w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[4 * a + e] += special[e];
-          }
+              for (int e = 0; e < 4; ++e) o[i][4 * a + e] += special[e];
+            }
       }
-      // Row `col`, dims 32 wave + 8 a + 4 half + 0..3 for a = 0..3: with 16-bit outputs the halves exchange what the other stores.
-      const int64_t at = (base + t0 + col) * p.sot + head * p.soh + 32 * wave;
+      // Row 32 i + col, dims 32 wave + 8 a + 4 half + 0..3 for a = 0..3: with 16-bit outputs the halves exchange what the other stores.
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[r] *= p.scale;
-      if (p.out_wide) {
+      for (int i = 0; i < IT; ++i) {
+        const int row = 32 * i + col;
+        const int64_t at = (base + t0 + row) * p.sot + head * p.soh + 32 * wave;
 #pragma unroll
-        for (int a = 0; a < 4; a += 2) {
-          uint32_t w[2][2];
+        for (int r = 0; r < 16; ++r) o[i][r] *= p.scale;
+        if (p.out_wide) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            w[0][j] = T::pack(o[4 * a + 2 * j], o[4 * a + 2 * j + 1]), w[1][j] = T::pack(o[4 * a + 4 + 2 * j], o[4 * a + 5 + 2 * j]);
-            const auto x = __builtin_amdgcn_permlane32_swap(w[0][j], w[1][j], false, false);
-            w[0][j] = x[0], w[1][j] = x[1];
+          for (int a = 0; a < 4; a += 2) {
+            uint32_t w[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              w[0][j] = T::pack(o[i][4 * a + 2 * j], o[i][4 * a + 2 * j + 1]), w[1][j] = T::pack(o[i][4 * a + 4 + 2 * j], o[i][4 * a + 5 + 2 * j]);
+              const auto x = __builtin_amdgcn_permlane32_swap(w[0][j], w[1][j], false, false);
+              w[0][j] = x[0], w[1][j] = x[1];
+            }
+            if (row < count) *reinterpret_cast<v4u32*>(reinterpret_cast<uint16_t*>(out) + at + 8 * a + 8 * half) = v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
           }
-          if (col < count) *reinterpret_cast<v4u32*>(reinterpret_cast<uint16_t*>(out) + at + 8 * a + 8 * half) = v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
-        }
-      } else if (col < count) {
-        if (p.out_dtype == VXA_F32) {
+        } else if (row < count) {
+          if (p.out_dtype == VXA_F32) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) reinterpret_cast<float*>(out)[at + 8 * (r / 4) + 4 * half + r % 4] = o[r];
-        } else {
+            for (int r = 0; r < 16; ++r) reinterpret_cast<float*>(out)[at + 8 * (r / 4) + 4 * half + r % 4] = o[i][r];
+          } else {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) store_f32_as(out, p.out_dtype, at + 8 * (r / 4) + 4 * half + r % 4, o[r]);
+            for (int r = 0; r < 16; ++r) store_f32_as(out, p.out_dtype, at + 8 * (r / 4) + 4 * half + r % 4, o[i][r]);
+          }
         }
       }
     }
-    if (kLate && t0 + kChunk < rows) fetch(t0 + kChunk);
-    const float decay = count == kChunk ? full : power(g, count);
+    if (kLate && t0 + C < rows) fetch(t0 + C);
+    // The state. Values are weighted and split into three parts, which keep the 24 bits of the products; the keys are exact.
+    const float decay = count == C ? full : power(g, count);
 #pragma unroll
-    for (int t = 0; t < DT; ++t) {
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[t][r] *= decay;
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < CT; ++c) {
+      float f[8];
+      floats<T>(v[c], f);
 #pragma unroll
-        for (int n = 0; n < 3; ++n) {
-          const v4u32 k = transposed(now, s_kd[n], c, t);
-          s[t] = BF16::mfma32(k, v[0][c], s[t]);
-          if constexpr (F16)
-            if (n < 2) s[t] = BF16::mfma32(k, v[1][c], s[t]);
+      for (int j = 0; j < 8; j += 4) {
+        const v4f w = *reinterpret_cast<const v4f*>(sh.left + 16 * c + 4 * (now >> 5) + 2 * j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[j + e] *= w[e];
+      }
+      v4u32 three[3];
+      split(f, three);
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const v4u32 k = transposed(now, sh.kt[0], c, t);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) s[t] = BF16::mfma32(k, three[n], s[t]);
+        if constexpr (F16) {
+          const v4u32 low = transposed(now, sh.kt[1], c, t);
+          s[t] = BF16::mfma32(low, three[0], s[t]);
+          s[t] = BF16::mfma32(low, three[1], s[t]);
         }
-      __builtin_amdgcn_sched_barrier(0);
+        if (D == 256 && t % 2) __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
   float* to = nullptr;
   if (!OUT)
-    to = kept + kept_at(p, part, part.part + 1, head, D * D);
+    to = kept + kept_at(p, part.lo, part.part + 1, head, D * D);
   else if (part.part == part.parts - 1 && slots.write >= 0)
     to = p.state + slots.write * p.sss + head * p.ssh;
   if (to) state_rows([&](int t, int r, int64_t at) { to[at] = s[t][r]; });
 }
 
-// The states before a long sequence's parts, from what each part adds: 4 values of one head a thread.
+// The states before a long sequence's third part and later, from what each part adds: 4 values of one head a thread.
 __global__ __launch_bounds__(256) void linear_parts_kernel(LinearParams p, float* kept, int size) {
   const int pieces = size / 1024, head = (int)(blockIdx.x / pieces) % p.H, seq = (int)(blockIdx.x / pieces) / p.H;
   const int lo = min(max(p.cu[seq], 0), p.total), len = min(max(p.cu[seq + 1], lo), p.total) - lo;
-  if (len <= kPart) return;
-  const Part part{seq, lo, len, 0, (len + kPart - 1) / kPart};
-  const int at = 4 * ((int)(blockIdx.x % pieces) * 256 + (int)threadIdx.x);
-  const int read = p.read ? p.read[seq] : -1;
-  v4f s = {0, 0, 0, 0};
-  if (read >= 0 && read < p.slots) s = *reinterpret_cast<const v4f*>(p.state + read * p.sss + head * p.ssh + at);
+  const int parts = (len + kPart - 1) / kPart;
+  if (parts < 3) return;
+  v4f* x = reinterpret_cast<v4f*>(kept + kept_at(p, lo, 1, head, size)) + (int)(blockIdx.x % pieces) * 256 + (int)threadIdx.x;
+  const int64_t step = (int64_t)p.H * size / 4;
   const float decay = power(p.log_decay[head], kPart);
-  for (int i = 0; i < part.parts; ++i) {
-    v4f* x = reinterpret_cast<v4f*>(kept + kept_at(p, part, i, head, size) + at);
-    if (i > 0) {
-      const v4f add = *x;
+  v4f s = *x;
+#pragma unroll 4
+  for (int i = 2; i < parts; ++i) {
+    const v4f add = x[(i - 1) * step];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] = fmaf(s[e], decay, add[e]);
-    }
-    *x = s;
+    for (int e = 0; e < 4; ++e) s[e] = fmaf(s[e], decay, add[e]);
+    x[(i - 1) * step] = s;
   }
 }
 
@@ -492,7 +542,7 @@ hipError_t launch_prompt(const LinearParams& p, float* kept, hipStream_t st) {
   if (!launchable(blocks, 2 * D) || !launchable(pieces, 256)) return hipErrorInvalidConfiguration;
   if (p.total > kPart) {  // some sequence may have several parts
     hipLaunchKernelGGL((linear_chunk_kernel<T, D, false>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
-    hipLaunchKernelGGL(linear_parts_kernel, dim3((unsigned)pieces), dim3(256), 0, st, p, kept, D * D);
+    if (p.total > 2 * kPart) hipLaunchKernelGGL(linear_parts_kernel, dim3((unsigned)pieces), dim3(256), 0, st, p, kept, D * D);
   }
   hipLaunchKernelGGL((linear_chunk_kernel<T, D, true>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
   return hipGetLastError();
