@@ -15,10 +15,10 @@
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kEach = 32;                  // values of a thread, in runs of 8
+constexpr int kEach = 64;                  // values of a thread, in runs of 8
 constexpr int kSlice = kThreads * kEach;   // values of a workgroup
 constexpr int kMost = 64;                  // of `count`: a wave has so many lane maxima
-constexpr int kWaveList = 128;             // candidates that a wave may list; more (many equal values) are picked one by one
+constexpr int kWaveList = 128;             // candidates that a wave may list; where more values are near (many equal ones) it looks closer
 constexpr int kMostSlices = 4096;          // of a request
 
 typedef unsigned long long u64;
@@ -64,16 +64,32 @@ __device__ inline double wave_sum(double x) {
   return x;
 }
 
-// exp(d) for d <= 0, off by a few 2^-25: the product with log2(e) is split into a whole part and a rest that keeps its bits.
+// exp(d) for -80 <= d <= 0, off by a few 2^-25: of the product with log2(e), the whole part goes to the exponent and the rest
+// keeps its bits.
 __device__ inline float exp_of(float d) {
   constexpr float kLog2e = 1.44269504f, kRest = 1.92596303e-8f;  // their sum: log2(e) to 48 bits
-  d = d < -200.0f ? -200.0f : d;  // 0, also of -inf; a NaN stays one
-  const float whole = __builtin_rintf(d * kLog2e);
-  return __builtin_amdgcn_ldexpf(exp2_hw(fmaf(d, kRest, fmaf(d, kLog2e, -whole))), (int)whole);
+  constexpr float kMagic = 12582912.0f;                          // 1.5 2^23: added, it rounds to a whole number in the lowest bits
+  const float m = fmaf(d, kLog2e, kMagic), whole = m - kMagic;
+  return __uint_as_float(__float_as_uint(exp2_hw(fmaf(d, kRest, fmaf(d, kLog2e, -whole)))) + (__float_as_uint(m) << 23));
 }
 
 template <int DTYPE>
-__global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamParams p) {
+struct Logits {
+  using Element = std::conditional_t<DTYPE == VXA_F32, float, uint16_t>;
+  const Element* row;  // which may start at any element
+  static __device__ inline float value(Element e) {
+    if constexpr (DTYPE == VXA_F32)
+      return e;
+    else if constexpr (DTYPE == VXA_BF16)
+      return bf16_to_f32(e);
+    else
+      return (float)__builtin_bit_cast(_Float16, e);
+  }
+  __device__ inline float at(int place) const { return value(row[place]); }
+};
+
+template <int DTYPE>
+__global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(BeamParams p) {
   __shared__ u64 s_list[kWaves * kWaveList];
   __shared__ int s_count;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -82,80 +98,109 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamParams p) {
   __syncthreads();
 
   // Run r of a thread: places slice * kSlice + r * 8 * kThreads + 8 * thread + 0..7.
+  const Logits<DTYPE> logits{reinterpret_cast<const typename Logits<DTYPE>::Element*>(p.logits) + (int64_t)row * p.stride};
+  auto place_of = [&](int i) { return slice * kSlice + (i / 8 * kThreads + (int)threadIdx.x) * 8 + i % 8; };
   float x[kEach];
-  const int64_t base = (int64_t)row * p.stride;
+  auto load = [&](auto whole_c) {
+    constexpr bool kWhole = decltype(whole_c)::value;  // the slice lies within the row; else its runs may pass the row's end
+    typename Logits<DTYPE>::Element e[kEach];
 #pragma unroll
-  for (int r = 0; r < kEach / 8; ++r) {
-    const int place = slice * kSlice + (r * kThreads + (int)threadIdx.x) * 8;
+    for (int r = 0; r < kEach; r += 8) __builtin_memcpy(e + r, logits.row + (kWhole ? place_of(r) : min(place_of(r), p.vocab - 8)), sizeof(e) / (kEach / 8));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float v = kNegInf;
-      if (place + j < p.vocab) {
-        if (DTYPE == VXA_F32)
-          v = reinterpret_cast<const float*>(p.logits)[base + place + j];
-        else if (DTYPE == VXA_BF16)
-          v = bf16_to_f32(reinterpret_cast<const uint16_t*>(p.logits)[base + place + j]);
-        else
-          v = (float)reinterpret_cast<const _Float16*>(p.logits)[base + place + j];
+    for (int r = 0; r < kEach; r += 8)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[r + j] = kWhole || place_of(r) + 8 <= p.vocab ? logits.value(e[r + j]) : kNegInf;
+  };
+  if ((slice + 1) * kSlice <= p.vocab) {
+    load(std::true_type{});
+  } else {
+    if (p.vocab >= 8)
+      load(std::false_type{});
+    else
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) x[i] = kNegInf;
+#pragma unroll
+    for (int r = 0; r < kEach; r += 8)
+      if (place_of(r) < p.vocab && place_of(r) + 8 > p.vocab) {  // the run that the row ends in
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (place_of(r) + j < p.vocab) x[r + j] = logits.at(place_of(r) + j);
       }
-      x[8 * r + j] = v;
-    }
   }
-  auto place_of = [&](int i) { return (uint32_t)(slice * kSlice + (i / 8 * kThreads + (int)threadIdx.x) * 8 + i % 8); };
 
-  float top = kNegInf;
+  float top = x[0];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) top = fmaxf(top, x[i]);
+  for (int i = 1; i < kEach; ++i) top = __builtin_elementwise_maximum(top, x[i]);  // a NaN where there is one
+  if (top != top) top = __builtin_nanf("");
   const uint32_t mine = order_of(top);
-  const float most = value_of((uint32_t)(wave_max((u64)mine << 32 | 1) >> 32));  // of order 0: a NaN, and then nothing is summed
-  const float ref = __any(mine != 0) ? most : 0.0f;
+  const uint32_t highest = (uint32_t)(wave_max((u64)mine << 32) >> 32);
+  const float most = value_of(highest);  // a NaN's order is above all others
   double sum = 0.0;
+  if (highest != 0 && !(most < __builtin_huge_valf())) {
+    sum = __builtin_nan("");
+  } else if (highest != 0) {  // what is more than 80 below counts as nothing in fp64 sums of 2^31 terms
 #pragma unroll
-  for (int i = 0; i < kEach; i += 4) {
-    float part = 0.0f;
+    for (int i = 0; i < kEach; i += 8) {
+      float part = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) part += exp_of(x[i + j] - ref);
-    sum += (double)part;
+      for (int j = 0; j < 8; ++j) part += exp_of(__builtin_amdgcn_fmed3f(x[i + j] - most, -80.0f, 0.0f));
+      sum += (double)part;
+    }
+    sum = wave_sum(sum);
   }
-  sum = wave_sum(sum);
-  const bool any = __any(mine != 0);
-  if (lane == 0) p.tops[(int64_t)blockIdx.x * kWaves + wave] = any ? most : kNegInf, p.sums[(int64_t)blockIdx.x * kWaves + wave] = sum;
+  if (lane == 0) p.tops[(int64_t)blockIdx.x * kWaves + wave] = highest ? most : kNegInf, p.sums[(int64_t)blockIdx.x * kWaves + wave] = sum;
 
-  // The count-th largest order among the lanes' maxima, bit by bit; at least 1.
+  // The count-th largest order among the lanes' maxima, bit by bit; at least 1. (Orders of 16-bit types differ in the upper bits.)
   uint32_t bar = 0;
 #pragma unroll
-  for (int b = 31; b >= (DTYPE == VXA_F32 ? 0 : 12); --b)
+  for (int b = 31; b >= (DTYPE == VXA_F32 ? 0 : DTYPE == VXA_BF16 ? 16 : 13); --b)
     if (__popcll(__ballot(mine >= (bar | 1u << b))) >= p.count) bar |= 1u << b;
-  if (bar == 0) bar = 1;
-  int many = 0;
+  const float least = bar == 0 ? -3.402823466e38f : value_of(bar);
+  uint64_t mask = 0;  // this lane's values that are not below the bar
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) many += order_of(x[i]) >= bar;
+  for (int i = 0; i < kEach; ++i)
+    if (x[i] >= least) mask |= 1ull << i;
+  const int many = __popcll(mask);
   const int before = wave_scan(many, [](int a, int b) { return a + b; });
   const int all = __builtin_amdgcn_readlane(before, 63);
   if (all <= kWaveList) {
     int at = 0;
     if (lane == 0 && all) at = atomicAdd(&s_count, all);
     at = __builtin_amdgcn_readfirstlane(at) + before - many;
-    if (many) {
-#pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (order_of(x[i]) >= bar) s_list[at++] = key_of(order_of(x[i]), place_of(i));
+    for (; mask; mask &= mask - 1) {  // a lane's only one is its maximum
+      const int place = place_of(__builtin_ctzll(mask));
+      s_list[at++] = key_of(order_of(many > 1 ? logits.at(place) : top), (uint32_t)place);
     }
-  } else {  // many values equal the bar: one after the other, each the largest below the last
+  } else {  // many values are near the bar: the wave's count-th largest value, then all above it and the first that equal it
+    uint32_t order = 0;
+#pragma unroll 1
+    for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1) {
+      const float v = value_of(order | bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) n += x[i] >= v;
+      if (wave_reduce(n, [](int a, int b) { return a + b; }) >= p.count) order |= bit;
+    }
+    const float kth = value_of(order);
     int at = 0;
     if (lane == 0) at = atomicAdd(&s_count, p.count);
     at = __builtin_amdgcn_readfirstlane(at);
-    u64 last = ~0ull;
-    for (int c = 0; c < p.count; ++c) {
-      u64 best = 0;
+    const int end = at + p.count;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const u64 key = key_of(order_of(x[i]), place_of(i));
-        if (key < last && key > best) best = key;
+    for (int equal = 0; equal < 2; ++equal)
+#pragma unroll
+      for (int r = 0; r < kEach; r += 8) {  // places rise with the run, then the lane, then within the run
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) n += equal ? x[r + j] == kth : x[r + j] > kth;
+        const int upto = wave_scan(n, [](int a, int b) { return a + b; });
+        int mine_at = at + upto - n;
+        if (n)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if ((equal ? x[r + j] == kth : x[r + j] > kth) && mine_at < end) s_list[mine_at++] = key_of(order_of(x[r + j]), (uint32_t)place_of(r + j));
+        at += __builtin_amdgcn_readlane(upto, 63);
       }
-      last = wave_max(best);
-      if (lane == 0) s_list[at + c] = last;
-    }
   }
   __syncthreads();
 
@@ -230,13 +275,17 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamParams p) {
   auto above = [](u64 o, uint32_t q, u64 order, uint32_t place) { return o > order || (o == order && q < place); };
   for (int g = threadIdx.x; g < groups; g += kJoin) score(g, 0, s_order[g], s_place[g]);
   __syncthreads();
-  // The slice whose best is the count-th: no candidate below it is among the best.
-  for (int g = threadIdx.x; g < groups; g += kJoin) {
-    const u64 order = s_order[g];
-    const uint32_t place = s_place[g];
+  // The slice whose best is the count-th: no candidate below it is among the best. 2^share threads compare one slice.
+  int share = 0;
+  while (share < 6 && groups << (share + 1) <= kJoin) ++share;
+  for (int g0 = 0; g0 < groups; g0 += kJoin >> share) {
+    const int g = g0 + ((int)threadIdx.x >> share);
+    const u64 order = g < groups ? s_order[g] : 0;
+    const uint32_t place = g < groups ? s_place[g] : 0;
     int rank = 0;
     if (order)
-      for (int j = 0; j < groups; ++j) rank += above(s_order[j], s_place[j], order, place);
+      for (int j = threadIdx.x & ((1 << share) - 1); j < groups; j += 1 << share) rank += above(s_order[j], s_place[j], order, place);
+    for (int m = 1; m < 1 << share; m *= 2) rank += __builtin_amdgcn_ds_bpermute(((int)threadIdx.x & 63 ^ m) << 2, rank);
     if (order && rank == p.count - 1) s_bar = g;
   }
   __syncthreads();
