@@ -15,8 +15,11 @@
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kEach = 64;                  // values of a thread, in runs of 8
-constexpr int kSlice = kThreads * kEach;   // values of a workgroup
+constexpr int kWords = 32;                 // of a thread's values, as they are in memory
+template <int DTYPE>
+constexpr int kEach = DTYPE == VXA_F32 ? kWords : 2 * kWords;  // values of a thread, in runs of 8
+template <int DTYPE>
+constexpr int kSlice = kThreads * kEach<DTYPE>;                // values of a workgroup
 constexpr int kMost = 64;                  // of `count`: a wave has so many lane maxima
 constexpr int kWaveList = 128;             // candidates that a wave may list; where more values are near (many equal ones) it looks closer
 constexpr int kMostSlices = 4096;          // of a request
@@ -73,23 +76,29 @@ __device__ inline float exp_of(float d) {
   return __uint_as_float(__float_as_uint(exp2_hw(fmaf(d, kRest, fmaf(d, kLog2e, -whole)))) + (__float_as_uint(m) << 23));
 }
 
+// Element of a row of logits, which may start at any element.
 template <int DTYPE>
-struct Logits {
-  using Element = std::conditional_t<DTYPE == VXA_F32, float, uint16_t>;
-  const Element* row;  // which may start at any element
-  static __device__ inline float value(Element e) {
-    if constexpr (DTYPE == VXA_F32)
-      return e;
-    else if constexpr (DTYPE == VXA_BF16)
-      return bf16_to_f32(e);
-    else
-      return (float)__builtin_bit_cast(_Float16, e);
-  }
-  __device__ inline float at(int place) const { return value(row[place]); }
-};
+using Element = std::conditional_t<DTYPE == VXA_F32, float, uint16_t>;
+template <int DTYPE>
+__device__ inline float value(Element<DTYPE> e) {
+  if constexpr (DTYPE == VXA_F32)
+    return e;
+  else if constexpr (DTYPE == VXA_BF16)
+    return bf16_to_f32(e);
+  else
+    return (float)__builtin_bit_cast(_Float16, e);
+}
+template <int DTYPE>
+__device__ inline uint32_t word(Element<DTYPE> e) {  // in the lower half, or the whole
+  if constexpr (DTYPE == VXA_F32)
+    return __float_as_uint(e);
+  else
+    return e;
+}
 
 template <int DTYPE>
-__global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(BeamParams p) {
+__global__ __launch_bounds__(kThreads, 6) void beam_slice_kernel(BeamParams p) {
+  constexpr int kEach = ::kEach<DTYPE>, kSlice = ::kSlice<DTYPE>, kRun = 8 * kWords / kEach;  // words of a run
   __shared__ u64 s_list[kWaves * kWaveList];
   __shared__ int s_count;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -97,45 +106,58 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(BeamParams p) {
   if (threadIdx.x == 0) s_count = 0;
   __syncthreads();
 
-  // Run r of a thread: places slice * kSlice + r * 8 * kThreads + 8 * thread + 0..7.
-  const Logits<DTYPE> logits{reinterpret_cast<const typename Logits<DTYPE>::Element*>(p.logits) + (int64_t)row * p.stride};
+  // Run r of a thread: places slice * kSlice + r * 8 * kThreads + 8 * thread + 0..7. Its values stay as they came; each pass takes
+  // them apart again, which costs less than the waves that twice as many registers would.
+  const Element<DTYPE>* logits = reinterpret_cast<const Element<DTYPE>*>(p.logits) + (int64_t)row * p.stride;
   auto place_of = [&](int i) { return slice * kSlice + (i / 8 * kThreads + (int)threadIdx.x) * 8 + i % 8; };
-  float x[kEach];
-  auto load = [&](auto whole_c) {
-    constexpr bool kWhole = decltype(whole_c)::value;  // the slice lies within the row; else its runs may pass the row's end
-    typename Logits<DTYPE>::Element e[kEach];
-#pragma unroll
-    for (int r = 0; r < kEach; r += 8) __builtin_memcpy(e + r, logits.row + (kWhole ? place_of(r) : min(place_of(r), p.vocab - 8)), sizeof(e) / (kEach / 8));
-#pragma unroll
-    for (int r = 0; r < kEach; r += 8)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[r + j] = kWhole || place_of(r) + 8 <= p.vocab ? logits.value(e[r + j]) : kNegInf;
-  };
-  if ((slice + 1) * kSlice <= p.vocab) {
-    load(std::true_type{});
-  } else {
-    if (p.vocab >= 8)
-      load(std::false_type{});
+  uint32_t w[kWords];
+  auto x = [&](int i) {
+    if constexpr (DTYPE == VXA_F32)
+      return __uint_as_float(w[i]);
+    else if constexpr (DTYPE == VXA_BF16)
+      return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
     else
+      return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i / 2] >> (16 * (i % 2))));
+  };
+  auto again = [&] {
+    if constexpr (DTYPE != VXA_F32)
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) x[i] = kNegInf;
+      for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+  };
+  constexpr uint32_t kNothing = DTYPE == VXA_F32 ? 0xFF800000u : DTYPE == VXA_BF16 ? 0xFF80FF80u : 0xFC00FC00u;  // -inf
+  const bool whole = (slice + 1) * kSlice <= p.vocab;
+  if (whole || p.vocab >= 8) {
 #pragma unroll
-    for (int r = 0; r < kEach; r += 8)
-      if (place_of(r) < p.vocab && place_of(r) + 8 > p.vocab) {  // the run that the row ends in
+    for (int r = 0; r < kEach / 8; ++r) __builtin_memcpy(w + r * kRun, logits + (whole ? place_of(8 * r) : min(place_of(8 * r), p.vocab - 8)), 4 * kRun);
+  }
+  if (!whole) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (place_of(r) + j < p.vocab) x[r + j] = logits.at(place_of(r) + j);
+    for (int r = 0; r < kEach / 8; ++r) {
+      const int place = place_of(8 * r);
+      if (place + 8 > p.vocab) {
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) w[r * kRun + j] = kNothing;
+        if (place < p.vocab) {  // the run that the row ends in
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t e = word<DTYPE>(logits[min(place + j, p.vocab - 1)]);
+            uint32_t& to = w[r * kRun + j * kRun / 8];
+            if (place + j < p.vocab) to = DTYPE == VXA_F32 ? e : j % 2 ? (to & 0xFFFFu) | e << 16 : (to & 0xFFFF0000u) | e;
+          }
+        }
       }
+    }
   }
 
-  float top = x[0];
+  float top = x(0);
 #pragma unroll
-  for (int i = 1; i < kEach; ++i) top = __builtin_elementwise_maximum(top, x[i]);  // a NaN where there is one
+  for (int i = 1; i < kEach; ++i) top = __builtin_elementwise_maximum(top, x(i));  // a NaN where there is one
   if (top != top) top = __builtin_nanf("");
   const uint32_t mine = order_of(top);
   const uint32_t highest = (uint32_t)(wave_max((u64)mine << 32) >> 32);
   const float most = value_of(highest);  // a NaN's order is above all others
   double sum = 0.0;
+  again();
   if (highest != 0 && !(most < __builtin_huge_valf())) {
     sum = __builtin_nan("");
   } else if (highest != 0) {  // what is more than 80 below counts as nothing in fp64 sums of 2^31 terms
@@ -143,7 +165,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(BeamParams p) {
     for (int i = 0; i < kEach; i += 8) {
       float part = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) part += exp_of(__builtin_amdgcn_fmed3f(x[i + j] - most, -80.0f, 0.0f));
+      for (int j = 0; j < 8; ++j) part += exp_of(__builtin_amdgcn_fmed3f(x(i + j) - most, -80.0f, 0.0f));
       sum += (double)part;
     }
     sum = wave_sum(sum);
@@ -156,10 +178,13 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(BeamParams p) {
   for (int b = 31; b >= (DTYPE == VXA_F32 ? 0 : DTYPE == VXA_BF16 ? 16 : 13); --b)
     if (__popcll(__ballot(mine >= (bar | 1u << b))) >= p.count) bar |= 1u << b;
   const float least = bar == 0 ? -3.402823466e38f : value_of(bar);
+  again();
   uint64_t mask = 0;  // this lane's values that are not below the bar
+  if (top >= least) {
 #pragma unroll
-  for (int i = 0; i < kEach; ++i)
-    if (x[i] >= least) mask |= 1ull << i;
+    for (int i = 0; i < kEach; ++i)
+      if (x(i) >= least) mask |= 1ull << i;
+  }
   const int many = __popcll(mask);
   const int before = wave_scan(many, [](int a, int b) { return a + b; });
   const int all = __builtin_amdgcn_readlane(before, 63);
@@ -169,16 +194,17 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(BeamParams p) {
     at = __builtin_amdgcn_readfirstlane(at) + before - many;
     for (; mask; mask &= mask - 1) {  // a lane's only one is its maximum
       const int place = place_of(__builtin_ctzll(mask));
-      s_list[at++] = key_of(order_of(many > 1 ? logits.at(place) : top), (uint32_t)place);
+      s_list[at++] = key_of(order_of(many > 1 ? value<DTYPE>(logits[place]) : top), (uint32_t)place);
     }
   } else {  // many values are near the bar: the wave's count-th largest value, then all above it and the first that equal it
     uint32_t order = 0;
 #pragma unroll 1
     for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1) {
       const float v = value_of(order | bit);
+      again();
       int n = 0;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) n += x[i] >= v;
+      for (int i = 0; i < kEach; ++i) n += x(i) >= v;
       if (wave_reduce(n, [](int a, int b) { return a + b; }) >= p.count) order |= bit;
     }
     const float kth = value_of(order);
@@ -187,20 +213,22 @@ __global__ __launch_bounds__(kThreads, 4) void beam_slice_kernel(BeamParams p) {
     at = __builtin_amdgcn_readfirstlane(at);
     const int end = at + p.count;
 #pragma unroll
-    for (int equal = 0; equal < 2; ++equal)
+    for (int equal = 0; equal < 2; ++equal) {
+      again();
 #pragma unroll
       for (int r = 0; r < kEach; r += 8) {  // places rise with the run, then the lane, then within the run
         int n = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) n += equal ? x[r + j] == kth : x[r + j] > kth;
+        for (int j = 0; j < 8; ++j) n += equal ? x(r + j) == kth : x(r + j) > kth;
         const int upto = wave_scan(n, [](int a, int b) { return a + b; });
         int mine_at = at + upto - n;
         if (n)
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if ((equal ? x[r + j] == kth : x[r + j] > kth) && mine_at < end) s_list[mine_at++] = key_of(order_of(x[r + j]), (uint32_t)place_of(r + j));
+            if ((equal ? x(r + j) == kth : x(r + j) > kth) && mine_at < end) s_list[mine_at++] = key_of(order_of(x(r + j)), (uint32_t)place_of(r + j));
         at += __builtin_amdgcn_readlane(upto, 63);
       }
+    }
   }
   __syncthreads();
 
@@ -285,7 +313,7 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamParams p) {
     int rank = 0;
     if (order)
       for (int j = threadIdx.x & ((1 << share) - 1); j < groups; j += 1 << share) rank += above(s_order[j], s_place[j], order, place);
-    for (int m = 1; m < 1 << share; m *= 2) rank += __builtin_amdgcn_ds_bpermute(((int)threadIdx.x & 63 ^ m) << 2, rank);
+    for (int m = 1; m < 1 << share; m *= 2) rank += __builtin_amdgcn_ds_bpermute((lane ^ m) << 2, rank);
     if (order && rank == p.count - 1) s_bar = g;
   }
   __syncthreads();
@@ -320,11 +348,11 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamParams p) {
     p.out_scores[out + i] = kNegInf, p.out_parents[out + i] = -1, p.out_tokens[out + i] = -1;
 }
 
-int64_t slices_of(int64_t vocab) { return cdiv<int64_t>(vocab, kSlice); }
+int64_t slices_of(int64_t vocab) { return cdiv<int64_t>(vocab, kSlice<VXA_F32>); }  // the most, of any type
 
 int check_sizes(int64_t n, int64_t beams, int64_t vocab, int64_t count) {
   if (n < 0 || beams <= 0 || vocab <= 0 || count <= 0) return VXA_ERR_ARG;
-  if (count > kMost || beams > kMost * 16 || vocab > (1LL << 31) - kSlice || beams * vocab >= 1LL << 31 || beams * slices_of(vocab) > kMostSlices ||
+  if (count > kMost || beams > kMost * 16 || vocab > (1LL << 31) - kSlice<VXA_BF16> || beams * vocab >= 1LL << 31 || beams * slices_of(vocab) > kMostSlices ||
       n > (1 << 30) || n * beams > (1LL << 31) - 1)
     return VXA_ERR_UNSUPPORTED;
   return VXA_OK;
@@ -352,7 +380,7 @@ extern "C" int vxa_beam_select(const void* logits, int64_t stride_row, int dtype
   if (!ws || (uintptr_t)ws % 16 || ws_bytes < bytes) return VXA_ERR_WORKSPACE;
   BeamParams p;
   p.logits = logits, p.stride = stride_row, p.scores = scores;
-  p.n = (int32_t)n, p.beams = (int32_t)beams, p.vocab = (int32_t)vocab, p.count = (int32_t)count, p.slices = (int32_t)slices_of(vocab);
+  p.n = (int32_t)n, p.beams = (int32_t)beams, p.vocab = (int32_t)vocab, p.count = (int32_t)count, p.slices = (int32_t)cdiv<int64_t>(vocab, dtype == VXA_F32 ? kSlice<VXA_F32> : kSlice<VXA_BF16>);
   const int64_t blocks = n * beams * p.slices;
   if (!launchable(blocks, kThreads) || !launchable(n, kJoin)) return VXA_ERR_UNSUPPORTED;
   p.sums = reinterpret_cast<double*>(ws);
