@@ -15,7 +15,7 @@ struct LinearParams {
   int64_t skt, skh;
   const uint16_t* v;
   int64_t svt, svh;
-  const int32_t* cu;  // null: sequence i is row i
+  const int32_t* cu;  // of prompts
   int32_t n, total, H, G;
   const float* log_decay;
   float scale;
@@ -47,68 +47,70 @@ __device__ inline Slots find_slots(const LinearParams& p, int seq) {
   return s;
 }
 
-constexpr int kCols = 32;    // columns of a state that a workgroup keeps
-constexpr int kTokens = 16;  // staged at a time
+// ---------------------------------------------------------------------------------- single tokens
+constexpr int kCols = 32;  // columns of a state that a workgroup takes
 
-// The recurrence as it stands: a workgroup keeps kCols columns of one head's state in registers.
+// A workgroup takes 32 columns of one head's state of one sequence: 128 bytes of each row, D / 8 rows a thread. It reads and writes
+// every value of the state once, and that is what bounds it.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void linear_recurrent_kernel(LinearParams p) {
+__global__ __launch_bounds__(256) void linear_step_kernel(LinearParams p) {
   constexpr int kRows = D / 8;  // of the state, of a thread
-  __shared__ float s_q[kTokens][D], s_k[kTokens][D], s_v[kTokens][kCols], s_o[8][kTokens][kCols];
-  const int slabs = D / kCols;
-  const int slab = blockIdx.x % slabs, head = (int)(blockIdx.x / slabs) % p.H, seq = (int)(blockIdx.x / slabs) / p.H;
+  __shared__ float s_q[D], s_k[D], s_o[8][kCols];
+  constexpr int kSlabs = D / kCols;
+  const int slab = blockIdx.x % kSlabs, head = (int)(blockIdx.x / kSlabs) % p.H, seq = (int)(blockIdx.x / kSlabs) / p.H;
   const int col = threadIdx.x & 31, part = threadIdx.x >> 5;
-  int lo = seq, hi = seq + 1;
-  if (p.cu) {
-    lo = min(max(p.cu[seq], 0), p.total);
-    hi = min(max(p.cu[seq + 1], lo), p.total);
-  }
   const Slots slots = find_slots(p, seq);
-  const int64_t at = (int64_t)head * p.soh + slab * kCols + col;
+  const int64_t at = seq * p.sot + head * p.soh + slab * kCols + col;
   if (slots.bad) {
-    for (int t = lo + part; t < hi; t += 8) store_f32_as(p.out, p.out_dtype, t * p.sot + at, __builtin_nanf(""));
+    if (part == 0) store_f32_as(p.out, p.out_dtype, at, __builtin_nanf(""));
     return;
   }
-  const int64_t place = (int64_t)head * p.ssh + (int64_t)part * kRows * D + slab * kCols + col;
+  const int64_t place = head * p.ssh + part * kRows * D + slab * kCols + col;
   float s[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) s[i] = slots.read >= 0 ? p.state[slots.read * p.sss + place + (int64_t)i * D] : 0.0f;
-  const float decay = expf(p.log_decay[head]);
-  for (int t0 = lo; t0 < hi; t0 += kTokens) {
-    const int count = min(kTokens, hi - t0);
-    __syncthreads();
-    for (int x = threadIdx.x; x < count * D; x += 256) {
-      const int64_t t = t0 + x / D;
-      s_q[x / D][x % D] = T::to_f32(p.q[t * p.sqt + head * p.sqh + x % D]);
-      s_k[x / D][x % D] = T::to_f32(p.k[t * p.skt + head / p.G * p.skh + x % D]);
-    }
-    for (int x = threadIdx.x; x < count * kCols; x += 256)
-      s_v[x / kCols][x % kCols] = T::to_f32(p.v[(int64_t)(t0 + x / kCols) * p.svt + head / p.G * p.svh + slab * kCols + x % kCols]);
-    __syncthreads();
-    for (int t = 0; t < count; ++t) {
-      const float v = s_v[t][col];
-      float o = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        s[i] = fmaf(s_k[t][part * kRows + i], v, decay * s[i]);
-        o = fmaf(s_q[t][part * kRows + i], s[i], o);
-      }
-      s_o[part][t][col] = o;
-    }
-    __syncthreads();
-    for (int t = part; t < count; t += 8) {
-      float o = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o += s_o[i][t][col];
-      store_f32_as(p.out, p.out_dtype, (t0 + t) * p.sot + at, o * p.scale);
-    }
+  for (int x = threadIdx.x; x < D; x += 256) {
+    s_q[x] = T::to_f32(p.q[seq * p.sqt + head * p.sqh + x]);
+    s_k[x] = T::to_f32(p.k[seq * p.skt + head / p.G * p.skh + x]);
   }
+  const float v = T::to_f32(p.v[seq * p.svt + head / p.G * p.svh + slab * kCols + col]);
+  // The decay in two parts: rounded to fp32, its error would grow with every step, as the state's own roundings do not.
+  const double exact = exp((double)p.log_decay[head]);
+  const float decay = (float)exact, rest = (float)(exact - (double)decay);
+  __syncthreads();
+  float o = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    s[i] = fmaf(s[i], decay, fmaf(s[i], rest, s_k[part * kRows + i] * v));
+    o = fmaf(s_q[part * kRows + i], s[i], o);
+  }
+  s_o[part][col] = o;
   if (slots.write >= 0) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) p.state[slots.write * p.sss + place + (int64_t)i * D] = s[i];
   }
+  __syncthreads();
+  if (part == 0) {
+    o = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o += s_o[i][col];
+    store_f32_as(p.out, p.out_dtype, at, o * p.scale);
+  }
 }
 
+template <typename T>
+hipError_t launch_step(int64_t D, const LinearParams& p, hipStream_t st) {
+  const int64_t blocks = (int64_t)p.n * p.H * (D / kCols);
+  if (!launchable(blocks, 256)) return hipErrorInvalidConfiguration;
+  const dim3 grid((unsigned)blocks);
+  if (D == 64)
+    hipLaunchKernelGGL((linear_step_kernel<T, 64>), grid, dim3(256), 0, st, p);
+  else if (D == 128)
+    hipLaunchKernelGGL((linear_step_kernel<T, 128>), grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((linear_step_kernel<T, 256>), grid, dim3(256), 0, st, p);
+  return hipGetLastError();
+}
 
 // ---------------------------------------------------------------------------------- prompts
 // Rows go in chunks: with S the state before a chunk of n rows and i, j the rows in it,
@@ -150,27 +152,48 @@ __device__ inline int again(int id) {
   return id;
 }
 
-// Part `part` of sequence seq, for workgroup `index` of the grid's floor(tokens / kPart) + n: sequence i has the places from
-// floor(cu[i] / kPart) + i on, at least as many as it has parts.
+// Part `part` of sequence seq. The grid has floor(tokens / kPart) + n places: the whole parts come first, then what is left of the
+// sequences (and empty ones), 64 sequences at a time the longest first, so that the last workgroups are short ones.
 struct Part {
   int seq, lo, len, part, parts;  // parts: of the sequence, at least 1
 };
 __device__ inline Part find_part(const LinearParams& p, int index) {
   const int lane = threadIdx.x & 63;
-  auto start = [&](int i) { return min(max(p.cu[i], 0), p.total); };
-  int seq = 0;
-  for (int j0 = 0; j0 < p.n; j0 += 64) {
-    const int j = j0 + lane;
-    const uint64_t past = __ballot(j < p.n && start(j) / kPart + j > index);
-    if (past) {
-      seq = j0 + __builtin_ctzll(past) - 1;
-      break;
+  auto add = [](int a, int b) { return a + b; };
+  auto lengths = [&](int j, int& lo, int& len) {
+    lo = len = 0;
+    if (j < p.n) {
+      lo = min(max(p.cu[j], 0), p.total);
+      len = max(min(p.cu[j + 1], p.total) - lo, 0);
     }
-    seq = min(j0 + 63, p.n - 1);
+  };
+  auto found = [&](int j, int lo, int len, int at, bool whole, int part) {  // of lane `at`
+    lo = __builtin_amdgcn_readlane(lo, at), len = __builtin_amdgcn_readlane(len, at);
+    return Part{j + at, lo, len, whole ? part : len / kPart, max(1, (len + kPart - 1) / kPart)};
+  };
+  for (int j0 = 0; j0 < p.n; j0 += 64) {
+    int lo, len;
+    lengths(j0 + lane, lo, len);
+    const int upto = wave_scan(len / kPart, add), all = __builtin_amdgcn_readlane(upto, 63);
+    if (index < all) {
+      const int at = __builtin_ctzll(__ballot(upto > index));
+      return found(j0, lo, len, at, true, index - __builtin_amdgcn_readlane(upto - len / kPart, at));
+    }
+    index -= all;
   }
-  seq = __builtin_amdgcn_readfirstlane(max(seq, 0));
-  const int lo = start(seq), hi = max(start(seq + 1), lo);
-  return Part{seq, lo, hi - lo, index - (lo / kPart + seq), max(1, (hi - lo + kPart - 1) / kPart)};
+  for (int j0 = 0; j0 < p.n; j0 += 64) {
+    int lo, len;
+    lengths(j0 + lane, lo, len);
+    const bool has = j0 + lane < p.n && (len % kPart != 0 || len == 0);
+    const int all = __popcll(__ballot(has)), key = has ? (len % kPart) * 64 + lane : -1;
+    if (index < all) {
+      int rank = 0;
+      for (int m = 0; m < min(64, p.n - j0); ++m) rank += __builtin_amdgcn_readlane(key, m) > key;
+      return found(j0, lo, len, __builtin_ctzll(__ballot(has && rank == index)), false, 0);
+    }
+    index -= all;
+  }
+  return Part{0, 0, 0, 0, 0};
 }
 // Where the state before part `part` of a sequence of several parts is kept: 2 floor(lo / kPart) + part. (The parts of a
 // sequence longer than kPart are at most twice its whole ones.)
@@ -210,7 +233,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   const int x = (int)(blockIdx.x % p.H);
   const int head = p.H % 8 == 0 ? (x % 8) * (p.H / 8) + x / 8 : x;  // heads of one KV head on one XCD
   const Part part = find_part(p, (int)(blockIdx.x / p.H));
-  if (part.part < 0 || part.part >= part.parts - (OUT ? 0 : 1)) return;
+  if (part.part >= part.parts - (OUT ? 0 : 1)) return;
   const Slots slots = find_slots(p, part.seq);
   const int row0 = part.part * kPart, rows = min(kPart, part.len - row0);
   const int64_t base = part.lo + row0;
@@ -554,20 +577,6 @@ hipError_t launch_prompt(int64_t D, const LinearParams& p, float* kept, hipStrea
   return launch_prompt<T, 256>(p, kept, st);
 }
 
-template <typename T>
-hipError_t launch_recurrent(int64_t D, const LinearParams& p, hipStream_t st) {
-  const int64_t blocks = (int64_t)p.n * p.H * (D / kCols);
-  if (!launchable(blocks, 256)) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)blocks);
-  if (D == 64)
-    hipLaunchKernelGGL((linear_recurrent_kernel<T, 64>), grid, dim3(256), 0, st, p);
-  else if (D == 128)
-    hipLaunchKernelGGL((linear_recurrent_kernel<T, 128>), grid, dim3(256), 0, st, p);
-  else
-    hipLaunchKernelGGL((linear_recurrent_kernel<T, 256>), grid, dim3(256), 0, st, p);
-  return hipGetLastError();
-}
-
 // What both entry points check, and their parameters.
 int linear_params(LinearParams& p, const void* q, int64_t sqt, int64_t sqh, const void* k, int64_t skt, int64_t skh, const void* v,
                   int64_t svt, int64_t svh, int dtype, int64_t n, int64_t tokens, const float* log_decay, float scale, void* out,
@@ -640,5 +649,5 @@ extern "C" int vxa_linear_step(const void* q, int64_t sqt, int64_t sqh, const vo
                                slots, sss, ssh, read_slots, write_slots, num_heads, num_kv_heads, head_dim);
   if (rc != VXA_OK || n == 0) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  return status_of(dtype == VXA_BF16 ? launch_recurrent<BF16>(head_dim, p, st) : launch_recurrent<FP16>(head_dim, p, st));
+  return status_of(dtype == VXA_BF16 ? launch_step<BF16>(head_dim, p, st) : launch_step<FP16>(head_dim, p, st));
 }
