@@ -38,11 +38,14 @@ struct Slots {
 __device__ inline Slots find_slots(const LinearParams& p, int seq) {
   Slots s{p.read ? p.read[seq] : -1, p.write ? p.write[seq] : -1, false};
   bool bad = s.read >= p.slots || s.write >= p.slots;
-  if (p.write)
-    for (int j = threadIdx.x; j < p.n; j += blockDim.x) {
-      const int w = p.write[j];
-      if (j != seq) bad |= (w >= 0 && (w == s.write || w == s.read)) || (p.read && s.write >= 0 && p.read[j] == s.write);
-    }
+  if (p.n == 1 || !p.write) {  // no other sequence writes
+    s.bad = bad;
+    return s;
+  }
+  for (int j = threadIdx.x; j < p.n; j += blockDim.x) {
+    const int w = p.write[j];
+    if (j != seq) bad |= (w >= 0 && (w == s.write || w == s.read)) || (p.read && s.write >= 0 && p.read[j] == s.write);
+  }
   s.bad = __syncthreads_or(bad);
   return s;
 }
@@ -232,18 +235,12 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   const int col = lane & 31, half = lane >> 5;
   const int x = (int)(blockIdx.x % p.H);
   const int head = p.H % 8 == 0 ? (x % 8) * (p.H / 8) + x / 8 : x;  // heads of one KV head on one XCD
+  const float g = p.log_decay[head];
   const Part part = find_part(p, (int)(blockIdx.x / p.H));
   if (part.part >= part.parts - (OUT ? 0 : 1)) return;
-  const Slots slots = find_slots(p, part.seq);
   const int row0 = part.part * kPart, rows = min(kPart, part.len - row0);
   const int64_t base = part.lo + row0;
   char* const out = reinterpret_cast<char*>(p.out);
-  if (slots.bad) {
-    if (OUT)
-      for (int i = threadIdx.x; i < rows * D; i += 2 * D) store_f32_as(out, p.out_dtype, (base + i / D) * p.sot + head * p.soh + i % D, __builtin_nanf(""));
-    return;
-  }
-  const float g = p.log_decay[head];
   const uint16_t* const qh = p.q + head * p.sqh;
   const uint16_t* const kh = p.k + head / p.G * p.skh;
   const uint16_t* const vh = p.v + head / p.G * p.svh;
@@ -312,6 +309,12 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
       for (int r = 0; r < 16; ++r) f(t, r, (int64_t)(32 * t + 8 * (r / 4) + r % 4) * D + corner);
   };
   fetch(0);
+  const Slots slots = find_slots(p, part.seq);
+  if (slots.bad) {
+    if (OUT)
+      for (int i = threadIdx.x; i < rows * D; i += 2 * D) store_f32_as(out, p.out_dtype, (base + i / D) * p.sot + head * p.soh + i % D, __builtin_nanf(""));
+    return;
+  }
   if ((int)threadIdx.x < C) sh.power[threadIdx.x] = sh.left[threadIdx.x] = power(g, C - 1 - (int)threadIdx.x);
   // A sequence of several parts that writes the slot that it reads keeps its first state apart: its last part may end before the first
   // begins.

@@ -123,8 +123,8 @@ __device__ int find_free(const TableParams& p, int wanted, int* s_wave, F&& give
   return min(found, wanted);
 }
 
-__device__ inline void copy_refs(const TableParams& p) {
-  for (int64_t i = (int64_t)(blockIdx.x - 1) * kPlan + threadIdx.x; i < p.num_blocks; i += (int64_t)(gridDim.x - 1) * kPlan) p.out_refs[i] = p.refs[i];
+__device__ inline void copy_refs(const TableParams& p, int share, int shares) {
+  for (int64_t i = (int64_t)share * kPlan + threadIdx.x; i < p.num_blocks; i += (int64_t)shares * kPlan) p.out_refs[i] = p.refs[i];
 }
 
 // Length of row r's parent, and the page of its partly filled end (-1: there is none, or not one of the cache).
@@ -144,7 +144,7 @@ __device__ inline Parent parent_of(const TableParams& p, int r) {
 
 __global__ __launch_bounds__(kPlan) void pages_fork_plan_kernel(TableParams p) {
   __shared__ int s_first[kMostRows], s_children[kMostRows], s_wave[kPlan / 64];
-  if (blockIdx.x > 0) return copy_refs(p);
+  if (blockIdx.x > 0) return copy_refs(p, blockIdx.x - 1, gridDim.x - 1);
   int32_t *children = p.ws, *source = p.ws + p.rows, *target = source + p.new_rows;
   for (int i = threadIdx.x; i < p.rows; i += kPlan) s_first[i] = 0x7FFFFFFF, s_children[i] = 0;
   __syncthreads();
@@ -222,9 +222,8 @@ __global__ __launch_bounds__(256) void pages_fork_copy_kernel(TableParams p, Vie
   if (source[r] >= 0 && target[r] >= 0) copy_page(views.at[blockIdx.y], p.page, source[r], target[r], threadIdx.x, 256);
 }
 
-__global__ __launch_bounds__(kPlan) void pages_resize_plan_kernel(TableParams p) {
-  __shared__ int s_wave[kPlan / 64];
-  if (blockIdx.x > 0) return copy_refs(p);
+// Where each row's new pages are in the list of free ones, and the list.
+__device__ inline void plan_resize(const TableParams& p, int* s_wave) {
   int32_t *base = p.ws, *list = p.ws + p.rows + 1;
   int wanted = 0;
   for (int r0 = 0; r0 < p.rows; r0 += kPlan) {
@@ -239,21 +238,37 @@ __global__ __launch_bounds__(kPlan) void pages_resize_plan_kernel(TableParams p)
   const int found = find_free(p, min(wanted, p.num_blocks), s_wave, [&](int rank, int page) { list[rank] = page; });
   if (threadIdx.x == 0) base[p.rows] = found, *p.missing = wanted - found;
 }
-
-__global__ __launch_bounds__(256) void pages_resize_kernel(TableParams p) {
+// Entry j of row r.
+__device__ inline void resize_entry(const TableParams& p, int r, int j) {
   const int32_t *base = p.ws, *list = p.ws + p.rows + 1;
-  const int r = blockIdx.x, had = min(pages_of(p.lens[r], p.page), p.cols), has = min(pages_of(p.new_lens[r], p.page), p.cols);
-  const int found = base[p.rows], at = base[r];
-  for (int j = threadIdx.x; j < p.cols; j += 256) {
-    int b = p.table[r * p.stride + j];
-    if (j >= has && j < had && b >= 0 && b < p.num_blocks) atomicAdd(&p.out_refs[b], -1);
-    if (j >= has) b = -1;
-    if (j >= had && j < has) {
-      b = at + j - had < found ? list[at + j - had] : -1;
-      if (b >= 0) atomicAdd(&p.out_refs[b], 1);
-    }
-    p.out_table[r * p.out_stride + j] = b;
+  const int had = min(pages_of(p.lens[r], p.page), p.cols), has = min(pages_of(p.new_lens[r], p.page), p.cols);
+  int b = p.table[r * p.stride + j];
+  if (j >= has && j < had && b >= 0 && b < p.num_blocks) atomicAdd(&p.out_refs[b], -1);
+  if (j >= has) b = -1;
+  if (j >= had && j < has) {
+    const int rank = base[r] + j - had;
+    b = rank < base[p.rows] ? list[rank] : -1;
+    if (b >= 0) atomicAdd(&p.out_refs[b], 1);
   }
+  p.out_table[r * p.out_stride + j] = b;
+}
+
+__global__ __launch_bounds__(kPlan) void pages_resize_plan_kernel(TableParams p) {
+  __shared__ int s_wave[kPlan / 64];
+  if (blockIdx.x > 0) return copy_refs(p, blockIdx.x - 1, gridDim.x - 1);
+  plan_resize(p, s_wave);
+}
+__global__ __launch_bounds__(256) void pages_resize_kernel(TableParams p) {
+  for (int j = threadIdx.x; j < p.cols; j += 256) resize_entry(p, blockIdx.x, j);
+}
+// All of it by one workgroup.
+__global__ __launch_bounds__(kPlan) void pages_resize_small_kernel(TableParams p) {
+  __shared__ int s_wave[kPlan / 64];
+  if (p.out_refs != p.refs) copy_refs(p, 0, 1);
+  plan_resize(p, s_wave);
+  __threadfence();  // the copied counts are where the atomic additions are made, before any of them
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.rows * p.cols; i += kPlan) resize_entry(p, i / p.cols, i % p.cols);
 }
 
 struct KeepParams {
@@ -332,6 +347,7 @@ Views views_of(const vxa_cache_view* caches, int64_t first, int64_t count) {
 }
 
 constexpr int64_t kMostBlocks = 1 << 28;
+constexpr int64_t kSmallTable = 4096, kSmallPool = 16384;  // a resize that one workgroup does: 4 entries and 16 counts a thread
 
 // What fork and resize check of a table and its counts.
 int check_table(int64_t rows, int64_t cols, int64_t num_blocks, int64_t page) {
@@ -423,6 +439,11 @@ extern "C" int vxa_pages_resize(const int32_t* block_table, int64_t stride_bt, i
   p.out_table = out_table, p.out_stride = stride_ot, p.refs = ref_count, p.out_refs = out_ref_count;
   p.num_blocks = (int32_t)num_blocks, p.page = (int32_t)block_size, p.missing = missing, p.ws = reinterpret_cast<int32_t*>(ws);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (rows * cols <= kSmallTable && num_blocks <= kSmallPool) {
+    hipLaunchKernelGGL(pages_resize_small_kernel, dim3(1), dim3(kPlan), 0, st, p);
+    VXA_CHECK_LAUNCH();
+    return VXA_OK;
+  }
   hipLaunchKernelGGL(pages_resize_plan_kernel, dim3(plan_grid(p)), dim3(kPlan), 0, st, p);
   VXA_CHECK_LAUNCH();
   if (rows == 0) return VXA_OK;
