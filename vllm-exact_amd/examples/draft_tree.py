@@ -2,15 +2,14 @@
 
     python vllm-exact_amd/examples/draft_tree.py
 
-The four serving operators as a decoding loop uses them:
+The serving operators as a decoding loop uses them:
 
 * prompts of different lengths, packed, go through ``prompt_attention``; their keys and values through ``write_cache``;
 * each step drafts a tree for every request: its root is the token that the last step decided, below it hang guesses from
   the request's own text. The nodes' keys and values are written behind the context and ``tree_decode`` scores all nodes of
   all requests in one call;
 * the longest path that the model agrees with is kept. Its keys and values lie apart in the cache where a sibling was drafted
-  between them: ``read_cache`` reads the drafted range back and ``write_cache`` puts the kept rows side by side. Rows
-  read back quantise to the same 8-bit values.
+  between them: ``keep_drafted`` moves them side by side, in the caches of all layers at once.
 
 ``generate(..., guesses=0)`` drafts nothing but the root: plain decoding, the same tokens.
 """
@@ -21,7 +20,8 @@ from pathlib import Path
 import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
-from vllm_exact.int8_cache import make_cache, read_cache, write_cache  # noqa: E402
+from vllm_exact.int8_cache import make_cache, write_cache  # noqa: E402
+from vllm_exact.pages import keep_drafted  # noqa: E402
 from vllm_exact.prompt_attn import prompt_attention  # noqa: E402
 from vllm_exact.tree_attn import tree_decode  # noqa: E402
 
@@ -133,8 +133,7 @@ def generate(model, prompts, count, guesses=7):
                                key_scale=key_scale, value_scale=value_scale)
 
         best = model.forward(ints([t for tree in trees for t, _ in tree], torch.int64), pos, attend_tree).argmax(-1).tolist()
-        moves = []  # (request, packed row of a kept node, its place)
-        row = 0
+        keep, row = [], 0  # of each request, the kept nodes as bits
         for i, tree in enumerate(trees):
             kept = [0]
             while True:
@@ -144,15 +143,10 @@ def generate(model, prompts, count, guesses=7):
                 if child is None:
                     break
                 kept.append(child)
-            moves += [(i, row + node, ctx[i] + at) for at, node in enumerate(kept) if node != at]
+            keep.append(masks[row + kept[-1]])
             row += len(tree)
-        if moves:
-            rows = ints([m[1] for m in moves], torch.int64)
-            where = slots([(m[0], m[2]) for m in moves])
-            for cache in caches:
-                k, v = (torch.empty(sum(sizes), model.kv_heads, dim, device=dev) for _ in "kv")
-                read_cache(*cache, table, qsl, k, v, first=first)
-                write_cache(k[rows], v[rows], *cache, where)
+        views = [view for cache in caches for view in cache]
+        keep_drafted(views, table, lens, qsl, ints(keep, torch.int64), PAGE, torch.empty_like(lens))
     return [t[len(p):len(p) + count] for t, p in zip(texts, prompts)], steps
 
 
