@@ -179,23 +179,32 @@ __global__ __launch_bounds__(kThreads, 6) void beam_slice_kernel(BeamParams p) {
     if (__popcll(__ballot(mine >= (bar | 1u << b))) >= p.count) bar |= 1u << b;
   const float least = bar == 0 ? -3.402823466e38f : value_of(bar);
   again();
-  uint64_t mask = 0;  // this lane's values that are not below the bar
-  if (top >= least) {
+  // This lane's values that are not below the bar, the first in the top bit of each 32: a comparison, and its outcome added to
+  // twice the bits before. (Written as a condition it is three longer instructions: 8.4 us in place of 6.8 for 4 rows of 151936.)
+  uint32_t mask[kEach / 32];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i)
-      if (x(i) >= least) mask |= 1ull << i;
+  for (int i = 0; i < kEach; i += 32) {
+    mask[i / 32] = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      asm("v_cmp_ge_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc" : "+v"(mask[i / 32]) : "v"(x(i + j)), "v"(least) : "vcc");
   }
-  const int many = __popcll(mask);
+  int many = 0;
+#pragma unroll
+  for (int i = 0; i < kEach / 32; ++i) many += __popc(mask[i]);
   const int before = wave_scan(many, [](int a, int b) { return a + b; });
   const int all = __builtin_amdgcn_readlane(before, 63);
   if (all <= kWaveList) {
     int at = 0;
     if (lane == 0 && all) at = atomicAdd(&s_count, all);
     at = __builtin_amdgcn_readfirstlane(at) + before - many;
-    for (; mask; mask &= mask - 1) {  // a lane's only one is its maximum
-      const int place = place_of(__builtin_ctzll(mask));
-      s_list[at++] = key_of(order_of(many > 1 ? value<DTYPE>(logits[place]) : top), (uint32_t)place);
-    }
+#pragma unroll
+    for (int i = 0; i < kEach / 32; ++i)
+      for (uint32_t left = mask[i]; left != 0;) {  // a lane's only one is its maximum
+        const int first = __builtin_clz(left), place = place_of(32 * i + first);
+        left &= 0x7FFFFFFFu >> first;
+        s_list[at++] = key_of(order_of(many > 1 ? value<DTYPE>(logits[place]) : top), (uint32_t)place);
+      }
   } else {  // many values are near the bar: the wave's count-th largest value, then all above it and the first that equal it
     uint32_t order = 0;
 #pragma unroll 1
@@ -232,18 +241,21 @@ __global__ __launch_bounds__(kThreads, 6) void beam_slice_kernel(BeamParams p) {
   }
   __syncthreads();
 
-  // A candidate's rank is how many are larger.
+  // A candidate's rank is how many are larger; 2^share threads compare one.
   const int listed = s_count;
   u64* keys = p.keys + (int64_t)blockIdx.x * p.count;
-  for (int i = threadIdx.x; i < listed; i += kThreads) {
-    const u64 key = s_list[i];
+  int share = 0, valid = 0;
+  while (share < 3 && listed << (share + 1) <= kThreads) ++share;
+  for (int i0 = 0; i0 < listed; i0 += kThreads >> share) {
+    const int i = i0 + ((int)threadIdx.x >> share), part = threadIdx.x & ((1 << share) - 1);
+    const u64 key = i < listed ? s_list[i] : 0;
     int rank = 0;
-    for (int j = 0; j < listed; ++j) rank += s_list[j] > key;
-    if (key != 0 && rank < p.count) keys[rank] = key;
+    if (key != 0)
+      for (int j = part; j < listed; j += 1 << share) rank += s_list[j] > key;
+    for (int m = 1; m < 1 << share; m *= 2) rank += __builtin_amdgcn_ds_bpermute((lane ^ m) << 2, rank);
+    if (key != 0 && rank < p.count && part == 0) keys[rank] = key;
+    valid += __syncthreads_count(key != 0 && part == 0);
   }
-  int valid = 0;
-  for (int i = threadIdx.x; i < listed; i += kThreads) valid += s_list[i] != 0;
-  valid = __syncthreads_count(valid > 0) + __syncthreads_count(valid > 1);
   for (int i = valid + (int)threadIdx.x; i < p.count; i += kThreads) keys[i] = 0;
 }
 
