@@ -303,3 +303,59 @@ def test_refusals():
                        (dict(scale="x"), TypeError), (dict(write="x"), TypeError)):
         with pytest.raises(kind):
             linear_prompt(*dict(ok, **over).values())
+
+
+def test_many_sequences_and_starts_beyond_the_rows():
+    """More sequences than a wave has lanes, empty ones among them, long ones at both ends: each as it is alone."""
+    g = torch.Generator().manual_seed(18)
+    lens = [600, 0] + torch.randint(0, 40, (195,), generator=g).tolist() + [512, 0, 1025]
+    H, D = 2, 64
+    q, k, v, cu = inputs(lens, H, 1, D, torch.bfloat16, seed=19)
+    gd, n = decays(H), len(lens)
+    state, out = torch.zeros(n, H, D, D, device=DEV), torch.empty(len(q), H, D, device=DEV)
+    linear_prompt(q, k, v, cu, gd, 0.125, out, state, None, ints(range(n)))
+    for i in [0, 1, 2, 63, 64, 65, 130, n - 3, n - 2, n - 1]:
+        lo, hi = int(cu[i]), int(cu[i + 1])
+        alone, o = torch.ones(1, H, D, D, device=DEV), torch.empty(hi - lo, H, D, device=DEV)
+        linear_prompt(q[lo:hi], k[lo:hi], v[lo:hi], ints([0, hi - lo]), gd, 0.125, o, alone, None, ints([0]))
+        assert torch.equal(o, out[lo:hi]) and torch.equal(alone[0], state[i]), i
+    # a last start beyond the rows ends at them; starts that fall back make sequences of no rows
+    rows = len(q)
+    other = torch.full_like(out, 5.0)
+    linear_prompt(q, k, v, ints([-3, 700, rows + 1000]), gd, 0.125, other)
+    again = torch.full_like(out, 5.0)
+    linear_prompt(q, k, v, ints([0, 700, rows]), gd, 0.125, again)
+    assert torch.equal(other, again)
+    linear_prompt(q, k, v, ints([10, 20, 5, 5]), gd, 0.125, other.fill_(5.0))
+    assert (other[:10] == 5).all() and (other[20:] == 5).all() and torch.isfinite(other).all()
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rows_of_the_output_anywhere(out_dtype):
+    lens, H, D = (40, 70), 2, 128
+    q, k, v, cu = inputs(lens, H, 1, D, torch.bfloat16, seed=20)
+    g, state = decays(H), torch.zeros(2, H, D, D, device=DEV)
+    wide = torch.full((110, 3, D + 3), 2.0, device=DEV, dtype=out_dtype)
+    out = wide[:, :H, 1:D + 1]  # rows at odd elements
+    linear_prompt(q, k, v, cu, g, 0.25, out, state, None, ints([0, 1]))
+    want, _ = linear64(q, k, v, lens, g, 0.25)
+    row_bound, _ = bounds(q, k, v, lens, g, 0.25)
+    check(out, want, row_bound, out_dtype)
+    assert (wide[:, H:] == 2).all() and (wide[..., 0] == 2).all() and (wide[..., D + 1:] == 2).all()
+    n = len(q)
+    linear_step(q, k, v, g, 0.25, out, torch.zeros(1, H, D, D, device=DEV), None, None)
+    want, _ = linear64(q, k, v, (1,) * n, g, 0.25)
+    check(out, want, bounds(q, k, v, (1,) * n, g, 0.25)[0], out_dtype)
+
+
+def test_a_step_in_many_steps_keeps_its_bits_of_the_decay():
+    """4000 tokens with a window of 10000: the decay's own rounding (2^-25) would add up to 4000 of it."""
+    H, D, n = 1, 64, 4000
+    g = torch.full((H,), -1e-4, device=DEV)
+    state = torch.ones(1, H, D, D, device=DEV)
+    zero, out = torch.zeros(1, H, D, device=DEV, dtype=torch.bfloat16), torch.empty(1, H, D, device=DEV)
+    for _ in range(n):
+        linear_step(zero, zero, zero, g, 1.0, out, state, ints([0]), ints([0]))
+    want = torch.exp(g.double() * n)
+    # one rounding of 2^-24 a step, to the nearest: a walk of sqrt(4000) of half steps, with room for six of its deviations
+    assert (state.double() / want - 1).abs().max() < 6 * n ** 0.5 * 2.0 ** -24
