@@ -413,7 +413,10 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] *= grow[i];
     };
+    // Waves in products go before those that stage or wait: 75 to 72 us for 8192 rows, and 34 to 33 without outputs.
+    __builtin_amdgcn_s_setprio(3);
     if constexpr (OUT) from_state();
+    __builtin_amdgcn_s_setprio(0);
     v4u32 v[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) v[c] = transposed(now, sh.v, c, wave);
@@ -500,6 +503,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
       }
     }
     if (kLate && t0 + C < rows) fetch(t0 + C);
+    __builtin_amdgcn_s_setprio(3);
     // The state. Values are weighted and split into three parts, which keep the 24 bits of the products; the keys are exact.
     const float decay = count == C ? full : power(g, count);
 #pragma unroll
@@ -531,6 +535,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
         if (D == 256 && t % 2) __builtin_amdgcn_sched_barrier(0);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
   }
   float* to = nullptr;
   if (!OUT)
