@@ -4,6 +4,8 @@
 // for every row t of a sequence, S a D x D matrix of each head in fp32, g the head's log_decay. A sequence starts from a slot of
 // a pool of states (or zeros) and ends in one.
 
+#include <algorithm>
+
 #include "attention_common.h"
 
 namespace {
@@ -140,6 +142,19 @@ __device__ inline void split(const float (&x)[8], v4u32 (&part)[N]) {
     }
   }
 }
+// Eight fp32 values as three bf16 operands whose sum they are exactly: cut off after 8 bits, and again.
+__device__ inline void split_exactly(const float (&x)[8], v4u32 (&part)[3]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    float a = x[j], b = x[j + 1];
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+      part[n][j / 2] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+      if (n < 2) a -= __uint_as_float(ua & 0xFFFF0000u), b -= __uint_as_float(ub & 0xFFFF0000u);
+    }
+  }
+}
 template <typename T>
 __device__ inline void floats(v4u32 w, float (&x)[8]) {
 #pragma unroll
@@ -214,7 +229,7 @@ struct Shared {
   char qs[OUT && F16 ? 2 : 1][OUT && F16 ? kTile : 16];                // fp16: queries as two bf16 parts
   char kt[F16 ? 2 : 1][kTile], v[kTile];                               // for transposed reads; fp16: keys as two bf16 parts
   char scores[OUT ? (C == 64 ? 6 : 2) : 1][2][OUT ? 1024 : 16];        // operands of 16 keys and 32 queries, two parts
-  float power[C];                                                      // exp(g (C - 1 - x))
+  float power[C];                                                      // scale exp(g (C - 1 - x))
   float left[C];                                                       // exp(g (n - 1 - j)) of row j of the chunk, 0 past its end
 };
 
@@ -229,7 +244,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   constexpr int C = S::C, kRow = 2 * D;
   constexpr int DT = D / 32, IT = C / 32, CT = C / 16;  // blocks of the state's rows, of queries, of keys
   constexpr int kPieces = C / 16;                       // of a row tile, 16 bytes each, of a thread
-  constexpr bool kLate = OUT && D == 256;               // the next rows are asked for when little but the state is held
+  constexpr bool kLate = OUT;                           // the next rows are asked for when little but the state is held
   __shared__ __attribute__((aligned(1024))) S sh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -247,17 +262,17 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
 
   // Staging: this thread's 16-byte pieces are chunk `piece` of rows srow + 16 r.
   v4u32 gq[kPieces], gk[kPieces], gv[kPieces];
-  auto fetch = [&](int t0) {
-    const int id = again(threadIdx.x), srow = id / (D / 8), piece = id % (D / 8);
+  auto fetch = [&](int t0) {  // rows past the end repeat the last one
+    const int id = again((int)threadIdx.x), srow = id / (D / 8), piece = id % (D / 8);
+    auto piece_of = [&](const uint16_t* head_rows, int64_t stride, int r) {
+      const char* chunk = reinterpret_cast<const char*>(head_rows + (base + t0) * stride);
+      return *reinterpret_cast<const v4u32*>(chunk + 2u * (__umul24(min(srow + 16 * r, rows - 1 - t0), (uint32_t)stride) + 8u * piece));
+    };
 #pragma unroll
     for (int r = 0; r < kPieces; ++r) {
-      const int row = t0 + srow + 16 * r;
-      gq[r] = gk[r] = gv[r] = v4u32{0, 0, 0, 0};
-      if (row < rows) {
-        if (OUT) gq[r] = *reinterpret_cast<const v4u32*>(qh + (base + row) * p.sqt + 8 * piece);
-        gk[r] = *reinterpret_cast<const v4u32*>(kh + (base + row) * p.skt + 8 * piece);
-        gv[r] = *reinterpret_cast<const v4u32*>(vh + (base + row) * p.svt + 8 * piece);
-      }
+      if (OUT) gq[r] = piece_of(qh, p.sqt, r);
+      gk[r] = piece_of(kh, p.skt, r);
+      gv[r] = piece_of(vh, p.svt, r);
     }
   };
   // For the scores, queries and keys lie with the dims of each 16 in the order 0-3, 8-11, 4-7, 12-15: the order in which a lane holds
@@ -269,7 +284,12 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
     *reinterpret_cast<v2u32*>(at + 16 * ((c + 1) ^ key_swizzle<D>(row))) = v2u32{w.z, w.w};
   };
   auto stage = [&](int count) {
-    const int id = again(threadIdx.x), srow = id / (D / 8), piece = id % (D / 8);
+    const int id = again((int)threadIdx.x), srow = id / (D / 8), piece = id % (D / 8);
+    if (count < C) {
+#pragma unroll
+      for (int r = 0; r < kPieces; ++r)
+        if (srow + 16 * r >= count) gq[r] = gk[r] = gv[r] = v4u32{0, 0, 0, 0};
+    }
 #pragma unroll
     for (int r = 0; r < kPieces; ++r) {
       const int row = srow + 16 * r;
@@ -308,14 +328,17 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
 #pragma unroll
       for (int r = 0; r < 16; ++r) f(t, r, (int64_t)(32 * t + 8 * (r / 4) + r % 4) * D + corner);
   };
-  fetch(0);
+  if (rows > 0) fetch(0);
   const Slots slots = find_slots(p, part.seq);
   if (slots.bad) {
     if (OUT)
       for (int i = threadIdx.x; i < rows * D; i += 2 * D) store_f32_as(out, p.out_dtype, (base + i / D) * p.sot + head * p.soh + i % D, __builtin_nanf(""));
     return;
   }
-  if ((int)threadIdx.x < C) sh.power[threadIdx.x] = sh.left[threadIdx.x] = power(g, C - 1 - (int)threadIdx.x);
+  if ((int)threadIdx.x < C) {
+    const float w = power(g, C - 1 - (int)threadIdx.x);
+    sh.power[threadIdx.x] = w * p.scale, sh.left[threadIdx.x] = w;
+  }
   // A sequence of several parts that writes the slot that it reads keeps its first state apart: its last part may end before the first
   // begins.
   const bool apart = part.parts > 1 && slots.read == slots.write;
@@ -342,7 +365,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   };
   float grow[IT];
 #pragma unroll
-  for (int i = 0; i < IT; ++i) grow[i] = OUT ? power(g, 32 * i + col + 1) : 0.0f;
+  for (int i = 0; i < IT; ++i) grow[i] = OUT ? p.scale * power(g, 32 * i + col + 1) : 0.0f;
   const float full = power(g, C);
 
   for (int t0 = 0; t0 < rows; t0 += C) {
@@ -353,31 +376,23 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
     __syncthreads();
     const int now = again(lane);
     v16f o[IT];
-    if constexpr (OUT) {
-      // Scores in blocks of 16 keys 16 jt + 4 (lane / 16) + r and 16 queries 16 it + lane % 16, those that some query sees and the
-      // ones beside them that complete an operand.
-      constexpr int kBlocks = C == 64 ? 12 : 4;
+    // Scores in blocks of 16 keys 16 jt + 4 (lane / 16) + r and 16 queries 16 it + lane % 16, those that some query sees and the
+    // ones beside them that complete an operand: block b of 4 (or 12) of the waves in turn. Their products come first, what is made
+    // of them after those with the state, which hide that they wait.
+    constexpr int kBlocks = C == 64 ? 12 : 4, kEach = (kBlocks + DT - 1) / DT;  // kEach of a wave
+    const bool scoring = OUT && (kBlocks % DT == 0 || wave < kBlocks);
+    auto query_of = [](int b) { return 16 * (b < 4 ? b >> 1 : 2 + ((b - 4) >> 2)); };
+    auto key_of = [](int b) { return 16 * (b < 4 ? b & 1 : (b - 4) & 3); };
+    v4f sc[kEach];
+    if (scoring) {
 #pragma unroll
-      for (int n = 0; n < (kBlocks + DT - 1) / DT; ++n) {
-        const int b = wave + n * DT;
-        if (b < kBlocks) {
-          const int it = b < 4 ? b >> 1 : 2 + ((b - 4) >> 2), jt = b < 4 ? b & 1 : (b - 4) & 3, l16 = now & 15, l4 = now >> 4;
-          const int krow = 16 * jt + l16, qrow = 16 * it + l16, key = 16 * jt + 4 * l4;
-          v4f sc = {0, 0, 0, 0};
+      for (int n = 0; n < kEach; ++n) {
+        const int b = wave + n * DT, l16 = now & 15, l4 = now >> 4;
+        sc[n] = v4f{0, 0, 0, 0};
 #pragma unroll
-          for (int u = 0; u < D / 32; ++u)
-            sc = T::mfma16(*reinterpret_cast<const v4u32*>(sh.k + krow * kRow + 16 * ((4 * u + l4) ^ key_swizzle<D>(krow))),
-                           *reinterpret_cast<const v4u32*>(sh.q + qrow * kRow + 16 * ((4 * u + l4) ^ key_swizzle<D>(qrow))), sc);
-          float w[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r)  // a later key's score may be an infinity
-            w[r] = qrow >= key + r ? sc[r] * sh.power[min(C - 1 - qrow + key + r, C - 1)] : 0.0f;
-          const v2u32 hi = {BF16::pack(w[0], w[1]), BF16::pack(w[2], w[3])};
-          const v2f h0 = BF16::unpack(hi.x), h1 = BF16::unpack(hi.y);
-          const v2u32 lo = {BF16::pack(w[0] - h0.x, w[1] - h0.y), BF16::pack(w[2] - h1.x, w[3] - h1.y)};
-          const int at = (32 * (l4 & 1) + (qrow & 31)) * 16 + 8 * (l4 >> 1), operand = (it < 2 ? 0 : 2) + jt;
-          *reinterpret_cast<v2u32*>(sh.scores[operand][0] + at) = hi;
-          *reinterpret_cast<v2u32*>(sh.scores[operand][1] + at) = lo;
+        for (int u = 0; u < D / 32; ++u) {
+          const int at = l16 * kRow + 16 * ((4 * u + l4) ^ key_swizzle<D>(l16));
+          sc[n] = T::mfma16(*reinterpret_cast<const v4u32*>(sh.k + key_of(b) * kRow + at), *reinterpret_cast<const v4u32*>(sh.q + query_of(b) * kRow + at), sc[n]);
         }
       }
     }
@@ -417,6 +432,23 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
     __builtin_amdgcn_s_setprio(3);
     if constexpr (OUT) from_state();
     __builtin_amdgcn_s_setprio(0);
+    if (scoring) {
+#pragma unroll
+      for (int n = 0; n < kEach; ++n) {
+        const int b = wave + n * DT, l16 = now & 15, l4 = now >> 4, query = query_of(b) + l16, key = key_of(b) + 4 * l4;
+        float x[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = sh.power[min(C - 1 - query + key + r, C - 1)];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = query >= key + r ? sc[n][r] * x[r] : 0.0f;  // a later key's score may be an infinity
+        const v2u32 hi = {BF16::pack(x[0], x[1]), BF16::pack(x[2], x[3])};
+        const v2f h0 = BF16::unpack(hi.x), h1 = BF16::unpack(hi.y);
+        const v2u32 lo = {BF16::pack(x[0] - h0.x, x[1] - h0.y), BF16::pack(x[2] - h1.x, x[3] - h1.y)};
+        const int at = (32 * (l4 & 1) + (query & 31)) * 16 + 8 * (l4 >> 1), operand = (b < 4 ? 0 : 2) + key_of(b) / 16;
+        *reinterpret_cast<v2u32*>(sh.scores[operand][0] + at) = hi;
+        *reinterpret_cast<v2u32*>(sh.scores[operand][1] + at) = lo;
+      }
+    }
     v4u32 v[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) v[c] = transposed(now, sh.v, c, wave);
@@ -473,12 +505,12 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
             }
       }
       // Row 32 i + col, dims 32 wave + 8 a + 4 half + 0..3 for a = 0..3: with 16-bit outputs the halves exchange what the other stores.
+      const int there = again(lane);
+      char* const chunk = out + (p.out_dtype == VXA_F32 ? 4 : 2) * ((base + t0) * p.sot + head * p.soh + 32 * wave);
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        const int row = 32 * i + col;
-        const int64_t at = (base + t0 + row) * p.sot + head * p.soh + 32 * wave;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][r] *= p.scale;
+        const int row = 32 * i + (there & 31);
+        const uint32_t at = __umul24(row, (uint32_t)p.sot);
         if (p.out_wide) {
 #pragma unroll
           for (int a = 0; a < 4; a += 2) {
@@ -489,16 +521,11 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
               const auto x = __builtin_amdgcn_permlane32_swap(w[0][j], w[1][j], false, false);
               w[0][j] = x[0], w[1][j] = x[1];
             }
-            if (row < count) *reinterpret_cast<v4u32*>(reinterpret_cast<uint16_t*>(out) + at + 8 * a + 8 * half) = v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
+            if (row < count) *reinterpret_cast<v4u32*>(chunk + 2u * (at + 8 * a + 8 * (there >> 5))) = v4u32{w[0][0], w[0][1], w[1][0], w[1][1]};
           }
         } else if (row < count) {
-          if (p.out_dtype == VXA_F32) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) reinterpret_cast<float*>(out)[at + 8 * (r / 4) + 4 * half + r % 4] = o[i][r];
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) store_f32_as(out, p.out_dtype, at + 8 * (r / 4) + 4 * half + r % 4, o[i][r]);
-          }
+          for (int r = 0; r < 16; ++r) store_f32_as(chunk, p.out_dtype, at + 8 * (r / 4) + 4 * (there >> 5) + r % 4, o[i][r]);
         }
       }
     }
@@ -521,7 +548,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
         for (int e = 0; e < 4; ++e) f[j + e] *= w[e];
       }
       v4u32 three[3];
-      split(f, three);
+      split_exactly(f, three);
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
         const v4u32 k = transposed(now, sh.kt[0], c, t);
@@ -598,6 +625,7 @@ int linear_params(LinearParams& p, const void* q, int64_t sqt, int64_t sqh, cons
   if (H > (1 << 16) || tokens > (1 << 30) || n > (1 << 30) || slots > (1 << 30)) return VXA_ERR_UNSUPPORTED;
   if (n == 0) return VXA_OK;
   if (!log_decay || (tokens && (!q || !k || !v || !out))) return VXA_ERR_ARG;
+  if (std::max({sqt, skt, svt, sot}) >= 1 << 23 || std::min({sqt, skt, svt, sot}) < 0) return VXA_ERR_UNSUPPORTED;  // 64 rows' bytes are a 32-bit number
   // Rows are read in 16-byte pieces.
   if ((uintptr_t)q % 16 || (uintptr_t)k % 16 || (uintptr_t)v % 16 || sqt % 8 || sqh % 8 || skt % 8 || skh % 8 || svt % 8 || svh % 8 ||
       (uintptr_t)state % 16 || sss % 4 || ssh % 4)
