@@ -133,6 +133,14 @@ def test_beam_statement():
     assert beam_select_torch(logits[2:3], scores[2:3], 1, 2)[1].tolist() == [[-1, -1]]
 
 
+@pytest.mark.parametrize("score", [float("nan"), float("inf")])
+def test_beam_statement_of_a_score_without_tokens(score):
+    logits = torch.full((2, 5), -torch.inf)
+    logits[0] = 1.0
+    best, parents, tokens = beam_select_torch(logits, torch.tensor([0.0, score]), 2, 3)
+    assert best.isnan().all() and parents.eq(-1).all() and tokens.eq(-1).all()
+
+
 def test_page_statements():
     ints = lambda x: torch.tensor(x, dtype=torch.int32)
     cache = torch.arange(8.0).view(8, 1, 1).repeat(1, 4, 1)

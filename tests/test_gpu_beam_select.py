@@ -97,6 +97,14 @@ def test_nan_and_infinities_make_their_request_nan(where):
     assert torch.isfinite(best[0]).all() and torch.isfinite(best[2]).all()
 
 
+@pytest.mark.parametrize("score", [float("nan"), float("inf")])
+def test_scores_count_where_a_beam_has_no_token(score):
+    logits, scores = inputs(2, 2, 300, torch.float32, 7)
+    logits[3], scores[3] = -torch.inf, score
+    best, parents, tokens = check(logits, scores, 2, 4)
+    assert torch.isnan(best[1]).all() and parents[1].eq(-1).all() and tokens[1].eq(-1).all() and torch.isfinite(best[0]).all()
+
+
 @pytest.mark.parametrize("scale", [1e-3, 30.0, 1e4, 1e30])
 def test_magnitudes(scale):
     logits, scores = inputs(2, 3, 10000, torch.float32, 6)

@@ -290,11 +290,12 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamParams p) {
     double s = 0.0;
     for (int i = lane; i < parts; i += 64) s += tops[i] == kNegInf ? sums[i] : sums[i] * exp((double)tops[i] - (double)m);
     s = wave_sum(s);
-    const double score = s == 0.0 ? -__builtin_huge_val() : (double)p.scores[row0 + b];  // no token, or a beam that has ended
+    const float given = p.scores[row0 + b];
+    const double score = s == 0.0 ? -__builtin_huge_val() : (double)given;  // no token, or a beam that has ended
     const double l = log(s);
     if (lane == 0) {
       s_top[b] = m, s_log[b] = l, s_score[b] = score;
-      if (score != -__builtin_huge_val() && !(score - l - (double)m < __builtin_huge_val() && l == l)) s_nan = 1;
+      if (!(given < __builtin_huge_valf()) || (score != -__builtin_huge_val() && !(score - l - (double)m < __builtin_huge_val() && l == l))) s_nan = 1;
     }
   }
   __syncthreads();

@@ -32,7 +32,7 @@ def beam_select_torch(logits, scores, beams, count):
     top = x.amax(dim=1, keepdim=True)
     total = scores.double()[:, None] + ((x - top) - (x - top).exp().sum(dim=1, keepdim=True).log())
     total = torch.where(live[:, None] & (x != -torch.inf), total, -torch.inf)
-    bad = ((total != total) | (total == torch.inf)).any(dim=1) | (live & (scores != scores))
+    bad = ((total != total) | (total == torch.inf)).any(dim=1) | ~(scores < torch.inf)
     best, at = total.view(-1, beams * V).sort(dim=1, descending=True, stable=True)
     best, at = best[:, :count], at[:, :count]
     if best.shape[1] < count:
