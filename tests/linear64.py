@@ -23,9 +23,14 @@ def linear64(q, k, v, lens, log_decay, scale, starts=None):
 def bounds(q, k, v, lens, log_decay, scale, starts=None):
     """How far fp32 kernels may be off: (rows, states). Every sum is of fp32 terms, one rounding of 2^-24 of the magnitudes for
     each of the D dims and the rows before, and one for each decay (2^-24 of its exponent, which is at most the rows times |g| where
-    the decay is not nothing); where operands of the matrix cores are split into two bf16 parts, 2^-18 is left of each of two, and 2^-27 of
-    three."""
+    the decay is not nothing).
+
+    Operands of the matrix cores are two bf16 parts: the first is off by at most 2^-8 where the value is in [1, 2), so the second, below
+    2^-8, by at most 2^-17. Every term of a row's sum meets one such operand, the state's or the score's: 2^-17. The other one of
+    fp16 rows is two parts as well, exactly (11 bits), but the product of both second parts is left out: 2^-8 of 2^-8 more. A state's
+    terms are exact parts; of fp16 keys the second part (2^-8) times the third of the value (below 2^-14) is left out, 2^-22."""
     out, ends = linear64(q.abs(), k.abs(), v.abs(), lens, log_decay, abs(scale), None if starts is None else starts.abs())
     n, d = max(lens) if lens else 0, q.shape[2]
     steps = (n + d + 64 + min(n * float(log_decay.abs().nan_to_num(posinf=0).max()), 90)) * 2.0 ** -24
-    return out * (2 * 2.0 ** -18 + steps), ends * (2.0 ** -26 + steps)
+    half = q.dtype == torch.float16
+    return out * (2.0 ** -17 + half * 2.0 ** -16 + steps), ends * (half * 2.0 ** -22 + steps)

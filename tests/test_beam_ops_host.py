@@ -42,6 +42,16 @@ def test_linear_attention_refusals():
     assert prompt(tokens=-1) == nx.VXA_ERR_ARG and prompt(cu=None) == nx.VXA_ERR_ARG and prompt(tokens=1 << 40) == nx.VXA_ERR_UNSUPPORTED
 
 
+def test_linear_attention_rows_too_far_apart():
+    rows = dict(q=FAKE, sqt=1024, sqh=128, k=FAKE, skt=256, skh=128, v=FAKE, svt=256, svh=128, dtype=BF)
+    rest = dict(g=FAKE, scale=0.1, out=FAKE, od=BF, sot=1024, soh=128, state=FAKE, slots=4, sss=8 * 128 * 128, ssh=128 * 128, read=FAKE, write=FAKE,
+                H=8, KV=2, D=128)
+    for call in (calls("vxa_linear_prompt", dict(rows, cu=FAKE, n=2, tokens=100, **rest, ws=FAKE, wsb=1 << 40, st=None)),
+                 calls("vxa_linear_step", dict(rows, n=2, **rest, st=None))):
+        for name in ("sqt", "skt", "svt", "sot"):
+            assert call(**{name: 1 << 23}) == nx.VXA_ERR_UNSUPPORTED and call(**{name: -8}) == nx.VXA_ERR_UNSUPPORTED, name
+
+
 def test_beam_select_refusals():
     call = calls("vxa_beam_select", dict(x=FAKE, stride=1000, dtype=BF, scores=FAKE, n=2, beams=4, vocab=1000, count=8, a=FAKE, b=FAKE, c=FAKE, ws=FAKE,
                                          wsb=1 << 30, st=None))

@@ -154,3 +154,21 @@ def test_refusals():
         beam_select(logits, scores, 2, *outs(2, 65))
     empty = logits[:0], scores[:0]
     assert beam_select(*empty, 2, *outs(0))[0].shape == (0, 4)
+
+
+def test_rows_far_apart():
+    """Rows past 2^31 elements from each other."""
+    logits, scores = inputs(1, 4, 9001, torch.bfloat16, 8)
+    stride = (1 << 30) + 1
+    far = torch.empty(3 * stride + 9001, device=DEV, dtype=torch.bfloat16).as_strided(logits.shape, (stride, 1)).copy_(logits)
+    a, b = select(far, scores, 4, 8), select(logits, scores, 4, 8)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_scores_updated_in_place():
+    """As many continuations as beams: the next step's scores may be written over this one's."""
+    logits, scores = inputs(5, 4, 1000, torch.float16, 9)
+    want = select(logits, scores, 4, 4)
+    parents, tokens = torch.empty(5, 4, device=DEV, dtype=torch.int32), torch.empty(5, 4, device=DEV, dtype=torch.int64)
+    beam_select(logits, scores, 4, scores.view(5, 4), parents, tokens)
+    assert torch.equal(scores.view(5, 4), want[0]) and torch.equal(parents, want[1]) and torch.equal(tokens, want[2])

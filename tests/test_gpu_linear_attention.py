@@ -359,3 +359,64 @@ def test_a_step_in_many_steps_keeps_its_bits_of_the_decay():
     want = torch.exp(g.double() * n)
     # one rounding of 2^-24 a step, to the nearest: a walk of sqrt(4000) of half steps, with room for six of its deviations
     assert (state.double() / want - 1).abs().max() < 6 * n ** 0.5 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("step", [False, True])
+def test_rows_and_states_far_apart(step):
+    """Rows of the longest stride there is, past 2^31 elements and 2^32 bytes; two states as far from each other."""
+    n, H, D, stride = 300, 2, 64, (1 << 23) - 8
+    q, k, v, cu = inputs((n,), H, 1, D, torch.bfloat16, seed=21)
+    g = decays(H)
+
+    def far(x):
+        y = torch.empty(stride * (n - 1) + x.shape[1] * D, device=DEV, dtype=x.dtype).as_strided(x.shape, (stride, D, 1))
+        return y.copy_(x)
+
+    fq, fk, fv, out = far(q), far(k), far(v), far(q)
+    pool = torch.empty((1 << 31) + 16 + H * D * D, device=DEV).as_strided((2, H, D, D), ((1 << 31) + 16, D * D, D, 1))
+    starts = torch.randn(n if step else 1, H, D, D, generator=torch.Generator().manual_seed(22)).to(DEV)
+    lens = (1,) * n if step else (n,)
+    if step:
+        pool[0], pool[1] = starts[0], 3.0
+        starts[:] = starts[0].clone()
+        read, write = ints([0] * n), ints([-1] * (n - 1) + [1])
+        linear_step(fq, fk, fv, g, 0.5, out, pool, read, write)
+    else:
+        pool[0], pool[1] = 3.0, starts[0]
+        linear_prompt(fq, fk, fv, cu, g, 0.5, out, pool, ints([1]), ints([1]))
+    want, ends = linear64(q, k, v, lens, g, 0.5, starts)
+    row_bound, state_bound = bounds(q, k, v, lens, g, 0.5, starts)
+    check(out, want, row_bound, torch.bfloat16)
+    check(pool[1], ends[-1], state_bound[-1])
+    assert torch.equal(pool[0], starts[0]) if step else (pool[0] == 3).all()
+
+
+def test_two_calls_at_once():
+    calls = []
+    for seed in (23, 24):
+        q, k, v, cu = inputs((3000, 40, 700), 4, 2, 128, torch.bfloat16, seed=seed)
+        calls.append((q, k, v, cu, decays(4), 0.1))
+    want = []
+    for c in calls:
+        state = torch.zeros(3, 4, 128, 128, device=DEV)
+        want.append((linear_prompt(*c, torch.empty_like(c[0]), state, None, ints([0, 1, 2])), state))
+    got = [(torch.empty_like(c[0]), torch.zeros(3, 4, 128, 128, device=DEV), ints([0, 1, 2])) for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, (out, state, slots), stream in zip(calls, got, streams):
+            with torch.cuda.stream(stream):
+                linear_prompt(*c, out, state, None, slots)
+    torch.cuda.synchronize()
+    for (out, state, _), (a, b) in zip(got, want):
+        assert torch.equal(out, a) and torch.equal(state, b)
+
+
+def test_outputs_over_the_inputs_are_refused():
+    q, k, v, cu = inputs((5,), 2, 2, 64, torch.bfloat16)
+    pool, slots = torch.zeros(5, 2, 64, 64, device=DEV), torch.arange(5, dtype=torch.int32, device=DEV)
+    for out in (q, k, v):
+        with pytest.raises(ValueError, match="out must not be"):
+            linear_prompt(q, k, v, cu, decays(2), 0.1, out)
+        with pytest.raises(ValueError, match="out must not be"):
+            linear_step(q, k, v, decays(2), 0.1, out, pool, slots, slots)

@@ -308,3 +308,21 @@ def test_refusals():
     big = torch.empty(8193, 1, dtype=torch.int32, device=DEV)
     with pytest.raises(NotImplementedError):
         resize_pages(big, big[:, 0].contiguous(), big[:, 0].contiguous(), refs, 16)
+
+
+def test_pages_far_apart():
+    """Pages past 2^32 bytes from each other: copied, forked and compacted."""
+    page, KV, D, stride = 4, 2, 64, (1 << 31) + 64
+    far = torch.empty(3 * stride + page * KV * D, device=DEV, dtype=torch.int8).as_strided((4, page, KV, D), (stride, KV * D, D, 1))
+    fill(far, torch.Generator().manual_seed(11))
+    copy_pages([far], page, ints([0]), ints([3]))
+    assert torch.equal(far[3], far[0])
+    table, lens, refs = ints([[3, 0]]), ints([6]), ints([1, 0, 0, 1])
+    out, out_lens, missing = fork([far], table, lens, ints([0, 0]), refs, page)  # the second row's end is copied to page 1
+    assert out.tolist() == [[3, 0], [3, 1]] and out_lens.tolist() == [6, 6] and int(missing) == 0 and torch.equal(far[1], far[0])
+    assert refs.tolist() == [1, 1, 0, 2]
+    fill(far, torch.Generator().manual_seed(12))
+    said = far.contiguous()
+    kept = keep_drafted_torch([said], out[:1], lens[:1], ints([0, 5]), ints([0b11000], torch.int64), page)
+    got = keep_drafted([far], out[:1], lens[:1], ints([0, 5]), ints([0b11000], torch.int64), page, torch.empty_like(lens))
+    assert torch.equal(got, kept) and torch.equal(far, said)

@@ -55,8 +55,9 @@ __device__ inline Slots find_slots(const LinearParams& p, int seq) {
 // ---------------------------------------------------------------------------------- single tokens
 constexpr int kCols = 32;  // columns of a state that a workgroup takes
 
-// A workgroup takes 32 columns of one head's state of one sequence: 128 bytes of each row, D / 8 rows a thread. It reads and writes
-// every value of the state once, and that is what bounds it.
+// A workgroup takes 32 columns of one head's state of one sequence: 128 bytes of each row, D / 8 rows a thread, so that a thread has
+// all its loads in flight at once and 64 sequences make 8192 workgroups. It reads and writes every value of the state once, and that is what
+// bounds it: 64 sequences, 32 heads of 128, 41 us, 6.6 TB/s. One sequence of 8 heads: 3.4 us, a launch and two dependent loads.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void linear_step_kernel(LinearParams p) {
   constexpr int kRows = D / 8;  // of the state, of a thread
@@ -121,28 +122,35 @@ hipError_t launch_step(int64_t D, const LinearParams& p, hipStream_t st) {
 // Rows go in chunks: with S the state before a chunk of n rows and i, j the rows in it,
 //   o_i = scale (exp(g (i + 1)) q_i S + sum_{j <= i} exp(g (i - j)) (q_i . k_j) v_j)
 //   S'  = exp(g n) S + sum_j k_j (exp(g (n - 1 - j)) v_j)^T
-constexpr int kPart = 512;  // rows of a part: long sequences are cut into parts whose states are computed first
+// All of it runs on the matrix cores, with sums in fp32. What is not 16 bits wide already goes there as several bf16 numbers:
+//   S in q S, and the weighted scores: two, off by at most 2^-17 of each term; an output of 16 bits is rounded to 2^-8 or 2^-11 afterwards.
+//   The weighted values, whose products add up to the state that later tokens start from: three, whose sum is the fp32 number itself.
+//   fp16 queries, keys and values beside them: two, exactly. Products of two second parts are left out (2^-16 of a term, in S 2^-22).
+// The weights are powers of a whole number of rows, at most 1, never quotients of two powers, which would overflow.
+//
+// A sequence is walked in order, so 32 heads of one prompt of 8192 rows would be 32 workgroups. It is cut into parts of 512 rows:
+// one launch computes what each part adds to the state (half the work of outputs, 32 us for 8192 rows of 32 heads of 128), one adds
+// these up (10.5 us, and only where a sequence may have three parts), one computes the outputs (68 us). A token at
+// a time, one after the other, the same call takes 4128 us. Where the cuts are goes by the sequence alone, and so do a row's bits.
+//
+// What bounds it: 17.2 GF are 15 us at the rate of a large product, 170 MB 35 us at that of a copy. A SIMD's matrix and vector instructions
+// do not overlap here (two waves a SIMD, which is what their registers allow): per chunk of 64 rows a wave has 98 products of 32
+// clocks and some 1000 vector instructions that split, weight and stage, of 13,200 clocks that two of them take together.
+constexpr int kPart = 512;
 
 __device__ inline float power(float g, int e) { return e == 0 ? 1.0f : expf(g * (float)e); }  // exp(-inf * 0) is 1 here
 
-// Eight fp32 values as bf16 operands whose sum they are, N parts: off by 2^-9 of a value for one part, 2^-18 for two, 2^-27 for three.
-template <int N>
-__device__ inline void split(const float (&x)[8], v4u32 (&part)[N]) {
+// Eight fp32 values as two bf16 operands, off by at most 2^-17 of a value; 16 significant bits are exact.
+__device__ inline void split(const float (&x)[8], v4u32 (&part)[2]) {
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
-    float a = x[j], b = x[j + 1];
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const uint32_t w = BF16::pack(a, b);
-      part[n][j / 2] = w;
-      if (n + 1 < N) {
-        const v2f f = BF16::unpack(w);
-        a -= f.x, b -= f.y;
-      }
-    }
+    part[0][j / 2] = BF16::pack(x[j], x[j + 1]);
+    const v2f f = BF16::unpack(part[0][j / 2]);
+    part[1][j / 2] = BF16::pack(x[j] - f.x, x[j + 1] - f.y);
   }
 }
-// Eight fp32 values as three bf16 operands whose sum they are exactly: cut off after 8 bits, and again.
+// Eight fp32 values as three bf16 operands whose sum they are exactly: cut off after 8 bits, and again. (Cutting takes one instruction
+// for two values where rounding takes two or three; with two operands its error would be four times as large.)
 __device__ inline void split_exactly(const float (&x)[8], v4u32 (&part)[3]) {
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
@@ -223,7 +231,9 @@ __device__ inline int64_t kept_at(const LinearParams& p, int lo, int part, int h
 template <typename T, int D, bool OUT>
 struct Shared {
   static constexpr bool F16 = std::is_same_v<T, FP16>;
-  static constexpr int C = !F16 && D <= 128 ? 64 : 32;  // rows of a chunk
+  // Rows of a chunk: 64 (the state is split and decayed half as often as with 32: 120 us in place of 132 for 8192 rows), where two workgroups'
+  // tiles fit a CU's LDS; 32 in fp16, whose queries and keys lie there twice, and at 256 dims.
+  static constexpr int C = !F16 && D <= 128 ? 64 : 32;
   static constexpr int kTile = C * 2 * D;
   char q[OUT ? kTile : 16], k[OUT ? kTile : 16];                       // for the scores
   char qs[OUT && F16 ? 2 : 1][OUT && F16 ? kTile : 16];                // fp16: queries as two bf16 parts
@@ -234,7 +244,8 @@ struct Shared {
 };
 
 // A workgroup of D / 32 waves takes one head of a part. A wave keeps 32 columns of the state in the accumulators of 32 x 32 x 16
-// MFMAs, where they are the operand of the next product as they lie.
+// MFMAs, where they are the operand of the next product as they lie. (Twice as many waves of 16 columns, four a SIMD: 80 us in place of 77
+// for the outputs of 8192 rows, since each of them splits, weights and waits as often.)
 // OUT: the rows' outputs from the state that the part starts from, and the sequence's end state. Else: the state that a
 // part leaves, for all parts but a sequence's last; the first starts from the sequence's state, the others from zeros.
 template <typename T, int D, bool OUT>
@@ -244,7 +255,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   constexpr int C = S::C, kRow = 2 * D;
   constexpr int DT = D / 32, IT = C / 32, CT = C / 16;  // blocks of the state's rows, of queries, of keys
   constexpr int kPieces = C / 16;                       // of a row tile, 16 bytes each, of a thread
-  constexpr bool kLate = OUT;                           // the next rows are asked for when little but the state is held
+  constexpr bool kLate = OUT;                           // the next rows are asked for when little but the state is held in registers
   __shared__ __attribute__((aligned(1024))) S sh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;

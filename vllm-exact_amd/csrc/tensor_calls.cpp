@@ -258,6 +258,8 @@ void check_linear(const char* what, const Linear& x, int64_t n, const at::Tensor
     refuse(what, ": inconsistent shapes");
   for (const at::Tensor* t : {&x.q, &x.k, &x.v, &x.out})
     if (t->size(2) && t->stride(2) != 1) refuse(what, ": the head dimension must be contiguous");
+  for (const at::Tensor* t : {&x.q, &x.k, &x.v})  // workgroups read rows whose outputs others have written
+    if (x.out.numel() && t->data_ptr() == x.out.data_ptr()) refuse(what, ": out must not be query, key or value");
   const int64_t H = x.q.size(1), D = x.q.size(2);
   if (!vector_of(x.decay, at::kFloat, H)) refuse(what, ": log_decay must be a contiguous fp32 vector, one number for each head");
   if ((x.read || x.write) && !x.state) refuse(what, ": slots need a pool of states");
