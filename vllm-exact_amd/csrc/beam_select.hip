@@ -9,6 +9,12 @@
 // count-th largest of a wave's 64 lane maxima, a handful more than `count`. A second kernel, a workgroup for each request,
 // joins the slices' sums and picks from their candidates in the same way.
 // A slice's place goes by the vocabulary alone, so a row's sums are the same bits in any batch and at any alignment.
+//
+// What bounds it: 256 rows of 248320 bf16 logits are 127 MB, 26 us at the rate of a large copy (19 at that of plain reads); the slices take
+// 42 us (3.0 TB/s) and the join 8. About 180 vector instructions for each eight logits' worth of words (a conversion, a
+// difference, an exponential, a sum, a maximum and a comparison of each) are 12 us where nothing else runs, the loads alone
+// 30, and a workgroup has one slice: while it computes only the other workgroups' loads are in flight. (Workgroups that stay and ask for
+// their next slice first need its registers as well, which costs as many waves: 58 us.) 4 rows of 151936: 6.6 + 5.2, two launches' latency.
 
 #include "attention_common.h"
 
@@ -67,13 +73,11 @@ __device__ inline double wave_sum(double x) {
   return x;
 }
 
-// exp(d) for -80 <= d <= 0, off by a few 2^-25: of the product with log2(e), the whole part goes to the exponent and the rest
-// keeps its bits.
+// exp(d) for -80 <= d <= 0, off by a few 2^-25 where |d| is not much above 10, as it is for what carries a sum of 2^17 terms: the power
+// of 2 of the rounded product with log2(e), and what the rounding left, d less the product times log(2), as a factor of 1 more than it.
 __device__ inline float exp_of(float d) {
-  constexpr float kLog2e = 1.44269504f, kRest = 1.92596303e-8f;  // their sum: log2(e) to 48 bits
-  constexpr float kMagic = 12582912.0f;                          // 1.5 2^23: added, it rounds to a whole number in the lowest bits
-  const float m = fmaf(d, kLog2e, kMagic), whole = m - kMagic;
-  return __uint_as_float(__float_as_uint(exp2_hw(fmaf(d, kRest, fmaf(d, kLog2e, -whole)))) + (__float_as_uint(m) << 23));
+  const float p = d * 1.44269504f, e = exp2_hw(p);
+  return fmaf(e, fmaf(p, -0.693147182f, d), e);
 }
 
 // Element of a row of logits, which may start at any element.
@@ -149,9 +153,14 @@ __global__ __launch_bounds__(kThreads, 6) void beam_slice_kernel(BeamParams p) {
     }
   }
 
-  float top = x(0);
+  float runs[kEach / 8], top = kNegInf;  // the largest values; a NaN where there is one
 #pragma unroll
-  for (int i = 1; i < kEach; ++i) top = __builtin_elementwise_maximum(top, x(i));  // a NaN where there is one
+  for (int r = 0; r < kEach / 8; ++r) {
+    runs[r] = x(8 * r);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) runs[r] = __builtin_elementwise_maximum(runs[r], x(8 * r + j));
+    top = __builtin_elementwise_maximum(top, runs[r]);
+  }
   if (top != top) top = __builtin_nanf("");
   const uint32_t mine = order_of(top);
   const uint32_t highest = (uint32_t)(wave_max((u64)mine << 32) >> 32);
@@ -178,33 +187,39 @@ __global__ __launch_bounds__(kThreads, 6) void beam_slice_kernel(BeamParams p) {
   for (int b = 31; b >= (DTYPE == VXA_F32 ? 0 : DTYPE == VXA_BF16 ? 16 : 13); --b)
     if (__popcll(__ballot(mine >= (bar | 1u << b))) >= p.count) bar |= 1u << b;
   const float least = bar == 0 ? -3.402823466e38f : value_of(bar);
-  again();
-  // This lane's values that are not below the bar, the first in the top bit of each 32: a comparison, and its outcome added to
-  // twice the bits before. (Written as a condition it is three longer instructions: 8.4 us in place of 6.8 for 4 rows of 151936.)
-  uint32_t mask[kEach / 32];
+  // This lane's values that are not below the bar, one bit each. Few runs have one: those are read again.
+  u64 mask = 0;
+  uint32_t near = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; i += 32) {
-    mask[i / 32] = 0;
+  for (int r = 0; r < kEach / 8; ++r) near |= runs[r] >= least ? 1u << r : 0u;
+  for (; near != 0; near &= near - 1) {
+    const int r = __builtin_ctz(near), place = place_of(8 * r);
+    Element<DTYPE> e[8];
+    int skip = 0;
+    if (whole || p.vocab >= 8) {
+      skip = max(place - (p.vocab - 8), 0);
+      __builtin_memcpy(e, logits + (place - skip), sizeof(e));
+    } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      asm("v_cmp_ge_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc" : "+v"(mask[i / 32]) : "v"(x(i + j)), "v"(least) : "vcc");
+      for (int j = 0; j < 8; ++j) e[j] = logits[min(j, p.vocab - 1)];
+    }
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits |= value<DTYPE>(e[j]) >= least ? 1u << j : 0u;
+    if (p.vocab < 8) bits &= (1u << p.vocab) - 1;
+    mask |= (u64)(bits >> skip) << (8 * r);
   }
-  int many = 0;
-#pragma unroll
-  for (int i = 0; i < kEach / 32; ++i) many += __popc(mask[i]);
+  const int many = __popcll(mask);
   const int before = wave_scan(many, [](int a, int b) { return a + b; });
   const int all = __builtin_amdgcn_readlane(before, 63);
   if (all <= kWaveList) {
     int at = 0;
     if (lane == 0 && all) at = atomicAdd(&s_count, all);
     at = __builtin_amdgcn_readfirstlane(at) + before - many;
-#pragma unroll
-    for (int i = 0; i < kEach / 32; ++i)
-      for (uint32_t left = mask[i]; left != 0;) {  // a lane's only one is its maximum
-        const int first = __builtin_clz(left), place = place_of(32 * i + first);
-        left &= 0x7FFFFFFFu >> first;
-        s_list[at++] = key_of(order_of(many > 1 ? value<DTYPE>(logits[place]) : top), (uint32_t)place);
-      }
+    for (; mask != 0; mask &= mask - 1) {  // a lane's only one is its maximum
+      const int place = place_of(__builtin_ctzll(mask));
+      s_list[at++] = key_of(order_of(many > 1 ? value<DTYPE>(logits[place]) : top), (uint32_t)place);
+    }
   } else {  // many values are near the bar: the wave's count-th largest value, then all above it and the first that equal it
     uint32_t order = 0;
 #pragma unroll 1
