@@ -326,3 +326,27 @@ def test_pages_far_apart():
     kept = keep_drafted_torch([said], out[:1], lens[:1], ints([0, 5]), ints([0b11000], torch.int64), page)
     got = keep_drafted([far], out[:1], lens[:1], ints([0, 5]), ints([0b11000], torch.int64), page, torch.empty_like(lens))
     assert torch.equal(got, kept) and torch.equal(far, said)
+
+
+@pytest.mark.parametrize("blocks", [1023, 1024, 1025, 4096, 4097, 8191, 16500])
+@pytest.mark.parametrize("rows", [1, 20, 33])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_resize_by_one_workgroup_or_several(blocks, rows, in_place):
+    """Both sides of the sizes at which a resize is one launch, with free pages in between and fewer than are wanted."""
+    page, cols = 4, 50
+    g = torch.Generator().manual_seed(blocks + rows)
+    lens = torch.randint(0, cols * page // 2, (rows,), generator=g).tolist()
+    table, refs = rows_of(lens, page, cols, blocks, g)
+    refs += (torch.rand(blocks, generator=g) < 0.7).to(torch.int32).to(DEV)  # others hold them
+    new = torch.randint(0, cols * page + 1, (rows,), generator=g)
+    lens, new = ints(lens), new.to(torch.int32).to(DEV)
+    want = resize_pages_torch(table.cpu(), lens.cpu(), new.cpu(), refs.cpu(), page)
+    if in_place:
+        missing = resize_pages(table, lens, new, refs, page)
+        out, counts = table, refs
+    else:
+        out, counts = torch.full_like(table, 5), torch.full_like(refs, 5)
+        before = table.clone(), refs.clone()
+        missing = resize_pages(table, lens, new, refs, page, out, counts)
+        assert torch.equal(table, before[0]) and torch.equal(refs, before[1])
+    assert torch.equal(out.cpu(), want[0]) and torch.equal(counts.cpu(), want[1]) and int(missing) == want[2]

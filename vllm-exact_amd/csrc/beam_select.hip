@@ -11,17 +11,18 @@
 // A slice's place goes by the vocabulary alone, so a row's sums are the same bits in any batch and at any alignment.
 //
 // What bounds it: 256 rows of 248320 bf16 logits are 127 MB, 26 us at the rate of a large copy (19 at that of plain reads); the slices take
-// 42 us (3.0 TB/s) and the join 8. About 180 vector instructions for each eight logits' worth of words (a conversion, a
-// difference, an exponential, a sum, a maximum and a comparison of each) are 12 us where nothing else runs, the loads alone
-// 30, and a workgroup has one slice: while it computes only the other workgroups' loads are in flight. (Workgroups that stay and ask for
-// their next slice first need its registers as well, which costs as many waves: 58 us.) 4 rows of 151936: 6.6 + 5.2, two launches' latency.
+// 40.6 us and the join 8.3. Vector instructions are in flight for 76 % of the slices' cycles: 19 a logit, of which 10 take a logit apart
+// twice and add its exponential (one of them at a quarter of the rate), the others find the bar, look through the runs near it and
+// rank the candidates, work that a slice has whatever its size (half as many logits a thread: 48.9 us, the join 13.5). Loads alone are 30:
+// a workgroup has one slice, and while it computes only the others' loads are in flight. (Workgroups that stay and ask for their
+// next slice first need its registers as well, which costs as many waves: 58 us.) 4 rows of 151936: 7.1 + 4.8, two launches' latency.
 
 #include "attention_common.h"
 
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kWords = 32;                 // of a thread's values, as they are in memory
+constexpr int kWords = 32;                 // of a thread's values, as they are in memory: 62 to 80 registers, 6 to 8 waves a SIMD
 template <int DTYPE>
 constexpr int kEach = DTYPE == VXA_F32 ? kWords : 2 * kWords;  // values of a thread, in runs of 8
 template <int DTYPE>
@@ -283,6 +284,8 @@ __device__ inline double score_of(u64 o) { return __builtin_bit_cast(double, o >
 
 constexpr int kJoin = 1024;
 
+// A request has at most 4096 slices, each with its `count` largest in order. Of the slices' first ones the count-th largest is a bar
+// that no candidate below passes, so at most count slices, count^2 candidates, are ranked in LDS.
 __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamParams p) {
   // Of beam b: its largest logit, the log of its sum of exp(x - largest), its score (-inf: no continuations).
   __shared__ float s_top[kMost * 16];

@@ -6,7 +6,10 @@
 // which workgroups run: counts are whole numbers, and new pages are the lowest free ones, in the order of rows and places.
 //
 // fork and resize are two launches: one workgroup decides which places get a page and finds the free ones, while others copy the
-// counts; then a workgroup for each row writes its entries and counts, and others copy the pages.
+// counts; then a workgroup for each row writes its entries and counts, and others copy the pages. They move few bytes (2.4 us at a
+// copy's rate for 256 rows and 4 layers) and are bound by launches and chains of dependent reads: parents, lengths, entries, counts,
+// then the page. fork of 256 rows, 16 views: 5.3 + 7.9 us, resize 4.7 + 4.0; keep of 64 trees of 40 nodes, 16 views: 6.4, resize 2.4 + 3.1.
+// A call takes 4 to 9 us on the host besides, most of it the views that it is given.
 
 #include <algorithm>
 
@@ -105,26 +108,60 @@ __device__ inline int block_scan(int x, int* s_wave, int& all) {
   return mine + before;
 }
 
-// give(rank, page) for the `wanted` lowest free pages; how many there were.
+// give(rank, page) for the `wanted` lowest free pages; how many there were. A wave looks at 64 counts with each load, all of them at
+// once; the free ones are the bits of a ballot. (8 counts a thread, one after the other in memory: 3.5 us for each
+// 8192 of them in place of 2. 16 loads a wave: more instructions than a small pool's plan has time to fetch, 7.0 us for a resize in place of 6.2.)
 template <typename F>
 __device__ int find_free(const TableParams& p, int wanted, int* s_wave, F&& give) {
+  constexpr int kMost = 8;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int loads = min(kMost, (p.num_blocks + kPlan - 1) / kPlan);  // of a wave: few counts are for all waves too
   int found = 0;
-  for (int64_t b0 = 0; b0 < p.num_blocks && found < wanted; b0 += 8 * kPlan) {
-    const int64_t b = b0 + 8 * (int)threadIdx.x;
-    uint32_t free = 0;
+  for (int b0 = 0; b0 < p.num_blocks && found < wanted; b0 += loads * kPlan) {
+    const int first = b0 + wave * 64 * loads + lane;
+    int32_t x[kMost];
+    uint64_t free[kMost];
+    int mine = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (b + j < p.num_blocks && p.refs[b + j] == 0) free |= 1u << j;
-    int all;
-    int rank = found + block_scan(__popc(free), s_wave, all) - __popc(free);
-    for (; free && rank < wanted; free &= free - 1) give(rank++, (int)b + __builtin_ctz(free));
-    found += all;
+    for (int j = 0; j < kMost; ++j)
+      if (j < loads) x[j] = p.refs[min(first + 64 * j, p.num_blocks - 1)];
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) {
+      free[j] = 0;
+      if (j < loads) free[j] = __ballot(first + 64 * j < p.num_blocks && x[j] == 0);
+      mine += __popcll(free[j]);
+    }
+    __syncthreads();  // the sums before have been read
+    if (lane == 0) s_wave[wave] = mine;
+    __syncthreads();
+    int rank = found;
+#pragma unroll
+    for (int w = 0; w < kPlan / 64; ++w) {
+      if (w < wave) rank += s_wave[w];
+      found += s_wave[w];
+    }
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) {
+      if (free[j] == 0) continue;
+      const int at = rank + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(free[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)free[j], 0u));
+      if ((free[j] >> lane & 1) && at < wanted) give(at, first + 64 * j);
+      rank += __popcll(free[j]);
+    }
   }
   return min(found, wanted);
 }
 
 __device__ inline void copy_refs(const TableParams& p, int share, int shares) {
-  for (int64_t i = (int64_t)share * kPlan + threadIdx.x; i < p.num_blocks; i += (int64_t)shares * kPlan) p.out_refs[i] = p.refs[i];
+  constexpr int N = 4;  // at once
+  const int step = shares * kPlan;
+  for (int i0 = share * kPlan + (int)threadIdx.x; i0 < p.num_blocks; i0 += N * step) {
+    int32_t x[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = p.refs[min(i0 + j * step, p.num_blocks - 1)];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i0 + j * step < p.num_blocks) p.out_refs[i0 + j * step] = x[j];
+  }
 }
 
 // Length of row r's parent, and the page of its partly filled end (-1: there is none, or not one of the cache).
@@ -261,14 +298,13 @@ __global__ __launch_bounds__(kPlan) void pages_resize_plan_kernel(TableParams p)
 __global__ __launch_bounds__(256) void pages_resize_kernel(TableParams p) {
   for (int j = threadIdx.x; j < p.cols; j += 256) resize_entry(p, blockIdx.x, j);
 }
-// All of it by one workgroup.
+// All of it by one workgroup, an entry a thread.
 __global__ __launch_bounds__(kPlan) void pages_resize_small_kernel(TableParams p) {
   __shared__ int s_wave[kPlan / 64];
   if (p.out_refs != p.refs) copy_refs(p, 0, 1);
   plan_resize(p, s_wave);
-  __threadfence();  // the copied counts are where the atomic additions are made, before any of them
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.rows * p.cols; i += kPlan) resize_entry(p, i / p.cols, i % p.cols);
+  __syncthreads();  // the copied counts, the plan
+  if ((int)threadIdx.x < p.rows * p.cols) resize_entry(p, threadIdx.x / p.cols, threadIdx.x % p.cols);
 }
 
 struct KeepParams {
@@ -283,7 +319,8 @@ struct KeepParams {
 constexpr int kKeepUnits = 8;                       // that a thread holds
 constexpr int kKeepWidth = kKeepUnits * 256 / 64;   // columns of a slab: a workgroup holds 64 rows of it
 
-// Workgroup (request, view, slab): the kept rows of columns (head, chunk) of the view. All are read before any is written.
+// Workgroup (request, view, slab): the kept rows of columns (head, chunk) of the view. A kept token moves to a place that another one
+// may still lie in, so all are read, into registers, before any is written: 64 rows of 32 chunks for 256 threads of 8.
 __global__ __launch_bounds__(256) void pages_keep_kernel(KeepParams p, Views views, bool lens) {
   __shared__ int64_t s_src[64], s_dst[64];  // of kept row j, -1: it stays where it is
   const int r = blockIdx.x;
@@ -347,7 +384,10 @@ Views views_of(const vxa_cache_view* caches, int64_t first, int64_t count) {
 }
 
 constexpr int64_t kMostBlocks = 1 << 28;
-constexpr int64_t kSmallTable = 4096, kSmallPool = 16384;  // a resize that one workgroup does: 4 entries and 16 counts a thread
+// A resize that one workgroup does, an entry and four counts a thread: 16 rows of 64 entries and 4096 counts, in a replayed graph, 5.7 us in place of
+// two launches' 6.0, and 4 us less of the host where it is called eagerly. Four entries a thread took 8.2 us in place of 6.0, 16 counts
+// besides 9.6 in place of 6.6.
+constexpr int64_t kSmallTable = kPlan, kSmallPool = 4 * kPlan;
 
 // What fork and resize check of a table and its counts.
 int check_table(int64_t rows, int64_t cols, int64_t num_blocks, int64_t page) {
