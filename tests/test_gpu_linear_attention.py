@@ -420,3 +420,20 @@ def test_outputs_over_the_inputs_are_refused():
             linear_prompt(q, k, v, cu, decays(2), 0.1, out)
         with pytest.raises(ValueError, match="out must not be"):
             linear_step(q, k, v, decays(2), 0.1, out, pool, slots, slots)
+
+
+@pytest.mark.parametrize("dtype,H,KV,D", [(torch.bfloat16, 16, 4, 64), (torch.bfloat16, 17, 17, 64), (torch.float16, 20, 5, 128), (torch.float16, 18, 2, 256), (torch.bfloat16, 6, 3, 256)])
+@pytest.mark.parametrize("lens", [(319, 320, 321), (511, 512, 513, 0, 3), (961, 1, 640), (383, 385, 769), (1536, 1537)])
+def test_lengths_about_the_parts(lens, dtype, H, KV, D):
+    """Sequences are cut into parts whose length goes by the heads: lengths beside their multiples, from states, in place."""
+    q, k, v, cu = inputs(lens, H, KV, D, dtype, seed=26, extra=1)
+    g, scale = decays(H), D ** -0.5
+    starts = torch.randn(len(lens), H, D, D, generator=torch.Generator().manual_seed(27)).to(DEV)
+    state, slots = starts.clone(), torch.arange(len(lens), dtype=torch.int32, device=DEV)
+    out = torch.full((len(q), H, D), 7.0, device=DEV)
+    linear_prompt(q, k, v, cu, g, scale, out, state, slots, slots)
+    want, ends = linear64(q, k, v, lens, g, scale, starts)
+    row_bound, state_bound = bounds(q, k, v, lens, g, scale, starts)
+    check(out[:-1], want[:-1], row_bound[:-1])
+    check(state, ends, state_bound)
+    assert (out[-1] == 7).all()

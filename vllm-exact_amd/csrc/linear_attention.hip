@@ -19,6 +19,7 @@ struct LinearParams {
   int64_t svt, svh;
   const int32_t* cu;  // of prompts
   int32_t n, total, H, G;
+  int32_t part;  // rows of a part of a long sequence
   const float* log_decay;
   float scale;
   void* out;
@@ -128,15 +129,22 @@ hipError_t launch_step(int64_t D, const LinearParams& p, hipStream_t st) {
 //   fp16 queries, keys and values beside them: two, exactly. Products of two second parts are left out (2^-16 of a term, in S 2^-22).
 // The weights are powers of a whole number of rows, at most 1, never quotients of two powers, which would overflow.
 //
-// A sequence is walked in order, so 32 heads of one prompt of 8192 rows would be 32 workgroups. It is cut into parts of 512 rows:
+// A sequence is walked in order, so 32 heads of one prompt of 8192 rows would be 32 workgroups. It is cut into parts of 320 to 512 rows:
 // one launch computes what each part adds to the state (half the work of outputs, 32 us for 8192 rows of 32 heads of 128), one adds
 // these up (10.5 us, and only where a sequence may have three parts), one computes the outputs (68 us). A token at
-// a time, one after the other, the same call takes 4128 us. Where the cuts are goes by the sequence alone, and so do a row's bits.
+// a time, one after the other, the same call takes 4128 us. Where the cuts are goes by the sequence
+// and the heads alone, and so do a row's bits.
 //
 // What bounds it: 17.2 GF are 15 us at the rate of a large product, 170 MB 35 us at that of a copy. A SIMD's matrix and vector instructions
 // do not overlap here (two waves a SIMD, which is what their registers allow): per chunk of 64 rows a wave has 98 products of 32
 // clocks and some 1000 vector instructions that split, weight and stage, of 13,200 clocks that two of them take together.
-constexpr int kPart = 512;
+//
+// Where there are up to 16 heads, a few prompts leave CUs idle with parts of 512 rows: nine calls of 4 to 16 heads of 128 dims take 55 us
+// in the geometric mean with 320 rows and 68 with 512. With 32 heads there are enough workgroups, and what counts is each part's
+// state: 8192 rows 100 us, 121 with 320; 16 prompts of 900 163 and 194. States of 256 dims are four times as large: 384 rows, 178 us
+// in the mean of 15 calls with 16 heads where 512 take 193, and 320 175 with a fifth more states to keep (one prompt of 4096 rows 121 us
+// and 114, eight of 700 114 and 142).
+inline int part_rows(int64_t heads, int64_t dims) { return heads > 16 ? 512 : dims > 128 ? 384 : 320; }
 
 __device__ inline float power(float g, int e) { return e == 0 ? 1.0f : expf(g * (float)e); }  // exp(-inf * 0) is 1 here
 
@@ -178,7 +186,7 @@ __device__ inline int again(int id) {
   return id;
 }
 
-// Part `part` of sequence seq. The grid has floor(tokens / kPart) + n places: the whole parts come first, then what is left of the
+// Part `part` of sequence seq. The grid has floor(tokens / rows of a part) + n places: the whole parts come first, then what is left of the
 // sequences (and empty ones), 64 sequences at a time the longest first, so that the last workgroups are short ones.
 struct Part {
   int seq, lo, len, part, parts;  // parts: of the sequence, at least 1
@@ -195,23 +203,25 @@ __device__ inline Part find_part(const LinearParams& p, int index) {
   };
   auto found = [&](int j, int lo, int len, int at, bool whole, int part) {  // of lane `at`
     lo = __builtin_amdgcn_readlane(lo, at), len = __builtin_amdgcn_readlane(len, at);
-    return Part{j + at, lo, len, whole ? part : len / kPart, max(1, (len + kPart - 1) / kPart)};
+    const int all = len / p.part;
+    return Part{j + at, lo, len, whole ? part : all, max(1, all + (len > all * p.part))};
   };
   for (int j0 = 0; j0 < p.n; j0 += 64) {
     int lo, len;
     lengths(j0 + lane, lo, len);
-    const int upto = wave_scan(len / kPart, add), all = __builtin_amdgcn_readlane(upto, 63);
+    const int mine = len / p.part, upto = wave_scan(mine, add), all = __builtin_amdgcn_readlane(upto, 63);
     if (index < all) {
       const int at = __builtin_ctzll(__ballot(upto > index));
-      return found(j0, lo, len, at, true, index - __builtin_amdgcn_readlane(upto - len / kPart, at));
+      return found(j0, lo, len, at, true, index - __builtin_amdgcn_readlane(upto - mine, at));
     }
     index -= all;
   }
   for (int j0 = 0; j0 < p.n; j0 += 64) {
     int lo, len;
     lengths(j0 + lane, lo, len);
-    const bool has = j0 + lane < p.n && (len % kPart != 0 || len == 0);
-    const int all = __popcll(__ballot(has)), key = has ? (len % kPart) * 64 + lane : -1;
+    const int rest = len % p.part;
+    const bool has = j0 + lane < p.n && (rest != 0 || len == 0);
+    const int all = __popcll(__ballot(has)), key = has ? rest * 64 + lane : -1;
     if (index < all) {
       int rank = 0;
       for (int m = 0; m < min(64, p.n - j0); ++m) rank += __builtin_amdgcn_readlane(key, m) > key;
@@ -221,10 +231,10 @@ __device__ inline Part find_part(const LinearParams& p, int index) {
   }
   return Part{0, 0, 0, 0, 0};
 }
-// Where the state before part `part` of a sequence of several parts is kept: 2 floor(lo / kPart) + part. (The parts of a
-// sequence longer than kPart are at most twice its whole ones.)
+// Where the state before part `part` of a sequence of several parts is kept: 2 floor(lo / rows of a part) + part. (The parts of a
+// sequence longer than one are at most twice its whole ones.)
 __device__ inline int64_t kept_at(const LinearParams& p, int lo, int part, int head, int size) {
-  return ((int64_t)(2 * (lo / kPart) + part) * p.H + head) * size;
+  return ((int64_t)(2 * (lo / p.part) + part) * p.H + head) * size;
 }
 
 // A tile's 16-byte chunks lie at chunk ^ swizzle(row): 16 rows that are read at one chunk meet 16 different ones.
@@ -264,7 +274,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   const float g = p.log_decay[head];
   const Part part = find_part(p, (int)(blockIdx.x / p.H));
   if (part.part >= part.parts - (OUT ? 0 : 1)) return;
-  const int row0 = part.part * kPart, rows = min(kPart, part.len - row0);
+  const int row0 = part.part * p.part, rows = min(p.part, part.len - row0);
   const int64_t base = part.lo + row0;
   char* const out = reinterpret_cast<char*>(p.out);
   const uint16_t* const qh = p.q + head * p.sqh;
@@ -588,11 +598,11 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
 __global__ __launch_bounds__(256) void linear_parts_kernel(LinearParams p, float* kept, int size) {
   const int pieces = size / 1024, head = (int)(blockIdx.x / pieces) % p.H, seq = (int)(blockIdx.x / pieces) / p.H;
   const int lo = min(max(p.cu[seq], 0), p.total), len = min(max(p.cu[seq + 1], lo), p.total) - lo;
-  const int parts = (len + kPart - 1) / kPart;
+  const int parts = (len + p.part - 1) / p.part;
   if (parts < 3) return;
   v4f* x = reinterpret_cast<v4f*>(kept + kept_at(p, lo, 1, head, size)) + (int)(blockIdx.x % pieces) * 256 + (int)threadIdx.x;
   const int64_t step = (int64_t)p.H * size / 4;
-  const float decay = power(p.log_decay[head], kPart);
+  const float decay = power(p.log_decay[head], p.part);
   v4f s = *x;
 #pragma unroll 4
   for (int i = 2; i < parts; ++i) {
@@ -603,16 +613,19 @@ __global__ __launch_bounds__(256) void linear_parts_kernel(LinearParams p, float
   }
 }
 
-int64_t kept_states(int64_t tokens) { return tokens > kPart ? 2 * (tokens / kPart) + 2 : 0; }
+int64_t kept_states(int64_t tokens, int64_t heads, int64_t dims) {
+  const int64_t part = part_rows(heads, dims);
+  return tokens > part ? 2 * (tokens / part) + 2 : 0;
+}
 
 template <typename T, int D>
 hipError_t launch_prompt(const LinearParams& p, float* kept, hipStream_t st) {
-  const int64_t blocks = (int64_t)p.H * (p.total / kPart + p.n);
+  const int64_t blocks = (int64_t)p.H * (p.total / p.part + p.n);
   const int64_t pieces = (int64_t)p.n * p.H * (D * D / 1024);
   if (!launchable(blocks, 2 * D) || !launchable(pieces, 256)) return hipErrorInvalidConfiguration;
-  if (p.total > kPart) {  // some sequence may have several parts
+  if (p.total > p.part) {  // some sequence may have several parts
     hipLaunchKernelGGL((linear_chunk_kernel<T, D, false>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
-    if (p.total > 2 * kPart) hipLaunchKernelGGL(linear_parts_kernel, dim3((unsigned)pieces), dim3(256), 0, st, p, kept, D * D);
+    if (p.total > 2 * p.part) hipLaunchKernelGGL(linear_parts_kernel, dim3((unsigned)pieces), dim3(256), 0, st, p, kept, D * D);
   }
   hipLaunchKernelGGL((linear_chunk_kernel<T, D, true>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
   return hipGetLastError();
@@ -645,7 +658,7 @@ int linear_params(LinearParams& p, const void* q, int64_t sqt, int64_t sqh, cons
   p.q = reinterpret_cast<const uint16_t*>(q), p.sqt = sqt, p.sqh = sqh;
   p.k = reinterpret_cast<const uint16_t*>(k), p.skt = skt, p.skh = skh;
   p.v = reinterpret_cast<const uint16_t*>(v), p.svt = svt, p.svh = svh;
-  p.cu = nullptr;
+  p.cu = nullptr, p.part = part_rows(H, D);
   p.n = (int32_t)n, p.total = (int32_t)tokens, p.H = (int32_t)H, p.G = (int32_t)(H / KV);
   p.log_decay = log_decay, p.scale = scale;
   p.out = out, p.sot = sot, p.soh = soh, p.out_dtype = out_dtype;
@@ -663,7 +676,7 @@ int status_of(hipError_t err) {
 
 extern "C" int vxa_linear_prompt_workspace(int64_t tokens, int64_t num_heads, int64_t head_dim, size_t* ws_bytes) {
   if (tokens < 0 || num_heads <= 0 || head_dim <= 0 || !ws_bytes) return VXA_ERR_ARG;
-  *ws_bytes = (size_t)product({kept_states(tokens), num_heads, head_dim, head_dim, 4});
+  *ws_bytes = (size_t)product({kept_states(tokens, num_heads, head_dim), num_heads, head_dim, head_dim, 4});
   return VXA_OK;
 }
 
