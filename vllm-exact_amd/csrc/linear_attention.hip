@@ -555,7 +555,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
         }
       }
     }
-    if (OUT && t0 + C >= rows && !to) break;  // nobody takes the state behind these rows (3 prompts of 2111, fp16, 256 dims: 142 to 139 us)
+    if (OUT && t0 + C >= rows && !to) break;  // nobody takes the state behind these rows (3 prompts of 2111, fp16, 256 dims, parts of 512: 142 to 139 us)
     if (kLate && t0 + C < rows) fetch(t0 + C);
     __builtin_amdgcn_s_setprio(3);
     // The state. Values are weighted and split into three parts, which keep the 24 bits of the products; the keys are exact.
