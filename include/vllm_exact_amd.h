@@ -364,7 +364,8 @@ int vxa_linear_step(const void* q, int64_t stride_qt, int64_t stride_qh, const v
 
 /*
  * Beam search's selection (beam.beam_select): of all continuations (beam b, token v) of a request, with the score
- * scores[b] + x_bv - log sum_u exp(x_bu) in more than 32 bits, the `count` (<= 64) best in order; equal scores by (b, v).
+ * scores[b] + x_bv - log sum_u exp(x_bu) in more than 32 bits, the `count` (<= 64) best in order: of one beam by x_bv, then v; of
+ * several by the score in fp64, then b.
  * logits [n * beams, vocab] with row stride stride_row (fp32, bf16 or fp16), scores [n * beams]; out_scores, out_parents (the
  * logits' row) and out_tokens [n, count]. A beam of score -inf has no continuations, nor a token of logit -inf; where a request
  * has fewer than `count`, the rest is -inf, -1, -1. A request with a NaN or +inf among the logits or scores of its other beams

@@ -1,8 +1,10 @@
 // Beam search's selection over beams and vocabulary (gfx950).
 //
 //   score(b, v) = scores[b] + x_bv - log sum_u exp(x_bu)
-// for the beams b of a request; the `count` largest, in order, equal scores by (b, v). An fp64 score of a beam's log-sum, whose
-// terms are fp32 and whose sums are fp64, orders beams against each other; within a beam the logits themselves do.
+// for the beams b of a request; the `count` largest, in order. An fp64 score of a beam's log-sum, whose terms are fp32 and whose sums
+// are fp64, orders beams against each other, equal ones by b; within a beam the logits themselves do, equal ones by v. (A score in which
+// the logits drown, as of a beam held at -1e30, is the same for all tokens of the beam. As a score rises with its logit, this
+// is one order of all continuations, by which slices and requests choose alike.)
 //
 // A row of logits is cut into slices, a workgroup each. A thread holds its values in registers, so the logits are read
 // once: maximum, sum of exponentials, and the slice's `count` largest. Those are among the values that are at least the
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamParams p) {
   __shared__ float s_top[kMost * 16];
   __shared__ double s_log[kMost * 16], s_score[kMost * 16];
   __shared__ u64 s_order[kMostSlices];        // of the slices' best, then of the candidates
-  __shared__ uint32_t s_place[kMostSlices];   // beam * vocab + token
+  __shared__ u64 s_tail[kMostSlices];         // order of the logit, then ~place, a place being beam * vocab + token
   __shared__ int s_count, s_bar, s_nan;
   const int request = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row0 = (int64_t)request * p.beams;
@@ -324,57 +326,72 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamParams p) {
   }
   const int groups = p.beams * p.slices;
   const u64* keys = p.keys + row0 * p.slices * p.count;
-  auto score = [&](int group, int rank, u64& order, uint32_t& place) {
+  auto score = [&](int group, int rank, u64& order, u64& tail) {
     const u64 key = keys[(int64_t)group * p.count + rank];
     const int b = group / p.slices;
     // the differences first: they are exact, or nearly, where logits are large
     order = key && s_score[b] != -__builtin_huge_val() ? order_of(s_score[b] + (((double)value_of((uint32_t)(key >> 32)) - (double)s_top[b]) - s_log[b])) : 0;
-    place = (uint32_t)b * (uint32_t)p.vocab + ~(uint32_t)key;
+    tail = key - (uint32_t)b * (uint32_t)p.vocab;  // ~(x + y) = ~x - y, and no borrow: places are less than 2^31
   };
-  auto above = [](u64 o, uint32_t q, u64 order, uint32_t place) { return o > order || (o == order && q < place); };
-  for (int g = threadIdx.x; g < groups; g += kJoin) score(g, 0, s_order[g], s_place[g]);
+  auto beam_of = [&](u64 tail) { return ~(uint32_t)tail / (uint32_t)p.vocab; };
+  // Scores, then beams, then logits, then tokens. With equal scores tails alone say it, but where two beams' logits differ.
+  auto above = [&](u64 o, u64 t, u64 order, u64 tail) {
+    return o != order ? o > order : beam_of(t) == beam_of(tail) ? t > tail : (uint32_t)t > (uint32_t)tail;
+  };
+  // f(i, how many are above number i), of the n in LDS, for one of the 2^share threads that compare number i together.
+  auto rank_all = [&](int n, auto&& f) {
+    int share = 0;  // at most 4
+    while (n >> share > 4 && n << (share + 1) <= kJoin) ++share;
+    const int part = threadIdx.x & ((1 << share) - 1);
+    for (int i0 = 0; i0 < n; i0 += kJoin >> share) {
+      const int i = i0 + ((int)threadIdx.x >> share);
+      const u64 order = i < n ? s_order[i] : 0, tail = i < n ? s_tail[i] : 0;
+      int rank = 0;
+      if (order) {
+        uint32_t differ = 0;
+        for (int j = part; j < n; j += 1 << share) {
+          const u64 o = s_order[j], t = s_tail[j];
+          rank += o > order || (o == order && t > tail);
+          differ |= o == order ? (uint32_t)((t ^ tail) >> 32) : 0u;
+        }
+        if (differ) {  // rare: scores in which logits drown
+          rank = 0;
+          for (int j = part; j < n; j += 1 << share) rank += above(s_order[j], s_tail[j], order, tail);
+        }
+      }
+      for (int m = 1; m < 1 << share; m *= 2) rank += __builtin_amdgcn_ds_bpermute((lane ^ m) << 2, rank);
+      if (order && part == 0) f(i, rank);
+    }
+  };
+  for (int g = threadIdx.x; g < groups; g += kJoin) score(g, 0, s_order[g], s_tail[g]);
   __syncthreads();
-  // The slice whose best is the count-th: no candidate below it is among the best. 2^share threads compare one slice.
-  int share = 0;
-  while (share < 6 && groups << (share + 1) <= kJoin) ++share;
-  for (int g0 = 0; g0 < groups; g0 += kJoin >> share) {
-    const int g = g0 + ((int)threadIdx.x >> share);
-    const u64 order = g < groups ? s_order[g] : 0;
-    const uint32_t place = g < groups ? s_place[g] : 0;
-    int rank = 0;
-    if (order)
-      for (int j = threadIdx.x & ((1 << share) - 1); j < groups; j += 1 << share) rank += above(s_order[j], s_place[j], order, place);
-    for (int m = 1; m < 1 << share; m *= 2) rank += __builtin_amdgcn_ds_bpermute((lane ^ m) << 2, rank);
-    if (order && rank == p.count - 1) s_bar = g;
-  }
+  // The slice whose best is the count-th: no candidate below it is among the best.
+  rank_all(groups, [&](int g, int rank) {
+    if (rank == p.count - 1) s_bar = g;
+  });
   __syncthreads();
   const int bar = s_bar;
-  const u64 least = bar >= 0 ? s_order[bar] : 1;
-  const uint32_t least_place = bar >= 0 ? s_place[bar] : ~0u;
+  const u64 least = bar >= 0 ? s_order[bar] : 1, least_tail = bar >= 0 ? s_tail[bar] : 0;
   __syncthreads();
-  // At most count slices have candidates from there on, of count each.
+  // At most count slices have candidates from there on, of count each: a slice's first one is its best in this order too.
   for (int i = threadIdx.x; i < groups * p.count; i += kJoin) {
-    u64 order;
-    uint32_t place;
-    score(i / p.count, i % p.count, order, place);
-    if (order && !above(least, least_place, order, place)) {
+    u64 order, tail;
+    score(i / p.count, i % p.count, order, tail);
+    if (order && !above(least, least_tail, order, tail)) {
       const int at = atomicAdd(&s_count, 1);
-      s_order[at] = order, s_place[at] = place;
+      s_order[at] = order, s_tail[at] = tail;
     }
   }
   __syncthreads();
   const int listed = s_count;
-  for (int i = threadIdx.x; i < listed; i += kJoin) {
-    const u64 order = s_order[i];
-    const uint32_t place = s_place[i];
-    int rank = 0;
-    for (int j = 0; j < listed; ++j) rank += above(s_order[j], s_place[j], order, place);
+  rank_all(listed, [&](int i, int rank) {
     if (rank < p.count) {
-      p.out_scores[out + rank] = (float)score_of(order);
-      p.out_parents[out + rank] = (int32_t)(row0 + place / p.vocab);
-      p.out_tokens[out + rank] = place % p.vocab;
+      const uint32_t place = ~(uint32_t)s_tail[i];
+      p.out_scores[out + rank] = (float)score_of(s_order[i]);
+      p.out_parents[out + rank] = (int32_t)(row0 + place / (uint32_t)p.vocab);
+      p.out_tokens[out + rank] = place % (uint32_t)p.vocab;
     }
-  }
+  });
   for (int i = listed + (int)threadIdx.x; i < p.count; i += kJoin)
     p.out_scores[out + i] = kNegInf, p.out_parents[out + i] = -1, p.out_tokens[out + i] = -1;
 }
