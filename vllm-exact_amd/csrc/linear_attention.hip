@@ -53,6 +53,19 @@ __device__ inline Slots find_slots(const LinearParams& p, int seq) {
   return s;
 }
 
+// exp(g rows), what a state decays by, as an fp32 number and its rest: rounded to fp32 alone, its error would grow with every step and
+// every call, as the states' own roundings do not.
+struct Decay {
+  float whole, rest;
+};
+__device__ inline Decay decay_of(float g, int rows) {
+  const double exact = exp((double)g * rows);
+  return {(float)exact, (float)(exact - (double)(float)exact)};
+}
+// A value that all lanes have, in a scalar register.
+__device__ inline float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
+__device__ inline Decay uniform(Decay x) { return {uniform(x.whole), uniform(x.rest)}; }
+
 // ---------------------------------------------------------------------------------- single tokens
 constexpr int kCols = 32;  // columns of a state that a workgroup takes
 
@@ -81,14 +94,12 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearParams p) {
     s_k[x] = T::to_f32(p.k[seq * p.skt + head / p.G * p.skh + x]);
   }
   const float v = T::to_f32(p.v[seq * p.svt + head / p.G * p.svh + slab * kCols + col]);
-  // The decay in two parts: rounded to fp32, its error would grow with every step, as the state's own roundings do not.
-  const double exact = exp((double)p.log_decay[head]);
-  const float decay = (float)exact, rest = (float)(exact - (double)decay);
+  const Decay decay = decay_of(p.log_decay[head], 1);
   __syncthreads();
   float o = 0.0f;
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    s[i] = fmaf(s[i], decay, fmaf(s[i], rest, s_k[part * kRows + i] * v));
+    s[i] = fmaf(s[i], decay.whole, fmaf(s[i], decay.rest, s_k[part * kRows + i] * v));
     o = fmaf(s_q[part * kRows + i], s[i], o);
   }
   s_o[part][col] = o;
@@ -276,6 +287,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   if (part.part >= part.parts - (OUT ? 0 : 1)) return;
   const int row0 = part.part * p.part, rows = min(p.part, part.len - row0);
   const int64_t base = part.lo + row0;
+  const Decay full = uniform(decay_of(g, C)), last = uniform(decay_of(g, (rows - 1) % C + 1));
   char* const out = reinterpret_cast<char*>(p.out);
   const uint16_t* const qh = p.q + head * p.sqh;
   const uint16_t* const kh = p.k + head / p.G * p.skh;
@@ -392,8 +404,6 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   float grow[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i) grow[i] = OUT ? p.scale * power(g, 32 * i + col + 1) : 0.0f;
-  const float full = power(g, C);
-
   for (int t0 = 0; t0 < rows; t0 += C) {
     const int count = min(C, rows - t0);
     __syncthreads();  // the last chunk's tiles have been read
@@ -559,11 +569,15 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
     if (kLate && t0 + C < rows) fetch(t0 + C);
     __builtin_amdgcn_s_setprio(3);
     // The state. Values are weighted and split into three parts, which keep the 24 bits of the products; the keys are exact.
-    const float decay = count == C ? full : power(g, count);
+    const Decay decay = t0 + C < rows ? full : last;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] *= decay;
+      for (int r = 0; r < 16; ++r) {
+        float less = s[t][r] * -decay.rest;
+        asm("" : "+v"(less));  // subtracted, as a sum would take its summand's register: 204 in place of more than there are, with 256 dims
+        s[t][r] = fmaf(s[t][r], decay.whole, -less);
+      }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       float f[8];
@@ -602,13 +616,13 @@ __global__ __launch_bounds__(256) void linear_parts_kernel(LinearParams p, float
   if (parts < 3) return;
   v4f* x = reinterpret_cast<v4f*>(kept + kept_at(p, lo, 1, head, size)) + (int)(blockIdx.x % pieces) * 256 + (int)threadIdx.x;
   const int64_t step = (int64_t)p.H * size / 4;
-  const float decay = power(p.log_decay[head], p.part);
+  const Decay decay = decay_of(p.log_decay[head], p.part);
   v4f s = *x;
 #pragma unroll 4
   for (int i = 2; i < parts; ++i) {
     const v4f add = x[(i - 1) * step];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = fmaf(s[e], decay, add[e]);
+    for (int e = 0; e < 4; ++e) s[e] = fmaf(s[e], decay.whole, fmaf(s[e], decay.rest, add[e]));
     x[(i - 1) * step] = s;
   }
 }
