@@ -62,6 +62,14 @@ __device__ inline Decay decay_of(float g, int rows) {
   const double exact = exp((double)g * rows);
   return {(float)exact, (float)(exact - (double)(float)exact)};
 }
+// exp(g) s + add of a state's value. The rest counts for finite values alone: an infinity times it would be NaN, or one of the other sign.
+// (Infinities are clamped. A NaN is what the first product is in any case.) Subtracted in place of added, through a register that
+// the compiler does not see into: an addition's result would take the place of its summand, and a state that is updated in place registers for two.
+__device__ inline float decayed(float s, Decay decay, float add) {
+  float less = fmaf(__builtin_amdgcn_fmed3f(s, kLowest, -kLowest), -decay.rest, -add);
+  asm("" : "+v"(less));
+  return fmaf(s, decay.whole, -less);
+}
 // A value that all lanes have, in a scalar register.
 __device__ inline float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 __device__ inline Decay uniform(Decay x) { return {uniform(x.whole), uniform(x.rest)}; }
@@ -99,7 +107,7 @@ __global__ __launch_bounds__(256) void linear_step_kernel(LinearParams p) {
   float o = 0.0f;
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    s[i] = fmaf(s[i], decay.whole, fmaf(s[i], decay.rest, s_k[part * kRows + i] * v));
+    s[i] = decayed(s[i], decay, s_k[part * kRows + i] * v);
     o = fmaf(s_q[part * kRows + i], s[i], o);
   }
   s_o[part][col] = o;
@@ -155,7 +163,8 @@ hipError_t launch_step(int64_t D, const LinearParams& p, hipStream_t st) {
 // state: 8192 rows 100 us, 121 with 320; 16 prompts of 900 163 and 194. States of 256 dims are four times as large: 384 rows, 178 us
 // in the mean of 15 calls with 16 heads where 512 take 193, and 320 175 with a fifth more states to keep (one prompt of 4096 rows 121 us
 // and 114, eight of 700 114 and 142).
-inline int part_rows(int64_t heads, int64_t dims) { return heads > 16 ? 512 : dims > 128 ? 384 : 320; }
+constexpr int kMostRows = 512;  // of a part
+inline int part_rows(int64_t heads, int64_t dims) { return heads > 16 ? kMostRows : dims > 128 ? 384 : 320; }
 
 __device__ inline float power(float g, int e) { return e == 0 ? 1.0f : expf(g * (float)e); }  // exp(-inf * 0) is 1 here
 
@@ -262,7 +271,108 @@ struct Shared {
   char scores[OUT ? (C == 64 ? 6 : 2) : 1][2][OUT ? 1024 : 16];        // operands of 16 keys and 32 queries, two parts
   float power[C];                                                      // scale exp(g (C - 1 - x))
   float left[C];                                                       // exp(g (n - 1 - j)) of row j of the chunk, 0 past its end
+  int met;                                                             // whether something was not finite
 };
+
+// The heads of one KV head on one XCD.
+__device__ inline int head_of(const LinearParams& p, int x) { return p.H % 8 == 0 ? (x % 8) * (p.H / 8) + x / 8 : x; }
+// A sequence of several parts that writes the slot that it reads keeps its first state apart: its last part may end before the first
+// begins.
+__device__ inline bool kept_apart(const Part& part, const Slots& slots) { return part.part == 0 && part.parts > 1 && slots.read >= 0 && slots.read == slots.write; }
+// Where the state before a part is (null: zeros), for its rows or for what it adds to a state, and where the one after it goes (null: nowhere).
+template <bool OUT>
+__device__ inline const float* state_before(const LinearParams& p, float* kept, const Part& part, const Slots& slots, int head, int size) {
+  if (OUT && (part.part > 0 || kept_apart(part, slots))) return kept + kept_at(p, part.lo, part.part, head, size);
+  return part.part == 0 && slots.read >= 0 ? p.state + slots.read * p.sss + head * p.ssh : nullptr;
+}
+template <bool OUT>
+__device__ inline float* state_after(const LinearParams& p, float* kept, const Part& part, const Slots& slots, int head, int size) {
+  if (!OUT) return kept + kept_at(p, part.lo, part.part + 1, head, size);
+  return part.part == part.parts - 1 && slots.write >= 0 ? p.state + slots.write * p.sss + head * p.ssh : nullptr;
+}
+
+// A part's rows through the recurrence, one after the other in fp32, where something was not finite: one of the rows, or the state that
+// they start from. Which sums are infinite, of which sign, and which are NaN the chunks' products do not tell (an infinity's second
+// part is NaN, and its products meet in another order). What is not finite here takes the place of what was stored, what is finite
+// keeps its bits. 32 rows of the state at a time: whether an output is infinite or NaN is the sum of what they say, bits of +inf (or
+// NaN) and of -inf (or NaN) for each row and lane, which lie in the tiles' place. s: the state after the rows from the chunks.
+// All arguments are read and found again, as they would keep scalar registers through all that comes before (8192 tokens: 104 us in
+// place of 107). Such a call of 8192 tokens takes 2 ms, one of 17 tokens 26 us.
+template <typename T, int D, bool OUT>
+__device__ inline void recurrence(const v16f (&s)[D / 32], uint64_t* signs) {
+  struct Args {
+    LinearParams p;
+    float* kept;
+  };
+  typedef const __attribute__((address_space(4))) Args ConstantArgs;
+  ConstantArgs* args = (ConstantArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const LinearParams p = *(const LinearParams*)&args->p;
+  float* const kept = args->kept;
+  int block = blockIdx.x, thread = threadIdx.x;
+  asm volatile("" : "+s"(block), "+v"(thread));
+  const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), half = lane >> 5, col = 32 * wave + (lane & 31);
+  const int head = head_of(p, block % p.H);
+  const Part part = find_part(p, block / p.H);
+  const Slots slots = find_slots(p, part.seq);
+  const float* const from = state_before<OUT>(p, kept, part, slots, head, D * D);
+  float* const to = state_after<OUT>(p, kept, part, slots, head, D * D);
+  const int rows = min(p.part, part.len - part.part * p.part);
+  const int64_t base = part.lo + part.part * p.part;
+  const uint16_t* const q = p.q + base * p.sqt + head * p.sqh;
+  const uint16_t* const k = p.k + base * p.skt + head / p.G * p.skh;
+  const uint16_t* const v = p.v + base * p.svt + head / p.G * p.svh + col;
+  const Decay one = uniform(decay_of(p.log_decay[head], 1));
+  signs += wave * 2 * p.part;
+  for (int i = lane; OUT && i < 2 * rows; i += 64) signs[i] = 0;
+  __threadfence_block();
+  static_for<D / 32>([&](auto t) {
+    v16f x;
+    auto each = [&](auto f) {  // value r: row 32 t + 8 (r / 4) + 4 half + r % 4 of column col
+#pragma unroll
+      for (int r = 0; r < 16; ++r) f(r, (int64_t)(32 * t + 8 * (r / 4) + 4 * half + r % 4) * D + col);
+    };
+    each([&](int r, int64_t) { x[r] = 0.0f; });
+    if (from) each([&](int r, int64_t at) { x[r] = from[at]; });
+#pragma unroll 1
+    for (int row = 0; row < rows; ++row) {
+      const float value = T::to_f32(v[row * p.svt]);
+      auto four = [&](const uint16_t* at, float (&f)[4]) {
+        const v2u32 w = *reinterpret_cast<const v2u32*>(at);
+        const v2f low = T::unpack(w.x), high = T::unpack(w.y);
+        f[0] = low.x, f[1] = low.y, f[2] = high.x, f[3] = high.y;
+      };
+      float o = 0.0f;
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        float f[4];
+        four(k + row * p.skt + 32 * t + 8 * a + 4 * half, f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * a + e] = decayed(x[4 * a + e], one, f[e] * value);
+        if constexpr (OUT) {
+          four(q + row * p.sqt + 32 * t + 8 * a + 4 * half, f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o = fmaf(f[e], x[4 * a + e], o);
+        }
+      }
+      if constexpr (OUT) {
+        const uint64_t plus = __ballot(!(o < __builtin_huge_valf())), minus = __ballot(!(o > kNegInf));
+        if (lane == 0) signs[2 * row] |= plus, signs[2 * row + 1] |= minus;
+      }
+    }
+    if (to) each([&](int r, int64_t at) { to[at] = __builtin_isfinite(x[r]) && __builtin_isfinite(s[t][r]) ? s[t][r] : x[r]; });
+  });
+  if constexpr (OUT) {
+    __threadfence_block();  // the bits; and other lanes of the wave have stored these rows
+#pragma unroll 1
+    for (int row = 0; row < rows; ++row) {
+      const uint64_t plus = signs[2 * row], minus = signs[2 * row + 1];
+      const bool high = (plus | plus >> 32) >> (lane & 31) & 1, low = (minus | minus >> 32) >> (lane & 31) & 1;
+      if (half == 0 && (high || low))
+        store_f32_as(p.out, p.out_dtype, (base + row) * p.sot + head * p.soh + col, p.scale * (high && low ? __builtin_nanf("") : high ? __builtin_huge_valf() : kNegInf));
+    }
+  }
+}
 
 // A workgroup of D / 32 waves takes one head of a part. A wave keeps 32 columns of the state in the accumulators of 32 x 32 x 16
 // MFMAs, where they are the operand of the next product as they lie. (Twice as many waves of 16 columns, four a SIMD: 80 us in place of 77
@@ -272,6 +382,7 @@ struct Shared {
 template <typename T, int D, bool OUT>
 __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, float* kept) {
   using S = Shared<T, D, OUT>;
+  static_assert(!OUT || sizeof(S) >= D / 32 * 2 * kMostRows * sizeof(uint64_t), "recurrence() keeps bits there");
   constexpr bool F16 = S::F16;
   constexpr int C = S::C, kRow = 2 * D;
   constexpr int DT = D / 32, IT = C / 32, CT = C / 16;  // blocks of the state's rows, of queries, of keys
@@ -280,8 +391,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   __shared__ __attribute__((aligned(1024))) S sh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int x = (int)(blockIdx.x % p.H);
-  const int head = p.H % 8 == 0 ? (x % 8) * (p.H / 8) + x / 8 : x;  // heads of one KV head on one XCD
+  const int head = head_of(p, (int)(blockIdx.x % p.H));
   const float g = p.log_decay[head];
   const Part part = find_part(p, (int)(blockIdx.x / p.H));
   if (part.part >= part.parts - (OUT ? 0 : 1)) return;
@@ -368,23 +478,18 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
       for (int i = threadIdx.x; i < rows * D; i += 2 * D) store_f32_as(out, p.out_dtype, (base + i / D) * p.sot + head * p.soh + i % D, __builtin_nanf(""));
     return;
   }
+  if (threadIdx.x == 0) sh.met = 0;
+  if (rows == 0) __syncthreads();
   if ((int)threadIdx.x < C) {
     const float w = power(g, C - 1 - (int)threadIdx.x);
     sh.power[threadIdx.x] = w * p.scale, sh.left[threadIdx.x] = w;
   }
-  // A sequence of several parts that writes the slot that it reads keeps its first state apart: its last part may end before the first
-  // begins.
-  const bool apart = part.parts > 1 && slots.read == slots.write;
-  const float* from = nullptr;
-  if (part.part > 0 ? OUT : OUT && apart && slots.read >= 0)
-    from = kept + kept_at(p, part.lo, part.part, head, D * D);
-  else if (part.part == 0 && slots.read >= 0)
-    from = p.state + slots.read * p.sss + head * p.ssh;
+  const float* const from = state_before<OUT>(p, kept, part, slots, head, D * D);
   if (from)
     state_rows([&](int t, int r, int64_t at) { s[t][r] = from[at]; });
   else
     state_rows([&](int t, int r, int64_t) { s[t][r] = 0.0f; });
-  if (!OUT && apart && part.part == 0 && slots.read >= 0) {
+  if (!OUT && kept_apart(part, slots)) {
     float* to = kept + kept_at(p, part.lo, 0, head, D * D);
     state_rows([&](int t, int r, int64_t at) { to[at] = s[t][r]; });
   }
@@ -396,14 +501,11 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
     const v2u32 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
     return v4u32{lo.x, lo.y, hi.x, hi.y};
   };
-  float* to = nullptr;  // of the state after the rows
-  if (!OUT)
-    to = kept + kept_at(p, part.lo, part.part + 1, head, D * D);
-  else if (part.part == part.parts - 1 && slots.write >= 0)
-    to = p.state + slots.write * p.sss + head * p.ssh;
+  float* const to = state_after<OUT>(p, kept, part, slots, head, D * D);
   float grow[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i) grow[i] = OUT ? p.scale * power(g, 32 * i + col + 1) : 0.0f;
+  bool met = false;  // sums that are not finite
   for (int t0 = 0; t0 < rows; t0 += C) {
     const int count = min(C, rows - t0);
     __syncthreads();  // the last chunk's tiles have been read
@@ -510,14 +612,14 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
         }
       };
       add_rows(v);
-      // 0 times an infinity or NaN of a later row is NaN. Where sums end up not finite, the rows are added again without such values,
-      // which then count for the rows from theirs on.
+      // 0 times an infinity or NaN of a later row is NaN. Where sums end up not finite, the rows are added again without such values:
+      // right for the rows before theirs. Those from theirs on are put right at the end.
       float odd = 0.0f;
 #pragma unroll
       for (int i = 0; i < IT; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) odd = fmaf(o[i][r], 0.0f, odd);
-      if (__any(odd != 0.0f)) {
+      if (__builtin_expect(__any(odd != 0.0f), 0)) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) asm volatile("" : "+v"(s[t]));  // computed again, not kept from above
         from_state();
@@ -527,18 +629,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
 #pragma unroll
           for (int j = 0; j < 4; ++j) fine[c][j] = only_finite<T>(v[c][j]);
         add_rows(fine);
-#pragma unroll
-        for (int i = 0; i < IT; ++i)
-#pragma unroll
-          for (int a = 0; a < 4; ++a)
-#pragma unroll 1
-            for (int j = 0; j <= 32 * i + col; ++j) {
-              const v2u32 w = *reinterpret_cast<const v2u32*>(sh.v + j * kRow + 16 * ((4 * wave + a) ^ value_swizzle<D>(j)) + 8 * half);
-              v4f special = {0, 0, 0, 0};
-              add_specials<T>(special, w);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[i][4 * a + e] += special[e];
-            }
+        met = true;
       }
       // Row 32 i + col, dims 32 wave + 8 a + 4 half + 0..3 for a = 0..3: with 16-bit outputs the halves exchange what the other stores.
       const int there = again(lane);
@@ -575,7 +666,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float less = s[t][r] * -decay.rest;
-        asm("" : "+v"(less));  // subtracted, as a sum would take its summand's register: 204 in place of more than there are, with 256 dims
+        asm("" : "+v"(less));  // as in decayed(): with 256 dims there would not be registers enough
         s[t][r] = fmaf(s[t][r], decay.whole, -less);
       }
 #pragma unroll
@@ -605,7 +696,15 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
     }
     __builtin_amdgcn_s_setprio(0);
   }
-  if (to) state_rows([&](int t, int r, int64_t at) { to[at] = s[t][r]; });
+  float odd = 0.0f, odd2 = 0.0f;
+  if (to) state_rows([&](int t, int r, int64_t) { (r % 2 ? odd2 : odd) = fmaf(s[t][r], 0.0f, r % 2 ? odd2 : odd); });
+  if (met || odd != 0.0f || odd2 != 0.0f) sh.met = 1;
+  __syncthreads();
+  if (__builtin_expect(sh.met == 0, 1)) {
+    if (to) state_rows([&](int t, int r, int64_t at) { to[at] = s[t][r]; });
+    return;
+  }
+  recurrence<T, D, OUT>(s, reinterpret_cast<uint64_t*>(&sh));
 }
 
 // The states before a long sequence's third part and later, from what each part adds: 4 values of one head a thread.
@@ -617,12 +716,13 @@ __global__ __launch_bounds__(256) void linear_parts_kernel(LinearParams p, float
   v4f* x = reinterpret_cast<v4f*>(kept + kept_at(p, lo, 1, head, size)) + (int)(blockIdx.x % pieces) * 256 + (int)threadIdx.x;
   const int64_t step = (int64_t)p.H * size / 4;
   const Decay decay = decay_of(p.log_decay[head], p.part);
+  const float one = power(p.log_decay[head], 1);  // an infinity is one still where exp(g rows) is 0 and exp(g) is not
   v4f s = *x;
 #pragma unroll 4
   for (int i = 2; i < parts; ++i) {
     const v4f add = x[(i - 1) * step];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] = fmaf(s[e], decay.whole, fmaf(s[e], decay.rest, add[e]));
+    for (int e = 0; e < 4; ++e) s[e] = __builtin_isfinite(s[e]) ? fmaf(s[e], decay.whole, fmaf(s[e], decay.rest, add[e])) : fmaf(s[e], one, add[e]);
     x[(i - 1) * step] = s;
   }
 }

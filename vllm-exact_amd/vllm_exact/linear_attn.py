@@ -5,8 +5,9 @@
 Kernels (libvllm_exact_amd.so, linear_attention.hip): whole prompts, packed one after the other, and one new token of every
 sequence. A state S is a D x D fp32 matrix of each head. States live in the slots of a pool: a sequence starts from one
 slot (or zeros) and leaves its state in one, the same or another, so beams that continue one parent read its slot and no
-state is copied. A row's bits depend on its own sequence, never on the rest of the batch. An infinity or NaN of a row makes
-this row and the later ones of its sequence that meet it infinite or NaN, never earlier ones.
+state is copied. A row's bits depend on its own sequence, never on the rest of the batch. An infinity or NaN of a row or of the state that
+a sequence starts from makes this row and the later ones that meet it, and the state, infinite or NaN as the recurrence
+has it (infinities of both signs in one sum are NaN), never earlier ones. Prompts with such values take 3 to 20 times as long.
 """
 import torch
 
