@@ -143,9 +143,12 @@ hipError_t launch_step(int64_t D, const LinearParams& p, hipStream_t st) {
 //   o_i = scale (exp(g (i + 1)) q_i S + sum_{j <= i} exp(g (i - j)) (q_i . k_j) v_j)
 //   S'  = exp(g n) S + sum_j k_j (exp(g (n - 1 - j)) v_j)^T
 // All of it runs on the matrix cores, with sums in fp32. What is not 16 bits wide already goes there as several bf16 numbers:
-//   S in q S, and the weighted scores: two, off by at most 2^-17 of each term; an output of 16 bits is rounded to 2^-8 or 2^-11 afterwards.
+//   S in q S, and the weighted scores: two where outputs have 16 bits, off by at most 2^-17 of each term; such an output is rounded to
+//   2^-8 or 2^-11 afterwards. Three where outputs have 32 bits, exactly. (Such outputs of 8192 rows, bf16 and 128 dims: 147 us of the call,
+//   178 with two parts and chunks of 64 rows, since scores of three parts take chunks of 32; fp16 and 256 dims: 235 and 203.)
 //   The weighted values, whose products add up to the state that later tokens start from: three, whose sum is the fp32 number itself.
-//   fp16 queries, keys and values beside them: two, exactly. Products of two second parts are left out (2^-16 of a term, in S 2^-22).
+//   fp16 queries, keys and values beside them: two, exactly. The product of the last parts of both is left out (of two parts 2^-16 of a
+//   term, of three 2^-24, in S 2^-22).
 // The weights are powers of a whole number of rows, at most 1, never quotients of two powers, which would overflow.
 //
 // A sequence is walked in order, so 32 heads of one prompt of 8192 rows would be 32 workgroups. It is cut into parts of 320 to 512 rows:
@@ -168,20 +171,22 @@ inline int part_rows(int64_t heads, int64_t dims) { return heads > 16 ? kMostRow
 
 __device__ inline float power(float g, int e) { return e == 0 ? 1.0f : expf(g * (float)e); }  // exp(-inf * 0) is 1 here
 
-// Eight fp32 values as two bf16 operands, off by at most 2^-17 of a value; 16 significant bits are exact.
-__device__ inline void split(const float (&x)[8], v4u32 (&part)[2]) {
+// Fp32 values as two bf16 operands, off by at most 2^-17 of a value; 16 significant bits are exact. N dwords of two values.
+template <int N, typename W>
+__device__ inline void split(const float (&x)[N], W (&part)[2]) {
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
+  for (int j = 0; j < N; j += 2) {
     part[0][j / 2] = BF16::pack(x[j], x[j + 1]);
     const v2f f = BF16::unpack(part[0][j / 2]);
     part[1][j / 2] = BF16::pack(x[j] - f.x, x[j + 1] - f.y);
   }
 }
-// Eight fp32 values as three bf16 operands whose sum they are exactly: cut off after 8 bits, and again. (Cutting takes one instruction
+// The same as three bf16 operands whose sum they are exactly: cut off after 8 bits, and again. (Cutting takes one instruction
 // for two values where rounding takes two or three; with two operands its error would be four times as large.)
-__device__ inline void split_exactly(const float (&x)[8], v4u32 (&part)[3]) {
+template <int N, typename W>
+__device__ inline void split(const float (&x)[N], W (&part)[3]) {
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
+  for (int j = 0; j < N; j += 2) {
     float a = x[j], b = x[j + 1];
 #pragma unroll
     for (int n = 0; n < 3; ++n) {
@@ -258,17 +263,18 @@ __device__ inline int64_t kept_at(const LinearParams& p, int lo, int part, int h
 }
 
 // A tile's 16-byte chunks lie at chunk ^ swizzle(row): 16 rows that are read at one chunk meet 16 different ones.
-template <typename T, int D, bool OUT>
+template <typename T, int D, bool OUT, bool WIDE>
 struct Shared {
   static constexpr bool F16 = std::is_same_v<T, FP16>;
   // Rows of a chunk: 64 (the state is split and decayed half as often as with 32: 120 us in place of 132 for 8192 rows), where two workgroups'
-  // tiles fit a CU's LDS; 32 in fp16, whose queries and keys lie there twice, and at 256 dims.
-  static constexpr int C = !F16 && D <= 128 ? 64 : 32;
+  // tiles fit a CU's LDS; 32 in fp16, whose queries and keys lie there twice, at 256 dims, and with scores of three parts at 128.
+  static constexpr int C = !F16 && D <= (WIDE ? 64 : 128) ? 64 : 32;
+  static constexpr int kParts = WIDE ? 3 : 2;  // of the state and the scores as operands
   static constexpr int kTile = C * 2 * D;
   char q[OUT ? kTile : 16], k[OUT ? kTile : 16];                       // for the scores
   char qs[OUT && F16 ? 2 : 1][OUT && F16 ? kTile : 16];                // fp16: queries as two bf16 parts
   char kt[F16 ? 2 : 1][kTile], v[kTile];                               // for transposed reads; fp16: keys as two bf16 parts
-  char scores[OUT ? (C == 64 ? 6 : 2) : 1][2][OUT ? 1024 : 16];        // operands of 16 keys and 32 queries, two parts
+  char scores[OUT ? (C == 64 ? 6 : 2) : 1][kParts][OUT ? 1024 : 16];   // operands of 16 keys and 32 queries
   float power[C];                                                      // scale exp(g (C - 1 - x))
   float left[C];                                                       // exp(g (n - 1 - j)) of row j of the chunk, 0 past its end
   int met;                                                             // whether something was not finite
@@ -377,14 +383,14 @@ __device__ inline void recurrence(const v16f (&s)[D / 32], uint64_t* signs) {
 // A workgroup of D / 32 waves takes one head of a part. A wave keeps 32 columns of the state in the accumulators of 32 x 32 x 16
 // MFMAs, where they are the operand of the next product as they lie. (Twice as many waves of 16 columns, four a SIMD: 80 us in place of 77
 // for the outputs of 8192 rows, since each of them splits, weights and waits as often.)
-// OUT: the rows' outputs from the state that the part starts from, and the sequence's end state. Else: the state that a
+// OUT: the rows' outputs from the state that the part starts from, and the sequence's end state (WIDE: outputs of 32 bits). Else: the state that a
 // part leaves, for all parts but a sequence's last; the first starts from the sequence's state, the others from zeros.
-template <typename T, int D, bool OUT>
+template <typename T, int D, bool OUT, bool WIDE>
 __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, float* kept) {
-  using S = Shared<T, D, OUT>;
+  using S = Shared<T, D, OUT, WIDE>;
   static_assert(!OUT || sizeof(S) >= D / 32 * 2 * kMostRows * sizeof(uint64_t), "recurrence() keeps bits there");
   constexpr bool F16 = S::F16;
-  constexpr int C = S::C, kRow = 2 * D;
+  constexpr int C = S::C, kRow = 2 * D, kParts = S::kParts;
   constexpr int DT = D / 32, IT = C / 32, CT = C / 16;  // blocks of the state's rows, of queries, of keys
   constexpr int kPieces = C / 16;                       // of a row tile, 16 bytes each, of a thread
   constexpr bool kLate = OUT;                           // the next rows are asked for when little but the state is held in registers
@@ -543,20 +549,21 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
         float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = s[u / 2][8 * (u % 2) + j];
-        v4u32 two[2];
-        split(f, two);
+        v4u32 part[kParts];
+        split(f, part);
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
           const int row = 32 * i + (now & 31), at = row * kRow + 16 * ((2 * u + (now >> 5)) ^ key_swizzle<D>(row));
           if constexpr (F16) {
             const v4u32 qhi = *reinterpret_cast<const v4u32*>(sh.qs[0] + at), qlo = *reinterpret_cast<const v4u32*>(sh.qs[1] + at);
-            o[i] = BF16::mfma32(two[0], qhi, o[i]);
-            o[i] = BF16::mfma32(two[1], qhi, o[i]);
-            o[i] = BF16::mfma32(two[0], qlo, o[i]);
+#pragma unroll
+            for (int n = 0; n < kParts; ++n) o[i] = BF16::mfma32(part[n], qhi, o[i]);
+#pragma unroll
+            for (int n = 0; n < kParts - 1; ++n) o[i] = BF16::mfma32(part[n], qlo, o[i]);
           } else {
             const v4u32 q = *reinterpret_cast<const v4u32*>(sh.q + at);
-            o[i] = BF16::mfma32(two[0], q, o[i]);
-            o[i] = BF16::mfma32(two[1], q, o[i]);
+#pragma unroll
+            for (int n = 0; n < kParts; ++n) o[i] = BF16::mfma32(part[n], q, o[i]);
           }
         }
         if (D == 256 && u % 2) __builtin_amdgcn_sched_barrier(0);
@@ -579,12 +586,11 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
         for (int r = 0; r < 4; ++r) x[r] = sh.power[min(C - 1 - query + key + r, C - 1)];
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] = query >= key + r ? sc[n][r] * x[r] : 0.0f;  // a later key's score may be an infinity
-        const v2u32 hi = {BF16::pack(x[0], x[1]), BF16::pack(x[2], x[3])};
-        const v2f h0 = BF16::unpack(hi.x), h1 = BF16::unpack(hi.y);
-        const v2u32 lo = {BF16::pack(x[0] - h0.x, x[1] - h0.y), BF16::pack(x[2] - h1.x, x[3] - h1.y)};
+        v2u32 part[kParts];
+        split(x, part);
         const int at = (32 * (l4 & 1) + (query & 31)) * 16 + 8 * (l4 >> 1), operand = (b < 4 ? 0 : 2) + key_of(b) / 16;
-        *reinterpret_cast<v2u32*>(sh.scores[operand][0] + at) = hi;
-        *reinterpret_cast<v2u32*>(sh.scores[operand][1] + at) = lo;
+#pragma unroll
+        for (int n = 0; n < kParts; ++n) *reinterpret_cast<v2u32*>(sh.scores[operand][n] + at) = part[n];
       }
     }
     v4u32 v[CT];
@@ -603,11 +609,13 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
           }
 #pragma unroll
           for (int i = c / 2; i < IT; ++i) {
-            const char* operand = sh.scores[(i ? 2 : 0) + c][0] + 16 * lane;
-            const v4u32 hi = *reinterpret_cast<const v4u32*>(operand), lo = *reinterpret_cast<const v4u32*>(operand + 1024);
-            o[i] = BF16::mfma32(two[0], hi, o[i]);
-            o[i] = BF16::mfma32(two[0], lo, o[i]);
-            if constexpr (F16) o[i] = BF16::mfma32(two[1], hi, o[i]);
+            v4u32 part[kParts];
+#pragma unroll
+            for (int n = 0; n < kParts; ++n) part[n] = *reinterpret_cast<const v4u32*>(sh.scores[(i ? 2 : 0) + c][n] + 16 * lane);
+#pragma unroll
+            for (int n = 0; n < kParts; ++n) o[i] = BF16::mfma32(two[0], part[n], o[i]);
+#pragma unroll
+            for (int n = 0; F16 && n < kParts - 1; ++n) o[i] = BF16::mfma32(two[1], part[n], o[i]);
           }
         }
       };
@@ -680,7 +688,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
         for (int e = 0; e < 4; ++e) f[j + e] *= w[e];
       }
       v4u32 three[3];
-      split_exactly(f, three);
+      split(f, three);
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
         const v4u32 k = transposed(now, sh.kt[0], c, t);
@@ -738,10 +746,13 @@ hipError_t launch_prompt(const LinearParams& p, float* kept, hipStream_t st) {
   const int64_t pieces = (int64_t)p.n * p.H * (D * D / 1024);
   if (!launchable(blocks, 2 * D) || !launchable(pieces, 256)) return hipErrorInvalidConfiguration;
   if (p.total > p.part) {  // some sequence may have several parts
-    hipLaunchKernelGGL((linear_chunk_kernel<T, D, false>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
+    hipLaunchKernelGGL((linear_chunk_kernel<T, D, false, false>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
     if (p.total > 2 * p.part) hipLaunchKernelGGL(linear_parts_kernel, dim3((unsigned)pieces), dim3(256), 0, st, p, kept, D * D);
   }
-  hipLaunchKernelGGL((linear_chunk_kernel<T, D, true>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
+  if (p.out_dtype == VXA_F32)
+    hipLaunchKernelGGL((linear_chunk_kernel<T, D, true, true>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
+  else
+    hipLaunchKernelGGL((linear_chunk_kernel<T, D, true, false>), dim3((unsigned)blocks), dim3(2 * D), 0, st, p, kept);
   return hipGetLastError();
 }
 template <typename T>

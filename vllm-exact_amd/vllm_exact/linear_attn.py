@@ -24,8 +24,8 @@ def linear_prompt(query, key, value, cu_seqlens, log_decay, scale, out, state=No
     sequence writes a slot that another reads or writes: where that is not so, or a slot is not in the pool, the sequence's
     rows are NaN and its state is not written. Rows after cu_seqlens[n] are left alone.
 
-    States and sums are fp32. Besides their roundings a row is off by at most 2^-17 (fp16: 3 2^-17) of the sum of its terms' magnitudes, and
-    by its output's rounding. Returns out."""
+    States and sums are fp32. An fp32 row is off by their roundings (fp16: and 2^-24 of the sum of its terms' magnitudes); rows of 16 bits
+    by their own rounding and at most 2^-17 (fp16: 3 2^-17) of that sum besides. Returns out."""
     status = (_nx._calls or _nx.calls()).linear_prompt(query, key, value, cu_seqlens, log_decay, scale, out, state, read_slots, write_slots)
     if status:
         _nx.check(status, "linear_prompt")
