@@ -144,8 +144,8 @@ hipError_t launch_step(int64_t D, const LinearParams& p, hipStream_t st) {
 //   S'  = exp(g n) S + sum_j k_j (exp(g (n - 1 - j)) v_j)^T
 // All of it runs on the matrix cores, with sums in fp32. What is not 16 bits wide already goes there as several bf16 numbers:
 //   S in q S, and the weighted scores: two where outputs have 16 bits, off by at most 2^-17 of each term; such an output is rounded to
-//   2^-8 or 2^-11 afterwards. Three where outputs have 32 bits, exactly. (Such outputs of 8192 rows, bf16 and 128 dims: 147 us of the call,
-//   178 with two parts and chunks of 64 rows, since scores of three parts take chunks of 32; fp16 and 256 dims: 235 and 203.)
+//   2^-8 or 2^-11 afterwards. Three where outputs have 32 bits, exactly. (A call of 8192 rows with such outputs, bf16 and 128 dims: 143 us,
+//   160 with two parts and chunks of 64 rows; three parts of the scores take chunks of 32. fp16 and 256 dims: 221 and 200.)
 //   The weighted values, whose products add up to the state that later tokens start from: three, whose sum is the fp32 number itself.
 //   fp16 queries, keys and values beside them: two, exactly. The product of the last parts of both is left out (of two parts 2^-16 of a
 //   term, of three 2^-24, in S 2^-22).
@@ -394,6 +394,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
   constexpr int DT = D / 32, IT = C / 32, CT = C / 16;  // blocks of the state's rows, of queries, of keys
   constexpr int kPieces = C / 16;                       // of a row tile, 16 bytes each, of a thread
   constexpr bool kLate = OUT;                           // the next rows are asked for when little but the state is held in registers
+  constexpr bool kFull = WIDE && F16 && D == 256;       // no registers to keep the values in for the state
   __shared__ __attribute__((aligned(1024))) S sh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -680,7 +681,7 @@ __global__ __launch_bounds__(2 * D, 2) void linear_chunk_kernel(LinearParams p, 
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       float f[8];
-      floats<T>(v[c], f);
+      floats<T>(kFull ? transposed(now, sh.v, c, wave) : v[c], f);
 #pragma unroll
       for (int j = 0; j < 8; j += 4) {
         const v4f w = *reinterpret_cast<const v4f*>(sh.left + 16 * c + 4 * (now >> 5) + 2 * j);
