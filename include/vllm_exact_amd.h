@@ -369,7 +369,8 @@ int vxa_linear_step(const void* q, int64_t stride_qt, int64_t stride_qh, const v
  * logits [n * beams, vocab] with row stride stride_row (fp32, bf16 or fp16), scores [n * beams]; out_scores, out_parents (the
  * logits' row) and out_tokens [n, count]. A beam of score -inf has no continuations, nor a token of logit -inf; where a request
  * has fewer than `count`, the rest is -inf, -1, -1. A request with a NaN or +inf among the logits or scores of its other beams
- * gets NaN, -1, -1. The workspace is on 16 bytes.
+ * gets NaN, -1, -1. The workspace is on 16 bytes. The outputs overlap neither each other nor the inputs, but out_scores may be
+ * `scores` where count is beams.
  */
 int vxa_beam_select_workspace(int64_t n, int64_t beams, int64_t vocab, int64_t count, size_t* ws_bytes);
 int vxa_beam_select(const void* logits, int64_t stride_row, int dtype, const float* scores, int64_t n, int64_t beams,

@@ -94,6 +94,55 @@ T* ptr(const at::Tensor* t) {
 }
 int64_t stride(const at::Tensor* t, int i) { return t ? t->stride(i) : 0; }
 
+// A tensor's memory: runs of `bytes` from `start` on, at all sums of the dims' strides. (Strides are not negative.)
+struct Memory {
+  struct Dim {
+    int64_t size, stride;  // bytes
+  };
+  int64_t start, bytes;
+  c10::SmallVector<Dim, 6> dims;  // the widest first
+  explicit Memory(const at::Tensor& t) : start((int64_t)(intptr_t)t.const_data_ptr()), bytes((int64_t)t.element_size()) {
+    const int64_t item = bytes;
+    for (int64_t i = 0; i < t.dim(); ++i)
+      if (t.size(i) > 1) dims.push_back({t.size(i), t.stride(i) * item});
+    std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
+    for (; !dims.empty() && dims.back().stride <= bytes; dims.pop_back()) bytes += (dims.back().size - 1) * dims.back().stride;
+  }
+  int64_t extent(size_t from = 0) const {  // from the first byte to the one behind the last, of the dims from `from` on
+    int64_t n = bytes;
+    for (size_t i = from; i < dims.size(); ++i) n += (dims[i].size - 1) * dims[i].stride;
+    return n;
+  }
+};
+// Whether b's runs, `apart` bytes behind a's, meet them, without the widest i dims of a and j of b. Of the widest left the places are
+// tried at which what is left of both meets: two, where rows and heads lie within each other. Layouts that take more than
+// `steps` trials count as meeting.
+bool meet(const Memory& a, size_t i, const Memory& b, size_t j, int64_t apart, int& steps) {
+  if (--steps < 0) return true;
+  const int64_t x = a.extent(i), y = b.extent(j);
+  if (apart >= x || -apart >= y) return false;
+  if (i == a.dims.size() && j == b.dims.size()) return true;
+  const int64_t sa = i < a.dims.size() ? a.dims[i].stride : -1, sb = j < b.dims.size() ? b.dims[j].stride : -1, s = std::max(sa, sb);
+  const int64_t most = sa == s ? a.dims[i].size - 1 : 0, least = sb == s ? 1 - b.dims[j].size : 0;  // places of a less those of b
+  i += sa == s, j += sb == s;
+  const int64_t p = a.extent(i), q = b.extent(j);
+  auto up = [](int64_t n, int64_t d) { return n >= 0 ? (n + d - 1) / d : -(-n / d); };  // n / d rounded up
+  for (int64_t k = std::max(least, up(apart - p + 1, s)); k <= most && k * s < apart + q; ++k)
+    if (meet(a, i, b, j, apart - k * s, steps)) return true;
+  return false;
+}
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const Memory x(a), y(b);
+  int steps = 1 << 14;
+  return meet(x, 0, y, 0, y.start - x.start, steps);
+}
+// Outputs that other workgroups' inputs, or other outputs, lie in.
+void check_apart(const char* what, const char* name, const at::Tensor& out, std::initializer_list<const at::Tensor*> others) {
+  for (const at::Tensor* t : others)
+    if (t && overlap(out, *t)) refuse(what, (std::string(": ") + name + " must not be, or overlap, another argument").c_str());
+}
+
 // The interpreter lock, given back while this lives: also where an exception ends the scope.
 struct Unlocked {
   PyThreadState* const state = PyEval_SaveThread();
@@ -325,6 +374,11 @@ int beam_select(PyObject* const* a) {
       best.size(0) != n || best.size(1) == 0 || parents.sizes() != best.sizes() || tokens.sizes() != best.sizes() || !best.is_contiguous() ||
       !parents.is_contiguous() || !tokens.is_contiguous())
     refuse(what, ": out_scores (fp32), out_parents (int32) and out_tokens (int64) are contiguous (requests, count)");
+  // A request's workgroup reads its scores before it writes as many in their place; with another count they would be others'.
+  const bool in_place = best.const_data_ptr() == scores.const_data_ptr() && best.numel() == scores.numel();
+  check_apart(what, "out_scores", best, {&x, in_place ? nullptr : &scores, &parents, &tokens});
+  check_apart(what, "out_parents", parents, {&x, &scores, &tokens});
+  check_apart(what, "out_tokens", tokens, {&x, &scores});
   if (n == 0) return VXA_OK;
   size_t bytes = 0;
   const int rc = beam_workspace_fn(n, beams, V, best.size(1), &bytes);
@@ -434,6 +488,17 @@ int resize_pages(PyObject* const* a) {
                    ptr(&ws), bytes);
 }
 
+// Whether two tensors have memory in common, for tests.
+PyObject* overlap_of(PyObject*, PyObject* const* args, Py_ssize_t given) {
+  HANDLE_TH_ERRORS
+  if (given != 2 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) {
+    PyErr_SetString(PyExc_TypeError, "overlap() takes two tensors");
+    return nullptr;
+  }
+  return PyBool_FromLong(overlap(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1])));
+  END_HANDLE_TH_ERRORS
+}
+
 int keep_drafted(PyObject* const* a) {
   const char* what = "keep_drafted";
   const at::Tensor &bt = *tensor(what, a[1]), &sl = *tensor(what, a[2]), &qsl = *tensor(what, a[3]), &keep = *tensor(what, a[4]);
@@ -495,6 +560,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t given) {
 
 #define VXA_METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {VXA_METHOD("bind", bind),
+                         VXA_METHOD("overlap", overlap_of),
                          VXA_METHOD("prompt_attention", (call<prompt_attention, 6>)),
                          VXA_METHOD("write_cache", (call<write_cache, 7>)),
                          VXA_METHOD("read_cache", (call<read_cache, 9>)),
