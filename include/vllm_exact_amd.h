@@ -343,7 +343,7 @@ int vxa_tree_decode(const void* q, int64_t stride_qt, int64_t stride_qh, int q_d
  * negative slot: zeros) and ends in write_slots[i] (null, negative: not kept), which may be the slot that it reads. A sequence
  * with a slot that the pool does not have, or one of whose slots another sequence writes, or that writes a slot which another
  * reads, gets NaN rows and writes no state.
- * out overlaps none of the others. Rows of q, k, v and out are less than 2^23 elements apart (strides 0 to 2^23 - 1).
+ * out overlaps none of the others, nor does a state that is written, or another state. Rows of q, k, v and out are less than 2^23 elements apart (strides 0 to 2^23 - 1).
  * prompt: sequence i is rows starts[i] .. starts[i + 1]; the workspace (on 16 bytes) holds states between parts of long sequences.
  * step: sequence i is row i.
  */

@@ -131,16 +131,27 @@ bool meet(const Memory& a, size_t i, const Memory& b, size_t j, int64_t apart, i
     if (meet(a, i, b, j, apart - k * s, steps)) return true;
   return false;
 }
+struct Range {  // from the first byte to behind the last
+  int64_t start, end;
+  explicit Range(const at::Tensor& t) : start((int64_t)(intptr_t)t.const_data_ptr()), end(start) {
+    if (t.numel() == 0) return;
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    end = start + (last + 1) * (int64_t)t.element_size();
+  }
+  bool apart(const Range& o) const { return start == end || o.start == o.end || end <= o.start || o.end <= start; }
+};
 bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  if (a.numel() == 0 || b.numel() == 0) return false;
+  if (Range(a).apart(Range(b))) return false;
   const Memory x(a), y(b);
   int steps = 1 << 14;
   return meet(x, 0, y, 0, y.start - x.start, steps);
 }
 // Outputs that other workgroups' inputs, or other outputs, lie in.
 void check_apart(const char* what, const char* name, const at::Tensor& out, std::initializer_list<const at::Tensor*> others) {
+  const Range range(out);
   for (const at::Tensor* t : others)
-    if (t && overlap(out, *t)) refuse(what, (std::string(": ") + name + " must not be, or overlap, another argument").c_str());
+    if (t && !range.apart(Range(*t)) && overlap(out, *t)) refuse(what, (std::string(": ") + name + " must not be, or overlap, another argument").c_str());
 }
 
 // The interpreter lock, given back while this lives: also where an exception ends the scope.
@@ -307,8 +318,6 @@ void check_linear(const char* what, const Linear& x, int64_t n, const at::Tensor
     refuse(what, ": inconsistent shapes");
   for (const at::Tensor* t : {&x.q, &x.k, &x.v, &x.out})
     if (t->size(2) && t->stride(2) != 1) refuse(what, ": the head dimension must be contiguous");
-  for (const at::Tensor* t : {&x.q, &x.k, &x.v})  // workgroups read rows whose outputs others have written
-    if (x.out.numel() && t->data_ptr() == x.out.data_ptr()) refuse(what, ": out must not be query, key or value");
   const int64_t H = x.q.size(1), D = x.q.size(2);
   if (!vector_of(x.decay, at::kFloat, H)) refuse(what, ": log_decay must be a contiguous fp32 vector, one number for each head");
   if ((x.read || x.write) && !x.state) refuse(what, ": slots need a pool of states");
@@ -317,9 +326,18 @@ void check_linear(const char* what, const Linear& x, int64_t n, const at::Tensor
     if (s.scalar_type() != at::kFloat) refuse(what, ": states must be fp32", PyExc_NotImplementedError);
     if (s.dim() != 4 || s.size(1) != H || s.size(2) != D || s.size(3) != D || s.stride(3) != 1 || s.stride(2) != D)
       refuse(what, ": states are (slots, H, D, D), each matrix contiguous");
+    if (x.write && s.numel()) {  // a workgroup writes each matrix
+      const bool slots_inside = s.stride(0) < s.stride(1);
+      const int64_t size = D * D, inner = s.size(slots_inside ? 0 : 1), inner_stride = s.stride(slots_inside ? 0 : 1), wide = s.stride(slots_inside ? 1 : 0);
+      if ((inner > 1 && inner_stride < size) || (s.size(slots_inside ? 1 : 0) > 1 && wide < (inner - 1) * inner_stride + size))
+        refuse(what, ": states must not overlap each other");
+      check_apart(what, "state", s, {&x.q, &x.k, &x.v, cu, &x.decay, x.read, x.write});
+    }
   }
   for (const at::Tensor* t : {x.read, x.write})
     if (t && !vector_of(*t, at::kInt, n)) refuse(what, ": slots must be contiguous int32 vectors, one for each sequence");
+  // Workgroups read rows whose outputs others have written.
+  check_apart(what, "out", x.out, {&x.q, &x.k, &x.v, cu, &x.decay, x.state, x.read, x.write});
 }
 
 int linear_prompt(PyObject* const* a) {
