@@ -387,12 +387,12 @@ int vxa_beam_select(const void* logits, int64_t stride_row, int dtype, const flo
  * fork: row r of out_table takes the pages of row parents[r] (negative, or no row: an empty one) and its length. Whole pages are
  * shared; a page that the length ends in is copied to the lowest free page, but for the first row of a parent where nobody else
  * holds that page. Rows r without children let go of their pages. Entries past a row's pages are -1.
- * out_table and out_lens are not block_table and seq_lens.
+ * The outputs overlap neither each other nor the inputs.
  * resize: rows that get longer take the lowest free pages (by ref_count as it was), in the order of rows and places, shorter ones
- * let go of theirs. Rows have at most `cols` pages. out_table may be block_table.
- * In both, out_ref_count may be ref_count, and `missing` [1] is the number of places that found no free page: they are -1.
+ * let go of theirs. Rows have at most `cols` pages. out_table may be block_table; else the outputs overlap nothing.
+ * In both, out_ref_count may be ref_count all the same, and `missing` [1] is the number of places that found no free page: they are -1.
  * keep: of the request's last T = starts[i + 1] - starts[i] <= 64 cached tokens those with bit j of keep[i] set move to
- * the places behind the others, in order, and out_lens is the length with them alone (not seq_lens itself). A request with
+ * the places behind the others, in order, and out_lens (apart from the inputs) is the length with them alone. A request with
  * more tokens than that, or fewer cached ones, stays as it is. No other request holds the pages of these tokens.
  */
 typedef struct {

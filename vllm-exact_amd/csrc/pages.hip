@@ -419,6 +419,7 @@ extern "C" int vxa_pages_copy(const vxa_cache_view* caches, int64_t count, int64
 
 extern "C" int vxa_pages_fork_workspace(int64_t rows, int64_t new_rows, size_t* ws_bytes) {
   if (rows < 0 || new_rows < 0 || !ws_bytes) return VXA_ERR_ARG;
+  if (std::max(rows, new_rows) > kMostRows) return VXA_ERR_UNSUPPORTED;
   *ws_bytes = (size_t)product({product({2, new_rows}) + rows, 4});
   return VXA_OK;
 }
@@ -459,6 +460,7 @@ extern "C" int vxa_pages_fork(const vxa_cache_view* caches, int64_t count, const
 
 extern "C" int vxa_pages_resize_workspace(int64_t rows, int64_t num_blocks, size_t* ws_bytes) {
   if (rows < 0 || num_blocks < 0 || !ws_bytes) return VXA_ERR_ARG;
+  if (rows > kMostRows) return VXA_ERR_UNSUPPORTED;
   *ws_bytes = (size_t)product({rows + 1 + num_blocks, 4});
   return VXA_OK;
 }

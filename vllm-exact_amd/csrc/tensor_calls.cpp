@@ -446,6 +446,12 @@ void check_tables(const char* what, const at::Tensor& table, const at::Tensor& o
   check_table(what, table);
   check_table(what, out);
   if (out.size(1) != table.size(1)) refuse(what, ": the tables must have the same columns");
+  if (out.size(0) > 1 && out.stride(0) < out.size(1)) refuse(what, ": the new table's rows must not overlap");
+}
+// Counts in their own place, or apart.
+void check_new_counts(const char* what, const at::Tensor& refs, const at::Tensor& out, std::initializer_list<const at::Tensor*> others) {
+  if (out.const_data_ptr() != refs.const_data_ptr()) check_apart(what, "out_ref_count", out, {&refs});
+  check_apart(what, "out_ref_count", out, others);
 }
 
 int copy_pages(PyObject* const* a) {
@@ -477,6 +483,10 @@ int fork_pages(PyObject* const* a) {
   size_t bytes = 0;
   const int rc = fork_workspace_fn(rows, many, &bytes);
   if (rc != VXA_OK) return rc;
+  // Rows read each other's pages and lengths while others are written.
+  check_apart(what, "out_table", out, {&bt, &sl, &parents, &refs, &out_lens, &out_refs, &missing});
+  check_apart(what, "out_lens", out_lens, {&bt, &sl, &parents, &refs, &out_refs, &missing});
+  check_new_counts(what, refs, out_refs, {&bt, &sl, &parents, &missing});
   at::Tensor ws;
   if (bytes) ws = at::empty({(int64_t)bytes / 4}, bt.options());
   return on_device(bt, pages_fork_fn, c.views.data(), (int64_t)c.views.size(), ptr<int32_t>(&bt), bt.stride(0), bt.size(1), ptr<int32_t>(&sl), rows,
@@ -500,6 +510,9 @@ int resize_pages(PyObject* const* a) {
   size_t bytes = 0;
   const int rc = resize_workspace_fn(rows, refs.size(0), &bytes);
   if (rc != VXA_OK) return rc;
+  const bool in_place = out.const_data_ptr() == bt.const_data_ptr() && (rows <= 1 || out.stride(0) == bt.stride(0));
+  check_apart(what, "out_table", out, {in_place ? nullptr : &bt, &sl, &lens, &refs, &out_refs, &missing});
+  check_new_counts(what, refs, out_refs, {&bt, &sl, &lens, &missing});
   const at::Tensor ws = at::empty({(int64_t)bytes / 4}, bt.options());
   return on_device(bt, pages_resize_fn, ptr<int32_t>(&bt), bt.stride(0), bt.size(1), ptr<int32_t>(&sl), ptr<int32_t>(&lens), rows,
                    ptr<int32_t>(&refs), refs.size(0), page, ptr<int32_t>(&out), out.stride(0), ptr<int32_t>(&out_refs), ptr<int32_t>(&missing),
@@ -529,6 +542,7 @@ int keep_drafted(PyObject* const* a) {
   if (!vector_of(sl, at::kInt, n) || !vector_of(qsl, at::kInt, n + 1) || !vector_of(out_lens, at::kInt, n))
     refuse(what, ": seq_lens, query_start_loc and out_lens must be contiguous int32 vectors, one length for each block-table row and the n + 1 starts");
   if (!vector_of(keep, at::kLong, n)) refuse(what, ": keep must be a contiguous int64 vector, one mask for each request");
+  check_apart(what, "out_lens", out_lens, {&bt, &sl, &qsl, &keep});
   if (n == 0) return VXA_OK;
   return on_device(bt, pages_keep_fn, c.views.data(), (int64_t)c.views.size(), ptr<int32_t>(&bt), bt.stride(0), bt.size(1), ptr<int32_t>(&sl),
                    ptr<int32_t>(&qsl), ptr<int64_t>(&keep), n, std::max<int64_t>(c.num_blocks, 0), page, ptr<int32_t>(&out_lens));

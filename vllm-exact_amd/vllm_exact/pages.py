@@ -25,9 +25,9 @@ def fork_pages(caches, block_table, seq_lens, parents, ref_count, block_size, ou
     """The rows of out_table continue those of block_table: row r takes row parents[r]'s pages and length (a negative parent, or
     one that is no row: an empty row). Whole pages are shared. A page that the length ends in is copied, in every cache, to the
     lowest free page, but for the first row of a parent where nobody else holds that page. Pages of rows that none
-    continues lose a holder. block_table (rows, max_blocks) and out_table (new rows, max_blocks) int32, not the same; entries
+    continues lose a holder. block_table (rows, max_blocks) and out_table (new rows, max_blocks) int32; entries
     behind a row's pages are -1. seq_lens (rows,), parents and out_lens (new rows,) int32. out_ref_count None: ref_count is
-    updated. Returns a (1,) int32 tensor: how many rows found no free page; theirs is -1, which the attention answers with
+    updated. Outputs have no memory in common with each other or the inputs. Returns a (1,) int32 tensor: how many rows found no free page; theirs is -1, which the attention answers with
     NaN."""
     missing = ref_count.new_empty(1)
     status = (_nx._calls or _nx.calls()).fork_pages(caches, block_table, seq_lens, parents, ref_count, block_size, out_table, out_lens,
@@ -41,7 +41,8 @@ def resize_pages(block_table, seq_lens, new_lens, ref_count, block_size, out_tab
     """Rows get the pages of new_lens tokens in place of seq_lens: the lowest free ones (free before the call) where they grow, in the order of
     rows and places; where they shrink, 0 for a row that has ended, the pages behind lose a holder and their entries
     are -1. A row has at most max_blocks pages. A grown row's last page is written to next: it should have no other holder, as
-    fork_pages leaves it. out_table and out_ref_count None: block_table and ref_count are updated. Returns a (1,) int32 tensor: how
+    fork_pages leaves it. out_table and out_ref_count None: block_table and ref_count are updated; others have no memory in common with
+    each other or the inputs. Returns a (1,) int32 tensor: how
     many pages were missing; their entries are -1."""
     missing = ref_count.new_empty(1)
     status = (_nx._calls or _nx.calls()).resize_pages(block_table, seq_lens, new_lens, ref_count, block_size,
@@ -55,7 +56,7 @@ def resize_pages(block_table, seq_lens, new_lens, ref_count, block_size, out_tab
 def keep_drafted(caches, block_table, seq_lens, query_start_loc, keep, block_size, out_lens):
     """After tree_attn.tree_decode: of each request's drafted tokens, the last query_start_loc[i + 1] - query_start_loc[i] (at most
     64) of its seq_lens[i] cached ones, those with bit j of keep[i] set (an accepted node's tree_mask) move side by side behind the
-    context, in every cache, bit for bit. keep (n,) int64; out_lens (n,) int32, not seq_lens itself, takes the lengths with the kept
+    context, in every cache, bit for bit. keep (n,) int64; out_lens (n,) int32, apart from the inputs, takes the lengths with the kept
     tokens alone, for resize_pages and the next step. No other row holds the drafted tokens' pages. A request with more drafted
     tokens than 64 or than cached ones stays as it is. Returns out_lens."""
     status = (_nx._calls or _nx.calls()).keep_drafted(caches, block_table, seq_lens, query_start_loc, keep, block_size, out_lens)
