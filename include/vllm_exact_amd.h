@@ -393,7 +393,8 @@ int vxa_beam_select(const void* logits, int64_t stride_row, int dtype, const flo
  * In both, out_ref_count may be ref_count all the same, and `missing` [1] is the number of places that found no free page: they are -1.
  * keep: of the request's last T = starts[i + 1] - starts[i] <= 64 cached tokens those with bit j of keep[i] set move to
  * the places behind the others, in order, and out_lens (apart from the inputs) is the length with them alone. A request with
- * more tokens than that, or fewer cached ones, stays as it is. No other request holds the pages of these tokens.
+ * more tokens than that, or fewer cached ones, stays as it is. No other request holds the pages of these tokens,
+ * no two views the same memory.
  */
 typedef struct {
   void* data;

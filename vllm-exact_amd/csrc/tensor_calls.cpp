@@ -141,8 +141,24 @@ struct Range {  // from the first byte to behind the last
   }
   bool apart(const Range& o) const { return start == end || o.start == o.end || end <= o.start || o.end <= start; }
 };
+// Whether two views of the same strides are rows beside each other, as keys and values in one buffer: a quick answer for most.
+bool side_by_side(const at::Tensor& a, const at::Tensor& b) {
+  const int64_t dims = a.dim(), size = a.element_size();
+  if (dims < 2 || b.dim() != dims || b.element_size() != size) return false;
+  int64_t step = INT64_MAX;  // all differences between the starts of two rows of one view are multiples of it
+  for (int64_t i = 0; i + 1 < dims; ++i) {
+    if (a.stride(i) != b.stride(i) || a.stride(i) == 0) return false;
+    step = std::min(step, a.stride(i));
+  }
+  for (int64_t i = 0; i + 1 < dims; ++i)
+    if (a.stride(i) % step != 0) return false;
+  const int64_t x = (a.size(dims - 1) - 1) * a.stride(dims - 1) + 1, y = (b.size(dims - 1) - 1) * b.stride(dims - 1) + 1;  // a row's elements
+  const int64_t bytes = (int64_t)(intptr_t)b.const_data_ptr() - (int64_t)(intptr_t)a.const_data_ptr(), apart = bytes / size;
+  const int64_t behind = (apart % step + step) % step;
+  return bytes % size == 0 && behind >= x && step - behind >= y;
+}
 bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  if (Range(a).apart(Range(b))) return false;
+  if (Range(a).apart(Range(b)) || side_by_side(a, b)) return false;
   const Memory x(a), y(b);
   int steps = 1 << 14;
   return meet(x, 0, y, 0, y.start - x.start, steps);
@@ -411,7 +427,8 @@ struct Caches {
   std::vector<vxa_cache_view> views;
   int64_t num_blocks = 0;
 };
-Caches caches_of(const char* what, PyObject* o, int64_t page, const at::Tensor& beside) {
+// apart: refused if they have memory in common, which is then moved twice.
+Caches caches_of(const char* what, PyObject* o, int64_t page, const at::Tensor& beside, bool apart = false) {
   PyObject* const list = PySequence_Fast(o, "");
   if (!list) {
     PyErr_Clear();
@@ -419,7 +436,10 @@ Caches caches_of(const char* what, PyObject* o, int64_t page, const at::Tensor& 
   }
   const THPObjectPtr kept(list);
   Caches c;
+  std::vector<std::pair<Range, const at::Tensor*>> ranges;
   c.num_blocks = -1;
+  c.views.reserve(PySequence_Fast_GET_SIZE(list));
+  if (apart) ranges.reserve(PySequence_Fast_GET_SIZE(list));
   for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(list); ++i) {
     const at::Tensor& t = *tensor(what, PySequence_Fast_GET_ITEM(list, i));
     check_gpu(what, {&beside, &t}, "the torch statements of pages.py");
@@ -428,6 +448,14 @@ Caches caches_of(const char* what, PyObject* o, int64_t page, const at::Tensor& 
     if (c.num_blocks >= 0 && t.size(0) != c.num_blocks) refuse(what, ": all caches must have the same blocks");
     c.num_blocks = t.size(0);
     const int64_t size = t.element_size();
+    if (apart && t.numel()) {
+      for (int64_t d = 0; d < t.dim(); ++d)
+        if (t.size(d) > 1 && t.stride(d) == 0) refuse(what, ": caches must not be expanded views");
+      const Range range(t);
+      for (size_t j = 0; j < ranges.size(); ++j)
+        if (!range.apart(ranges[j].first) && overlap(t, *ranges[j].second)) refuse(what, ": caches must not have memory in common");
+      ranges.emplace_back(range, &t);
+    }
     if (t.numel())
       c.views.push_back({t.data_ptr(), t.stride(0) * size, t.stride(1) * size, t.stride(2) * size, t.size(2), (t.dim() == 4 ? t.size(3) : 1) * size});
   }
@@ -536,7 +564,7 @@ int keep_drafted(PyObject* const* a) {
   const int64_t page = block_size(what, a[5]);
   const at::Tensor& out_lens = *tensor(what, a[6]);
   check_gpu(what, {&bt, &sl, &qsl, &keep, &out_lens}, "keep_drafted_torch");
-  const Caches c = caches_of(what, a[0], page, bt);
+  const Caches c = caches_of(what, a[0], page, bt, true);
   check_table(what, bt);
   const int64_t n = bt.size(0);
   if (!vector_of(sl, at::kInt, n) || !vector_of(qsl, at::kInt, n + 1) || !vector_of(out_lens, at::kInt, n))

@@ -57,7 +57,8 @@ def keep_drafted(caches, block_table, seq_lens, query_start_loc, keep, block_siz
     """After tree_attn.tree_decode: of each request's drafted tokens, the last query_start_loc[i + 1] - query_start_loc[i] (at most
     64) of its seq_lens[i] cached ones, those with bit j of keep[i] set (an accepted node's tree_mask) move side by side behind the
     context, in every cache, bit for bit. keep (n,) int64; out_lens (n,) int32, apart from the inputs, takes the lengths with the kept
-    tokens alone, for resize_pages and the next step. No other row holds the drafted tokens' pages. A request with more drafted
+    tokens alone, for resize_pages and the next step. No other row holds the drafted tokens' pages, and no two caches the same memory (values that are a slice of
+    the keys are moved with them). A request with more drafted
     tokens than 64 or than cached ones stays as it is. Returns out_lens."""
     status = (_nx._calls or _nx.calls()).keep_drafted(caches, block_table, seq_lens, query_start_loc, keep, block_size, out_lens)
     if status:
