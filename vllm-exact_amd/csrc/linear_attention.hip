@@ -161,13 +161,16 @@ hipError_t launch_step(int64_t D, const LinearParams& p, hipStream_t st) {
 // do not overlap here (two waves a SIMD, which is what their registers allow): per chunk of 64 rows a wave has 98 products of 32
 // clocks and some 1000 vector instructions that split, weight and stage, of 13,200 clocks that two of them take together.
 //
-// Where there are up to 16 heads, a few prompts leave CUs idle with parts of 512 rows: nine calls of 4 to 16 heads of 128 dims take 55 us
-// in the geometric mean with 320 rows and 68 with 512. With 32 heads there are enough workgroups, and what counts is each part's
-// state: 8192 rows 100 us, 121 with 320; 16 prompts of 900 163 and 194. States of 256 dims are four times as large: 384 rows, 178 us
-// in the mean of 15 calls with 16 heads where 512 take 193, and 320 175 with a fifth more states to keep (one prompt of 4096 rows 121 us
-// and 114, eight of 700 114 and 142).
+// Few heads of a few prompts leave CUs idle with long parts; with many there are enough workgroups, and what counts is each part's state,
+// which is written and read. us of a call, bf16, the geometric mean over prompts of 1024, 2048, 4096 and 8192 rows and batches of
+// 4 x 1024, 16 x 700 and 3 x 3000, with parts of 320, 384 and 512 rows:
+//   64 dims:   8 heads 38, 42, 51;    16: 42, 45, 53;     20: 45, 47, 57;    24: 47, 48, 56;     32: 53, 53, 58;     64: 72, 71, 77
+//   128 dims:  8 heads 51, 55, 68;    16: 62, 64, 73;     20: 73, 72, 81;    24: 77, 76, 82;     32: 90, 88, 92;     64: 143, 139, 135
+//   256 dims:                         16: 166, 172, 189;                     24: 237, 222, 231;  32: 278, 265, 260
+// (32 heads of 128, one of 8192 rows: 136, 129, 115; 16 of 700: 169, 135, 141. 256 dims and 16 heads take 384, as 320 keep a fifth more
+// states. Parts of 256 rows: as those of 320, within 9 %.)
 constexpr int kMostRows = 512;  // of a part
-inline int part_rows(int64_t heads, int64_t dims) { return heads > 16 ? kMostRows : dims > 128 ? 384 : 320; }
+inline int part_rows(int64_t heads, int64_t dims) { return heads <= 16 && dims <= 128 ? 320 : heads < 32 || dims <= 64 ? 384 : kMostRows; }
 
 __device__ inline float power(float g, int e) { return e == 0 ? 1.0f : expf(g * (float)e); }  // exp(-inf * 0) is 1 here
 
