@@ -13,11 +13,11 @@
 // A slice's place goes by the vocabulary alone, so a row's sums are the same bits in any batch and at any alignment.
 //
 // What bounds it: 256 rows of 248320 bf16 logits are 127 MB, 26 us at the rate of a large copy (19 at that of plain reads); the slices take
-// 40.6 us and the join 8.3. Vector instructions are in flight for 76 % of the slices' cycles: 19 a logit, of which 10 take a logit apart
+// 41.0 us and the join 8.5. Vector instructions are in flight for 76 % of the slices' cycles: 19 a logit, of which 10 take a logit apart
 // twice and add its exponential (one of them at a quarter of the rate), the others find the bar, look through the runs near it and
 // rank the candidates, work that a slice has whatever its size (half as many logits a thread: 48.9 us, the join 13.5). Loads alone are 30:
 // a workgroup has one slice, and while it computes only the others' loads are in flight. (Workgroups that stay and ask for their
-// next slice first need its registers as well, which costs as many waves: 58 us.) 4 rows of 151936: 7.1 + 4.8, two launches' latency.
+// next slice first need its registers as well, which costs as many waves: 58 us.) 4 rows of 151936: 7.0 + 5.5, two launches' latency.
 
 #include "attention_common.h"
 

@@ -79,7 +79,8 @@ constexpr int kCols = 32;  // columns of a state that a workgroup takes
 
 // A workgroup takes 32 columns of one head's state of one sequence: 128 bytes of each row, D / 8 rows a thread, so that a thread has
 // all its loads in flight at once and 64 sequences make 8192 workgroups. It reads and writes every value of the state once, and that is what
-// bounds it: 64 sequences, 32 heads of 128, 41 us, 6.6 TB/s. One sequence of 8 heads: 3.4 us, a launch and two dependent loads.
+// bounds it: 64 sequences, 32 heads of 128, that read 40 different slots, 219 MB: 41 us where a part of the states is in the last cache (62 MB
+// fetched, 132 written), 50 us, 4.4 TB/s, where none is. One sequence of 8 heads: 3.7 us, a launch and two dependent loads.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void linear_step_kernel(LinearParams p) {
   constexpr int kRows = D / 8;  // of the state, of a thread
@@ -145,21 +146,23 @@ hipError_t launch_step(int64_t D, const LinearParams& p, hipStream_t st) {
 // All of it runs on the matrix cores, with sums in fp32. What is not 16 bits wide already goes there as several bf16 numbers:
 //   S in q S, and the weighted scores: two where outputs have 16 bits, off by at most 2^-17 of each term; such an output is rounded to
 //   2^-8 or 2^-11 afterwards. Three where outputs have 32 bits, exactly. (A call of 8192 rows with such outputs, bf16 and 128 dims: 143 us,
-//   160 with two parts and chunks of 64 rows; three parts of the scores take chunks of 32. fp16 and 256 dims: 221 and 200.)
+//   160 with two parts and chunks of 64 rows; three parts of the scores take chunks of 32. fp16 and 256 dims: 221 and 200. With outputs of 16
+//   bits three parts would take 118 us in place of 104, and 195 in place of 174, for last bits of 2 values in 1000.)
 //   The weighted values, whose products add up to the state that later tokens start from: three, whose sum is the fp32 number itself.
 //   fp16 queries, keys and values beside them: two, exactly. The product of the last parts of both is left out (of two parts 2^-16 of a
 //   term, of three 2^-24, in S 2^-22).
 // The weights are powers of a whole number of rows, at most 1, never quotients of two powers, which would overflow.
 //
 // A sequence is walked in order, so 32 heads of one prompt of 8192 rows would be 32 workgroups. It is cut into parts of 320 to 512 rows:
-// one launch computes what each part adds to the state (half the work of outputs, 32 us for 8192 rows of 32 heads of 128), one adds
-// these up (10.5 us, and only where a sequence may have three parts), one computes the outputs (68 us). A token at
+// one launch computes what each part adds to the state (half the work of outputs, 34 us for 8192 rows of 32 heads of 128), one adds
+// these up (11 us, and only where a sequence may have three parts), one computes the outputs (69 us). A token at
 // a time, one after the other, the same call takes 4128 us. Where the cuts are goes by the sequence
 // and the heads alone, and so do a row's bits.
 //
-// What bounds it: 17.2 GF are 15 us at the rate of a large product, 170 MB 35 us at that of a copy. A SIMD's matrix and vector instructions
-// do not overlap here (two waves a SIMD, which is what their registers allow): per chunk of 64 rows a wave has 98 products of 32
-// clocks and some 1000 vector instructions that split, weight and stage, of 13,200 clocks that two of them take together.
+// What bounds it: 17.2 GF are 15 us at the rate of a large product, 170 MB 35 us at that of a copy. Behind a 32 x 32 x 16
+// product go four vector instructions, and more add up (a loop of products with 0, 4, 8 and 12 fmas to each, two waves a SIMD: 37, 37,
+// 47 and 57 clocks a product). Per chunk of 64 rows a wave has 98 products and some 1000 vector instructions that split, weight and
+// stage; registers allow two waves a SIMD. Of the outputs' cycles matrix pipes are busy for 31 %, vector instructions in flight for 44 %.
 //
 // Few heads of a few prompts leave CUs idle with long parts; with many there are enough workgroups, and what counts is each part's state,
 // which is written and read. us of a call, bf16, the geometric mean over prompts of 1024, 2048, 4096 and 8192 rows and batches of
@@ -260,7 +263,8 @@ __device__ inline Part find_part(const LinearParams& p, int index) {
   return Part{0, 0, 0, 0, 0};
 }
 // Where the state before part `part` of a sequence of several parts is kept: 2 floor(lo / rows of a part) + part. (The parts of a
-// sequence longer than one are at most twice its whole ones.)
+// sequence longer than one are at most twice its whole ones. Half of the places stay empty: the first state of a sequence needs one where
+// it is kept apart alone, and where the sequences before end only their lengths say.)
 __device__ inline int64_t kept_at(const LinearParams& p, int lo, int part, int head, int size) {
   return ((int64_t)(2 * (lo / p.part) + part) * p.H + head) * size;
 }

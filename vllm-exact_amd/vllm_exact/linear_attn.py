@@ -16,7 +16,7 @@ from . import _native as _nx
 
 def linear_prompt(query, key, value, cu_seqlens, log_decay, scale, out, state=None, read_slots=None, write_slots=None):
     """query (tokens, H, D), key/value (tokens, KV, D) bf16 or fp16, rows [cu_seqlens[i], cu_seqlens[i + 1]) of sequence i;
-    cu_seqlens (n + 1,) int32 on the GPU; log_decay (H,) fp32, <= 0; out (tokens, H, D) fp32, bf16 or fp16; rows and heads
+    cu_seqlens (n + 1,) int32 on the GPU, ascending; log_decay (H,) fp32, <= 0; out (tokens, H, D) fp32, bf16 or fp16; rows and heads
     may be strided (rows by less than 2^23 elements, all by multiples of 8 but for out), D is 64, 128 or 256 and contiguous. out has no memory in
     common with the others, a state that is written none with them or another state. state (slots, H, D, D) fp32, each matrix [key dim][value dim]
     contiguous. Sequence i starts from slot read_slots[i] (n,) int32 (None or negative: from zeros), and its state after its last
